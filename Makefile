@@ -16,7 +16,8 @@ all: $(LIB) $(CLI) oracle
 # device-linked into the shared library.
 SRCS      := $(CSRC)/voltattn_api.cu $(CSRC)/host_util.cu $(CSRC)/launch_tc.cu $(CSRC)/launch_tcg.cu \
              $(CSRC)/launch_mma.cu $(CSRC)/launch_prefill.cu $(CSRC)/launch_stream_g1.cu \
-             $(CSRC)/launch_stream_g2.cu $(CSRC)/launch_stream_g4.cu $(CSRC)/launch_stream_g8.cu
+             $(CSRC)/launch_stream_g2.cu $(CSRC)/launch_stream_g4.cu $(CSRC)/launch_stream_g8.cu \
+             $(CSRC)/launch_tree_d64.cu $(CSRC)/launch_tree_d128.cu $(CSRC)/launch_cache.cu $(CSRC)/cache_api.cu
 OBJDIR    := voltattn_b200/_build
 OBJS      := $(patsubst $(CSRC)/%.cu,$(OBJDIR)/%.o,$(SRCS))
 

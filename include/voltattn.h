@@ -372,6 +372,102 @@ VA_API int va_decode_noalloc(int fmt, const va_bufs* bufs, int H, int L, int D, 
  * the flag of the current device; *code = 0 when no kernel reported one. */
 VA_API int va_device_error(int* code);
 
+/* ---- Speculative decoding over a paged cache (no reference counterpart) -------
+ * The cache is the pool of va_decode_paged: K/V [num_pages][Hkv][page_rows] rows,
+ * scales alike, row j of a sequence in page block_table[b * max_pages +
+ * j / page_rows]. Lengths and tables live on the device; nothing is read back,
+ * so a whole step can be captured in a CUDA graph. */
+
+/* Tree attention: sequence b's cache holds lens[b] rows (device int32 [B]; 0 is
+ * an unused slot), of which the last n = nodes[b] (device int32 [B], or NULL: Q
+ * each; at most Q and lens[b]) are its drafted tokens' K/V, appended in node
+ * order. Node i < n of query head h attends to all rows before the drafted ones,
+ * and to drafted row j for each bit j < n of tree_mask[b * Q + i] (device uint64
+ * [B][Q]; a node sees itself only if its own bit is set). Rows that it does not
+ * attend to have no influence on it, whatever they hold. Nodes i >= n, and nodes
+ * that see no row, give 0. Q <= 64; a plain chain or one token per sequence (Q = 1)
+ * are trees like any other.
+ * q, out: __half, element (b, i, h, d) at b * strides[0] + i * strides[1] +
+ * h * strides[2] + d (host arrays of 3, multiples of 8; NULL: contiguous
+ * [B][Q][Hq][D]); q 16-byte, out 8-byte aligned. Any Hq / Hkv. Formats f16+ / bf16+ /
+ * f8+ / q8+ / q4+ / q3+ at D = 64 or 128, page_rows a multiple of 8 (else
+ * VA_ERR_UNSUPPORTED). bf16 rows are taken as fp16 values (beyond fp16's range:
+ * infinite). Table entries outside [0, num_pages) read page 0.
+ * S: splits of a sequence's rows over CTAs (<= 128; 0: chosen by
+ * va_suggest_tree_splits' rule and what ws holds). ws: 16-byte aligned,
+ * ws_bytes >= va_tree_workspace_bytes(B, Hq, Hkv, Q, D, max(S, 1)), zeroed before
+ * first use (va_workspace_init). A completed call leaves the counters at its front
+ * zero, so one workspace serves calls of any shape in order on one stream. Splits
+ * (S > 1) take at most 16384 row tiles (B * Hkv * (Hq / Hkv * Q / 32, rounded up)). */
+VA_API size_t va_tree_workspace_bytes(int B, int Hq, int Hkv, int Q, int D, int S);
+VA_API int va_suggest_tree_splits(int fmt, int B, int Hq, int Hkv, int Q, int Lmax, int D, int* S);
+VA_API int va_decode_tree(int fmt, const va_bufs* bufs, const long long* q_strides, const long long* out_strides,
+                          const uint64_t* tree_mask, const int* lens, const int* nodes, const int* block_table,
+                          int max_pages, int B, int Hq, int Hkv, int Q, int page_rows, int num_pages, int D, int S,
+                          void* ws, size_t ws_bytes, void* stream);
+
+/* Types of the rows that va_append_packed takes. */
+typedef enum va_dtype { VA_FP32 = 0, VA_FP16 = 1, VA_BF16 = 2 } va_dtype;
+
+/* Appends packed tokens: token x (0 <= x < T) of K at element x * k_strides[0] +
+ * h * k_strides[1] + d (V alike; host arrays of 2, multiples of 8, or 4 for fp32;
+ * NULL: contiguous [T][Hkv][D]) belongs to the sequence b with cu_tokens[b] <= x <
+ * cu_tokens[b + 1] (device int32 [B + 1], ascending) and goes to its row
+ * pos[b] + x - cu_tokens[b] (device int32 [B]) of the pool bufs->K / V / scK / scV,
+ * with the arithmetic of va_quantize (q8 / q4 / q3), va_quantize_f8 (f8+) or one
+ * rounding (f16, bf16+) of the values in fp32. Tokens past cu_tokens[B], and rows
+ * whose page is not in the table, are skipped. Every format but q4c+; k and v
+ * 16-byte aligned; bufs->q and out are not used. */
+VA_API int va_append_packed(int fmt, const void* k, const void* v, int in_type, const long long* k_strides,
+                            const long long* v_strides, const va_bufs* bufs, const int* block_table, int max_pages,
+                            const int* cu_tokens, const int* pos, int T, int B, int Hkv, int page_rows, int num_pages,
+                            int D, void* stream);
+
+/* After a tree has been verified: moves the accepted drafted rows together.
+ * path: device int32 [B][P] (P <= 64), node indices from the root down,
+ * ascending; the first accepted[b] of sequence b's are accepted (the path ends
+ * at the first entry that does not ascend inside [0, nodes[b])). Row ctx + path[i]
+ * becomes row ctx + i, ctx = lens[b] - nodes[b], in every KV head of every layer;
+ * new_lens[b] = ctx + accepted (device int32 [B], not lens itself). Pool
+ * of `layers` layers, each [num_pages][Hkv][page_rows] rows, one after the other, that
+ * share the table (layers of separate allocations: one call each). Every
+ * format but q4c+. */
+VA_API int va_accept_tree(int fmt, const va_bufs* bufs, const int* block_table, int max_pages, const int* lens,
+                          const int* nodes, const int* path, const int* accepted, int* new_lens, int B, int P, int Hkv,
+                          int page_rows, int num_pages, int D, int layers, void* stream);
+
+/* Forks, reorders and frees sequences: new sequence i < Bout continues sequence
+ * parent[i] of the Bin old ones (device int32 [Bout]; any value outside
+ * [0, Bin): an empty sequence). Old sequences that nothing continues are freed.
+ * refs (device int32 [num_pages]) counts the table entries that hold a page, 0 =
+ * free. The first new sequence of a parent keeps all of its pages; the others
+ * share its full pages (lens / page_rows of them), and get a page of their own
+ * for the rest, into which the rows are copied (in blocks of 8, in every layer).
+ * Each new sequence then has pages for lens + reserve rows, as far as max_pages
+ * go. Pages are given out lowest number first, in order of sequence and place,
+ * from those with refs 0 before the call (pages that the call frees serve the
+ * next one). *shortage (device int32) = how many it did not find: their entries
+ * are -1, and a sequence that got none for its copied rows ends at its last full
+ * page. Outputs new_refs [num_pages], new_table [Bout][max_pages], new_lens
+ * [Bout]: separate buffers from the inputs. Bin, Bout <= 4000; page_rows a
+ * multiple of 8; every format but q4c+; layers as va_accept_tree. ws: 4-byte
+ * aligned scratch of va_pages_workspace_bytes(Bout, max_pages, num_pages)
+ * (not one that va_decode_tree uses: it does not stay zero). */
+VA_API size_t va_pages_workspace_bytes(int B, int max_pages, int num_pages);
+VA_API int va_fork_pages(int fmt, const va_bufs* bufs, const int* refs, const int* block_table, const int* lens,
+                         const int* parent, int* new_refs, int* new_table, int* new_lens, int* shortage, int Bin,
+                         int Bout, int max_pages, int reserve, int Hkv, int page_rows, int num_pages, int D,
+                         int layers, void* ws, size_t ws_bytes, void* stream);
+
+/* Compacts a pool: with n pages in use (refs > 0; *used = n, device int32), the
+ * m-th used page at or past n moves to the m-th free page below n, in every
+ * layer; new_refs [num_pages] and new_table [B][max_pages] (separate buffers)
+ * are renumbered to match (table entries outside the pool are kept). Afterwards pages
+ * [0, n) are in use and the rest of the pool is free. Arguments as va_fork_pages. */
+VA_API int va_compact_pages(int fmt, const va_bufs* bufs, const int* refs, const int* block_table, int* new_refs,
+                            int* new_table, int* used, int B, int max_pages, int Hkv, int page_rows, int num_pages,
+                            int D, int layers, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -90,6 +90,20 @@ def _load():
     lib.va_decode_paged.restype = i
     lib.va_append_kv_paged.argtypes = [i, vp, vp, vp, vp, i, i, i, i, i, i, vp, vp]
     lib.va_append_kv_paged.restype = i
+    ll2 = C.POINTER(C.c_longlong)
+    lib.va_tree_workspace_bytes.argtypes = [i] * 6; lib.va_tree_workspace_bytes.restype = sz
+    lib.va_suggest_tree_splits.argtypes = [i] * 7 + [C.POINTER(i)]; lib.va_suggest_tree_splits.restype = i
+    lib.va_decode_tree.argtypes = [i, C.POINTER(VaBufs), ll2, ll2, vp, vp, vp, vp] + [i] * 9 + [vp, sz, vp]
+    lib.va_decode_tree.restype = i
+    lib.va_append_packed.argtypes = ([i, vp, vp, i, ll2, ll2, C.POINTER(VaBufs), vp, i, vp, vp] + [i] * 6 + [vp])
+    lib.va_append_packed.restype = i
+    lib.va_accept_tree.argtypes = [i, C.POINTER(VaBufs), vp, i, vp, vp, vp, vp, vp] + [i] * 7 + [vp]
+    lib.va_accept_tree.restype = i
+    lib.va_pages_workspace_bytes.argtypes = [i, i, i]; lib.va_pages_workspace_bytes.restype = sz
+    lib.va_fork_pages.argtypes = [i, C.POINTER(VaBufs)] + [vp] * 8 + [i] * 9 + [vp, sz, vp]
+    lib.va_fork_pages.restype = i
+    lib.va_compact_pages.argtypes = [i, C.POINTER(VaBufs)] + [vp] * 5 + [i] * 7 + [vp, sz, vp]
+    lib.va_compact_pages.restype = i
     lib.va_device_error.argtypes = [C.POINTER(i)]; lib.va_device_error.restype = i
     return lib
 
@@ -400,6 +414,111 @@ def decode_paged(fmt, b: DeviceBufs, block_table, max_pages: int, lens, B: int, 
     _check(_lib.va_decode_paged(int(Fmt.parse(fmt)), C.byref(vb), _ptr(block_table), max_pages, _ptr(lens), B, Hq,
                                 Hkv, page_rows, num_pages, D, S, _ptr(b.ws), b.ws.numel() * b.ws.element_size(),
                                 _stream_ptr(stream)), "decode_paged")
+
+
+# ---- speculative decoding over a paged cache (no reference counterpart) ----
+
+
+def _nbytes(t) -> int:
+    return 0 if t is None else t.numel() * t.element_size()
+
+
+def _strides(t, n: int):
+    """The strides of a tensor's first n dimensions (its last one dense), None for a flat or contiguous one."""
+    if t.dim() != n + 1 or t.is_contiguous():
+        if not t.is_contiguous():
+            raise ValueError(f"expected a contiguous tensor or one of {n + 1} dimensions")
+        return None
+    if t.stride(-1) != 1:
+        raise ValueError("the last dimension must be dense")
+    return (C.c_longlong * n)(*t.stride()[:n])
+
+
+def tree_workspace_bytes(B: int, Hq: int, Hkv: int, Q: int, D: int, S: int) -> int:
+    return int(_lib.va_tree_workspace_bytes(B, Hq, Hkv, Q, D, S))
+
+
+def suggest_tree_splits(f, B: int, Hq: int, Hkv: int, Q: int, Lmax: int, D: int) -> int:
+    s = C.c_int(0)
+    _check(_lib.va_suggest_tree_splits(int(Fmt.parse(f)), B, Hq, Hkv, Q, Lmax, D, C.byref(s)), "suggest_tree_splits")
+    return s.value
+
+
+def decode_tree(fmt, b: DeviceBufs, tree_mask, lens, nodes, block_table, max_pages: int, B: int, Hq: int, Hkv: int,
+                Q: int, page_rows: int, num_pages: int, D: int, S: int = 0, stream=None):
+    """Attention of a tree of drafted tokens over a paged cache (va_decode_tree):
+    node i of sequence b sees the lens[b] - nodes[b] rows before the drafted ones
+    and the drafted rows j whose bit is set in tree_mask[b][i] (int64 or uint64
+    CUDA tensor [B][Q], Q <= 64). b.q, b.out: fp16 [B][Q][Hq][D] (four-dimensional
+    tensors may be strided, the last dimension dense); lens, nodes int32 [B]
+    (nodes None: Q each), block_table int32 [B][max_pages]. S = 0: the library
+    splits the rows as the workspace b.ws (zeroed once, tree_workspace_bytes) allows."""
+    vb = b.va()
+    _check(_lib.va_decode_tree(int(Fmt.parse(fmt)), C.byref(vb), _strides(b.q, 3), _strides(b.out, 3),
+                               _ptr(tree_mask), _ptr(lens), _ptr(nodes), _ptr(block_table), max_pages, B, Hq, Hkv, Q,
+                               page_rows, num_pages, D, S, _ptr(b.ws), _nbytes(b.ws), _stream_ptr(stream)),
+           "decode_tree")
+
+
+def append_packed(fmt, k, v, b: DeviceBufs, block_table, max_pages: int, cu_tokens, pos, B: int, Hkv: int,
+                  page_rows: int, num_pages: int, D: int, stream=None):
+    """K/V rows of packed tokens (k, v [T][Hkv][D], fp32 / fp16 / bf16, three-dimensional
+    tensors may be strided as slices of one projection are) quantized into the
+    pages of the pool in b: sequence b's tokens cu_tokens[b] .. cu_tokens[b+1] go
+    to its rows from pos[b] on (int32 CUDA tensors [B+1], [B])."""
+    import torch
+    kinds = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    if k.dtype != v.dtype or k.dtype not in kinds or k.shape != v.shape:
+        raise ValueError("append_packed: k and v must be float32, float16 or bfloat16 tensors of one shape")
+    T = k.shape[0] if k.dim() == 3 else k.numel() // (Hkv * D)
+    if T * Hkv * D != k.numel():
+        raise ValueError("append_packed: k and v must hold T * Hkv * D elements")
+    vb = b.va()
+    _check(_lib.va_append_packed(int(Fmt.parse(fmt)), _ptr(k), _ptr(v), kinds[k.dtype], _strides(k, 2), _strides(v, 2),
+                                 C.byref(vb), _ptr(block_table), max_pages, _ptr(cu_tokens), _ptr(pos), T, B, Hkv,
+                                 page_rows, num_pages, D, _stream_ptr(stream)), "append_packed")
+
+
+def accept_tree(fmt, b: DeviceBufs, block_table, max_pages: int, lens, nodes, path, accepted, new_lens, B: int, P: int,
+                Hkv: int, page_rows: int, num_pages: int, D: int, layers: int = 1, stream=None):
+    """Moves the accepted drafted rows together (va_accept_tree): row
+    lens - nodes + path[b][i] becomes row lens - nodes + i for i < accepted[b], in
+    every layer of the pool; new_lens[b] = lens[b] - nodes[b] + accepted. path:
+    int32 [B][P] ascending node indices (P <= 64)."""
+    vb = b.va()
+    _check(_lib.va_accept_tree(int(Fmt.parse(fmt)), C.byref(vb), _ptr(block_table), max_pages, _ptr(lens), _ptr(nodes),
+                               _ptr(path), _ptr(accepted), _ptr(new_lens), B, P, Hkv, page_rows, num_pages, D, layers,
+                               _stream_ptr(stream)), "accept_tree")
+
+
+def pages_workspace_bytes(B: int, max_pages: int, num_pages: int) -> int:
+    return int(_lib.va_pages_workspace_bytes(B, max_pages, num_pages))
+
+
+def fork_pages(fmt, b: DeviceBufs, refs, block_table, lens, parent, new_refs, new_table, new_lens, shortage, Bin: int,
+               Bout: int, max_pages: int, reserve: int, Hkv: int, page_rows: int, num_pages: int, D: int,
+               layers: int = 1, stream=None):
+    """Forks, reorders and frees sequences (va_fork_pages): new sequence i
+    continues old sequence parent[i] (outside [0, Bin): empty), sharing its full
+    pages and getting a copy of its last one, then pages for `reserve` more rows.
+    All tensors int32 CUDA; refs counts a page's table entries (0: free). b.ws:
+    scratch of pages_workspace_bytes(Bout, max_pages, num_pages)."""
+    vb = b.va()
+    _check(_lib.va_fork_pages(int(Fmt.parse(fmt)), C.byref(vb), _ptr(refs), _ptr(block_table), _ptr(lens), _ptr(parent),
+                              _ptr(new_refs), _ptr(new_table), _ptr(new_lens), _ptr(shortage), Bin, Bout, max_pages,
+                              reserve, Hkv, page_rows, num_pages, D, layers, _ptr(b.ws), _nbytes(b.ws),
+                              _stream_ptr(stream)), "fork_pages")
+
+
+def compact_pages(fmt, b: DeviceBufs, refs, block_table, new_refs, new_table, used, B: int, max_pages: int, Hkv: int,
+                  page_rows: int, num_pages: int, D: int, layers: int = 1, stream=None):
+    """Moves the pages in use to the front of the pool (va_compact_pages) and
+    renumbers refs and block_table into new_refs and new_table; used[0] = their
+    number. b.ws: scratch of pages_workspace_bytes(B, max_pages, num_pages)."""
+    vb = b.va()
+    _check(_lib.va_compact_pages(int(Fmt.parse(fmt)), C.byref(vb), _ptr(refs), _ptr(block_table), _ptr(new_refs),
+                                 _ptr(new_table), _ptr(used), B, max_pages, Hkv, page_rows, num_pages, D, layers,
+                                 _ptr(b.ws), _nbytes(b.ws), _stream_ptr(stream)), "compact_pages")
 
 
 def probe_ceiling(device: int = 0, nbytes: int = 0, reps: int = 0, method: Optional[int] = None) -> float:

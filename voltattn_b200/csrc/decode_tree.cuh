@@ -1,0 +1,760 @@
+// Attention of a tree of drafted tokens over a paged, quantized KV cache: the
+// verification step of speculative decoding (no reference counterpart; the
+// reference decodes one token at a time).
+//
+// Sequence b has lens[b] rows in its cache, of which the last n = nodes[b] are
+// the drafted tokens'; ctx = lens[b] - n. Node i of sequence b sees the rows
+//   A(b, i) = [0, ctx)  and  ctx + j for every bit j < n of mask[b][i]
+// and for every query head h, with KV head h / G,
+//   out[b][i][h] = sum_{p in A} w_p V_p / sum_{p in A} w_p,   w_p = exp(q . K_p / sqrt(D))
+// in the running form of a softmax; a row that sees nothing gives 0.
+//
+// All G * Q query rows of a (sequence, KV head) read the same cache rows, so
+// a CTA takes a tile of 16 or 32 query rows (row r: node r / G, query head
+// r % G of the group) over a range of the sequence's positions, and streams
+// the codes once. Its four warps take blocks of positions in turn, each with
+// its own running statistics and its own ring of shared-memory stages that one
+// lane set fills by bulk copies; they merge at the end, and the last CTA of a
+// row tile merges the ranges.
+//
+// The products run on mma.sync m16n8k16 straight from the codes: a code is
+// placed into an fp16 mantissa with a shift and a bit operation, the result is
+// exact, and no scale is multiplied in fp16.
+//   S = Q K^T: the K scale of (row, 64-dim group) multiplies the group's fp32
+//     partial score. The offset of the placed codes (x = offset + code * step)
+//     is taken off as -offset * sum(q) in the accumulator's initial value.
+//   O += P V: the V scale multiplies the fp32 weight before its one rounding to
+//     fp16 (P' = fp16(w * scale), one P' per group).
+// The rounding of P' is the only one below 32 bits: it is relative (2^-11)
+// because the exponent's reference is kept so that P' of the largest weight
+// lies in [2^13, 2^15): ref = max over blocks of (row maximum + exponent of
+// the block's largest V scale - 13), in log2 units.
+//
+// Rows that a query row does not see have no influence at all on it: their
+// scores are replaced, their weights selected to 0 before the scale (which may
+// be anything, nan included) is applied, and float formats' rows past the end
+// are cleared. A drafted float row with inf or nan entries reaches only the rows
+// that see it (`special` below).
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+#include "formats.cuh"
+
+namespace va {
+
+struct TreeParams {
+    const uint8_t* K;
+    const uint8_t* V;
+    const __half* scK;
+    const __half* scV;
+    const __half* q;
+    __half* out;
+    const unsigned long long* mask;  // [B][Q]
+    const int* lens;                 // [B]
+    const int* nodes;                // [B] or null (Q each)
+    const int* table;                // [B][max_pages]
+    float* ws_o;                     // [B*Hkv][R][S][D] partial outputs
+    float* ws_ml;                    // [B*Hkv][R][S][2] reference and sum
+    unsigned* counters;              // [B*Hkv*tiles]
+    long long qs_b, qs_t, qs_h;      // element strides of q and out: sequence, node, head
+    long long os_b, os_t, os_h;
+    int B, Hkv, G, Q, R, tiles, S;
+    int max_pages, page_rows, num_pages;
+};
+
+// Splits of a sequence of len rows: whole units of kTreeUnit rows, at most S.
+constexpr int kTreeUnit = 128;
+__device__ __forceinline__ int tree_chunk(int len, int S) {
+    const int units = (len + kTreeUnit - 1) / kTreeUnit;
+    return max(1, (units + S - 1) / S) * kTreeUnit;
+}
+
+template <Kind K, int kDim, int kMTiles>
+struct TreeCfg {
+    static constexpr Kind kKind = K;
+    static constexpr int kD = kDim;
+    static constexpr int kMT = kMTiles;           // 16-row tiles of query rows
+    static constexpr int kRows = 16 * kMTiles;    // query rows of a CTA
+    static constexpr int kNG = kDim / 64;         // scale groups
+    static constexpr bool kScaled = !(K == Kind::F16 || K == Kind::BF16);
+    static constexpr bool kFloat = is_float_kind(K);  // rows that can hold inf / nan
+    static constexpr int kRb = kDim * KindTraits<K>::kBits / 8;
+    static constexpr int kSb = kScaled ? 2 * kNG : 0;
+    // positions of a block: 32, or 16 where 32 rows of 256 bytes would leave
+    // room for one CTA per SM only
+    static constexpr int kPb = (kScaled || kDim == 64) ? 32 : 16;
+    static constexpr int kWarps = 4;
+    static constexpr int kThreads = 32 * kWarps;
+    static constexpr int kOffV = kPb * kRb;
+    static constexpr int kOffSK = 2 * kPb * kRb;
+    static constexpr int kOffSV = kOffSK + kPb * kSb;
+    static constexpr int kTx = kOffSV + kPb * kSb;
+    static constexpr int kStageBytes = (kTx + 127) / 128 * 128;
+    static constexpr int kStages = kStageBytes > 8000 ? 2 : kStageBytes > 5000 ? 3 : 4;
+    static constexpr int kRing = kWarps * kStages * kStageBytes;
+    static constexpr int kOStride = kDim + 4;     // floats of a merged row
+    static constexpr int kMerge = kWarps * kRows * kOStride * 4;
+    static constexpr int kBig = kRing > kMerge ? kRing : kMerge;
+    // + barriers, masks, (ref, l) of every warp and row, the ticket
+    static constexpr int kSmemBytes = kBig + kWarps * kStages * 8 + kRows * 8 + kWarps * kRows * 8 + 16;
+    static constexpr int kMinCtas = kMTiles == 1 ? 3 : 2;
+};
+
+__device__ __forceinline__ void mma_f16_16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+        "%2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
+__device__ __forceinline__ uint32_t bf2_to_h2(uint32_t w) {
+    const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+    return h2_bits(__float22half2_rn(f));
+}
+__device__ __forceinline__ uint32_t f8x2_to_h2(uint32_t b) {
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(b & 0xFFFFu), __NV_E4M3);
+    return (uint32_t)r.x | ((uint32_t)r.y << 16);
+}
+
+// What a placed code stands for: x = kOffset + code * kStep, code = the signed
+// code. q4: 1 + nibble / 16; q3: 1 + field / 8; q8: 1024 + byte.
+template <Kind K>
+struct TreeCode {
+    static constexpr float kOffset = K == Kind::Q4 ? 1.5f : K == Kind::Q3 ? 1.5f : K == Kind::Q8 ? 1152.f : 0.f;
+    static constexpr float kInvStep = K == Kind::Q4 ? 16.f : K == Kind::Q3 ? 8.f : 1.f;
+};
+
+// Eight 3-bit fields of a (low halves) and b (high halves) placed at bits 7..9
+// of an fp16 1.0: lo = their bits 0..15, hi = their bits 9..23 (fields 3..7).
+__device__ __forceinline__ void q3_place(uint32_t a, uint32_t b, uint32_t* h) {
+    constexpr uint32_t kM = 0x03800380u, kOne = 0x3C003C00u;
+    const uint32_t lo = __byte_perm(a, b, 0x5410), hi = __byte_perm(a >> 9, b >> 9, 0x5410);
+    h[0] = ((lo << 7) & kM) | kOne;
+    h[1] = ((lo << 4) & kM) | kOne;
+    h[2] = ((lo << 1) & kM) | kOne;
+    h[3] = ((lo >> 2) & kM) | kOne;
+    h[4] = ((lo >> 5) & kM) | kOne;
+    h[5] = ((hi << 1) & kM) | kOne;
+    h[6] = ((hi >> 2) & kM) | kOne;
+    h[7] = ((hi >> 5) & kM) | kOne;
+}
+
+// Sixteen consecutive dims (chunk t of group gr) of a K row in shared memory
+// as eight fp16 pairs. Pair i holds the dims k_dim(i, 0), k_dim(i, 1) of the
+// chunk; the query is loaded in the same order.
+template <Kind K>
+__device__ __forceinline__ constexpr int k_dim(int i, int e) {
+    return K == Kind::Q4 ? 8 * (i >> 2) + (i & 3) + 4 * e : K == Kind::Q3 ? i + 8 * e : 2 * i + e;
+}
+
+template <Kind K>
+__device__ __forceinline__ void k_chunk(const uint8_t* row, int gr, int t, uint32_t* h) {
+    if constexpr (K == Kind::F16 || K == Kind::BF16) {
+        const uint4* p = reinterpret_cast<const uint4*>(row + 128 * gr + 32 * t);
+        const uint4 a = p[0], b = p[1];
+        h[0] = a.x; h[1] = a.y; h[2] = a.z; h[3] = a.w;
+        h[4] = b.x; h[5] = b.y; h[6] = b.z; h[7] = b.w;
+        if constexpr (K == Kind::BF16) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[i] = bf2_to_h2(h[i]);
+        }
+    } else if constexpr (K == Kind::Q8 || K == Kind::F8) {
+        const uint4 a = *reinterpret_cast<const uint4*>(row + 64 * gr + 16 * t);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (K == Kind::Q8) {
+                const uint32_t u = w[i] ^ 0x80808080u;
+                h[2 * i] = __byte_perm(u, 0x64646464u, 0x4140);
+                h[2 * i + 1] = __byte_perm(u, 0x64646464u, 0x4342);
+            } else {
+                h[2 * i] = f8x2_to_h2(w[i]);
+                h[2 * i + 1] = f8x2_to_h2(w[i] >> 16);
+            }
+        }
+    } else if constexpr (K == Kind::Q4) {
+        constexpr uint32_t kM = 0x03C003C0u, kOne = 0x3C003C00u;
+        const uint2 a = *reinterpret_cast<const uint2*>(row + 32 * gr + 8 * t);
+        const uint32_t w[2] = {a.x, a.y};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            h[4 * i + 0] = ((w[i] << 6) & kM) | kOne;
+            h[4 * i + 1] = ((w[i] << 2) & kM) | kOne;
+            h[4 * i + 2] = ((w[i] >> 2) & kM) | kOne;
+            h[4 * i + 3] = ((w[i] >> 6) & kM) | kOne;
+        }
+    } else {
+        // bytes 6 t .. 6 t + 5 of the group's 24: two aligned words, shifted by 16 for odd t
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(row + 24 * gr + ((6 * t) & ~3));
+        const uint32_t sh = (t & 1) * 16;
+        const uint32_t w0 = p[0], w1 = p[1];
+        const uint32_t lo = __funnelshift_r(w0, w1, sh), hi = w1 >> sh;
+        q3_place(lo, (lo >> 24) | (hi << 8), h);
+    }
+}
+
+// Dims 8 g .. 8 g + 7 of group gr of two V rows as pairs (row a, row b): pair i
+// is dim 8 g + i, the code itself times the step (offset taken off exactly).
+template <Kind K>
+__device__ __forceinline__ void v_pairs(const uint8_t* ra, const uint8_t* rb, int gr, int g, uint32_t* h) {
+    if constexpr (K == Kind::F16 || K == Kind::BF16) {
+        const uint4 a4 = *reinterpret_cast<const uint4*>(ra + 128 * gr + 16 * g);
+        const uint4 b4 = *reinterpret_cast<const uint4*>(rb + 128 * gr + 16 * g);
+        uint32_t a[4] = {a4.x, a4.y, a4.z, a4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (K == Kind::BF16) {
+                a[i] = bf2_to_h2(a[i]);
+                b[i] = bf2_to_h2(b[i]);
+            }
+            h[2 * i] = __byte_perm(a[i], b[i], 0x5410);
+            h[2 * i + 1] = __byte_perm(a[i], b[i], 0x7632);
+        }
+    } else if constexpr (K == Kind::Q8 || K == Kind::F8) {
+        const uint2 a2 = *reinterpret_cast<const uint2*>(ra + 64 * gr + 8 * g);
+        const uint2 b2 = *reinterpret_cast<const uint2*>(rb + 64 * gr + 8 * g);
+        const uint32_t a[2] = {a2.x, a2.y}, b[2] = {b2.x, b2.y};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint32_t lo = __byte_perm(a[i], b[i], 0x5140), hi = __byte_perm(a[i], b[i], 0x7362);
+            if constexpr (K == Kind::Q8) {
+                const __half2 off = __float2half2_rn(1152.f);
+                lo ^= 0x80808080u;
+                hi ^= 0x80808080u;
+                h[4 * i + 0] = h2_bits(__hsub2(bits_h2(__byte_perm(lo, 0x64646464u, 0x4140)), off));
+                h[4 * i + 1] = h2_bits(__hsub2(bits_h2(__byte_perm(lo, 0x64646464u, 0x4342)), off));
+                h[4 * i + 2] = h2_bits(__hsub2(bits_h2(__byte_perm(hi, 0x64646464u, 0x4140)), off));
+                h[4 * i + 3] = h2_bits(__hsub2(bits_h2(__byte_perm(hi, 0x64646464u, 0x4342)), off));
+            } else {
+                h[4 * i + 0] = f8x2_to_h2(lo);
+                h[4 * i + 1] = f8x2_to_h2(lo >> 16);
+                h[4 * i + 2] = f8x2_to_h2(hi);
+                h[4 * i + 3] = f8x2_to_h2(hi >> 16);
+            }
+        }
+    } else {
+        const __half2 off = __float2half2_rn(1.5f);
+        if constexpr (K == Kind::Q4) {
+            constexpr uint32_t kM = 0x03C003C0u, kOne = 0x3C003C00u;
+            const uint32_t a = *reinterpret_cast<const uint32_t*>(ra + 32 * gr + 4 * g);
+            const uint32_t b = *reinterpret_cast<const uint32_t*>(rb + 32 * gr + 4 * g);
+            const uint32_t w[2] = {__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632)};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                h[4 * i + 0] = ((w[i] << 6) & kM) | kOne;
+                h[4 * i + 1] = ((w[i] << 2) & kM) | kOne;
+                h[4 * i + 2] = ((w[i] >> 2) & kM) | kOne;
+                h[4 * i + 3] = ((w[i] >> 6) & kM) | kOne;
+            }
+        } else {
+            // bytes 3 g .. 3 g + 2 of the group's 24; the second word only where they straddle
+            const int o = 24 * gr + ((3 * g) & ~3);
+            const uint32_t sh = 8u * ((3 * g) & 3);
+            const uint32_t* pa = reinterpret_cast<const uint32_t*>(ra + o);
+            const uint32_t* pb = reinterpret_cast<const uint32_t*>(rb + o);
+            const bool two = sh > 8;
+            const uint32_t a = __funnelshift_r(pa[0], two ? pa[1] : 0u, sh);
+            const uint32_t b = __funnelshift_r(pb[0], two ? pb[1] : 0u, sh);
+            q3_place(a, b, h);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = h2_bits(__hsub2(bits_h2(h[i]), off));
+    }
+}
+
+// One dim of a float row (f16 / bf16 / f8 codes) in shared memory.
+template <Kind K>
+__device__ __forceinline__ float v_one(const uint8_t* row, int d) {
+    if constexpr (K == Kind::F16) return __half2float(reinterpret_cast<const __half*>(row)[d]);
+    else if constexpr (K == Kind::BF16) return __half2float(__float2half_rn(__bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[d])));
+    else return __low2float(bits_h2(f8x2_to_h2(row[d])));
+}
+
+__device__ __forceinline__ bool h2_not_finite(uint32_t u) {
+    return (u & 0x7C00u) == 0x7C00u || (u & 0x7C000000u) == 0x7C000000u;
+}
+
+template <class C>
+__global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(const TreeParams p) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int D = C::kD, NG = C::kNG, MT = C::kMT, PB = C::kPb;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBig);
+    unsigned long long* s_mask = reinterpret_cast<unsigned long long*>(bars + C::kWarps * C::kStages);
+    float2* s_ml = reinterpret_cast<float2*>(s_mask + C::kRows);
+    unsigned* s_ticket = reinterpret_cast<unsigned*>(s_ml + C::kWarps * C::kRows);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int split = (int)(blockIdx.x % p.S);
+    const int rest = (int)(blockIdx.x / p.S);
+    const int tile = rest % p.tiles, stream = rest / p.tiles;
+    const int b = stream / p.Hkv, hk = stream - b * p.Hkv;
+    const int r0 = tile * C::kRows;
+
+    grid_dependency_wait();
+    const long long cap = (long long)p.max_pages * p.page_rows;
+    const int len = (int)max(0ll, min((long long)__ldg(p.lens + b), cap));
+    const int n = max(0, min(min(p.nodes ? __ldg(p.nodes + b) : p.Q, p.Q), len));
+    const int ctx = len - n;
+    const int chunk = tree_chunk(len, p.S);
+    const int nsplit = max(1, (len + chunk - 1) / chunk);
+    if (split >= nsplit) return;
+    const int p0 = split * chunk, p1 = min(len, p0 + chunk);
+    const bool dead = r0 / p.G >= n;  // every row of the tile is past the sequence's nodes
+    if (dead && split > 0) return;
+
+    uint8_t* ring = smem + warp * (C::kStages * C::kStageBytes);
+    uint64_t* bar = bars + warp * C::kStages;
+    if (lane == 0) {
+#pragma unroll
+        for (int s = 0; s < C::kStages; ++s) mbar_init(bar + s, 1);
+        fence_mbar_init();
+    }
+    if (tid < C::kRows) {
+        const int r = r0 + tid, node = r / p.G;
+        s_mask[tid] = (r < p.R && node < n) ? __ldg(p.mask + (size_t)b * p.Q + node) : 0ull;
+    }
+    __syncthreads();
+
+    // this warp's blocks: warp, warp + 4, ... of the range's PB-row blocks
+    const int nblk = dead ? 0 : (p1 - p0 + PB - 1) / PB;
+    const int mine = nblk > warp ? (nblk - warp + C::kWarps - 1) / C::kWarps : 0;
+    const uint64_t policy = l2_policy_evict_first();
+    const int* trow = p.table + (size_t)b * p.max_pages;
+    // rows of one copy: the whole block when it lies inside a page, else runs of 8
+    const bool whole = p.page_rows % PB == 0;
+    const int run = whole ? PB : 8, nrun = PB / run;
+    const auto issue = [&](int i) {
+        const int s = i % C::kStages;
+        uint8_t* st = ring + s * C::kStageBytes;
+        if (lane == 0) mbar_arrive_expect_tx(bar + s, C::kTx);
+        __syncwarp();
+        const int pos = p0 + (warp + i * C::kWarps) * PB + (lane >> 2) * run;
+        if (lane < 4 * nrun) {
+            const int pi = pos / p.page_rows;
+            int pg = pi < p.max_pages ? __ldg(trow + pi) : 0;
+            pg = (pg >= 0 && pg < p.num_pages) ? pg : 0;
+            const size_t row = ((size_t)pg * p.Hkv + hk) * p.page_rows + (pos - pi * p.page_rows);
+            const int o = (lane >> 2) * run;
+            if ((lane & 3) == 0) bulk_g2s(st + o * C::kRb, p.K + row * C::kRb, run * C::kRb, bar + s, policy);
+            else if ((lane & 3) == 1)
+                bulk_g2s(st + C::kOffV + o * C::kRb, p.V + row * C::kRb, run * C::kRb, bar + s, policy);
+            else if constexpr (C::kScaled) {
+                if ((lane & 3) == 2)
+                    bulk_g2s(st + C::kOffSK + o * C::kSb, p.scK + row * NG, run * C::kSb, bar + s, policy);
+                else
+                    bulk_g2s(st + C::kOffSV + o * C::kSb, p.scV + row * NG, run * C::kSb, bar + s, policy);
+            }
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < C::kStages; ++i)
+        if (i < mine) issue(i);
+
+    // the query rows as A fragments, 16 dims (64 gr + 16 t ..) of rows g and
+    // g + 8 per lane, in the order of k_chunk's pairs; sums of q per group
+    uint32_t qa[MT][NG][4][4];
+    float qsum[MT][NG][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = r0 + 16 * m + g + 8 * e;
+            const int node = r / p.G;
+            const bool ok = r < p.R && node < n;
+            const __half* src = p.q + b * p.qs_b + (ok ? node : 0) * p.qs_t + (long long)(hk * p.G + (ok ? r - node * p.G : 0)) * p.qs_h;
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) {
+                uint4 v[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+                if (ok) {
+                    const uint4* s4 = reinterpret_cast<const uint4*>(src + 64 * gr + 16 * t);
+                    v[0] = __ldg(s4);
+                    v[1] = __ldg(s4 + 1);
+                }
+                const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    constexpr Kind KK = C::kKind;
+                    const int d0 = k_dim<KK>(i, 0), d1 = k_dim<KK>(i, 1);
+                    const uint32_t sel = ((d0 & 1) ? 0x32u : 0x10u) | ((d1 & 1) ? 0x7600u : 0x5400u);
+                    qa[m][gr][i >> 1][e + 2 * (i & 1)] = __byte_perm(w[d0 >> 1], w[d1 >> 1], sel);
+                    const float2 f = __half22float2(bits_h2(w[i]));
+                    sum += f.x + f.y;
+                }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                qsum[m][gr][e] = -TreeCode<C::kKind>::kOffset * sum;
+            }
+        }
+    }
+
+    float o[MT][NG][8][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[m][gr][i][k] = 0.f;
+    float ref[MT][2], l[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) ref[m][0] = ref[m][1] = kNegMax, l[m][0] = l[m][1] = 0.f;
+    // scores in log2 units per unit of the raw product
+    const float c2 = rsqrtf((float)D) * kLog2e * TreeCode<C::kKind>::kInvStep;
+
+    bool failed = false;
+    int done = 0;
+    for (int i = 0; i < mine; ++i) {
+        done = i;
+        const int s = i % C::kStages;
+        if (!mbar_wait_bounded(bar + s, (uint32_t)(i / C::kStages) & 1u)) {
+            failed = true;
+            if (lane == 0) report_error(kErrFullWait);
+            break;
+        }
+        const uint8_t* st = ring + s * C::kStageBytes;
+        const int pb = p0 + (warp + i * C::kWarps) * PB;
+        const bool tail = pb + PB > ctx;  // holds drafted rows or the end
+
+        constexpr int NT = PB / 8;  // 8-position tiles of S
+        float x[MT][NT][4];         // scores, then weights
+        __half2 vmax = __float2half2_rn(0.f);
+        uint32_t vsc[NT][2];        // V scales of this lane's positions (both groups)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            // S of 8 positions: lane g decodes row (g >> 1) + 4 (g & 1) (+ 8 for odd tiles) of the 16
+            const uint8_t* krow = st + (16 * (nt >> 1) + (g >> 1) + 4 * (g & 1) + 8 * (nt & 1)) * C::kRb;
+            float acc[MT][NG][4];
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) {
+                uint32_t h[8];
+                k_chunk<C::kKind>(krow, gr, t, h);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    float* a = acc[m][C::kScaled ? gr : 0];
+                    if (C::kScaled || gr == 0) {
+                        a[0] = a[1] = C::kFloat ? 0.f : qsum[m][gr][0];
+                        a[2] = a[3] = C::kFloat ? 0.f : qsum[m][gr][1];
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mma_f16_16816(a, qa[m][gr][k], h[2 * k], h[2 * k + 1]);
+                }
+            }
+            // this lane's columns: positions t and t + 4 (+ 8) of the 16
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int pr = 16 * (nt >> 1) + t + 4 * e + 8 * (nt & 1);
+                if constexpr (C::kScaled) {
+                    float ks[NG];
+                    if constexpr (NG == 2) {
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(st + C::kOffSK + 4 * pr));
+                        ks[0] = f.x;
+                        ks[1] = f.y;
+                        vsc[nt][e] = *reinterpret_cast<const uint32_t*>(st + C::kOffSV + 4 * pr);
+                    } else {
+                        ks[0] = __half2float(*reinterpret_cast<const __half*>(st + C::kOffSK + 2 * pr));
+                        vsc[nt][e] = *reinterpret_cast<const uint16_t*>(st + C::kOffSV + 2 * pr);
+                    }
+                    uint32_t va = vsc[nt][e] & 0x7FFF7FFFu;
+                    if (tail) {
+                        if (pb + pr >= len) vsc[nt][e] = va = 0u;
+                        // an infinite scale of a row that not all rows see is no measure
+                        if ((va & 0x7FFFu) >= 0x7C00u) va &= 0x7FFF0000u;
+                        if ((va >> 16) >= 0x7C00u) va &= 0x7FFFu;
+                    }
+                    vmax = __hmax2(vmax, bits_h2(va));
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            float v = acc[m][0][2 * r + e] * ks[0];
+                            if constexpr (NG == 2) v = fmaf(acc[m][1][2 * r + e], ks[1], v);
+                            x[m][nt][2 * r + e] = v;
+                        }
+                } else {
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) x[m][nt][2 * r + e] = acc[m][0][2 * r + e];
+                }
+            }
+        }
+        uint32_t seen[MT][2];  // tail blocks: which of this lane's columns a row sees (bit 2 nt + e)
+        if (tail) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const unsigned long long mk = s_mask[16 * m + g + 8 * r];
+                    uint32_t bits = 0;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int j = pb + 16 * (nt >> 1) + t + 4 * e + 8 * (nt & 1) - ctx;
+                            const bool v = j < 0 || (j < n && ((mk >> (j & 63)) & 1ull));
+                            bits |= (v ? 1u : 0u) << (2 * nt + e);
+                            if (!v) x[m][nt][2 * r + e] = kNegMax;
+                        }
+                    seen[m][r] = bits;
+                }
+        }
+        // running reference: the block's row maximum and its largest V scale
+        float ev = -13.f;
+        if constexpr (C::kScaled) {
+            float vm = fmaxf(__low2float(vmax), __high2float(vmax));
+            vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 1));
+            vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 2));
+            // floor(log2 vm) from the exponent field; 0, inf (and an all-zero block) need no shift
+            const int ex = (int)(__float_as_uint(vm) >> 23);
+            ev += (ex == 0 || ex == 255) ? 0.f : (float)(ex - 127);
+        }
+        bool moved = false;
+        float corr[MT][2];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float bm = x[m][0][2 * r];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) bm = fmaxf(bm, fmaxf(x[m][nt][2 * r], x[m][nt][2 * r + 1]));
+                bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
+                bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
+                // (a block that the row does not see at all leaves the reference)
+                const float want = bm == kNegMax ? kNegMax : fmaf(bm, c2, ev);
+                const float nr = fmaxf(ref[m][r], want);
+                corr[m][r] = fast_exp2(ref[m][r] - nr);
+                moved |= nr != ref[m][r];
+                ref[m][r] = nr;
+            }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                l[m][0] *= corr[m][0];
+                l[m][1] *= corr[m][1];
+#pragma unroll
+                for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        o[m][gr][k][0] *= corr[m][0];
+                        o[m][gr][k][1] *= corr[m][0];
+                        o[m][gr][k][2] *= corr[m][1];
+                        o[m][gr][k][3] *= corr[m][1];
+                    }
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float sum = 0.f;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float w = fast_exp2(fmaf(x[m][nt][2 * r + e], c2, -ref[m][r]));
+                        if (tail && !((seen[m][r] >> (2 * nt + e)) & 1u)) w = 0.f;
+                        x[m][nt][2 * r + e] = w;
+                        sum += w;
+                    }
+                l[m][r] += sum;
+            }
+        // O += P' V, 16 positions at a time
+        bool special = false;
+#pragma unroll
+        for (int j = 0; j < PB / 16; ++j) {
+            const uint8_t* vb = st + C::kOffV + (16 * j + t) * C::kRb;
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) {
+                uint32_t pa[MT][4];
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    const int nt = 2 * j + hf;
+                    float s0 = 1.f, s1 = 1.f;
+                    if constexpr (C::kScaled) {
+                        s0 = __half2float(gr ? __high2half(bits_h2(vsc[nt][0])) : __low2half(bits_h2(vsc[nt][0])));
+                        s1 = __half2float(gr ? __high2half(bits_h2(vsc[nt][1])) : __low2half(bits_h2(vsc[nt][1])));
+                    }
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            float w0 = x[m][nt][2 * r], w1 = x[m][nt][2 * r + 1];
+                            if constexpr (C::kScaled) {
+                                w0 *= s0;
+                                w1 *= s1;
+                                if (tail) {  // an unseen row's scale may be nan
+                                    if (!((seen[m][r] >> (2 * nt)) & 1u)) w0 = 0.f;
+                                    if (!((seen[m][r] >> (2 * nt + 1)) & 1u)) w1 = 0.f;
+                                }
+                            }
+                            pa[m][2 * hf + r] = h2_bits(__floats2half2_rn(w0, w1));
+                        }
+                }
+                uint32_t h0[8], h1[8];
+                v_pairs<C::kKind>(vb, vb + 4 * C::kRb, gr, g, h0);
+                v_pairs<C::kKind>(vb + 8 * C::kRb, vb + 12 * C::kRb, gr, g, h1);
+                if constexpr (C::kFloat) {
+                    if (tail) {
+                        const int q0 = pb + 16 * j + t;
+                        const uint32_t k0 = (q0 < len ? 0xFFFFu : 0u) | (q0 + 4 < len ? 0xFFFF0000u : 0u);
+                        const uint32_t k1 = (q0 + 8 < len ? 0xFFFFu : 0u) | (q0 + 12 < len ? 0xFFFF0000u : 0u);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            h0[k] &= k0;
+                            h1[k] &= k1;
+                            if (h2_not_finite(h0[k])) {  // left to `special`
+                                special = true;
+                                if ((h0[k] & 0x7C00u) == 0x7C00u) h0[k] &= 0xFFFF0000u;
+                                if ((h0[k] & 0x7C000000u) == 0x7C000000u) h0[k] &= 0xFFFFu;
+                            }
+                            if (h2_not_finite(h1[k])) {
+                                special = true;
+                                if ((h1[k] & 0x7C00u) == 0x7C00u) h1[k] &= 0xFFFF0000u;
+                                if ((h1[k] & 0x7C000000u) == 0x7C000000u) h1[k] &= 0xFFFFu;
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) mma_f16_16816(o[m][gr][k], pa[m], h0[k], h1[k]);
+            }
+        }
+        if constexpr (C::kFloat) {
+            // inf and nan entries of the block's rows, added to the rows that see them: what a
+            // positive weight times such an entry gives
+            if (tail && __any_sync(0xffffffffu, special)) {
+                for (int pr = 0; pr < PB; ++pr) {
+                    const int j = pb + pr - ctx;
+                    if (j >= n) break;
+                    const uint8_t* vr = st + C::kOffV + pr * C::kRb;
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            if (!(j < 0 || ((s_mask[16 * m + g + 8 * r] >> (j & 63)) & 1ull))) continue;
+#pragma unroll
+                            for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+                                for (int k = 0; k < 8; ++k)
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e) {
+                                        const float v = v_one<C::kKind>(vr, 64 * gr + 16 * t + 8 * e + k);
+                                        if (!(fabsf(v) <= 65504.f)) o[m][gr][k][2 * r + e] += v;
+                                    }
+                        }
+                }
+            }
+        }
+        __syncwarp();
+        if (i + C::kStages < mine) issue(i + C::kStages);
+    }
+    if (failed) {
+        // let the copies in flight land (bounded) before the shared memory is given back
+        for (int k = done; k < min(done + C::kStages, mine); ++k)
+            (void)mbar_wait_bounded(bar + k % C::kStages, (uint32_t)(k / C::kStages) & 1u);
+    }
+    if (__syncthreads_or(failed)) return;
+
+    // merge the four warps: o and (ref, l) through shared memory
+    float* so = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float sum = l[m][r];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            const int row = 16 * m + g + 8 * r;
+            if (t == 0) s_ml[warp * C::kRows + row] = make_float2(ref[m][r], sum);
+            float* dst = so + (size_t)(warp * C::kRows + row) * C::kOStride;
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int k = 0; k < 8; k += 4)
+                        *reinterpret_cast<float4*>(dst + 64 * gr + 16 * t + 8 * e + k) =
+                            make_float4(o[m][gr][k][2 * r + e], o[m][gr][k + 1][2 * r + e], o[m][gr][k + 2][2 * r + e],
+                                        o[m][gr][k + 3][2 * r + e]);
+        }
+    __syncthreads();
+    grid_launch_dependents();
+    constexpr int Q4 = D / 4;  // float4 columns of a row
+    const bool direct = nsplit == 1 || dead;
+    const auto store_out = [&](int r, int c, float4 v, float inv) {
+        const int node = r / p.G;
+        __half* dst = p.out + b * p.os_b + node * p.os_t + (long long)(hk * p.G + (r - node * p.G)) * p.os_h + 4 * c;
+        const bool live = node < n && inv != 0.f;
+        const __half2 a = __floats2half2_rn(live ? v.x * inv : 0.f, live ? v.y * inv : 0.f);
+        const __half2 d = __floats2half2_rn(live ? v.z * inv : 0.f, live ? v.w * inv : 0.f);
+        *reinterpret_cast<uint2*>(dst) = make_uint2(h2_bits(a), h2_bits(d));
+    };
+    for (int i = tid; i < C::kRows * Q4; i += C::kThreads) {
+        const int row = i / Q4, c = i - row * Q4, r = r0 + row;
+        if (r >= p.R) break;
+        float mx = kNegMax, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < C::kWarps; ++w) mx = fmaxf(mx, s_ml[w * C::kRows + row].x);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < C::kWarps; ++w) {
+            const float2 ml = s_ml[w * C::kRows + row];
+            const float a = fast_exp2(ml.x - mx);
+            const float4 u = *reinterpret_cast<const float4*>(so + (size_t)(w * C::kRows + row) * C::kOStride + 4 * c);
+            sum = fmaf(ml.y, a, sum);
+            v.x = fmaf(u.x, a, v.x);
+            v.y = fmaf(u.y, a, v.y);
+            v.z = fmaf(u.z, a, v.z);
+            v.w = fmaf(u.w, a, v.w);
+        }
+        if (direct) {
+            store_out(r, c, v, sum == 0.f ? 0.f : TreeCode<C::kKind>::kInvStep / sum);
+        } else {
+            const size_t slot = ((size_t)stream * p.R + r) * p.S + split;
+            __stcg(reinterpret_cast<float4*>(p.ws_o + slot * D + 4 * c), v);
+            if (c == 0) __stcg(reinterpret_cast<float2*>(p.ws_ml + slot * 2), make_float2(mx, sum));
+        }
+    }
+    if (direct) return;
+    __syncthreads();
+    unsigned* counter = p.counters + (size_t)stream * p.tiles + tile;
+    if (tid == 0) *s_ticket = atomic_add_acq_rel_gpu(counter, 1u);
+    __syncthreads();
+    if (*s_ticket != (unsigned)(nsplit - 1)) return;
+    if (tid == 0) store_relaxed_gpu(counter, 0u);
+    // the last range of the row tile merges all of them, in order
+    for (int i = tid; i < C::kRows * Q4; i += C::kThreads) {
+        const int row = i / Q4, c = i - row * Q4, r = r0 + row;
+        if (r >= p.R) break;
+        const size_t slot = ((size_t)stream * p.R + r) * p.S;
+        const float2* ml = reinterpret_cast<const float2*>(p.ws_ml + slot * 2);
+        float mx = kNegMax, sum = 0.f;
+        for (int s = 0; s < nsplit; ++s) mx = fmaxf(mx, __ldcg(ml + s).x);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int s = 0; s < nsplit; ++s) {
+            const float2 w = __ldcg(ml + s);
+            const float a = fast_exp2(w.x - mx);
+            const float4 u = __ldcg(reinterpret_cast<const float4*>(p.ws_o + (slot + s) * D + 4 * c));
+            sum = fmaf(w.y, a, sum);
+            v.x = fmaf(u.x, a, v.x);
+            v.y = fmaf(u.y, a, v.y);
+            v.z = fmaf(u.z, a, v.z);
+            v.w = fmaf(u.w, a, v.w);
+        }
+        store_out(r, c, v, sum == 0.f ? 0.f : TreeCode<C::kKind>::kInvStep / sum);
+    }
+}
+
+}  // namespace va

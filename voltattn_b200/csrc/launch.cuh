@@ -18,6 +18,11 @@
 namespace va {
 
 struct PrefillParams;
+struct TreeParams;
+struct AppendParams;
+struct AcceptParams;
+struct ForkParams;
+struct CompactParams;
 
 namespace host {
 
@@ -68,6 +73,14 @@ int launch_prefill_fmt(int fmt, const PrefillParams& p, cudaStream_t st);
 int prefill_stage_rows(int L);
 size_t prefill_stage_bytes(int Hkv, int L, int D);
 int launch_prefill_staged_fmt(int fmt, const PrefillParams& p, void* ws, cudaStream_t st);
+// Tree attention (launch_tree_d*.cu): rows = query rows of a CTA (16 or 32).
+int launch_tree_d64(int fmt, const TreeParams& p, int rows, cudaStream_t st);
+int launch_tree_d128(int fmt, const TreeParams& p, int rows, cudaStream_t st);
+// Rows and pages of a paged cache (launch_cache.cu).
+int launch_append_packed(int fmt, int in_type, const AppendParams& p, cudaStream_t st);
+int launch_accept_tree(const AcceptParams& p, int B, int layers, cudaStream_t st);
+int launch_fork_pages(const ForkParams& p, cudaStream_t st);
+int launch_compact_pages(const CompactParams& p, cudaStream_t st);
 // fp16 [rows][128] tensor map, 64-element x box_rows boxes, 128-byte swizzle.
 int encode_f16_rows_map(CUtensorMap* m, const void* base, long long rows, int box_rows);
 

@@ -29,25 +29,15 @@ __device__ __forceinline__ int lrint_narrow(float y) {
 // rounded to nearest even with saturation to +-448 (nan stays nan).
 constexpr int kBitsF8 = -8;
 
-// One 64-element group, eight consecutive elements per thread (8 lanes per
-// group, lane-aligned): loads, reduces amax over the 8 lanes, quantizes and
-// packs. `src` points at this thread's 8 inputs; element `e0` (a multiple of
-// 8) and scale index `sidx` place the result. All 32 lanes must call it.
+// One 64-element group from registers, eight consecutive elements v[] per
+// thread (8 lanes per group, lane-aligned): reduces amax over the 8 lanes,
+// quantizes and packs. Element `e0` (a multiple of 8) and scale index `sidx`
+// place the result. All 32 lanes must call it; inactive ones pass zeros.
 template <int BITS>
-__device__ __forceinline__ void quantize_group_part(const float* src, bool active, int part, long long e0,
-                                                    long long sidx, uint8_t* __restrict__ codes,
-                                                    __half* __restrict__ scales) {
+__device__ __forceinline__ void quantize_group_values(const float (&v)[8], bool active, int part, long long e0,
+                                                      long long sidx, uint8_t* __restrict__ codes,
+                                                      __half* __restrict__ scales) {
     constexpr int lim = BITS == 8 ? 127 : BITS == 4 ? 7 : BITS == kBitsF8 ? 448 : 3;
-    float v[8];
-    if (active) {
-        const float4* p = reinterpret_cast<const float4*>(src);
-        const float4 a = __ldg(p), b = __ldg(p + 1);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    }
     float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));  // fmaxf drops nan operands
@@ -96,6 +86,24 @@ __device__ __forceinline__ void quantize_group_part(const float* src, bool activ
         dst[2] = (uint8_t)(w >> 16);
     }
     if (part == 0) scales[sidx] = hs;
+}
+
+// The same with the thread's eight fp32 values loaded from `src`.
+template <int BITS>
+__device__ __forceinline__ void quantize_group_part(const float* src, bool active, int part, long long e0,
+                                                    long long sidx, uint8_t* __restrict__ codes,
+                                                    __half* __restrict__ scales) {
+    float v[8];
+    if (active) {
+        const float4* p = reinterpret_cast<const float4*>(src);
+        const float4 a = __ldg(p), b = __ldg(p + 1);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    }
+    quantize_group_values<BITS>(v, active, part, e0, sidx, codes, scales);
 }
 
 template <int BITS>
