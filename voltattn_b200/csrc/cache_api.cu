@@ -2,6 +2,7 @@
 // in include/voltattn.h): argument checks, workspace layout and launch.
 #include <algorithm>
 #include <climits>
+#include <cstdlib>
 
 #include "../../include/voltattn.h"
 #include "cache_rows.cuh"
@@ -15,7 +16,7 @@ using namespace va::host;
 namespace {
 
 constexpr int kMaxNodes = 64;
-constexpr int kMaxSplits = 128;
+constexpr int kMaxSplits = kTreeMaxSplits;
 constexpr int kMaxForks = 4000;
 
 bool pool_fmt(int f) { return f >= VA_F16 && f < VA_Q4CP; }
@@ -38,8 +39,16 @@ int check_pool(int fmt, const va_bufs* b, int B, int max_pages, int Hkv, int pag
     return VA_OK;
 }
 
-// Rows of a CTA's tile of query rows: 16 while one such tile holds them all.
-int tree_rows(int R) { return R <= 16 ? 16 : 32; }
+// Rows of a CTA's tile of query rows: 16 or 32 (decode_tree.cuh), 128 or 256
+// (decode_tree_tc.cuh). VOLTATTN_TREE_ROWS overrides for measurements.
+int tree_rows(int R) {
+    static const int forced = [] {
+        const char* e = std::getenv("VOLTATTN_TREE_ROWS");
+        return e ? std::atoi(e) : 0;
+    }();
+    if (forced) return forced;
+    return R <= 16 ? 16 : R <= 128 ? 128 : 256;
+}
 
 // Completion counters, one per (sequence, KV head, row tile), at the front of the
 // workspace: a fixed number, so the slots of a call never lie where a call of
@@ -54,7 +63,7 @@ int tree_splits(int nsm, int B, int Hkv, int R, int Lmax) {
     const int rows = tree_rows(R);
     const long long ctas = (long long)B * Hkv * ((R + rows - 1) / rows);
     if (ctas > kCounters) return 1;
-    const long long cap = (long long)nsm * (rows == 16 ? 3 : 2);
+    const long long cap = (long long)nsm * (rows == 16 ? 3 : rows == 32 ? 2 : 1);
     const int most = std::max(1, std::min(kMaxSplits, (Lmax + kTreeUnit - 1) / kTreeUnit));
     double best = 1e300;
     int S = 1;
@@ -170,6 +179,13 @@ int va_decode_tree(int fmt, const va_bufs* b, const long long* q_strides, const 
     p.max_pages = max_pages;
     p.page_rows = page_rows;
     p.num_pages = num_pages;
+    // division by the page size as a multiplication (round-up method): with
+    // 2^(l-1) < d <= 2^l and m = floor(2^32 (2^l - d) / d) + 1, floor(n / d) =
+    // (mulhi(n, m) + n) >> l for every n < 2^31
+    unsigned l = 0;
+    while ((1ll << l) < page_rows) ++l;
+    p.page_shift = l;
+    p.page_mul = (unsigned)((((unsigned long long)1 << 32) * ((1ull << l) - (unsigned)page_rows)) / (unsigned)page_rows + 1);
     uint8_t* w = static_cast<uint8_t*>(ws);
     p.counters = reinterpret_cast<unsigned*>(w);
     w += kCounterBytes;

@@ -64,10 +64,13 @@ struct TreeParams {
     long long os_b, os_t, os_h;
     int B, Hkv, G, Q, R, tiles, S;
     int max_pages, page_rows, num_pages;
+    // pos / page_rows = (umulhi(pos, page_mul) + pos) >> page_shift for 0 <= pos < 2^31
+    unsigned page_mul, page_shift;
 };
 
 // Splits of a sequence of len rows: whole units of kTreeUnit rows, at most S.
 constexpr int kTreeUnit = 128;
+constexpr int kTreeMaxSplits = 128;
 __device__ __forceinline__ int tree_chunk(int len, int S) {
     const int units = (len + kTreeUnit - 1) / kTreeUnit;
     return max(1, (units + S - 1) / S) * kTreeUnit;
@@ -112,6 +115,16 @@ __device__ __forceinline__ void mma_f16_16816(float* c, const uint32_t* a, uint3
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The same with the accumulator's initial values (rows g and g + 8) in c0, c1.
+__device__ __forceinline__ void mma_f16_16816_init(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, float c0,
+                                                   float c1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, "
+        "%11, %11};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
+
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 __device__ __forceinline__ uint32_t bf2_to_h2(uint32_t w) {
@@ -123,12 +136,12 @@ __device__ __forceinline__ uint32_t f8x2_to_h2(uint32_t b) {
     return (uint32_t)r.x | ((uint32_t)r.y << 16);
 }
 
-// What a placed code stands for: x = kOffset + code * kStep, code = the signed
-// code. q4: 1 + nibble / 16; q3: 1 + field / 8; q8: 1024 + byte.
+// What a placed K code stands for: x = kOffset + code / kInvStep, code = the
+// signed code. q4: 1 + nibble / 64; q3: 1 + field / 8; q8: 1024 + byte.
 template <Kind K>
 struct TreeCode {
-    static constexpr float kOffset = K == Kind::Q4 ? 1.5f : K == Kind::Q3 ? 1.5f : K == Kind::Q8 ? 1152.f : 0.f;
-    static constexpr float kInvStep = K == Kind::Q4 ? 16.f : K == Kind::Q3 ? 8.f : 1.f;
+    static constexpr float kOffset = K == Kind::Q4 ? 1.125f : K == Kind::Q3 ? 1.5f : K == Kind::Q8 ? 1152.f : 0.f;
+    static constexpr float kInvStep = K == Kind::Q4 ? 64.f : K == Kind::Q3 ? 8.f : 1.f;
 };
 
 // Eight 3-bit fields of a (low halves) and b (high halves) placed at bits 7..9
@@ -180,15 +193,15 @@ __device__ __forceinline__ void k_chunk(const uint8_t* row, int gr, int t, uint3
             }
         }
     } else if constexpr (K == Kind::Q4) {
-        constexpr uint32_t kM = 0x03C003C0u, kOne = 0x3C003C00u;
+        constexpr uint32_t kM = 0x00F000F0u, kOne = 0x3C003C00u;
         const uint2 a = *reinterpret_cast<const uint2*>(row + 32 * gr + 8 * t);
         const uint32_t w[2] = {a.x, a.y};
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            h[4 * i + 0] = ((w[i] << 6) & kM) | kOne;
-            h[4 * i + 1] = ((w[i] << 2) & kM) | kOne;
-            h[4 * i + 2] = ((w[i] >> 2) & kM) | kOne;
-            h[4 * i + 3] = ((w[i] >> 6) & kM) | kOne;
+            h[4 * i + 0] = ((w[i] << 4) & kM) | kOne;
+            h[4 * i + 1] = (w[i] & kM) | kOne;
+            h[4 * i + 2] = ((w[i] >> 4) & kM) | kOne;
+            h[4 * i + 3] = ((w[i] >> 8) & kM) | kOne;
         }
     } else {
         // bytes 6 t .. 6 t + 5 of the group's 24: two aligned words, shifted by 16 for odd t
@@ -201,7 +214,16 @@ __device__ __forceinline__ void k_chunk(const uint8_t* row, int gr, int t, uint3
 }
 
 // Dims 8 g .. 8 g + 7 of group gr of two V rows as pairs (row a, row b): pair i
-// is dim 8 g + i, the code itself times the step (offset taken off exactly).
+// is dim 8 g + i, the code times v_step(i), exact: packed codes are placed where
+// they lie in the word, so the step differs between dims (a factor of the
+// output's column, applied once at the end) and no shift is spent on them.
+template <Kind K>
+__host__ __device__ constexpr float v_step(int i) {
+    // q4: nibbles 0, 2 of a half word (after one shift by 8) at bits 0..3, nibbles 1, 3 at bits 4..7;
+    // q3: fields 0, 3, 6 at bits 0..2, fields 1, 4, 7 at 3..5, fields 2, 5 at 6..8
+    return K == Kind::Q4 ? ((i & 1) ? 64.f : 1024.f) : K == Kind::Q3 ? (i % 3 == 0 ? 1024.f : i % 3 == 1 ? 128.f : 16.f) : 1.f;
+}
+
 template <Kind K>
 __device__ __forceinline__ void v_pairs(const uint8_t* ra, const uint8_t* rb, int gr, int g, uint32_t* h) {
     if constexpr (K == Kind::F16 || K == Kind::BF16) {
@@ -239,33 +261,39 @@ __device__ __forceinline__ void v_pairs(const uint8_t* ra, const uint8_t* rb, in
                 h[4 * i + 3] = f8x2_to_h2(hi >> 16);
             }
         }
-    } else {
-        const __half2 off = __float2half2_rn(1.5f);
-        if constexpr (K == Kind::Q4) {
-            constexpr uint32_t kM = 0x03C003C0u, kOne = 0x3C003C00u;
-            const uint32_t a = *reinterpret_cast<const uint32_t*>(ra + 32 * gr + 4 * g);
-            const uint32_t b = *reinterpret_cast<const uint32_t*>(rb + 32 * gr + 4 * g);
-            const uint32_t w[2] = {__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632)};
+    } else if constexpr (K == Kind::Q4) {
+        constexpr uint32_t kOne = 0x3C003C00u;
+        const __half2 off0 = __float2half2_rn(1.f + 8.f / 1024.f), off1 = __float2half2_rn(1.f + 8.f / 64.f);
+        const uint32_t a = *reinterpret_cast<const uint32_t*>(ra + 32 * gr + 4 * g);
+        const uint32_t b = *reinterpret_cast<const uint32_t*>(rb + 32 * gr + 4 * g);
+        const uint32_t w[2] = {__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632)};
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                h[4 * i + 0] = ((w[i] << 6) & kM) | kOne;
-                h[4 * i + 1] = ((w[i] << 2) & kM) | kOne;
-                h[4 * i + 2] = ((w[i] >> 2) & kM) | kOne;
-                h[4 * i + 3] = ((w[i] >> 6) & kM) | kOne;
-            }
-        } else {
-            // bytes 3 g .. 3 g + 2 of the group's 24; the second word only where they straddle
-            const int o = 24 * gr + ((3 * g) & ~3);
-            const uint32_t sh = 8u * ((3 * g) & 3);
-            const uint32_t* pa = reinterpret_cast<const uint32_t*>(ra + o);
-            const uint32_t* pb = reinterpret_cast<const uint32_t*>(rb + o);
-            const bool two = sh > 8;
-            const uint32_t a = __funnelshift_r(pa[0], two ? pa[1] : 0u, sh);
-            const uint32_t b = __funnelshift_r(pb[0], two ? pb[1] : 0u, sh);
-            q3_place(a, b, h);
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t u = w[i] >> 8;
+            h[4 * i + 0] = h2_bits(__hsub2(bits_h2((w[i] & 0x000F000Fu) | kOne), off0));
+            h[4 * i + 1] = h2_bits(__hsub2(bits_h2((w[i] & 0x00F000F0u) | kOne), off1));
+            h[4 * i + 2] = h2_bits(__hsub2(bits_h2((u & 0x000F000Fu) | kOne), off0));
+            h[4 * i + 3] = h2_bits(__hsub2(bits_h2((u & 0x00F000F0u) | kOne), off1));
         }
+    } else {
+        constexpr uint32_t kOne = 0x3C003C00u;
+        const __half2 off[3] = {__float2half2_rn(1.f + 4.f / 1024.f), __float2half2_rn(1.f + 4.f / 128.f),
+                                __float2half2_rn(1.f + 4.f / 16.f)};
+        constexpr uint32_t kM[3] = {0x00070007u, 0x00380038u, 0x01C001C0u};
+        // bytes 3 g .. 3 g + 2 of the group's 24; the second word only where they straddle
+        const int o = 24 * gr + ((3 * g) & ~3);
+        const uint32_t sh = 8u * ((3 * g) & 3);
+        const uint32_t* pa = reinterpret_cast<const uint32_t*>(ra + o);
+        const uint32_t* pb = reinterpret_cast<const uint32_t*>(rb + o);
+        const int two = sh > 8 ? 1 : 0;  // (else the first word again: its bits are not used)
+        const uint32_t a = __funnelshift_r(pa[0], pa[two], sh);
+        const uint32_t b = __funnelshift_r(pb[0], pb[two], sh);
+        const uint32_t lo = __byte_perm(a, b, 0x5410), hi = __byte_perm(a >> 9, b >> 9, 0x5410), up = hi >> 9;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = h2_bits(__hsub2(bits_h2(h[i]), off));
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t w = i < 3 ? lo : i < 6 ? hi : up;
+            h[i] = h2_bits(__hsub2(bits_h2((w & kM[i % 3]) | kOne), off[i % 3]));
+        }
     }
 }
 
@@ -279,6 +307,68 @@ __device__ __forceinline__ float v_one(const uint8_t* row, int d) {
 
 __device__ __forceinline__ bool h2_not_finite(uint32_t u) {
     return (u & 0x7C00u) == 0x7C00u || (u & 0x7C000000u) == 0x7C000000u;
+}
+
+// The last range of a row tile merges all of them, in order: first the weights of
+// every (row, range) into shared memory (kRows * (kTreeMaxSplits + 1) floats), then the
+// outputs with the loads of several rows in flight. kThreads threads take part.
+template <int D, int kRows, int kThreads, class Store>
+__device__ __forceinline__ void tree_merge(const TreeParams& p, int stream, int r0, int rows, int nsplit, float* sw,
+                                           int tid, const Store& store_out) {
+    const int lane = tid & 31;
+    float* sl = sw + kRows * kTreeMaxSplits;  // [kRows] sums
+    for (int row = tid >> 5; row < rows; row += kThreads / 32) {
+        const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + ((size_t)stream * p.R + r0 + row) * p.S;
+        float2 w[kTreeMaxSplits / 32];
+        float mx = kNegMax, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kTreeMaxSplits / 32; ++k) {
+            const int s = 32 * k + lane;
+            w[k] = s < nsplit ? __ldcg(ml + s) : make_float2(kNegMax, 0.f);
+            mx = fmaxf(mx, w[k].x);
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+#pragma unroll
+        for (int k = 0; k < kTreeMaxSplits / 32; ++k) {
+            const float a = fast_exp2(w[k].x - mx);
+            sum = fmaf(w[k].y, a, sum);
+            if (32 * k + lane < nsplit) sw[row * kTreeMaxSplits + 32 * k + lane] = a;
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (lane == 0) sl[row] = sum;
+    }
+    named_barrier_sync(1, kThreads);
+    constexpr int Q4 = D / 4;
+    static_assert(kThreads % Q4 == 0, "a thread keeps its column");
+    constexpr int kRowStep = kThreads / Q4, kItems = 4;
+    const int c = tid % Q4;
+    for (int rw = tid / Q4; rw < rows; rw += kItems * kRowStep) {
+        float4 v[kItems];
+#pragma unroll
+        for (int k = 0; k < kItems; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+        for (int s = 0; s < nsplit; ++s) {
+#pragma unroll
+            for (int k = 0; k < kItems; ++k) {
+                const int row = rw + k * kRowStep;
+                if (row >= rows) break;
+                const float4 u = __ldcg(
+                    reinterpret_cast<const float4*>(p.ws_o + (((size_t)stream * p.R + r0 + row) * p.S + s) * D + 4 * c));
+                const float a = sw[row * kTreeMaxSplits + s];
+                v[k].x = fmaf(u.x, a, v[k].x);
+                v[k].y = fmaf(u.y, a, v[k].y);
+                v[k].z = fmaf(u.z, a, v[k].z);
+                v[k].w = fmaf(u.w, a, v[k].w);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kItems; ++k) {
+            const int row = rw + k * kRowStep;
+            if (row < rows) store_out(r0 + row, c, v[k], sl[row] == 0.f ? 0.f : 1.f / sl[row]);
+        }
+    }
 }
 
 template <class C>
@@ -327,35 +417,37 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
     const int mine = nblk > warp ? (nblk - warp + C::kWarps - 1) / C::kWarps : 0;
     const uint64_t policy = l2_policy_evict_first();
     const int* trow = p.table + (size_t)b * p.max_pages;
-    // rows of one copy: the whole block when it lies inside a page, else runs of 8
+    // rows of one copy: the whole block when it lies inside a page, else runs of 8.
+    // Lane 4 r + k copies run r of buffer k (K, V and their scales): its source at
+    // page 0 and the bytes of a page and of a row there
     const bool whole = p.page_rows % PB == 0;
     const int run = whole ? PB : 8, nrun = PB / run;
-    const auto issue = [&](int i) {
-        const int s = i % C::kStages;
-        uint8_t* st = ring + s * C::kStageBytes;
+    const int buf = lane & 3, run_at = (lane >> 2) * run;
+    const int lane_row = buf < 2 ? C::kRb : C::kSb;
+    const uint32_t lane_bytes = (uint32_t)(run * lane_row);
+    const bool copies = lane < 4 * nrun && lane_bytes > 0;
+    const uint8_t* lane_src = buf == 0   ? p.K
+                              : buf == 1 ? p.V
+                              : buf == 2 ? reinterpret_cast<const uint8_t*>(p.scK)
+                                         : reinterpret_cast<const uint8_t*>(p.scV);
+    lane_src += (size_t)hk * p.page_rows * lane_row;
+    const long long lane_page = (long long)p.Hkv * p.page_rows * lane_row;
+    uint8_t* lane_dst = ring + (buf == 0 ? 0 : buf == 1 ? C::kOffV : buf == 2 ? C::kOffSK : C::kOffSV) + run_at * lane_row;
+    const auto issue = [&](int i, int s) {
         if (lane == 0) mbar_arrive_expect_tx(bar + s, C::kTx);
         __syncwarp();
-        const int pos = p0 + (warp + i * C::kWarps) * PB + (lane >> 2) * run;
-        if (lane < 4 * nrun) {
-            const int pi = pos / p.page_rows;
+        if (copies) {
+            const int pos = p0 + (warp + i * C::kWarps) * PB + run_at;
+            const int pi = (int)((__umulhi((unsigned)pos, p.page_mul) + (unsigned)pos) >> p.page_shift);
             int pg = pi < p.max_pages ? __ldg(trow + pi) : 0;
-            pg = (pg >= 0 && pg < p.num_pages) ? pg : 0;
-            const size_t row = ((size_t)pg * p.Hkv + hk) * p.page_rows + (pos - pi * p.page_rows);
-            const int o = (lane >> 2) * run;
-            if ((lane & 3) == 0) bulk_g2s(st + o * C::kRb, p.K + row * C::kRb, run * C::kRb, bar + s, policy);
-            else if ((lane & 3) == 1)
-                bulk_g2s(st + C::kOffV + o * C::kRb, p.V + row * C::kRb, run * C::kRb, bar + s, policy);
-            else if constexpr (C::kScaled) {
-                if ((lane & 3) == 2)
-                    bulk_g2s(st + C::kOffSK + o * C::kSb, p.scK + row * NG, run * C::kSb, bar + s, policy);
-                else
-                    bulk_g2s(st + C::kOffSV + o * C::kSb, p.scV + row * NG, run * C::kSb, bar + s, policy);
-            }
+            pg = (unsigned)pg < (unsigned)p.num_pages ? pg : 0;
+            bulk_g2s(lane_dst + s * C::kStageBytes, lane_src + pg * lane_page + (pos - pi * p.page_rows) * lane_row,
+                     lane_bytes, bar + s, policy);
         }
     };
 #pragma unroll
     for (int i = 0; i < C::kStages; ++i)
-        if (i < mine) issue(i);
+        if (i < mine) issue(i, i);
 
     // the query rows as A fragments, 16 dims (64 gr + 16 t ..) of rows g and
     // g + 8 per lane, in the order of k_chunk's pairs; sums of q per group
@@ -410,20 +502,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
     // scores in log2 units per unit of the raw product
     const float c2 = rsqrtf((float)D) * kLog2e * TreeCode<C::kKind>::kInvStep;
 
-    bool failed = false;
-    int done = 0;
-    for (int i = 0; i < mine; ++i) {
-        done = i;
-        const int s = i % C::kStages;
-        if (!mbar_wait_bounded(bar + s, (uint32_t)(i / C::kStages) & 1u)) {
-            failed = true;
-            if (lane == 0) report_error(kErrFullWait);
-            break;
-        }
-        const uint8_t* st = ring + s * C::kStageBytes;
-        const int pb = p0 + (warp + i * C::kWarps) * PB;
-        const bool tail = pb + PB > ctx;  // holds drafted rows or the end
-
+    // One block of positions in stage st. tail: it holds drafted rows or the end
+    // of the sequence (two instantiations: the others spend nothing on masks).
+    const auto block = [&](auto is_tail, const uint8_t* st, int pb) {
+        constexpr bool tail = decltype(is_tail)::value;
         constexpr int NT = PB / 8;  // 8-position tiles of S
         float x[MT][NT][4];         // scores, then weights
         __half2 vmax = __float2half2_rn(0.f);
@@ -440,12 +522,13 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                     float* a = acc[m][C::kScaled ? gr : 0];
-                    if (C::kScaled || gr == 0) {
-                        a[0] = a[1] = C::kFloat ? 0.f : qsum[m][gr][0];
-                        a[2] = a[3] = C::kFloat ? 0.f : qsum[m][gr][1];
-                    }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) mma_f16_16816(a, qa[m][gr][k], h[2 * k], h[2 * k + 1]);
+                    for (int k = 0; k < 4; ++k) {
+                        if (k == 0 && (C::kScaled || gr == 0))
+                            mma_f16_16816_init(a, qa[m][gr][k], h[0], h[1], C::kFloat ? 0.f : qsum[m][gr][0],
+                                               C::kFloat ? 0.f : qsum[m][gr][1]);
+                        else mma_f16_16816(a, qa[m][gr][k], h[2 * k], h[2 * k + 1]);
+                    }
                 }
             }
             // this lane's columns: positions t and t + 4 (+ 8) of the 16
@@ -464,7 +547,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
                         vsc[nt][e] = *reinterpret_cast<const uint16_t*>(st + C::kOffSV + 2 * pr);
                     }
                     uint32_t va = vsc[nt][e] & 0x7FFF7FFFu;
-                    if (tail) {
+                    if constexpr (tail) {
                         if (pb + pr >= len) vsc[nt][e] = va = 0u;
                         // an infinite scale of a row that not all rows see is no measure
                         if ((va & 0x7FFFu) >= 0x7C00u) va &= 0x7FFF0000u;
@@ -487,8 +570,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
                 }
             }
         }
-        uint32_t seen[MT][2];  // tail blocks: which of this lane's columns a row sees (bit 2 nt + e)
-        if (tail) {
+        uint32_t seen[MT][2];  // which of this lane's columns a row sees (bit 2 nt + e)
+        if constexpr (tail) {
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -518,36 +601,40 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
             ev += (ex == 0 || ex == 255) ? 0.f : (float)(ex - 127);
         }
         bool moved = false;
-        float corr[MT][2];
+        float want[MT][2];
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                float bm = x[m][0][2 * r];
+                float bm = fmaxf(x[m][0][2 * r], x[m][0][2 * r + 1]);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) bm = fmaxf(bm, fmaxf(x[m][nt][2 * r], x[m][nt][2 * r + 1]));
+                for (int nt = 1; nt < NT; ++nt) bm = fmaxf(bm, fmaxf(x[m][nt][2 * r], x[m][nt][2 * r + 1]));
                 bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
                 bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
+                want[m][r] = fmaf(bm, c2, ev);
                 // (a block that the row does not see at all leaves the reference)
-                const float want = bm == kNegMax ? kNegMax : fmaf(bm, c2, ev);
-                const float nr = fmaxf(ref[m][r], want);
-                corr[m][r] = fast_exp2(ref[m][r] - nr);
-                moved |= nr != ref[m][r];
-                ref[m][r] = nr;
+                if (tail && bm == kNegMax) want[m][r] = kNegMax;
+                moved |= want[m][r] > ref[m][r];
             }
         if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                l[m][0] *= corr[m][0];
-                l[m][1] *= corr[m][1];
+                float corr[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float nr = fmaxf(ref[m][r], want[m][r]);
+                    corr[r] = fast_exp2(ref[m][r] - nr);
+                    ref[m][r] = nr;
+                    l[m][r] *= corr[r];
+                }
 #pragma unroll
                 for (int gr = 0; gr < NG; ++gr)
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        o[m][gr][k][0] *= corr[m][0];
-                        o[m][gr][k][1] *= corr[m][0];
-                        o[m][gr][k][2] *= corr[m][1];
-                        o[m][gr][k][3] *= corr[m][1];
+                        o[m][gr][k][0] *= corr[0];
+                        o[m][gr][k][1] *= corr[0];
+                        o[m][gr][k][2] *= corr[1];
+                        o[m][gr][k][3] *= corr[1];
                     }
             }
         }
@@ -561,7 +648,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         float w = fast_exp2(fmaf(x[m][nt][2 * r + e], c2, -ref[m][r]));
-                        if (tail && !((seen[m][r] >> (2 * nt + e)) & 1u)) w = 0.f;
+                        if constexpr (tail) w = (seen[m][r] >> (2 * nt + e)) & 1u ? w : 0.f;
                         x[m][nt][2 * r + e] = w;
                         sum += w;
                     }
@@ -591,7 +678,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
                             if constexpr (C::kScaled) {
                                 w0 *= s0;
                                 w1 *= s1;
-                                if (tail) {  // an unseen row's scale may be nan
+                                if constexpr (tail) {  // an unseen row's scale may be nan
                                     if (!((seen[m][r] >> (2 * nt)) & 1u)) w0 = 0.f;
                                     if (!((seen[m][r] >> (2 * nt + 1)) & 1u)) w1 = 0.f;
                                 }
@@ -602,8 +689,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
                 uint32_t h0[8], h1[8];
                 v_pairs<C::kKind>(vb, vb + 4 * C::kRb, gr, g, h0);
                 v_pairs<C::kKind>(vb + 8 * C::kRb, vb + 12 * C::kRb, gr, g, h1);
-                if constexpr (C::kFloat) {
-                    if (tail) {
+                if constexpr (C::kFloat && tail) {
+                    {
                         const int q0 = pb + 16 * j + t;
                         const uint32_t k0 = (q0 < len ? 0xFFFFu : 0u) | (q0 + 4 < len ? 0xFFFF0000u : 0u);
                         const uint32_t k1 = (q0 + 8 < len ? 0xFFFFu : 0u) | (q0 + 12 < len ? 0xFFFF0000u : 0u);
@@ -630,10 +717,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
                     for (int m = 0; m < MT; ++m) mma_f16_16816(o[m][gr][k], pa[m], h0[k], h1[k]);
             }
         }
-        if constexpr (C::kFloat) {
+        if constexpr (C::kFloat && tail) {
             // inf and nan entries of the block's rows, added to the rows that see them: what a
             // positive weight times such an entry gives
-            if (tail && __any_sync(0xffffffffu, special)) {
+            if (__any_sync(0xffffffffu, special)) {
                 for (int pr = 0; pr < PB; ++pr) {
                     const int j = pb + pr - ctx;
                     if (j >= n) break;
@@ -656,8 +743,23 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
                 }
             }
         }
+    };
+    bool failed = false;
+    int done = 0;
+    uint32_t phase = 0;
+    for (int i = 0, s = 0; i < mine; ++i) {
+        done = i;
+        if (!mbar_wait_bounded(bar + s, phase)) {
+            failed = true;
+            if (lane == 0) report_error(kErrFullWait);
+            break;
+        }
+        const int pb = p0 + (warp + i * C::kWarps) * PB;
+        if (pb + PB > ctx) block(std::true_type{}, ring + s * C::kStageBytes, pb);
+        else block(std::false_type{}, ring + s * C::kStageBytes, pb);
         __syncwarp();
-        if (i + C::kStages < mine) issue(i + C::kStages);
+        if (i + C::kStages < mine) issue(i + C::kStages, s);
+        if (++s == C::kStages) s = 0, phase ^= 1u;
     }
     if (failed) {
         // let the copies in flight land (bounded) before the shared memory is given back
@@ -685,8 +787,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
 #pragma unroll
                     for (int k = 0; k < 8; k += 4)
                         *reinterpret_cast<float4*>(dst + 64 * gr + 16 * t + 8 * e + k) =
-                            make_float4(o[m][gr][k][2 * r + e], o[m][gr][k + 1][2 * r + e], o[m][gr][k + 2][2 * r + e],
-                                        o[m][gr][k + 3][2 * r + e]);
+                            make_float4(o[m][gr][k][2 * r + e] * v_step<C::kKind>(k),
+                                        o[m][gr][k + 1][2 * r + e] * v_step<C::kKind>(k + 1),
+                                        o[m][gr][k + 2][2 * r + e] * v_step<C::kKind>(k + 2),
+                                        o[m][gr][k + 3][2 * r + e] * v_step<C::kKind>(k + 3));
         }
     __syncthreads();
     grid_launch_dependents();
@@ -719,7 +823,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
             v.w = fmaf(u.w, a, v.w);
         }
         if (direct) {
-            store_out(r, c, v, sum == 0.f ? 0.f : TreeCode<C::kKind>::kInvStep / sum);
+            store_out(r, c, v, sum == 0.f ? 0.f : 1.f / sum);
         } else {
             const size_t slot = ((size_t)stream * p.R + r) * p.S + split;
             __stcg(reinterpret_cast<float4*>(p.ws_o + slot * D + 4 * c), v);
@@ -733,28 +837,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
     __syncthreads();
     if (*s_ticket != (unsigned)(nsplit - 1)) return;
     if (tid == 0) store_relaxed_gpu(counter, 0u);
-    // the last range of the row tile merges all of them, in order
-    for (int i = tid; i < C::kRows * Q4; i += C::kThreads) {
-        const int row = i / Q4, c = i - row * Q4, r = r0 + row;
-        if (r >= p.R) break;
-        const size_t slot = ((size_t)stream * p.R + r) * p.S;
-        const float2* ml = reinterpret_cast<const float2*>(p.ws_ml + slot * 2);
-        float mx = kNegMax, sum = 0.f;
-        for (int s = 0; s < nsplit; ++s) mx = fmaxf(mx, __ldcg(ml + s).x);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int s = 0; s < nsplit; ++s) {
-            const float2 w = __ldcg(ml + s);
-            const float a = fast_exp2(w.x - mx);
-            const float4 u = __ldcg(reinterpret_cast<const float4*>(p.ws_o + (slot + s) * D + 4 * c));
-            sum = fmaf(w.y, a, sum);
-            v.x = fmaf(u.x, a, v.x);
-            v.y = fmaf(u.y, a, v.y);
-            v.z = fmaf(u.z, a, v.z);
-            v.w = fmaf(u.w, a, v.w);
-        }
-        store_out(r, c, v, sum == 0.f ? 0.f : TreeCode<C::kKind>::kInvStep / sum);
-    }
+    tree_merge<D, C::kRows, C::kThreads>(p, stream, r0, min(C::kRows, p.R - r0), nsplit, reinterpret_cast<float*>(smem),
+                                         tid, store_out);
 }
 
 }  // namespace va

@@ -1,0 +1,780 @@
+// Tree attention over a paged cache on the Blackwell tensor cores: the
+// operator of decode_tree.cuh (its mathematics, masks, splits and slots) for many
+// query rows, with tcgen05.mma and accumulators in tensor memory.
+//
+// One CTA per (sequence, KV head, tile of query rows, range of positions), one
+// per SM, 17 warps:
+//   warps 0-3, 4-7  two softmax warpgroups; thread r owns query row r (TMEM lane r);
+//   warps 8-15      producers: codes -> exact fp16 codes in swizzled tiles;
+//   warp 16         one thread issues every tcgen05.mma.
+// A job is one warpgroup's work on one block of 64 positions. kTwo = false (up
+// to 128 query rows): the warpgroups take the blocks in turn, each with its own
+// O and statistics, merged at the end. kTwo = true (up to 256): both take every
+// block, for query rows 0..127 and 128..255, so a decoded tile serves twice.
+//
+// Per job j (MMA order S(0) S(1), then S(j + 2) PV(j)):
+//   S_g = Q_g K_g^T (M = 128 rows, N = 64 positions) for each 64-dim group g, in
+//     TMEM. The K tile holds the exact codes (times a power of two), so the group
+//     scales multiply fp32 scores, as in decode_tree.cuh;
+//   the softmax thread loads its row's scores, x = S_0 k_0 + S_1 k_1, hands the
+//     S columns back, and writes P'_g = fp16(w v_g) into shared memory;
+//   O_g += P'_g V_g (A = P' from shared memory, B = the V tile read MN-major).
+// O is rescaled only when a row's reference grows by more than 4 (log2): P' of the
+// largest weight stays in [2^6, 2^15), its rounding relative.
+//
+// The K and V tiles are the canonical 128-byte-swizzled layout, one panel of 64
+// rows per 64-dim group. Packed codes are placed two dims apart by 4 in each
+// 32-bit word ((0, 4), (1, 5), ...), which costs no byte permutes; Q's columns are
+// stored in the same order and the output's are put back.
+#pragma once
+
+#include "decode_tree.cuh"
+#include "prefill_tc.cuh"
+
+namespace va {
+
+template <Kind K, int kDim, bool kTwoTiles>
+struct TreeTcCfg {
+    static constexpr Kind kKind = K;
+    static constexpr int kD = kDim;
+    static constexpr bool kTwo = kTwoTiles;
+    static constexpr int kRows = kTwoTiles ? 256 : 128;
+    static constexpr int kNG = kDim / 64;
+    static constexpr bool kScaled = !(K == Kind::F16 || K == Kind::BF16);
+    static constexpr bool kFloat = is_float_kind(K);
+    static constexpr bool kPairs4 = K == Kind::Q4 || K == Kind::Q3;  // dims (p, p + 4) in a word
+    static constexpr int kSG = kScaled ? kNG : 1;  // score accumulators, weight copies
+    static constexpr int kRb = kDim * KindTraits<K>::kBits / 8;
+    static constexpr int kNb = 64;                 // positions of a block
+    static constexpr int kProducers = 256;
+    static constexpr int kThreads = 17 * 32;
+    static constexpr int kQTile = 128 * kDim * 2;
+    static constexpr int kTile = kNb * kDim * 2;   // one K or V tile
+    static constexpr int kPTile = 128 * kNb * 2;
+    static constexpr int kKS = 3;
+    static constexpr int kVS = (kTwoTiles && kScaled && kDim == 128) ? 2 : 3;
+    static constexpr int kOffP = (kTwoTiles ? 2 : 1) * kQTile;
+    static constexpr int kOffK = kOffP + 2 * kSG * kPTile;
+    static constexpr int kOffV = kOffK + kKS * kTile;
+    static constexpr int kOffScales = kOffV + kVS * kTile;     // [4 slots][K, V][kNG][64] floats
+    static constexpr int kScaleSlots = 4;
+    static constexpr int kOffMask = kOffScales + (kScaled ? kScaleSlots * 2 * kNG * kNb * 4 : 0);
+    static constexpr int kOffMl = kOffMask + kRows * 8;        // [2][128] (reference, sum)
+    static constexpr int kOffBars = kOffMl + 2 * 128 * 8;
+    static constexpr int kBars = 2 * kKS + 2 * kVS + 2 * 4 + 1 + kScaleSlots;
+    static constexpr int kOffMisc = kOffBars + kBars * 8;      // ev[4], TMEM slot, fail, special, ticket
+    static constexpr int kSmemBytes = 1024 + kOffMisc + 64;
+    static constexpr int kPrefetch = 6;                        // blocks ahead into L2
+    static_assert(kSmemBytes <= 227 * 1024, "one CTA per SM");
+};
+
+// Placed K codes: the code / kTcInvStep.
+template <Kind K>
+__host__ __device__ constexpr float tc_k_inv_step() {
+    return K == Kind::Q4 ? 64.f : K == Kind::Q3 ? 128.f : 1.f;
+}
+// Placed V codes: the code of pair p (dims p, p + 4) / this.
+template <Kind K>
+__host__ __device__ constexpr float tc_v_step(int p) {
+    return K == Kind::Q4 ? ((p & 1) ? 64.f : 1024.f)
+                         : K == Kind::Q3 ? (p == 1 ? 128.f : p == 2 ? 16.f : 1024.f) : 1.f;
+}
+
+// The codes of kDim / 4 consecutive dims of one row (quarter q).
+template <Kind K, int kDim>
+struct TcRaw {
+    static constexpr int kDims = kDim / 4;
+    static constexpr int kWords = K == Kind::Q3 ? (kDims == 32 ? 3 : 2) : kDims * KindTraits<K>::kBits / 32;
+    uint32_t w[kWords];
+};
+
+template <Kind K, int kDim>
+__device__ __forceinline__ void tc_load(TcRaw<K, kDim>& r, const uint8_t* row, int q) {
+    constexpr int kBytes = TcRaw<K, kDim>::kDims * KindTraits<K>::kBits / 8;
+    if constexpr (K == Kind::Q3) {
+        // 12 bytes of 4-byte alignment, or the two words around 6
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(row + ((q * kBytes) & ~3));
+#pragma unroll
+        for (int i = 0; i < TcRaw<K, kDim>::kWords; ++i) r.w[i] = __ldg(p + i);
+        if constexpr (kBytes == 6) {
+            const uint32_t sh = (q & 1) * 16;
+            r.w[0] = __funnelshift_r(r.w[0], r.w[1], sh);
+            r.w[1] >>= sh;
+        }
+    } else if constexpr (kBytes == 8) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(row) + q);
+        r.w[0] = v.x;
+        r.w[1] = v.y;
+    } else {
+        const uint4* p = reinterpret_cast<const uint4*>(row) + q * (kBytes / 16);
+#pragma unroll
+        for (int i = 0; i < kBytes / 16; ++i) {
+            const uint4 v = __ldg(p + i);
+            r.w[4 * i] = v.x;
+            r.w[4 * i + 1] = v.y;
+            r.w[4 * i + 2] = v.z;
+            r.w[4 * i + 3] = v.w;
+        }
+    }
+}
+
+// Eight dims (chunk j of the slice) as fp16, centred: exact.
+template <Kind K, int kDim, bool kIsV>
+__device__ __forceinline__ uint4 tc_convert(const TcRaw<K, kDim>& r, int j) {
+    constexpr uint32_t kOne = 0x3C003C00u;
+    uint32_t h[4];
+    if constexpr (K == Kind::F16) {
+        return make_uint4(r.w[4 * j], r.w[4 * j + 1], r.w[4 * j + 2], r.w[4 * j + 3]);
+    } else if constexpr (K == Kind::BF16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = bf2_to_h2(r.w[4 * j + i]);
+    } else if constexpr (K == Kind::F8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = f8x2_to_h2(r.w[2 * j + (i >> 1)] >> (16 * (i & 1)));
+    } else if constexpr (K == Kind::Q8) {
+        const __half2 off = __float2half2_rn(1152.f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t u = r.w[2 * j + (i >> 1)] ^ 0x80808080u;
+            h[i] = h2_bits(__hsub2(bits_h2(__byte_perm(u, 0x64646464u, (i & 1) ? 0x4342 : 0x4140)), off));
+        }
+    } else if constexpr (K == Kind::Q4) {
+        const uint32_t w = r.w[j];
+        const __half2 o64 = __float2half2_rn(1.f + 8.f / 64.f), o1024 = __float2half2_rn(1.f + 8.f / 1024.f);
+        if constexpr (kIsV) {
+            const uint32_t u = w >> 8;
+            h[0] = h2_bits(__hsub2(bits_h2((w & 0x000F000Fu) | kOne), o1024));
+            h[1] = h2_bits(__hsub2(bits_h2((w & 0x00F000F0u) | kOne), o64));
+            h[2] = h2_bits(__hsub2(bits_h2((u & 0x000F000Fu) | kOne), o1024));
+            h[3] = h2_bits(__hsub2(bits_h2((u & 0x00F000F0u) | kOne), o64));
+        } else {
+            h[0] = h2_bits(__hsub2(bits_h2(((w << 4) & 0x00F000F0u) | kOne), o64));
+            h[1] = h2_bits(__hsub2(bits_h2((w & 0x00F000F0u) | kOne), o64));
+            h[2] = h2_bits(__hsub2(bits_h2(((w >> 4) & 0x00F000F0u) | kOne), o64));
+            h[3] = h2_bits(__hsub2(bits_h2(((w >> 8) & 0x00F000F0u) | kOne), o64));
+        }
+    } else {
+        // bits 24 j .. 24 j + 23 of the slice: fields 0..3 to the low half, 4..7 to the high one
+        const int i0 = (24 * j) >> 5, sh = (24 * j) & 31;
+        const uint32_t w = sh > 8 && i0 + 1 < TcRaw<K, kDim>::kWords ? __funnelshift_r(r.w[i0], r.w[i0 + 1], sh) : r.w[i0] >> sh;
+        const uint32_t u = __byte_perm(w, w >> 12, 0x5410);
+        const __half2 o128 = __float2half2_rn(1.f + 4.f / 128.f);
+        if constexpr (kIsV) {
+            const __half2 o1024 = __float2half2_rn(1.f + 4.f / 1024.f), o16 = __float2half2_rn(1.f + 4.f / 16.f);
+            h[0] = h2_bits(__hsub2(bits_h2((u & 0x00070007u) | kOne), o1024));
+            h[1] = h2_bits(__hsub2(bits_h2((u & 0x00380038u) | kOne), o128));
+            h[2] = h2_bits(__hsub2(bits_h2((u & 0x01C001C0u) | kOne), o16));
+            h[3] = h2_bits(__hsub2(bits_h2(((u >> 9) & 0x00070007u) | kOne), o1024));
+        } else {
+            h[0] = h2_bits(__hsub2(bits_h2(((u << 3) & 0x00380038u) | kOne), o128));
+            h[1] = h2_bits(__hsub2(bits_h2((u & 0x00380038u) | kOne), o128));
+            h[2] = h2_bits(__hsub2(bits_h2(((u >> 3) & 0x00380038u) | kOne), o128));
+            h[3] = h2_bits(__hsub2(bits_h2(((u >> 6) & 0x00380038u) | kOne), o128));
+        }
+    }
+    return make_uint4(h[0], h[1], h[2], h[3]);
+}
+
+__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+        "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+        "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// 16 consecutive fp32 columns of this thread's TMEM lane, without the wait (as
+// tmem_ld32_nowait), and the tie to it.
+__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_tie16(uint32_t* r) {
+    asm volatile(""
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15]));
+}
+
+__device__ __forceinline__ void prefetch_l2(const void* src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
+
+// Clears the entries of eight fp16 values that are not finite; true if there were any.
+__device__ __forceinline__ bool clear_not_finite(uint4& v) {
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if ((w[i] & 0x7C00u) == 0x7C00u) w[i] &= 0xFFFF0000u, any = true;
+        if ((w[i] & 0x7C000000u) == 0x7C000000u) w[i] &= 0xFFFFu, any = true;
+    }
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+    return any;
+}
+
+template <class C>
+__global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const TreeParams p) {
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    constexpr int D = C::kD, NG = C::kNG, NB = C::kNb, KS = C::kKS, VS = C::kVS, SG = C::kSG;
+    constexpr Kind KK = C::kKind;
+    unsigned long long* s_mask = reinterpret_cast<unsigned long long*>(smem + C::kOffMask);
+    float2* s_ml = reinterpret_cast<float2*>(smem + C::kOffMl);
+    uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
+    uint64_t *kempty = kfull + KS, *vfull = kempty + KS, *vempty = vfull + VS, *sfull = vempty + VS;
+    uint64_t *sempty = sfull + 2, *pfull = sempty + 2, *odone = pfull + 2, *fin = odone + 2, *scfull = fin + 1;
+    float* s_ev = reinterpret_cast<float*>(smem + C::kOffMisc);
+    uint32_t* tslot = reinterpret_cast<uint32_t*>(s_ev + 4);
+    volatile int* fail = reinterpret_cast<volatile int*>(tslot + 1);
+    volatile int* special = fail + 1;
+    unsigned* s_ticket = tslot + 3;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int split = (int)(blockIdx.x % p.S);
+    const int rest = (int)(blockIdx.x / p.S);
+    const int tile = rest % p.tiles, stream = rest / p.tiles;
+    const int b = stream / p.Hkv, hk = stream - b * p.Hkv;
+    const int r0 = tile * C::kRows;
+
+    grid_dependency_wait();
+    const long long cap = (long long)p.max_pages * p.page_rows;
+    const int len = (int)max(0ll, min((long long)__ldg(p.lens + b), cap));
+    const int n = max(0, min(min(p.nodes ? __ldg(p.nodes + b) : p.Q, p.Q), len));
+    const int ctx = len - n;
+    const int chunk = tree_chunk(len, p.S);
+    const int nsplit = max(1, (len + chunk - 1) / chunk);
+    if (split >= nsplit) return;
+    const int p0 = split * chunk, p1 = min(len, p0 + chunk);
+    const int live = min(p.R, n * p.G) - r0;  // rows of the tile that belong to a node; none: zeros
+    if (live <= 0 && split > 0) return;
+    const int rows_here = min(C::kRows, p.R - r0);
+
+    const auto store_out = [&](int r, int c, float4 v, float inv) {
+        const int node = r / p.G;
+        __half* dst = p.out + b * p.os_b + node * p.os_t + (long long)(hk * p.G + (r - node * p.G)) * p.os_h + 4 * c;
+        const bool on = node < n && inv != 0.f;
+        const __half2 a = __floats2half2_rn(on ? v.x * inv : 0.f, on ? v.y * inv : 0.f);
+        const __half2 d = __floats2half2_rn(on ? v.z * inv : 0.f, on ? v.w * inv : 0.f);
+        *reinterpret_cast<uint2*>(dst) = make_uint2(h2_bits(a), h2_bits(d));
+    };
+    if (live <= 0) {
+        for (int i = tid; i < rows_here * (D / 4); i += C::kThreads)
+            store_out(r0 + i / (D / 4), i % (D / 4), make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
+        return;
+    }
+
+    const int nblk = (p1 - p0 + NB - 1) / NB;
+    const int njobs = C::kTwo ? 2 * nblk : nblk;
+    if (warp == 16) tmem_alloc(tslot, 512);
+    if (tid == 0) {
+        for (int i = 0; i < KS; ++i) mbar_init(kfull + i, C::kProducers / 32), mbar_init(kempty + i, 1);
+        for (int i = 0; i < VS; ++i) mbar_init(vfull + i, C::kProducers / 32), mbar_init(vempty + i, 1);
+        for (int i = 0; i < 2; ++i)
+            mbar_init(sfull + i, 1), mbar_init(sempty + i, 4), mbar_init(pfull + i, 4), mbar_init(odone + i, 1);
+        mbar_init(fin, 1);
+        for (int i = 0; i < C::kScaleSlots; ++i) mbar_init(scfull + i, 1);
+        *fail = 0;
+        *special = 0;
+        fence_mbar_init();
+    }
+    const int* trow = p.table + (size_t)b * p.max_pages;
+    const auto page_of = [&](int pos, int& off) {
+        const int pi = (int)((__umulhi((unsigned)pos, p.page_mul) + (unsigned)pos) >> p.page_shift);
+        off = pos - pi * p.page_rows;
+        const int pg = pi < p.max_pages ? __ldg(trow + pi) : 0;
+        return (unsigned)pg < (unsigned)p.num_pages ? pg : 0;
+    };
+    // L2 prefetch of block i by one warp: lane = buffer + 4 * run of 8 rows (or the
+    // whole block in one run)
+    const bool whole = p.page_rows % NB == 0;
+    const auto prefetch = [&](int i) {
+        const int buf = lane & 3, run = whole ? NB : 8, at = (lane >> 2) * run;
+        const int rb = buf < 2 ? C::kRb : 2 * NG;
+        if (at >= NB || (buf >= 2 && !C::kScaled)) return;
+        int off;
+        const int pg = page_of(p0 + i * NB + at, off);
+        const uint8_t* base = buf == 0   ? p.K
+                              : buf == 1 ? p.V
+                              : buf == 2 ? reinterpret_cast<const uint8_t*>(p.scK)
+                                         : reinterpret_cast<const uint8_t*>(p.scV);
+        prefetch_l2(base + (((size_t)pg * p.Hkv + hk) * p.page_rows + off) * rb, (uint32_t)(run * rb));
+    };
+    if (warp >= 8 && warp < 16)
+        for (int i = warp - 8; i < min(C::kPrefetch, nblk); i += 8) prefetch(i);
+
+    // the query rows into shared memory in the tiles' order of dims, and their masks
+    for (int i = tid; i < C::kRows * (D / 8); i += C::kThreads) {
+        const int row = i / (D / 8), c = i - row * (D / 8);
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (row < live) {
+            const int r = r0 + row, node = r / p.G;
+            v = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.qs_b + node * p.qs_t +
+                                                     (long long)(hk * p.G + (r - node * p.G)) * p.qs_h) + c);
+            if constexpr (C::kPairs4)
+                v = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
+                               __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+        }
+        const int rr = row & 127;
+        *reinterpret_cast<uint4*>(smem + (row >> 7) * C::kQTile + (c >> 3) * 16384 + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
+    }
+    const unsigned long long nodes_mask = n >= 64 ? ~0ull : (1ull << n) - 1ull;
+    for (int i = tid; i < C::kRows; i += C::kThreads) {
+        const int node = (r0 + i) / p.G;
+        s_mask[i] = i < live ? __ldg(p.mask + (size_t)b * p.Q + node) & nodes_mask : 0ull;
+    }
+    fence_proxy_async_smem();
+    tc05_fence_before();
+    __syncthreads();
+    tc05_fence_after();
+    const uint32_t tbase = *tslot;
+    const uint32_t sbase = smem_u32(smem);
+
+    float m_ref = kNegMax, l_sum = 0.f;  // softmax threads: their row's reference (log2 units) and sum
+    if (warp < 8) {
+        // ---- softmax -------------------------------------------------------------
+        const int w = warp >> 2;
+        const int row = tid & 127, qrow = C::kTwo ? w * 128 + row : row;
+        const int jobs = C::kTwo ? nblk : (nblk - w + 1) / 2;
+        const bool idle = (C::kTwo ? w * 128 : 0) + (warp & 3) * 32 >= live;  // no row of this warp is live
+        const uint32_t tS = tbase + w * 256 + ((uint32_t)((warp & 3) * 32) << 16), tO = tS + 128;
+        uint8_t* sP = smem + C::kOffP + w * SG * C::kPTile + row * 128;
+        const float c2 = rsqrtf((float)D) * kLog2e * tc_k_inv_step<KK>();
+        const unsigned long long mk = s_mask[qrow];
+        for (int k = 0; k < jobs; ++k) {
+            const int blk = C::kTwo ? k : 2 * k + w;
+            const int pb = p0 + blk * NB;
+            const float* sc = reinterpret_cast<const float*>(smem + C::kOffScales) + (blk % C::kScaleSlots) * 2 * NG * NB;
+            bool ok = mbar_wait_fast(sfull + w, (uint32_t)k & 1u);
+            // (a slot of scales is written again only after this block's PV, so this phase
+            // cannot be passed twice before it is seen here)
+            if constexpr (C::kScaled)
+                ok = ok && mbar_wait_fast(scfull + blk % C::kScaleSlots, (uint32_t)(blk / C::kScaleSlots) & 1u);
+            if (!ok) {
+                if (lane == 0) report_error(kErrFullWait);
+                *fail = 1;
+                break;
+            }
+            tc05_fence_after();
+            float x[NB];
+            if (!idle) {
+#pragma unroll
+                for (int cb = 0; cb < NB; cb += 16) {
+                    uint32_t s[SG][16];
+#pragma unroll
+                    for (int g = 0; g < SG; ++g) tmem_ld16_nowait(tS + 64 * g + cb, s[g]);
+                    tmem_wait_ld_only();
+#pragma unroll
+                    for (int g = 0; g < SG; ++g) tmem_tie16(s[g]);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        float2 a = make_float2(__uint_as_float(s[0][j]), __uint_as_float(s[0][j + 1]));
+                        float2 c = make_float2(__uint_as_float(s[0][j + 2]), __uint_as_float(s[0][j + 3]));
+                        if constexpr (C::kScaled) {
+                            const float4 k0 = *reinterpret_cast<const float4*>(sc + cb + j);
+                            a = fmul2(a, make_float2(k0.x, k0.y));
+                            c = fmul2(c, make_float2(k0.z, k0.w));
+                            if constexpr (NG == 2) {
+                                const float4 k1 = *reinterpret_cast<const float4*>(sc + NB + cb + j);
+                                a = ffma2(make_float2(__uint_as_float(s[SG - 1][j]), __uint_as_float(s[SG - 1][j + 1])),
+                                          make_float2(k1.x, k1.y), a);
+                                c = ffma2(make_float2(__uint_as_float(s[SG - 1][j + 2]), __uint_as_float(s[SG - 1][j + 3])),
+                                          make_float2(k1.z, k1.w), c);
+                            }
+                        }
+                        x[cb + j] = a.x;
+                        x[cb + j + 1] = a.y;
+                        x[cb + j + 2] = c.x;
+                        x[cb + j + 3] = c.y;
+                    }
+                }
+            }
+            tc05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sempty + w);  // the next S of this warpgroup may be computed
+            // which of the 64 columns the row sees
+            const bool tail = pb + NB > ctx;
+            unsigned long long vis = ~0ull;
+            if (tail) {
+                const int d = ctx - pb;  // < 64
+                vis = d > 0 ? (mk << d) | ((1ull << d) - 1ull) : -d < 64 ? mk >> -d : 0ull;
+                if (!idle) {
+#pragma unroll
+                    for (int j = 0; j < NB; ++j)
+                        if (!(vis >> j & 1ull)) x[j] = kNegMax;
+                }
+            }
+            float nref = m_ref;
+            if (!idle) {
+                float b0 = x[0], b1 = x[1];
+#pragma unroll
+                for (int j = 2; j < NB; j += 4) {
+                    b0 = fmax3f(b0, x[j], x[j + 1]);
+                    if (j + 2 < NB) b1 = fmax3f(b1, x[j + 2], x[j + 3]);
+                }
+                const float bm = fmaxf(b0, b1);
+                const float ev = C::kScaled ? s_ev[blk % C::kScaleSlots] : 0.f;
+                const float want = bm == kNegMax ? kNegMax : fmaf(bm, c2, ev - 10.f);
+                if (want > m_ref + 4.f) nref = want;
+            }
+            // P' and O of this warpgroup are free once its previous PV is done
+            if (k > 0 && !mbar_wait_fast(odone + w, (uint32_t)(k - 1) & 1u)) {
+                if (lane == 0) report_error(kErrFullWait);
+                *fail = 1;
+                break;
+            }
+            if (!idle) {
+                tc05_fence_after();
+                const float corr = fast_exp2(m_ref - nref);
+                if (__any_sync(0xffffffffu, nref != m_ref)) {
+                    l_sum *= corr;
+                    if (k > 0) {
+#pragma unroll 1
+                        for (int cb = 0; cb < D; cb += 32) {
+                            float o[32];
+                            tmem_ld32(tO + cb, o);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] *= corr;
+                            tmem_st32(tO + cb, o);
+                        }
+                        tmem_wait_st();
+                    }
+                }
+                m_ref = nref;
+                float2 sum = make_float2(0.f, 0.f);
+                const float2 sc2 = make_float2(c2, c2), nm = make_float2(-nref, -nref);
+#pragma unroll
+                for (int j = 0; j < NB; j += 8) {
+                    float2 e[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 y = ffma2(make_float2(x[j + 2 * i], x[j + 2 * i + 1]), sc2, nm);
+                        e[i] = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+                        if (tail) {
+                            if (!(vis >> (j + 2 * i) & 1ull)) e[i].x = 0.f;
+                            if (!(vis >> (j + 2 * i + 1) & 1ull)) e[i].y = 0.f;
+                        }
+                        sum = fadd2(sum, e[i]);
+                    }
+#pragma unroll
+                    for (int g = 0; g < SG; ++g) {
+                        uint32_t h[4];
+                        float2 v[4];
+                        if constexpr (C::kScaled) {
+                            const float4 v0 = *reinterpret_cast<const float4*>(sc + (NG + g) * NB + j);
+                            const float4 v1 = *reinterpret_cast<const float4*>(sc + (NG + g) * NB + j + 4);
+                            v[0] = fmul2(e[0], make_float2(v0.x, v0.y));
+                            v[1] = fmul2(e[1], make_float2(v0.z, v0.w));
+                            v[2] = fmul2(e[2], make_float2(v1.x, v1.y));
+                            v[3] = fmul2(e[3], make_float2(v1.z, v1.w));
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[i] = e[i];
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (C::kScaled && tail) {  // an unseen row's scale may be nan
+                                if (!(vis >> (j + 2 * i) & 1ull)) v[i].x = 0.f;
+                                if (!(vis >> (j + 2 * i + 1) & 1ull)) v[i].y = 0.f;
+                            }
+                            h[i] = h2_bits(__floats2half2_rn(v[i].x, v[i].y));
+                        }
+                        *reinterpret_cast<uint4*>(sP + g * C::kPTile + (((j >> 3) ^ (row & 7)) << 4)) =
+                            make_uint4(h[0], h[1], h[2], h[3]);
+                    }
+                }
+                l_sum += sum.x + sum.y;
+                fence_proxy_async_smem();
+            }
+            tc05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pfull + w);
+        }
+        if (jobs > 0 && !*fail && !mbar_wait_fast(odone + w, (uint32_t)(jobs - 1) & 1u)) {
+            if (lane == 0) report_error(kErrFullWait);
+            *fail = 1;
+        }
+        tc05_fence_after();
+    } else if (warp < 16) {
+        // ---- producers: thread = (row of the block, quarter of the dims) -------------
+        const int pw = warp - 8;
+        // lane bits: quarter bit 0, row bits 0..1, quarter bit 1, row bit 2: eight
+        // neighbouring lanes store to eight different 16-byte banks
+        const int q = (lane & 1) | ((lane >> 2) & 2), row = pw * 8 + ((lane >> 1) & 3) + ((lane >> 4) << 2);
+        using Raw = TcRaw<KK, D>;
+        constexpr int kChunks = Raw::kDims / 8;
+        Raw rk, rv, nk, nv;
+        const auto load = [&](int i, Raw& a, Raw& c) {
+            int off;
+            const int pg = page_of(p0 + i * NB + row, off);
+            const size_t r = ((size_t)pg * p.Hkv + hk) * p.page_rows + off;
+            tc_load<KK, D>(a, p.K + r * C::kRb, q);
+            tc_load<KK, D>(c, p.V + r * C::kRb, q);
+        };
+        const auto put = [&](uint8_t* dst, int j, uint4 v) {
+            const int c = q * kChunks + j;
+            *reinterpret_cast<uint4*>(dst + (c >> 3) * (NB * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+        };
+        load(0, rk, rv);
+        for (int i = 0; i < nblk; ++i) {
+            const int pb = p0 + i * NB;
+            if (pw == (i & 7) && i + C::kPrefetch < nblk) prefetch(i + C::kPrefetch);
+            if (i + 1 < nblk) load(i + 1, nk, nv);
+            // scales of the block: warp i % 8, two positions a lane
+            uint32_t ks[2], vs[2];
+            const bool scales = C::kScaled && pw == ((i + 4) & 7);
+            if (scales) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    int off;
+                    const int pg = page_of(pb + lane + 32 * e, off);
+                    const size_t r = ((size_t)pg * p.Hkv + hk) * p.page_rows + off;
+                    if constexpr (NG == 2) {
+                        ks[e] = __ldg(reinterpret_cast<const uint32_t*>(p.scK) + r);
+                        vs[e] = __ldg(reinterpret_cast<const uint32_t*>(p.scV) + r);
+                    } else {
+                        ks[e] = __ldg(reinterpret_cast<const uint16_t*>(p.scK) + r);
+                        vs[e] = __ldg(reinterpret_cast<const uint16_t*>(p.scV) + r);
+                    }
+                }
+            }
+            const int u = i / KS, x = i / VS;
+            if (u > 0 && !mbar_wait_bounded(kempty + i % KS, (uint32_t)(u - 1) & 1u)) {
+                if (lane == 0) report_error(kErrEmptyWait);
+                *fail = 1;
+                break;
+            }
+            if (scales) {
+                float* sc = reinterpret_cast<float*>(smem + C::kOffScales) + (i % C::kScaleSlots) * 2 * NG * NB;
+                __half2 big = __float2half2_rn(0.f);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float2 fk = __half22float2(bits_h2(ks[e])), fv = __half22float2(bits_h2(vs[e]));
+                    sc[lane + 32 * e] = fk.x;
+                    sc[NG * NB + lane + 32 * e] = fv.x;
+                    if constexpr (NG == 2) {
+                        sc[NB + lane + 32 * e] = fk.y;
+                        sc[3 * NB + lane + 32 * e] = fv.y;
+                    }
+                    // rows past the end and scales that are not finite are no measure
+                    uint32_t a = vs[e] & 0x7FFF7FFFu;
+                    if (pb + lane + 32 * e >= len) a = 0u;
+                    if ((a & 0x7FFFu) >= 0x7C00u) a &= 0x7FFF0000u;
+                    if ((a >> 16) >= 0x7C00u) a &= 0x7FFFu;
+                    big = __hmax2(big, bits_h2(a));
+                }
+                const float vm = fmaxf(__low2float(big), __high2float(big));
+                __syncwarp();
+                const unsigned vb = __reduce_max_sync(0xffffffffu, __float_as_uint(vm));
+                if (lane == 0) {
+                    s_ev[i % C::kScaleSlots] = vb ? (float)((int)(vb >> 23) - 127) : 0.f;
+                    mbar_arrive(scfull + i % C::kScaleSlots);  // (the reduction came after all lanes' stores)
+                }
+            }
+            uint8_t* kt = smem + C::kOffK + (i % KS) * C::kTile;
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) put(kt, j, tc_convert<KK, D, false>(rk, j));
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(kfull + i % KS);
+            if (x > 0 && !mbar_wait_bounded(vempty + i % VS, (uint32_t)(x - 1) & 1u)) {
+                if (lane == 0) report_error(kErrEmptyWait);
+                *fail = 1;
+                break;
+            }
+            uint8_t* vt = smem + C::kOffV + (i % VS) * C::kTile;
+            const int pos = pb + row;
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) {
+                uint4 v = tc_convert<KK, D, true>(rv, j);
+                if constexpr (C::kFloat) {
+                    // rows past the end are cleared; entries of drafted rows that are not finite
+                    // are left to the epilogue, which adds them to the rows that see them
+                    if (pos >= len) v = make_uint4(0u, 0u, 0u, 0u);
+                    else if (pos >= ctx && clear_not_finite(v)) *special = 1;
+                }
+                put(vt, j, v);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(vfull + i % VS);
+            rk = nk;
+            rv = nv;
+        }
+    } else if (lane == 0) {
+        // ---- the MMA thread ----------------------------------------------------------
+        constexpr uint32_t kIdescS = umma_idesc_f16(128, NB, false);
+        constexpr uint32_t kIdescO = umma_idesc_f16(128, C::kScaled ? 64 : D, true);
+        bool ok = true;
+        for (int j = 0; ok && j < njobs + 2; ++j) {
+            if (j < njobs) {
+                const int w = j & 1, k = j >> 1, i = C::kTwo ? j >> 1 : j, s = i % KS;
+                ok = mbar_wait_fast(kfull + s, (uint32_t)(i / KS) & 1u);
+                if (k > 0) ok = ok && mbar_wait_fast(sempty + w, (uint32_t)(k - 1) & 1u);
+                if (!ok) break;
+                tc05_fence_after();
+                const uint32_t qa = sbase + (C::kTwo ? w * C::kQTile : 0), ka = sbase + C::kOffK + s * C::kTile;
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        umma_f16(tbase + w * 256 + (C::kScaled ? 64 * g : 0),
+                                 umma_desc_sw128(qa + g * 16384 + kk * 32, 16, 1024),
+                                 umma_desc_sw128(ka + g * (NB * 128) + kk * 32, 16, 1024), kIdescS,
+                                 kk > 0 || (!C::kScaled && g > 0));
+                umma_commit(sfull + w);
+                if (!C::kTwo || w == 1) umma_commit(kempty + s);
+            }
+            if (j >= 2) {
+                const int jj = j - 2, w = jj & 1, k = jj >> 1, i = C::kTwo ? jj >> 1 : jj, s = i % VS;
+                ok = mbar_wait_fast(vfull + s, (uint32_t)(i / VS) & 1u);
+                ok = ok && mbar_wait_fast(pfull + w, (uint32_t)k & 1u);
+                if (!ok) break;
+                tc05_fence_after();
+                const uint32_t pa = sbase + C::kOffP + w * SG * C::kPTile, va = sbase + C::kOffV + s * C::kTile;
+#pragma unroll
+                for (int g = 0; g < SG; ++g)
+#pragma unroll
+                    for (int kk = 0; kk < NB / 16; ++kk)
+                        umma_f16(tbase + w * 256 + 128 + 64 * g,
+                                 umma_desc_sw128(pa + g * C::kPTile + kk * 32, 16, 1024),
+                                 umma_desc_sw128(va + g * (NB * 128) + kk * 2048, NB * 128, 1024), kIdescO,
+                                 k > 0 || kk > 0);
+                umma_commit(odone + w);
+                if (!C::kTwo || w == 1) umma_commit(vempty + s);
+            }
+        }
+        if (!ok) {  // every MMA issued so far ends before the tensor memory is given back
+            report_error(kErrFullWait);
+            *fail = 1;
+            umma_commit(fin);
+            (void)mbar_wait_bounded(fin, 0);
+        }
+    }
+    tc05_fence_before();
+    __syncthreads();
+    tc05_fence_after();
+    if (*fail) {
+        if (warp == 16) tmem_dealloc(tbase, 512);
+        return;
+    }
+    grid_launch_dependents();
+
+    // ---- epilogue: a thread's row, its half of the dims (one tile) or all of them ------
+    const bool direct = nsplit == 1;
+    if (warp < 8) {
+        const int w = warp >> 2, row = tid & 127, qrow = C::kTwo ? w * 128 + row : row, r = r0 + qrow;
+        const uint32_t tO = tbase + w * 256 + 128 + ((uint32_t)((warp & 3) * 32) << 16);
+        const bool idle = (C::kTwo ? w * 128 : 0) + (warp & 3) * 32 >= live;
+        float mx = m_ref, sum = l_sum, a0 = 1.f, a1 = 0.f;
+        float* xch = reinterpret_cast<float*>(smem + C::kOffK);  // [D][128]: the other warpgroup's half
+        constexpr int kCols = C::kTwo ? D : D / 2;               // dims this thread finishes
+        const int c0 = C::kTwo ? 0 : w * kCols;
+        const bool has = C::kTwo || w == 0 || nblk > 1;          // (one block: warpgroup 1 had no job)
+        if constexpr (!C::kTwo) {
+            s_ml[w * 128 + row] = make_float2(m_ref, l_sum);
+            if (!idle && has) {
+                const int o0 = (1 - w) * kCols;
+#pragma unroll 1
+                for (int cb = 0; cb < kCols; cb += 32) {
+                    float o[32];
+                    tmem_ld32(tO + o0 + cb, o);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) xch[(o0 + cb + i) * 128 + row] = o[i];
+                }
+            }
+            named_barrier_sync(1, 256);
+            const float2 other = s_ml[(1 - w) * 128 + row];
+            mx = fmaxf(m_ref, other.x);
+            a0 = has ? fast_exp2(m_ref - mx) : 0.f;
+            a1 = (w == 1 || nblk > 1) ? fast_exp2(other.x - mx) : 0.f;
+            sum = l_sum * a0 + other.y * a1;
+        }
+        if (!idle) {
+            const size_t slot = ((size_t)stream * p.R + r) * p.S + split;
+            const unsigned long long mk = s_mask[qrow];
+#pragma unroll 1
+            for (int cb = 0; cb < kCols; cb += 32) {
+                float o[32];
+                if (has) {
+                    tmem_ld32(tO + c0 + cb, o);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0.f;
+                }
+                if constexpr (!C::kTwo) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        o[i] = a1 != 0.f ? fmaf(xch[(c0 + cb + i) * 128 + row], a1, o[i] * a0) : o[i] * a0;
+                }
+                if constexpr (C::kFloat) {
+                    if (*special && qrow < live) {
+                        for (int j = max(0, p0 - ctx); j < n && ctx + j < p1; ++j) {
+                            if (!(mk >> j & 1ull)) continue;
+                            int off;
+                            const int pg = page_of(ctx + j, off);
+                            const uint8_t* vr = p.V + (((size_t)pg * p.Hkv + hk) * p.page_rows + off) * C::kRb;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const float v = v_one<KK>(vr, c0 + cb + i);
+                                if (!(fabsf(v) <= 65504.f)) o[i] += v;
+                            }
+                        }
+                    }
+                }
+                if (qrow >= rows_here) continue;
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    float v[8];
+#pragma unroll
+                    for (int d = 0; d < 8; ++d)
+                        v[d] = C::kPairs4 ? o[i + 2 * (d & 3) + (d >> 2)] * tc_v_step<KK>(d & 3) : o[i + d];
+                    const float4 lo = make_float4(v[0], v[1], v[2], v[3]), hi = make_float4(v[4], v[5], v[6], v[7]);
+                    const int c = (c0 + cb + i) / 4;
+                    if (direct) {
+                        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                        store_out(r, c, lo, inv);
+                        store_out(r, c + 1, hi, inv);
+                    } else {
+                        float4* dst = reinterpret_cast<float4*>(p.ws_o + slot * D) + c;
+                        __stcg(dst, lo);
+                        __stcg(dst + 1, hi);
+                    }
+                }
+            }
+            if (!direct && qrow < rows_here && (C::kTwo || w == 0))
+                __stcg(reinterpret_cast<float2*>(p.ws_ml) + slot, make_float2(mx, sum));
+        } else if (qrow < rows_here && (C::kTwo || w == 0)) {
+            // rows past the sequence's nodes
+            if (direct) {
+                for (int c = 0; c < D / 4; ++c) store_out(r, c, make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
+            } else {
+                __stcg(reinterpret_cast<float2*>(p.ws_ml) + ((size_t)stream * p.R + r) * p.S + split, make_float2(kNegMax, 0.f));
+            }
+        }
+    }
+    tc05_fence_before();
+    __syncthreads();
+    if (warp == 16) {
+        tc05_fence_after();
+        tmem_dealloc(tbase, 512);
+    }
+    if (direct) return;
+    unsigned* counter = p.counters + (size_t)stream * p.tiles + tile;
+    if (tid == 0) *s_ticket = atomic_add_acq_rel_gpu(counter, 1u);
+    __syncthreads();
+    if (*s_ticket != (unsigned)(nsplit - 1) || tid >= 512) return;
+    if (tid == 0) store_relaxed_gpu(counter, 0u);
+    tree_merge<D, C::kRows, 512>(p, stream, r0, min(rows_here, live), nsplit, reinterpret_cast<float*>(smem), tid, store_out);
+    for (int i = tid; i < (rows_here - min(rows_here, live)) * (D / 4); i += 512)
+        store_out(r0 + live + i / (D / 4), i % (D / 4), make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
+}
+
+}  // namespace va

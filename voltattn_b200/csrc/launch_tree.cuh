@@ -6,13 +6,14 @@
 #include <mutex>
 
 #include "decode_tree.cuh"
+#include "decode_tree_tc.cuh"
 #include "launch.cuh"
 
 namespace va {
 namespace host {
 
 template <class C>
-int launch_tree_cfg(const TreeParams& p, cudaStream_t st) {
+int launch_tree_cfg(void (*kernel)(const TreeParams), const TreeParams& p, cudaStream_t st) {
     int dev;
     int rc = current_device(&dev);
     if (rc) return rc;
@@ -21,8 +22,7 @@ int launch_tree_cfg(const TreeParams& p, cudaStream_t st) {
     {
         std::lock_guard<std::mutex> lock(mu);
         if (!attr_set[dev]) {
-            VA_CUDA(cudaFuncSetAttribute(decode_tree_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         C::kSmemBytes));
+            VA_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
             attr_set[dev] = true;
         }
     }
@@ -36,15 +36,20 @@ int launch_tree_cfg(const TreeParams& p, cudaStream_t st) {
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    VA_CUDA(cudaLaunchKernelEx(&cfg, decode_tree_kernel<C>, p));
+    VA_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
     return VA_OK;
 }
 
 template <int D>
 int launch_tree_dim(int fmt, const TreeParams& p, int rows, cudaStream_t st) {
-#define VA_TREE_KIND(kind)                                              \
-    return rows == 16 ? launch_tree_cfg<TreeCfg<kind, D, 1>>(p, st)     \
-                      : launch_tree_cfg<TreeCfg<kind, D, 2>>(p, st)
+#define VA_TREE_CFG(kernel, ...) return launch_tree_cfg<__VA_ARGS__>(kernel<__VA_ARGS__>, p, st)
+#define VA_TREE_KIND(kind)                                                                       \
+    do {                                                                                         \
+        if (rows == 16) VA_TREE_CFG(decode_tree_kernel, TreeCfg<kind, D, 1>);                    \
+        if (rows == 32) VA_TREE_CFG(decode_tree_kernel, TreeCfg<kind, D, 2>);                    \
+        if (rows == 128) VA_TREE_CFG(decode_tree_tc_kernel, TreeTcCfg<kind, D, false>);          \
+        VA_TREE_CFG(decode_tree_tc_kernel, TreeTcCfg<kind, D, true>);                            \
+    } while (0)
     switch (fmt) {
         case VA_F16P: VA_TREE_KIND(Kind::F16);
         case VA_BF16P: VA_TREE_KIND(Kind::BF16);
@@ -55,6 +60,7 @@ int launch_tree_dim(int fmt, const TreeParams& p, int rows, cudaStream_t st) {
         default: return VA_ERR_UNSUPPORTED;
     }
 #undef VA_TREE_KIND
+#undef VA_TREE_CFG
 }
 
 }  // namespace host
