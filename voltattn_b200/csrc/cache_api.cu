@@ -57,20 +57,21 @@ int tree_rows(int R) {
 constexpr long long kCounters = 16384;
 constexpr size_t kCounterBytes = kCounters * sizeof(unsigned);
 
-// The splits that fill the device in the fewest rows a CTA has to take: cost =
-// waves * (rows of a split + a CTA's fixed work in rows), smallest S first.
+// The splits with the least cost: the CTAs' rows (of sequences that fill 5/8 of
+// their tables on average, plus a CTA's fixed work in rows) shared by the device's
+// slots, and half of the longest range for the uneven end; smallest S first.
 int tree_splits(int nsm, int B, int Hkv, int R, int Lmax) {
     const int rows = tree_rows(R);
-    const long long ctas = (long long)B * Hkv * ((R + rows - 1) / rows);
-    if (ctas > kCounters) return 1;
-    const long long cap = (long long)nsm * (rows == 16 ? 3 : rows == 32 ? 2 : 1);
-    const int most = std::max(1, std::min(kMaxSplits, (Lmax + kTreeUnit - 1) / kTreeUnit));
+    const double ctas = (double)B * Hkv * ((R + rows - 1) / rows);
+    if (ctas > (double)kCounters) return 1;
+    const double cap = (double)nsm * (rows == 16 ? 3 : rows == 32 ? 2 : 1);
+    const double fixed = rows <= 32 ? 128.0 : 384.0;
+    const int units = (Lmax + kTreeUnit - 1) / kTreeUnit;
     double best = 1e300;
     int S = 1;
-    for (int s = 1; s <= most; ++s) {
-        const int units = (Lmax + kTreeUnit - 1) / kTreeUnit;
+    for (int s = 1; s <= std::min(kMaxSplits, units); ++s) {
         const double chunk = (double)((units + s - 1) / s) * kTreeUnit;
-        const double cost = (double)((ctas * s + cap - 1) / cap) * (chunk + 192.0) + 2.0 * s;
+        const double cost = std::max(1.0, ctas * s / cap) * (0.625 * chunk + fixed) + 0.5 * chunk;
         if (cost < best - 1e-9) {
             best = cost;
             S = s;

@@ -3,10 +3,12 @@
 // query rows, with tcgen05.mma and accumulators in tensor memory.
 //
 // One CTA per (sequence, KV head, tile of query rows, range of positions), one
-// per SM, 17 warps:
+// per SM, 14 warps (4 on an SM sub-partition at most: 128 registers a thread, which hold
+// a row's 64 scores; with 18 warps and 96 registers the spills took half of the time):
 //   warps 0-3, 4-7  two softmax warpgroups; thread r owns query row r (TMEM lane r);
-//   warps 8-15      producers: codes -> exact fp16 codes in swizzled tiles;
-//   warp 16         one thread issues every tcgen05.mma.
+//   warps 8-11      producers: codes -> exact fp16 codes in swizzled tiles;
+//   warp 12         one thread issues every tcgen05.mma;
+//   warp 13         copies blocks of codes and scales into a ring, several ahead.
 // A job is one warpgroup's work on one block of 64 positions. kTwo = false (up
 // to 128 query rows): the warpgroups take the blocks in turn, each with its own
 // O and statistics, merged at the end. kTwo = true (up to 256): both take every
@@ -46,25 +48,37 @@ struct TreeTcCfg {
     static constexpr int kSG = kScaled ? kNG : 1;  // score accumulators, weight copies
     static constexpr int kRb = kDim * KindTraits<K>::kBits / 8;
     static constexpr int kNb = 64;                 // positions of a block
-    static constexpr int kProducers = 256;
-    static constexpr int kThreads = 17 * 32;
+    static constexpr int kProducers = 128;
+    static constexpr int kThreads = 14 * 32;
     static constexpr int kQTile = 128 * kDim * 2;
     static constexpr int kTile = kNb * kDim * 2;   // one K or V tile
     static constexpr int kPTile = 128 * kNb * 2;
-    static constexpr int kKS = 3;
-    static constexpr int kVS = (kTwoTiles && kScaled && kDim == 128) ? 2 : 3;
+    static constexpr int kKS = 2;
+    // (two tiles of query rows and blocks of 8 bits or more: room for one V tile)
+    static constexpr int kVS = kTwoTiles && kDim == 128 && KindTraits<K>::kBits >= 8 ? 1 : 2;
     static constexpr int kOffP = (kTwoTiles ? 2 : 1) * kQTile;
     static constexpr int kOffK = kOffP + 2 * kSG * kPTile;
     static constexpr int kOffV = kOffK + kKS * kTile;
-    static constexpr int kOffScales = kOffV + kVS * kTile;     // [4 slots][K, V][kNG][64] floats
+    static constexpr int kOffRaw = kOffV + kVS * kTile;        // ring of blocks as they lie in the cache
+    static constexpr int kSb = kScaled ? 2 * kNG : 0;
+    static constexpr int kRawV = kNb * kRb, kRawSK = 2 * kNb * kRb, kRawSV = kRawSK + kNb * kSb;
+    static constexpr int kRawTx = kRawSV + kNb * kSb;
+    static constexpr int kRawStage = (kRawTx + 127) / 128 * 128;
+    // what follows the ring: scales as floats [4 slots][K, V][kNG][64], masks, [2][128]
+    // (reference, sum), barriers, ev[4], TMEM slot, fail, special, ticket
     static constexpr int kScaleSlots = 4;
-    static constexpr int kOffMask = kOffScales + (kScaled ? kScaleSlots * 2 * kNG * kNb * 4 : 0);
-    static constexpr int kOffMl = kOffMask + kRows * 8;        // [2][128] (reference, sum)
+    static constexpr int kScaleBytes = kScaled ? kScaleSlots * 2 * kNG * kNb * 4 : 0;
+    static constexpr int kRest = kScaleBytes + kRows * 8 + 2 * 128 * 8 + 512 + 64;
+    static constexpr int kRoom = (227 * 1024 - 1024 - kOffRaw - kRest) / kRawStage;
+    static constexpr int kRawStages = kRoom < 8 ? kRoom : 8;
+    static constexpr int kOffScales = kOffRaw + kRawStages * kRawStage;
+    static constexpr int kOffMask = kOffScales + kScaleBytes;
+    static constexpr int kOffMl = kOffMask + kRows * 8;
     static constexpr int kOffBars = kOffMl + 2 * 128 * 8;
-    static constexpr int kBars = 2 * kKS + 2 * kVS + 2 * 4 + 1 + kScaleSlots;
-    static constexpr int kOffMisc = kOffBars + kBars * 8;      // ev[4], TMEM slot, fail, special, ticket
+    static constexpr int kBars = 2 * kKS + 2 * kVS + 2 * 4 + 1 + kScaleSlots + 2 * kRawStages;
+    static constexpr int kOffMisc = kOffBars + kBars * 8;
     static constexpr int kSmemBytes = 1024 + kOffMisc + 64;
-    static constexpr int kPrefetch = 6;                        // blocks ahead into L2
+    static_assert(kRawStages >= 2 && kBars * 8 <= 512, "two blocks in flight");
     static_assert(kSmemBytes <= 227 * 1024, "one CTA per SM");
 };
 
@@ -80,7 +94,7 @@ __host__ __device__ constexpr float tc_v_step(int p) {
                          : K == Kind::Q3 ? (p == 1 ? 128.f : p == 2 ? 16.f : 1024.f) : 1.f;
 }
 
-// The codes of kDim / 4 consecutive dims of one row (quarter q).
+// The codes of kDim / 4 consecutive dims of one row in shared memory (quarter q).
 template <Kind K, int kDim>
 struct TcRaw {
     static constexpr int kDims = kDim / 4;
@@ -95,21 +109,21 @@ __device__ __forceinline__ void tc_load(TcRaw<K, kDim>& r, const uint8_t* row, i
         // 12 bytes of 4-byte alignment, or the two words around 6
         const uint32_t* p = reinterpret_cast<const uint32_t*>(row + ((q * kBytes) & ~3));
 #pragma unroll
-        for (int i = 0; i < TcRaw<K, kDim>::kWords; ++i) r.w[i] = __ldg(p + i);
+        for (int i = 0; i < TcRaw<K, kDim>::kWords; ++i) r.w[i] = p[i];
         if constexpr (kBytes == 6) {
             const uint32_t sh = (q & 1) * 16;
             r.w[0] = __funnelshift_r(r.w[0], r.w[1], sh);
             r.w[1] >>= sh;
         }
     } else if constexpr (kBytes == 8) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(row) + q);
+        const uint2 v = reinterpret_cast<const uint2*>(row)[q];
         r.w[0] = v.x;
         r.w[1] = v.y;
     } else {
         const uint4* p = reinterpret_cast<const uint4*>(row) + q * (kBytes / 16);
 #pragma unroll
         for (int i = 0; i < kBytes / 16; ++i) {
-            const uint4 v = __ldg(p + i);
+            const uint4 v = p[i];
             r.w[4 * i] = v.x;
             r.w[4 * i + 1] = v.y;
             r.w[4 * i + 2] = v.z;
@@ -203,8 +217,12 @@ __device__ __forceinline__ void tmem_tie16(uint32_t* r) {
                    "+r"(r[15]));
 }
 
-__device__ __forceinline__ void prefetch_l2(const void* src, uint32_t bytes) {
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+// Four floats of shared memory. Not volatile: the compiler may move the load over
+// stores (the caller's address comes out of a statement that follows the wait).
+__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
+    float4 v;
+    asm("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+    return v;
 }
 
 // Clears the entries of eight fp16 values that are not finite; true if there were any.
@@ -223,7 +241,8 @@ __device__ __forceinline__ bool clear_not_finite(uint4& v) {
 template <class C>
 __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const TreeParams p) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    // (an offset, not a rounded address: the compiler keeps seeing shared memory)
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     constexpr int D = C::kD, NG = C::kNG, NB = C::kNb, KS = C::kKS, VS = C::kVS, SG = C::kSG;
     constexpr Kind KK = C::kKind;
     unsigned long long* s_mask = reinterpret_cast<unsigned long long*>(smem + C::kOffMask);
@@ -231,6 +250,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
     uint64_t *kempty = kfull + KS, *vfull = kempty + KS, *vempty = vfull + VS, *sfull = vempty + VS;
     uint64_t *sempty = sfull + 2, *pfull = sempty + 2, *odone = pfull + 2, *fin = odone + 2, *scfull = fin + 1;
+    uint64_t *rfull = scfull + C::kScaleSlots, *rempty = rfull + C::kRawStages;
     float* s_ev = reinterpret_cast<float*>(smem + C::kOffMisc);
     uint32_t* tslot = reinterpret_cast<uint32_t*>(s_ev + 4);
     volatile int* fail = reinterpret_cast<volatile int*>(tslot + 1);
@@ -273,7 +293,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
 
     const int nblk = (p1 - p0 + NB - 1) / NB;
     const int njobs = C::kTwo ? 2 * nblk : nblk;
-    if (warp == 16) tmem_alloc(tslot, 512);
+    if (warp == 12) tmem_alloc(tslot, 512);
     if (tid == 0) {
         for (int i = 0; i < KS; ++i) mbar_init(kfull + i, C::kProducers / 32), mbar_init(kempty + i, 1);
         for (int i = 0; i < VS; ++i) mbar_init(vfull + i, C::kProducers / 32), mbar_init(vempty + i, 1);
@@ -281,6 +301,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
             mbar_init(sfull + i, 1), mbar_init(sempty + i, 4), mbar_init(pfull + i, 4), mbar_init(odone + i, 1);
         mbar_init(fin, 1);
         for (int i = 0; i < C::kScaleSlots; ++i) mbar_init(scfull + i, 1);
+        for (int i = 0; i < C::kRawStages; ++i) mbar_init(rfull + i, 1), mbar_init(rempty + i, C::kProducers / 32);
         *fail = 0;
         *special = 0;
         fence_mbar_init();
@@ -292,24 +313,6 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
         const int pg = pi < p.max_pages ? __ldg(trow + pi) : 0;
         return (unsigned)pg < (unsigned)p.num_pages ? pg : 0;
     };
-    // L2 prefetch of block i by one warp: lane = buffer + 4 * run of 8 rows (or the
-    // whole block in one run)
-    const bool whole = p.page_rows % NB == 0;
-    const auto prefetch = [&](int i) {
-        const int buf = lane & 3, run = whole ? NB : 8, at = (lane >> 2) * run;
-        const int rb = buf < 2 ? C::kRb : 2 * NG;
-        if (at >= NB || (buf >= 2 && !C::kScaled)) return;
-        int off;
-        const int pg = page_of(p0 + i * NB + at, off);
-        const uint8_t* base = buf == 0   ? p.K
-                              : buf == 1 ? p.V
-                              : buf == 2 ? reinterpret_cast<const uint8_t*>(p.scK)
-                                         : reinterpret_cast<const uint8_t*>(p.scV);
-        prefetch_l2(base + (((size_t)pg * p.Hkv + hk) * p.page_rows + off) * rb, (uint32_t)(run * rb));
-    };
-    if (warp >= 8 && warp < 16)
-        for (int i = warp - 8; i < min(C::kPrefetch, nblk); i += 8) prefetch(i);
-
     // the query rows into shared memory in the tiles' order of dims, and their masks
     for (int i = tid; i < C::kRows * (D / 8); i += C::kThreads) {
         const int row = i / (D / 8), c = i - row * (D / 8);
@@ -351,7 +354,6 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
         for (int k = 0; k < jobs; ++k) {
             const int blk = C::kTwo ? k : 2 * k + w;
             const int pb = p0 + blk * NB;
-            const float* sc = reinterpret_cast<const float*>(smem + C::kOffScales) + (blk % C::kScaleSlots) * 2 * NG * NB;
             bool ok = mbar_wait_fast(sfull + w, (uint32_t)k & 1u);
             // (a slot of scales is written again only after this block's PV, so this phase
             // cannot be passed twice before it is seen here)
@@ -363,6 +365,8 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                 break;
             }
             tc05_fence_after();
+            uint32_t sc = sbase + C::kOffScales + (blk % C::kScaleSlots) * 2 * NG * NB * 4;
+            asm volatile("" : "+r"(sc));  // the loads of scales come after the waits
             float x[NB];
             if (!idle) {
 #pragma unroll
@@ -378,11 +382,11 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                         float2 a = make_float2(__uint_as_float(s[0][j]), __uint_as_float(s[0][j + 1]));
                         float2 c = make_float2(__uint_as_float(s[0][j + 2]), __uint_as_float(s[0][j + 3]));
                         if constexpr (C::kScaled) {
-                            const float4 k0 = *reinterpret_cast<const float4*>(sc + cb + j);
+                            const float4 k0 = lds_f4(sc + 4 * (cb + j));
                             a = fmul2(a, make_float2(k0.x, k0.y));
                             c = fmul2(c, make_float2(k0.z, k0.w));
                             if constexpr (NG == 2) {
-                                const float4 k1 = *reinterpret_cast<const float4*>(sc + NB + cb + j);
+                                const float4 k1 = lds_f4(sc + 4 * (NB + cb + j));
                                 a = ffma2(make_float2(__uint_as_float(s[SG - 1][j]), __uint_as_float(s[SG - 1][j + 1])),
                                           make_float2(k1.x, k1.y), a);
                                 c = ffma2(make_float2(__uint_as_float(s[SG - 1][j + 2]), __uint_as_float(s[SG - 1][j + 3])),
@@ -449,47 +453,52 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                 }
                 m_ref = nref;
                 float2 sum = make_float2(0.f, 0.f);
-                const float2 sc2 = make_float2(c2, c2), nm = make_float2(-nref, -nref);
+                // (two instantiations: only blocks with drafted rows or the end select)
+                const auto weights = [&](auto is_tail) {
+                    const float2 sc2 = make_float2(c2, c2), nm = make_float2(-nref, -nref);
 #pragma unroll
-                for (int j = 0; j < NB; j += 8) {
-                    float2 e[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 y = ffma2(make_float2(x[j + 2 * i], x[j + 2 * i + 1]), sc2, nm);
-                        e[i] = make_float2(fast_exp2(y.x), fast_exp2(y.y));
-                        if (tail) {
-                            if (!(vis >> (j + 2 * i) & 1ull)) e[i].x = 0.f;
-                            if (!(vis >> (j + 2 * i + 1) & 1ull)) e[i].y = 0.f;
-                        }
-                        sum = fadd2(sum, e[i]);
-                    }
-#pragma unroll
-                    for (int g = 0; g < SG; ++g) {
-                        uint32_t h[4];
-                        float2 v[4];
-                        if constexpr (C::kScaled) {
-                            const float4 v0 = *reinterpret_cast<const float4*>(sc + (NG + g) * NB + j);
-                            const float4 v1 = *reinterpret_cast<const float4*>(sc + (NG + g) * NB + j + 4);
-                            v[0] = fmul2(e[0], make_float2(v0.x, v0.y));
-                            v[1] = fmul2(e[1], make_float2(v0.z, v0.w));
-                            v[2] = fmul2(e[2], make_float2(v1.x, v1.y));
-                            v[3] = fmul2(e[3], make_float2(v1.z, v1.w));
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) v[i] = e[i];
-                        }
+                    for (int j = 0; j < NB; j += 8) {
+                        float2 e[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            if (C::kScaled && tail) {  // an unseen row's scale may be nan
-                                if (!(vis >> (j + 2 * i) & 1ull)) v[i].x = 0.f;
-                                if (!(vis >> (j + 2 * i + 1) & 1ull)) v[i].y = 0.f;
+                            const float2 y = ffma2(make_float2(x[j + 2 * i], x[j + 2 * i + 1]), sc2, nm);
+                            e[i] = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+                            if constexpr (decltype(is_tail)::value) {
+                                if (!(vis >> (j + 2 * i) & 1ull)) e[i].x = 0.f;
+                                if (!(vis >> (j + 2 * i + 1) & 1ull)) e[i].y = 0.f;
                             }
-                            h[i] = h2_bits(__floats2half2_rn(v[i].x, v[i].y));
+                            sum = fadd2(sum, e[i]);
                         }
-                        *reinterpret_cast<uint4*>(sP + g * C::kPTile + (((j >> 3) ^ (row & 7)) << 4)) =
-                            make_uint4(h[0], h[1], h[2], h[3]);
+#pragma unroll
+                        for (int g = 0; g < SG; ++g) {
+                            uint32_t h[4];
+                            float2 v[4];
+                            if constexpr (C::kScaled) {
+                                const float4 v0 = lds_f4(sc + 4 * ((NG + g) * NB + j));
+                                const float4 v1 = lds_f4(sc + 4 * ((NG + g) * NB + j + 4));
+                                v[0] = fmul2(e[0], make_float2(v0.x, v0.y));
+                                v[1] = fmul2(e[1], make_float2(v0.z, v0.w));
+                                v[2] = fmul2(e[2], make_float2(v1.x, v1.y));
+                                v[3] = fmul2(e[3], make_float2(v1.z, v1.w));
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) v[i] = e[i];
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if constexpr (C::kScaled && decltype(is_tail)::value) {  // an unseen row's scale may be nan
+                                    if (!(vis >> (j + 2 * i) & 1ull)) v[i].x = 0.f;
+                                    if (!(vis >> (j + 2 * i + 1) & 1ull)) v[i].y = 0.f;
+                                }
+                                h[i] = h2_bits(__floats2half2_rn(v[i].x, v[i].y));
+                            }
+                            *reinterpret_cast<uint4*>(sP + g * C::kPTile + (((j >> 3) ^ (row & 7)) << 4)) =
+                                make_uint4(h[0], h[1], h[2], h[3]);
+                        }
                     }
-                }
+                };
+                if (tail) weights(std::true_type{});
+                else weights(std::false_type{});
                 l_sum += sum.x + sum.y;
                 fence_proxy_async_smem();
             }
@@ -502,70 +511,49 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
             *fail = 1;
         }
         tc05_fence_after();
-    } else if (warp < 16) {
-        // ---- producers: thread = (row of the block, quarter of the dims) -------------
+    } else if (warp < 12) {
+        // ---- producers: K of block i + 1 before V of block i, so the next scores never
+        // wait for this block's PV. A thread takes two slices (row, quarter of the dims) -----
         const int pw = warp - 8;
         // lane bits: quarter bit 0, row bits 0..1, quarter bit 1, row bit 2: eight
         // neighbouring lanes store to eight different 16-byte banks
-        const int q = (lane & 1) | ((lane >> 2) & 2), row = pw * 8 + ((lane >> 1) & 3) + ((lane >> 4) << 2);
+        const int q = (lane & 1) | ((lane >> 2) & 2), row0 = pw * 16 + ((lane >> 1) & 3) + ((lane >> 4) << 2);
         using Raw = TcRaw<KK, D>;
         constexpr int kChunks = Raw::kDims / 8;
-        Raw rk, rv, nk, nv;
-        const auto load = [&](int i, Raw& a, Raw& c) {
-            int off;
-            const int pg = page_of(p0 + i * NB + row, off);
-            const size_t r = ((size_t)pg * p.Hkv + hk) * p.page_rows + off;
-            tc_load<KK, D>(a, p.K + r * C::kRb, q);
-            tc_load<KK, D>(c, p.V + r * C::kRb, q);
-        };
-        const auto put = [&](uint8_t* dst, int j, uint4 v) {
+        const auto put = [&](uint8_t* dst, int row, int j, uint4 v) {
             const int c = q * kChunks + j;
             *reinterpret_cast<uint4*>(dst + (c >> 3) * (NB * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
         };
-        load(0, rk, rv);
-        for (int i = 0; i < nblk; ++i) {
-            const int pb = p0 + i * NB;
-            if (pw == (i & 7) && i + C::kPrefetch < nblk) prefetch(i + C::kPrefetch);
-            if (i + 1 < nblk) load(i + 1, nk, nv);
-            // scales of the block: warp i % 8, two positions a lane
-            uint32_t ks[2], vs[2];
-            const bool scales = C::kScaled && pw == ((i + 4) & 7);
-            if (scales) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    int off;
-                    const int pg = page_of(pb + lane + 32 * e, off);
-                    const size_t r = ((size_t)pg * p.Hkv + hk) * p.page_rows + off;
-                    if constexpr (NG == 2) {
-                        ks[e] = __ldg(reinterpret_cast<const uint32_t*>(p.scK) + r);
-                        vs[e] = __ldg(reinterpret_cast<const uint32_t*>(p.scV) + r);
-                    } else {
-                        ks[e] = __ldg(reinterpret_cast<const uint16_t*>(p.scK) + r);
-                        vs[e] = __ldg(reinterpret_cast<const uint16_t*>(p.scV) + r);
-                    }
-                }
-            }
-            const int u = i / KS, x = i / VS;
-            if (u > 0 && !mbar_wait_bounded(kempty + i % KS, (uint32_t)(u - 1) & 1u)) {
-                if (lane == 0) report_error(kErrEmptyWait);
-                *fail = 1;
-                break;
-            }
-            if (scales) {
+        const auto raw_of = [&](int i) { return smem + C::kOffRaw + (i % C::kRawStages) * C::kRawStage; };
+        const auto make_k = [&](int i) {
+            const int u = i / KS;
+            if (!mbar_wait_bounded(rfull + i % C::kRawStages, (uint32_t)(i / C::kRawStages) & 1u)) return false;
+            const uint8_t* raw = raw_of(i);
+            if (u > 0 && !mbar_wait_bounded(kempty + i % KS, (uint32_t)(u - 1) & 1u)) return false;
+            if (C::kScaled && pw == (i & 3)) {  // the block's scales: two positions a lane
                 float* sc = reinterpret_cast<float*>(smem + C::kOffScales) + (i % C::kScaleSlots) * 2 * NG * NB;
                 __half2 big = __float2half2_rn(0.f);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float2 fk = __half22float2(bits_h2(ks[e])), fv = __half22float2(bits_h2(vs[e]));
-                    sc[lane + 32 * e] = fk.x;
-                    sc[NG * NB + lane + 32 * e] = fv.x;
+                    const int at = lane + 32 * e;
+                    uint32_t ks, vs;
                     if constexpr (NG == 2) {
-                        sc[NB + lane + 32 * e] = fk.y;
-                        sc[3 * NB + lane + 32 * e] = fv.y;
+                        ks = reinterpret_cast<const uint32_t*>(raw + C::kRawSK)[at];
+                        vs = reinterpret_cast<const uint32_t*>(raw + C::kRawSV)[at];
+                    } else {
+                        ks = reinterpret_cast<const uint16_t*>(raw + C::kRawSK)[at];
+                        vs = reinterpret_cast<const uint16_t*>(raw + C::kRawSV)[at];
+                    }
+                    const float2 fk = __half22float2(bits_h2(ks)), fv = __half22float2(bits_h2(vs));
+                    sc[at] = fk.x;
+                    sc[NG * NB + at] = fv.x;
+                    if constexpr (NG == 2) {
+                        sc[NB + at] = fk.y;
+                        sc[3 * NB + at] = fv.y;
                     }
                     // rows past the end and scales that are not finite are no measure
-                    uint32_t a = vs[e] & 0x7FFF7FFFu;
-                    if (pb + lane + 32 * e >= len) a = 0u;
+                    uint32_t a = vs & 0x7FFF7FFFu;
+                    if (p0 + i * NB + at >= len) a = 0u;
                     if ((a & 0x7FFFu) >= 0x7C00u) a &= 0x7FFF0000u;
                     if ((a >> 16) >= 0x7C00u) a &= 0x7FFFu;
                     big = __hmax2(big, bits_h2(a));
@@ -579,35 +567,91 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                 }
             }
             uint8_t* kt = smem + C::kOffK + (i % KS) * C::kTile;
+            Raw r[2];
 #pragma unroll
-            for (int j = 0; j < kChunks; ++j) put(kt, j, tc_convert<KK, D, false>(rk, j));
+            for (int h = 0; h < 2; ++h) tc_load<KK, D>(r[h], raw + (row0 + 8 * h) * C::kRb, q);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < kChunks; ++j) put(kt, row0 + 8 * h, j, tc_convert<KK, D, false>(r[h], j));
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(kfull + i % KS);
-            if (x > 0 && !mbar_wait_bounded(vempty + i % VS, (uint32_t)(x - 1) & 1u)) {
-                if (lane == 0) report_error(kErrEmptyWait);
-                *fail = 1;
-                break;
-            }
-            uint8_t* vt = smem + C::kOffV + (i % VS) * C::kTile;
-            const int pos = pb + row;
+            return true;
+        };
+        const auto make_v = [&](int i) {
+            const int x = i / VS;
+            const uint8_t* raw = raw_of(i) + C::kRawV;
+            Raw r[2];
 #pragma unroll
-            for (int j = 0; j < kChunks; ++j) {
-                uint4 v = tc_convert<KK, D, true>(rv, j);
-                if constexpr (C::kFloat) {
-                    // rows past the end are cleared; entries of drafted rows that are not finite
-                    // are left to the epilogue, which adds them to the rows that see them
-                    if (pos >= len) v = make_uint4(0u, 0u, 0u, 0u);
-                    else if (pos >= ctx && clear_not_finite(v)) *special = 1;
+            for (int h = 0; h < 2; ++h) tc_load<KK, D>(r[h], raw + (row0 + 8 * h) * C::kRb, q);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(rempty + i % C::kRawStages);
+            if (x > 0 && !mbar_wait_bounded(vempty + i % VS, (uint32_t)(x - 1) & 1u)) return false;
+            uint8_t* vt = smem + C::kOffV + (i % VS) * C::kTile;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int pos = p0 + i * NB + row0 + 8 * h;
+#pragma unroll
+                for (int j = 0; j < kChunks; ++j) {
+                    uint4 v = tc_convert<KK, D, true>(r[h], j);
+                    if constexpr (C::kFloat) {
+                        // rows past the end are cleared; entries of drafted rows that are not finite
+                        // are left to the epilogue, which adds them to the rows that see them
+                        if (pos >= len) v = make_uint4(0u, 0u, 0u, 0u);
+                        else if (pos >= ctx && clear_not_finite(v)) *special = 1;
+                    }
+                    put(vt, row0 + 8 * h, j, v);
                 }
-                put(vt, j, v);
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(vfull + i % VS);
-            rk = nk;
-            rv = nv;
+            return true;
+        };
+        bool ok = make_k(0);
+        for (int i = 0; ok && i < nblk; ++i) {
+            if (i + 1 < nblk) ok = make_k(i + 1);
+            ok = ok && make_v(i);
         }
+        if (!ok) {
+            if (lane == 0) report_error(kErrEmptyWait);
+            *fail = 1;
+        }
+    } else if (warp == 13) {
+        // ---- copies: lane 4 r + k brings run r of buffer k (K, V, their scales): the
+        // whole block when it lies inside a page, else runs of 8 rows
+        const bool whole = p.page_rows % NB == 0;
+        const int run = whole ? NB : 8, nrun = NB / run, buf = lane & 3, at = (lane >> 2) * run;
+        const int rb = buf < 2 ? C::kRb : C::kSb;
+        const uint32_t bytes = (uint32_t)(run * rb);
+        const bool copies = lane < 4 * nrun && bytes > 0;
+        const uint8_t* src = buf == 0   ? p.K
+                             : buf == 1 ? p.V
+                             : buf == 2 ? reinterpret_cast<const uint8_t*>(p.scK)
+                                        : reinterpret_cast<const uint8_t*>(p.scV);
+        const int dst = C::kOffRaw + (buf == 0 ? 0 : buf == 1 ? C::kRawV : buf == 2 ? C::kRawSK : C::kRawSV) + at * rb;
+        const uint64_t policy = l2_policy_evict_first();
+        int i = 0;
+        for (; i < nblk; ++i) {
+            const int rs = i % C::kRawStages, u = i / C::kRawStages;
+            if (u > 0 && !mbar_wait_bounded(rempty + rs, (uint32_t)(u - 1) & 1u)) {
+                if (lane == 0) report_error(kErrEmptyWait);
+                *fail = 1;
+                break;
+            }
+            if (lane == 0) mbar_arrive_expect_tx(rfull + rs, C::kRawTx);
+            __syncwarp();
+            if (copies) {
+                int off;
+                const int pg = page_of(p0 + i * NB + at, off);
+                bulk_g2s(smem + dst + rs * C::kRawStage, src + (((size_t)pg * p.Hkv + hk) * p.page_rows + off) * rb, bytes,
+                         rfull + rs, policy);
+            }
+        }
+        // the copies in flight land (bounded) before the shared memory is given back
+        for (int k = max(0, i - C::kRawStages); k < i; ++k)
+            if (!mbar_wait_bounded(rfull + k % C::kRawStages, (uint32_t)(k / C::kRawStages) & 1u)) *fail = 1;
     } else if (lane == 0) {
         // ---- the MMA thread ----------------------------------------------------------
         constexpr uint32_t kIdescS = umma_idesc_f16(128, NB, false);
@@ -662,7 +706,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     __syncthreads();
     tc05_fence_after();
     if (*fail) {
-        if (warp == 16) tmem_dealloc(tbase, 512);
+        if (warp == 12) tmem_dealloc(tbase, 512);
         return;
     }
     grid_launch_dependents();
@@ -762,7 +806,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     }
     tc05_fence_before();
     __syncthreads();
-    if (warp == 16) {
+    if (warp == 12) {
         tc05_fence_after();
         tmem_dealloc(tbase, 512);
     }
@@ -770,10 +814,10 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     unsigned* counter = p.counters + (size_t)stream * p.tiles + tile;
     if (tid == 0) *s_ticket = atomic_add_acq_rel_gpu(counter, 1u);
     __syncthreads();
-    if (*s_ticket != (unsigned)(nsplit - 1) || tid >= 512) return;
+    if (*s_ticket != (unsigned)(nsplit - 1)) return;
     if (tid == 0) store_relaxed_gpu(counter, 0u);
-    tree_merge<D, C::kRows, 512>(p, stream, r0, min(rows_here, live), nsplit, reinterpret_cast<float*>(smem), tid, store_out);
-    for (int i = tid; i < (rows_here - min(rows_here, live)) * (D / 4); i += 512)
+    tree_merge<D, C::kRows, C::kThreads>(p, stream, r0, min(rows_here, live), nsplit, reinterpret_cast<float*>(smem), tid, store_out);
+    for (int i = tid; i < (rows_here - min(rows_here, live)) * (D / 4); i += C::kThreads)
         store_out(r0 + live + i / (D / 4), i % (D / 4), make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
 }
 
