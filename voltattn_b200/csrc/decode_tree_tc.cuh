@@ -14,13 +14,17 @@
 // O and statistics, merged at the end. kTwo = true (up to 256): both take every
 // block, for query rows 0..127 and 128..255, so a decoded tile serves twice.
 //
-// Per job j (MMA order S(0) S(1), then S(j + 2) PV(j)):
+// Per job j (MMA order S(0) S(1), then PV(j) S(j + 2)):
 //   S_g = Q_g K_g^T (M = 128 rows, N = 64 positions) for each 64-dim group g, in
 //     TMEM. The K tile holds the exact codes (times a power of two), so the group
 //     scales multiply fp32 scores, as in decode_tree.cuh;
-//   the softmax thread loads its row's scores, x = S_0 k_0 + S_1 k_1, hands the
-//     S columns back, and writes P'_g = fp16(w v_g) into shared memory;
-//   O_g += P'_g V_g (A = P' from shared memory, B = the V tile read MN-major).
+//   the softmax thread loads its row's scores, x = S_0 k_0 + S_1 k_1, and writes
+//     P'_g = fp16(w v_g) over them;
+//   O_g += P'_g V_g (A = P' read from TMEM, B = the V tile read MN-major).
+// The MMAs of one thread execute in issue order, so S(j + 2) follows PV(j) into the
+// same columns, and a completed S implies every earlier PV of its warpgroup. Shared
+// memory's bandwidth is what bounds the kernel (A operands and weights read from it
+// took 2840 cycles a block against ... with P' in TMEM).
 // O is rescaled only when a row's reference grows by more than 4 (log2): P' of the
 // largest weight stays in [2^6, 2^15), its rounding relative.
 //
@@ -52,12 +56,9 @@ struct TreeTcCfg {
     static constexpr int kThreads = 14 * 32;
     static constexpr int kQTile = 128 * kDim * 2;
     static constexpr int kTile = kNb * kDim * 2;   // one K or V tile
-    static constexpr int kPTile = 128 * kNb * 2;
     static constexpr int kKS = 2;
-    // (two tiles of query rows and blocks of 8 bits or more: room for one V tile)
-    static constexpr int kVS = kTwoTiles && kDim == 128 && KindTraits<K>::kBits >= 8 ? 1 : 2;
-    static constexpr int kOffP = (kTwoTiles ? 2 : 1) * kQTile;
-    static constexpr int kOffK = kOffP + 2 * kSG * kPTile;
+    static constexpr int kVS = 2;
+    static constexpr int kOffK = (kTwoTiles ? 2 : 1) * kQTile;
     static constexpr int kOffV = kOffK + kKS * kTile;
     static constexpr int kOffRaw = kOffV + kVS * kTile;        // ring of blocks as they lie in the cache
     static constexpr int kSb = kScaled ? 2 * kNG : 0;
@@ -75,7 +76,7 @@ struct TreeTcCfg {
     static constexpr int kOffMask = kOffScales + kScaleBytes;
     static constexpr int kOffMl = kOffMask + kRows * 8;
     static constexpr int kOffBars = kOffMl + 2 * 128 * 8;
-    static constexpr int kBars = 2 * kKS + 2 * kVS + 2 * 4 + 1 + kScaleSlots + 2 * kRawStages;
+    static constexpr int kBars = 2 * kKS + 2 * kVS + 2 * 2 + 2 + kScaleSlots + 2 * kRawStages;
     static constexpr int kOffMisc = kOffBars + kBars * 8;
     static constexpr int kSmemBytes = 1024 + kOffMisc + 64;
     static_assert(kRawStages >= 2 && kBars * 8 <= 512, "two blocks in flight");
@@ -217,6 +218,20 @@ __device__ __forceinline__ void tmem_tie16(uint32_t* r) {
                    "+r"(r[15]));
 }
 
+// True in one lane of the (converged) warp. The values around it stay warp-uniform,
+// so the operands of the MMAs need no move from vector to uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
+}
+
+__device__ __forceinline__ void tmem_st8_u(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
 // Four floats of shared memory. Not volatile: the compiler may move the load over
 // stores (the caller's address comes out of a statement that follows the wait).
 __device__ __forceinline__ float4 lds_f4(uint32_t addr) {
@@ -249,7 +264,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     float2* s_ml = reinterpret_cast<float2*>(smem + C::kOffMl);
     uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
     uint64_t *kempty = kfull + KS, *vfull = kempty + KS, *vempty = vfull + VS, *sfull = vempty + VS;
-    uint64_t *sempty = sfull + 2, *pfull = sempty + 2, *odone = pfull + 2, *fin = odone + 2, *scfull = fin + 1;
+    uint64_t *pfull = sfull + 2, *odone = pfull + 2, *fin = odone + 1, *scfull = fin + 1;
     uint64_t *rfull = scfull + C::kScaleSlots, *rempty = rfull + C::kRawStages;
     float* s_ev = reinterpret_cast<float*>(smem + C::kOffMisc);
     uint32_t* tslot = reinterpret_cast<uint32_t*>(s_ev + 4);
@@ -298,7 +313,8 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
         for (int i = 0; i < KS; ++i) mbar_init(kfull + i, C::kProducers / 32), mbar_init(kempty + i, 1);
         for (int i = 0; i < VS; ++i) mbar_init(vfull + i, C::kProducers / 32), mbar_init(vempty + i, 1);
         for (int i = 0; i < 2; ++i)
-            mbar_init(sfull + i, 1), mbar_init(sempty + i, 4), mbar_init(pfull + i, 4), mbar_init(odone + i, 1);
+            mbar_init(sfull + i, 1), mbar_init(pfull + i, 4);
+        mbar_init(odone, 1);
         mbar_init(fin, 1);
         for (int i = 0; i < C::kScaleSlots; ++i) mbar_init(scfull + i, 1);
         for (int i = 0; i < C::kRawStages; ++i) mbar_init(rfull + i, 1), mbar_init(rempty + i, C::kProducers / 32);
@@ -348,7 +364,6 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
         const int jobs = C::kTwo ? nblk : (nblk - w + 1) / 2;
         const bool idle = (C::kTwo ? w * 128 : 0) + (warp & 3) * 32 >= live;  // no row of this warp is live
         const uint32_t tS = tbase + w * 256 + ((uint32_t)((warp & 3) * 32) << 16), tO = tS + 128;
-        uint8_t* sP = smem + C::kOffP + w * SG * C::kPTile + row * 128;
         const float c2 = rsqrtf((float)D) * kLog2e * tc_k_inv_step<KK>();
         const unsigned long long mk = s_mask[qrow];
         for (int k = 0; k < jobs; ++k) {
@@ -400,9 +415,6 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                     }
                 }
             }
-            tc05_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(sempty + w);  // the next S of this warpgroup may be computed
             // which of the 64 columns the row sees
             const bool tail = pb + NB > ctx;
             unsigned long long vis = ~0ull;
@@ -428,14 +440,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                 const float want = bm == kNegMax ? kNegMax : fmaf(bm, c2, ev - 10.f);
                 if (want > m_ref + 4.f) nref = want;
             }
-            // P' and O of this warpgroup are free once its previous PV is done
-            if (k > 0 && !mbar_wait_fast(odone + w, (uint32_t)(k - 1) & 1u)) {
-                if (lane == 0) report_error(kErrFullWait);
-                *fail = 1;
-                break;
-            }
             if (!idle) {
-                tc05_fence_after();
                 const float corr = fast_exp2(m_ref - nref);
                 if (__any_sync(0xffffffffu, nref != m_ref)) {
                     l_sum *= corr;
@@ -457,56 +462,53 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                 const auto weights = [&](auto is_tail) {
                     const float2 sc2 = make_float2(c2, c2), nm = make_float2(-nref, -nref);
 #pragma unroll
-                    for (int j = 0; j < NB; j += 8) {
-                        float2 e[4];
+                    for (int jj = 0; jj < NB; jj += 16) {
+                        uint32_t h[SG][8];  // P' of 16 positions, fp16 pairs
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float2 y = ffma2(make_float2(x[j + 2 * i], x[j + 2 * i + 1]), sc2, nm);
-                            e[i] = make_float2(fast_exp2(y.x), fast_exp2(y.y));
-                            if constexpr (decltype(is_tail)::value) {
-                                if (!(vis >> (j + 2 * i) & 1ull)) e[i].x = 0.f;
-                                if (!(vis >> (j + 2 * i + 1) & 1ull)) e[i].y = 0.f;
-                            }
-                            sum = fadd2(sum, e[i]);
-                        }
+                        for (int j = jj; j < jj + 16; j += 4) {
+                            float2 e[2];
 #pragma unroll
-                        for (int g = 0; g < SG; ++g) {
-                            uint32_t h[4];
-                            float2 v[4];
-                            if constexpr (C::kScaled) {
-                                const float4 v0 = lds_f4(sc + 4 * ((NG + g) * NB + j));
-                                const float4 v1 = lds_f4(sc + 4 * ((NG + g) * NB + j + 4));
-                                v[0] = fmul2(e[0], make_float2(v0.x, v0.y));
-                                v[1] = fmul2(e[1], make_float2(v0.z, v0.w));
-                                v[2] = fmul2(e[2], make_float2(v1.x, v1.y));
-                                v[3] = fmul2(e[3], make_float2(v1.z, v1.w));
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) v[i] = e[i];
-                            }
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                if constexpr (C::kScaled && decltype(is_tail)::value) {  // an unseen row's scale may be nan
-                                    if (!(vis >> (j + 2 * i) & 1ull)) v[i].x = 0.f;
-                                    if (!(vis >> (j + 2 * i + 1) & 1ull)) v[i].y = 0.f;
+                            for (int i = 0; i < 2; ++i) {
+                                const float2 y = ffma2(make_float2(x[j + 2 * i], x[j + 2 * i + 1]), sc2, nm);
+                                e[i] = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+                                if constexpr (decltype(is_tail)::value) {
+                                    if (!(vis >> (j + 2 * i) & 1ull)) e[i].x = 0.f;
+                                    if (!(vis >> (j + 2 * i + 1) & 1ull)) e[i].y = 0.f;
                                 }
-                                h[i] = h2_bits(__floats2half2_rn(v[i].x, v[i].y));
+                                sum = fadd2(sum, e[i]);
                             }
-                            *reinterpret_cast<uint4*>(sP + g * C::kPTile + (((j >> 3) ^ (row & 7)) << 4)) =
-                                make_uint4(h[0], h[1], h[2], h[3]);
+#pragma unroll
+                            for (int g = 0; g < SG; ++g) {
+                                float2 v[2] = {e[0], e[1]};
+                                if constexpr (C::kScaled) {
+                                    const float4 v0 = lds_f4(sc + 4 * ((NG + g) * NB + j));
+                                    v[0] = fmul2(e[0], make_float2(v0.x, v0.y));
+                                    v[1] = fmul2(e[1], make_float2(v0.z, v0.w));
+                                }
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) {
+                                    if constexpr (C::kScaled && decltype(is_tail)::value) {  // an unseen row's scale may be nan
+                                        if (!(vis >> (j + 2 * i) & 1ull)) v[i].x = 0.f;
+                                        if (!(vis >> (j + 2 * i + 1) & 1ull)) v[i].y = 0.f;
+                                    }
+                                    h[g][(j - jj) / 2 + i] = h2_bits(__floats2half2_rn(v[i].x, v[i].y));
+                                }
+                            }
                         }
+#pragma unroll
+                        for (int g = 0; g < SG; ++g) tmem_st8_u(tS + 32 * g + jj / 2, h[g]);
                     }
                 };
                 if (tail) weights(std::true_type{});
                 else weights(std::false_type{});
                 l_sum += sum.x + sum.y;
-                fence_proxy_async_smem();
+                tmem_wait_st();
             }
             tc05_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(pfull + w);
         }
-        if (jobs > 0 && !*fail && !mbar_wait_fast(odone + w, (uint32_t)(jobs - 1) & 1u)) {
+        if (!*fail && !mbar_wait_fast(odone, 0)) {  // every MMA of the CTA
             if (lane == 0) report_error(kErrFullWait);
             *fail = 1;
         }
@@ -652,55 +654,67 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
         // the copies in flight land (bounded) before the shared memory is given back
         for (int k = max(0, i - C::kRawStages); k < i; ++k)
             if (!mbar_wait_bounded(rfull + k % C::kRawStages, (uint32_t)(k / C::kRawStages) & 1u)) *fail = 1;
-    } else if (lane == 0) {
-        // ---- the MMA thread ----------------------------------------------------------
+    } else {
+        // ---- the MMA warp: one elected lane issues -----------------------------------
         constexpr uint32_t kIdescS = umma_idesc_f16(128, NB, false);
         constexpr uint32_t kIdescO = umma_idesc_f16(128, C::kScaled ? 64 : D, true);
-        bool ok = true;
-        for (int j = 0; ok && j < njobs + 2; ++j) {
-            if (j < njobs) {
-                const int w = j & 1, k = j >> 1, i = C::kTwo ? j >> 1 : j, s = i % KS;
-                ok = mbar_wait_fast(kfull + s, (uint32_t)(i / KS) & 1u);
-                if (k > 0) ok = ok && mbar_wait_fast(sempty + w, (uint32_t)(k - 1) & 1u);
-                if (!ok) break;
-                tc05_fence_after();
-                const uint32_t qa = sbase + (C::kTwo ? w * C::kQTile : 0), ka = sbase + C::kOffK + s * C::kTile;
+        const uint32_t ub = __shfl_sync(0xffffffffu, sbase, 0), ut = __shfl_sync(0xffffffffu, tbase, 0);
+        // descriptors differ in their start addresses only (16-byte units, no carry out of them)
+        const uint64_t dq = umma_desc_sw128(ub, 16, 1024), dk = umma_desc_sw128(ub + C::kOffK, 16, 1024);
+        const uint64_t dv = umma_desc_sw128(ub + C::kOffV, NB * 128, 1024);
+        const auto issue_s = [&](int j) {
+            const int w = j & 1, i = C::kTwo ? j >> 1 : j, s = i % KS;
+            if (!mbar_wait_fast(kfull + s, (uint32_t)(i / KS) & 1u)) return false;
+            tc05_fence_after();
+            const uint64_t qa = dq + (C::kTwo ? w * (C::kQTile / 16) : 0), ka = dk + s * (C::kTile / 16);
+            const uint32_t d = ut + w * 256;
+            if (elect_one()) {
 #pragma unroll
                 for (int g = 0; g < NG; ++g)
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk)
-                        umma_f16(tbase + w * 256 + (C::kScaled ? 64 * g : 0),
-                                 umma_desc_sw128(qa + g * 16384 + kk * 32, 16, 1024),
-                                 umma_desc_sw128(ka + g * (NB * 128) + kk * 32, 16, 1024), kIdescS,
-                                 kk > 0 || (!C::kScaled && g > 0));
+                        umma_f16(d + (C::kScaled ? 64 * g : 0), qa + (g * 16384 + kk * 32) / 16, ka + (g * (NB * 128) + kk * 32) / 16,
+                                 kIdescS, kk > 0 || (!C::kScaled && g > 0));
                 umma_commit(sfull + w);
                 if (!C::kTwo || w == 1) umma_commit(kempty + s);
             }
-            if (j >= 2) {
-                const int jj = j - 2, w = jj & 1, k = jj >> 1, i = C::kTwo ? jj >> 1 : jj, s = i % VS;
-                ok = mbar_wait_fast(vfull + s, (uint32_t)(i / VS) & 1u);
-                ok = ok && mbar_wait_fast(pfull + w, (uint32_t)k & 1u);
-                if (!ok) break;
-                tc05_fence_after();
-                const uint32_t pa = sbase + C::kOffP + w * SG * C::kPTile, va = sbase + C::kOffV + s * C::kTile;
+            __syncwarp();
+            return true;
+        };
+        const auto issue_pv = [&](int j) {
+            const int w = j & 1, k = j >> 1, i = C::kTwo ? j >> 1 : j, s = i % VS;
+            if (!mbar_wait_fast(vfull + s, (uint32_t)(i / VS) & 1u)) return false;
+            if (!mbar_wait_fast(pfull + w, (uint32_t)k & 1u)) return false;
+            tc05_fence_after();
+            const uint64_t va = dv + s * (C::kTile / 16);
+            const uint32_t d = ut + w * 256;
+            if (elect_one()) {
 #pragma unroll
                 for (int g = 0; g < SG; ++g)
 #pragma unroll
                     for (int kk = 0; kk < NB / 16; ++kk)
-                        umma_f16(tbase + w * 256 + 128 + 64 * g,
-                                 umma_desc_sw128(pa + g * C::kPTile + kk * 32, 16, 1024),
-                                 umma_desc_sw128(va + g * (NB * 128) + kk * 2048, NB * 128, 1024), kIdescO,
-                                 k > 0 || kk > 0);
-                umma_commit(odone + w);
+                        umma_f16_ts(d + 128 + 64 * g, d + 32 * g + 8 * kk, va + (g * (NB * 128) + kk * 2048) / 16, kIdescO,
+                                    k > 0 || kk > 0);
                 if (!C::kTwo || w == 1) umma_commit(vempty + s);
             }
+            __syncwarp();
+            return true;
+        };
+        bool ok = issue_s(0);
+        if (njobs > 1) ok = ok && issue_s(1);
+        for (int j = 0; ok && j < njobs; ++j) {
+            ok = issue_pv(j);
+            if (j + 2 < njobs) ok = ok && issue_s(j + 2);
         }
-        if (!ok) {  // every MMA issued so far ends before the tensor memory is given back
-            report_error(kErrFullWait);
+        if (ok) {
+            if (elect_one()) umma_commit(odone);
+        } else {  // every MMA issued so far ends before the tensor memory is given back
+            if (lane == 0) report_error(kErrFullWait);
             *fail = 1;
-            umma_commit(fin);
+            if (elect_one()) umma_commit(fin);
             (void)mbar_wait_bounded(fin, 0);
         }
+        __syncwarp();
     }
     tc05_fence_before();
     __syncthreads();
