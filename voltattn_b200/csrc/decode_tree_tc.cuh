@@ -3,30 +3,30 @@
 // query rows, with tcgen05.mma and accumulators in tensor memory.
 //
 // One CTA per (sequence, KV head, tile of query rows, range of positions), one
-// per SM, 14 warps (4 on an SM sub-partition at most: 128 registers a thread, which hold
-// a row's 64 scores; with 18 warps and 96 registers the spills took half of the time):
-//   warps 0-3, 4-7  two softmax warpgroups; thread r owns query row r (TMEM lane r);
-//   warps 8-11      producers: codes -> exact fp16 codes in swizzled tiles;
-//   warp 12         one thread issues every tcgen05.mma;
-//   warp 13         copies blocks of codes and scales into a ring, several ahead.
-// A job is one warpgroup's work on one block of 64 positions. kTwo = false (up
-// to 128 query rows): the warpgroups take the blocks in turn, each with its own
-// O and statistics, merged at the end. kTwo = true (up to 256): both take every
-// block, for query rows 0..127 and 128..255, so a decoded tile serves twice.
+// per SM, 14 warps (4 on an SM sub-partition at most: 128 registers a thread):
+//   warps 0-7    softmax: thread (half hf, row r) has 32 of a job's 64 positions of
+//                query row r (TMEM lane r);
+//   warps 8-11   producers: codes -> exact fp16 codes in swizzled tiles;
+//   warp 12      one elected lane issues every tcgen05.mma;
+//   warp 13      copies: blocks of codes and scales into a ring, several ahead (fp16
+//                rows by tensor copies straight into the swizzled tiles).
+// A job is one block of 64 positions against 128 query rows; the jobs alternate
+// between two sets w of TMEM columns (S_w, O_w, 256 each). kTwo = false (up to 128
+// query rows): job j is block j, and O_0, O_1 (even and odd blocks) merge at the end.
+// kTwo = true (up to 256): jobs 2 i, 2 i + 1 are block i against rows 0..127 and
+// 128..255, so a decoded tile serves twice.
 //
 // Per job j (MMA order S(0) S(1), then PV(j) S(j + 2)):
 //   S_g = Q_g K_g^T (M = 128 rows, N = 64 positions) for each 64-dim group g, in
 //     TMEM. The K tile holds the exact codes (times a power of two), so the group
 //     scales multiply fp32 scores, as in decode_tree.cuh;
-//   the softmax thread loads its row's scores, x = S_0 k_0 + S_1 k_1, and writes
-//     P'_g = fp16(w v_g) over them;
+//   the softmax threads load their scores, x = S_0 k_0 + S_1 k_1, exchange the row's
+//     maximum, and write P'_g = fp16(w v_g) over the scores;
 //   O_g += P'_g V_g (A = P' read from TMEM, B = the V tile read MN-major).
 // The MMAs of one thread execute in issue order, so S(j + 2) follows PV(j) into the
-// same columns, and a completed S implies every earlier PV of its warpgroup. Shared
-// memory's bandwidth is what bounds the kernel (A operands and weights read from it
-// took 2840 cycles a block against ... with P' in TMEM).
+// same columns, and a completed S implies every earlier PV into its set.
 // O is rescaled only when a row's reference grows by more than 4 (log2): P' of the
-// largest weight stays in [2^6, 2^15), its rounding relative.
+// largest weight stays in [2^6, 2^15), its one rounding relative.
 //
 // The K and V tiles are the canonical 128-byte-swizzled layout, one panel of 64
 // rows per 64-dim group. Packed codes are placed two dims apart by 4 in each
@@ -56,8 +56,9 @@ struct TreeTcCfg {
     static constexpr int kThreads = 14 * 32;
     static constexpr int kQTile = 128 * kDim * 2;
     static constexpr int kTile = kNb * kDim * 2;   // one K or V tile
-    static constexpr int kKS = 2;
-    static constexpr int kVS = 2;
+    static constexpr bool kDirect = K == Kind::F16;  // tiles by tensor copies
+    static constexpr int kKS = kDirect ? (kTwoTiles ? 3 : 4) : 2;
+    static constexpr int kVS = kKS;
     static constexpr int kOffK = (kTwoTiles ? 2 : 1) * kQTile;
     static constexpr int kOffV = kOffK + kKS * kTile;
     static constexpr int kOffRaw = kOffV + kVS * kTile;        // ring of blocks as they lie in the cache
@@ -65,21 +66,23 @@ struct TreeTcCfg {
     static constexpr int kRawV = kNb * kRb, kRawSK = 2 * kNb * kRb, kRawSV = kRawSK + kNb * kSb;
     static constexpr int kRawTx = kRawSV + kNb * kSb;
     static constexpr int kRawStage = (kRawTx + 127) / 128 * 128;
-    // what follows the ring: scales as floats [4 slots][K, V][kNG][64], masks, [2][128]
-    // (reference, sum), barriers, ev[4], TMEM slot, fail, special, ticket
+    // what follows the ring: scales as floats [4 slots][K, V][kNG][64], masks,
+    // [2][2][128] maxima or sums, barriers, ev[4], TMEM slot, fail, special, ticket
     static constexpr int kScaleSlots = 4;
-    static constexpr int kScaleBytes = kScaled ? kScaleSlots * 2 * kNG * kNb * 4 : 0;
+    static constexpr int kScaleSlot = 2 * kNG * kNb * 4;
+    static constexpr int kScaleV = kNG * kNb * 4;  // where a slot's V scales begin
+    static constexpr int kScaleBytes = kScaled ? kScaleSlots * kScaleSlot : 0;
     static constexpr int kRest = kScaleBytes + kRows * 8 + 2 * 128 * 8 + 512 + 64;
     static constexpr int kRoom = (227 * 1024 - 1024 - kOffRaw - kRest) / kRawStage;
-    static constexpr int kRawStages = kRoom < 8 ? kRoom : 8;
-    static constexpr int kOffScales = kOffRaw + kRawStages * kRawStage;
+    static constexpr int kRawStages = kDirect ? 1 : kRoom < 8 ? kRoom : 8;
+    static constexpr int kOffScales = kOffRaw + (kDirect ? 0 : kRawStages * kRawStage);
     static constexpr int kOffMask = kOffScales + kScaleBytes;
     static constexpr int kOffMl = kOffMask + kRows * 8;
     static constexpr int kOffBars = kOffMl + 2 * 128 * 8;
-    static constexpr int kBars = 2 * kKS + 2 * kVS + 2 * 2 + 2 + kScaleSlots + 2 * kRawStages;
+    static constexpr int kBars = 2 * kKS + 3 * kVS + 2 * 2 + 2 + kScaleSlots + 2 * kRawStages;
     static constexpr int kOffMisc = kOffBars + kBars * 8;
     static constexpr int kSmemBytes = 1024 + kOffMisc + 64;
-    static_assert(kRawStages >= 2 && kBars * 8 <= 512, "two blocks in flight");
+    static_assert((kDirect || kRawStages >= 2) && kBars * 8 <= 512, "two blocks in flight");
     static_assert(kSmemBytes <= 227 * 1024, "one CTA per SM");
 };
 
@@ -200,36 +203,12 @@ __device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
     return d;
 }
 
-// 16 consecutive fp32 columns of this thread's TMEM lane, without the wait (as
-// tmem_ld32_nowait), and the tie to it.
-__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_tie16(uint32_t* r) {
-    asm volatile(""
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                   "+r"(r[15]));
-}
-
 // True in one lane of the (converged) warp. The values around it stay warp-uniform,
 // so the operands of the MMAs need no move from vector to uniform registers.
 __device__ __forceinline__ bool elect_one() {
     uint32_t ok;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
     return ok != 0;
-}
-
-__device__ __forceinline__ void tmem_st8_u(uint32_t taddr, const uint32_t* r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
-                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                 : "memory");
 }
 
 // Four floats of shared memory. Not volatile: the compiler may move the load over
@@ -253,19 +232,50 @@ __device__ __forceinline__ bool clear_not_finite(uint4& v) {
     return any;
 }
 
+// fp16 rows: the V tiles of blocks that hold drafted rows or the end are mended where
+// they landed (rows past the end cleared, entries that are not finite too), and every
+// tile is passed on to the MMAs. 128 threads: thread (row, half of the dims).
 template <class C>
-__global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const TreeParams p) {
+__device__ __forceinline__ void tree_tc_fix_v(int p0, int len, int ctx, int nblk, uint8_t* smem, uint64_t* vraw,
+                                              uint64_t* vfull, volatile int* special, volatile int* fail) {
+    const int t = (int)threadIdx.x - 256, lane = t & 31, row = t >> 1;
+    for (int i = 0; i < nblk; ++i) {
+        const int s = i % C::kVS, pb = p0 + i * C::kNb;
+        if (!mbar_wait_bounded(vraw + s, (uint32_t)(i / C::kVS) & 1u)) {
+            if (lane == 0) report_error(kErrFullWait);
+            *fail = 1;
+            return;
+        }
+        if (pb + C::kNb > ctx && pb + row >= ctx) {
+            uint8_t* tile = smem + C::kOffV + s * C::kTile;
+            for (int c = (t & 1) * (C::kD / 16); c < ((t & 1) + 1) * (C::kD / 16); ++c) {
+                uint4* at = reinterpret_cast<uint4*>(tile + (c >> 3) * (C::kNb * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+                uint4 v = *at;
+                if (pb + row >= len) *at = make_uint4(0u, 0u, 0u, 0u);
+                else if (clear_not_finite(v)) *special = 1, *at = v;
+            }
+            fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(vfull + s);
+    }
+}
+
+template <class C>
+__global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const TreeParams p,
+                                                                           const __grid_constant__ CUtensorMap tmK,
+                                                                           const __grid_constant__ CUtensorMap tmV) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
     // (an offset, not a rounded address: the compiler keeps seeing shared memory)
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     constexpr int D = C::kD, NG = C::kNG, NB = C::kNb, KS = C::kKS, VS = C::kVS, SG = C::kSG;
     constexpr Kind KK = C::kKind;
     unsigned long long* s_mask = reinterpret_cast<unsigned long long*>(smem + C::kOffMask);
-    float2* s_ml = reinterpret_cast<float2*>(smem + C::kOffMl);
+    float* s_xch = reinterpret_cast<float*>(smem + C::kOffMl);  // [2][2][128]
     uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
     uint64_t *kempty = kfull + KS, *vfull = kempty + KS, *vempty = vfull + VS, *sfull = vempty + VS;
     uint64_t *pfull = sfull + 2, *odone = pfull + 2, *fin = odone + 1, *scfull = fin + 1;
-    uint64_t *rfull = scfull + C::kScaleSlots, *rempty = rfull + C::kRawStages;
+    uint64_t *rfull = scfull + C::kScaleSlots, *rempty = rfull + C::kRawStages, *vraw = rempty + C::kRawStages;
     float* s_ev = reinterpret_cast<float*>(smem + C::kOffMisc);
     uint32_t* tslot = reinterpret_cast<uint32_t*>(s_ev + 4);
     volatile int* fail = reinterpret_cast<volatile int*>(tslot + 1);
@@ -310,14 +320,16 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     const int njobs = C::kTwo ? 2 * nblk : nblk;
     if (warp == 12) tmem_alloc(tslot, 512);
     if (tid == 0) {
-        for (int i = 0; i < KS; ++i) mbar_init(kfull + i, C::kProducers / 32), mbar_init(kempty + i, 1);
+        for (int i = 0; i < KS; ++i) mbar_init(kfull + i, C::kDirect ? 1 : C::kProducers / 32), mbar_init(kempty + i, 1);
         for (int i = 0; i < VS; ++i) mbar_init(vfull + i, C::kProducers / 32), mbar_init(vempty + i, 1);
         for (int i = 0; i < 2; ++i)
-            mbar_init(sfull + i, 1), mbar_init(pfull + i, 4);
+            mbar_init(sfull + i, 1), mbar_init(pfull + i, 8);
         mbar_init(odone, 1);
         mbar_init(fin, 1);
         for (int i = 0; i < C::kScaleSlots; ++i) mbar_init(scfull + i, 1);
         for (int i = 0; i < C::kRawStages; ++i) mbar_init(rfull + i, 1), mbar_init(rempty + i, C::kProducers / 32);
+        if constexpr (C::kDirect)
+            for (int i = 0; i < VS; ++i) mbar_init(vraw + i, 1);
         *fail = 0;
         *special = 0;
         fence_mbar_init();
@@ -356,18 +368,15 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     const uint32_t tbase = *tslot;
     const uint32_t sbase = smem_u32(smem);
 
-    float m_ref = kNegMax, l_sum = 0.f;  // softmax threads: their row's reference (log2 units) and sum
+    // softmax threads: the reference (log2 units) and their half's sum of each set
+    float m_ref[2] = {kNegMax, kNegMax}, l_sum[2] = {0.f, 0.f};
+    const int hf = warp >> 2, row = tid & 127, quad = warp & 3;
+    const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
     if (warp < 8) {
         // ---- softmax -------------------------------------------------------------
-        const int w = warp >> 2;
-        const int row = tid & 127, qrow = C::kTwo ? w * 128 + row : row;
-        const int jobs = C::kTwo ? nblk : (nblk - w + 1) / 2;
-        const bool idle = (C::kTwo ? w * 128 : 0) + (warp & 3) * 32 >= live;  // no row of this warp is live
-        const uint32_t tS = tbase + w * 256 + ((uint32_t)((warp & 3) * 32) << 16), tO = tS + 128;
         const float c2 = rsqrtf((float)D) * kLog2e * tc_k_inv_step<KK>();
-        const unsigned long long mk = s_mask[qrow];
-        for (int k = 0; k < jobs; ++k) {
-            const int blk = C::kTwo ? k : 2 * k + w;
+        for (int j = 0; j < njobs; ++j) {
+            const int w = j & 1, k = j >> 1, blk = C::kTwo ? k : j;
             const int pb = p0 + blk * NB;
             bool ok = mbar_wait_fast(sfull + w, (uint32_t)k & 1u);
             // (a slot of scales is written again only after this block's PV, so this phase
@@ -380,128 +389,129 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                 break;
             }
             tc05_fence_after();
-            uint32_t sc = sbase + C::kOffScales + (blk % C::kScaleSlots) * 2 * NG * NB * 4;
-            asm volatile("" : "+r"(sc));  // the loads of scales come after the waits
-            float x[NB];
-            if (!idle) {
-#pragma unroll
-                for (int cb = 0; cb < NB; cb += 16) {
-                    uint32_t s[SG][16];
-#pragma unroll
-                    for (int g = 0; g < SG; ++g) tmem_ld16_nowait(tS + 64 * g + cb, s[g]);
+            // a quadrant without live rows only keeps the barriers' count
+            if ((C::kTwo ? w * 128 : 0) + quad * 32 < live) {
+                uint32_t sc = sbase + C::kOffScales + (blk % C::kScaleSlots) * C::kScaleSlot;
+                asm volatile("" : "+r"(sc));  // the loads of scales come after the waits
+                const uint32_t tS = tbase + w * 256 + lane_addr, tO = tS + 128;
+                float x[32];
+                {
+                    uint32_t s0[32], s1[32];
+                    tmem_ld32_nowait(tS + 32 * hf, s0);
+                    if constexpr (SG == 2) tmem_ld32_nowait(tS + 64 + 32 * hf, s1);
                     tmem_wait_ld_only();
+                    tmem_tie32(s0);
+                    if constexpr (SG == 2) tmem_tie32(s1);
 #pragma unroll
-                    for (int g = 0; g < SG; ++g) tmem_tie16(s[g]);
-#pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
-                        float2 a = make_float2(__uint_as_float(s[0][j]), __uint_as_float(s[0][j + 1]));
-                        float2 c = make_float2(__uint_as_float(s[0][j + 2]), __uint_as_float(s[0][j + 3]));
+                    for (int c = 0; c < 32; c += 4) {
+                        float2 u = make_float2(__uint_as_float(s0[c]), __uint_as_float(s0[c + 1]));
+                        float2 v = make_float2(__uint_as_float(s0[c + 2]), __uint_as_float(s0[c + 3]));
                         if constexpr (C::kScaled) {
-                            const float4 k0 = lds_f4(sc + 4 * (cb + j));
-                            a = fmul2(a, make_float2(k0.x, k0.y));
-                            c = fmul2(c, make_float2(k0.z, k0.w));
-                            if constexpr (NG == 2) {
-                                const float4 k1 = lds_f4(sc + 4 * (NB + cb + j));
-                                a = ffma2(make_float2(__uint_as_float(s[SG - 1][j]), __uint_as_float(s[SG - 1][j + 1])),
-                                          make_float2(k1.x, k1.y), a);
-                                c = ffma2(make_float2(__uint_as_float(s[SG - 1][j + 2]), __uint_as_float(s[SG - 1][j + 3])),
-                                          make_float2(k1.z, k1.w), c);
+                            const float4 k0 = lds_f4(sc + 4 * (32 * hf + c));
+                            u = fmul2(u, make_float2(k0.x, k0.y));
+                            v = fmul2(v, make_float2(k0.z, k0.w));
+                            if constexpr (SG == 2) {
+                                const float4 k1 = lds_f4(sc + 4 * (NB + 32 * hf + c));
+                                u = ffma2(make_float2(__uint_as_float(s1[c]), __uint_as_float(s1[c + 1])),
+                                          make_float2(k1.x, k1.y), u);
+                                v = ffma2(make_float2(__uint_as_float(s1[c + 2]), __uint_as_float(s1[c + 3])),
+                                          make_float2(k1.z, k1.w), v);
                             }
                         }
-                        x[cb + j] = a.x;
-                        x[cb + j + 1] = a.y;
-                        x[cb + j + 2] = c.x;
-                        x[cb + j + 3] = c.y;
+                        x[c] = u.x;
+                        x[c + 1] = u.y;
+                        x[c + 2] = v.x;
+                        x[c + 3] = v.y;
                     }
                 }
-            }
-            // which of the 64 columns the row sees
-            const bool tail = pb + NB > ctx;
-            unsigned long long vis = ~0ull;
-            if (tail) {
-                const int d = ctx - pb;  // < 64
-                vis = d > 0 ? (mk << d) | ((1ull << d) - 1ull) : -d < 64 ? mk >> -d : 0ull;
-                if (!idle) {
+                // which of its 32 columns the row sees
+                const bool tail = pb + NB > ctx;
+                uint32_t vis = 0xFFFFFFFFu;
+                if (tail) {
+                    const unsigned long long mk = s_mask[(C::kTwo ? w * 128 : 0) + row];
+                    const int d = ctx - pb;  // < 64
+                    const unsigned long long all = d > 0 ? (mk << d) | ((1ull << d) - 1ull) : -d < 64 ? mk >> -d : 0ull;
+                    vis = (uint32_t)(all >> (32 * hf));
 #pragma unroll
-                    for (int j = 0; j < NB; ++j)
-                        if (!(vis >> j & 1ull)) x[j] = kNegMax;
+                    for (int c = 0; c < 32; ++c)
+                        if (!(vis >> c & 1u)) x[c] = kNegMax;
                 }
-            }
-            float nref = m_ref;
-            if (!idle) {
-                float b0 = x[0], b1 = x[1];
+                float b0 = fmaxf(x[0], x[1]), b1 = fmaxf(x[2], x[3]);
 #pragma unroll
-                for (int j = 2; j < NB; j += 4) {
-                    b0 = fmax3f(b0, x[j], x[j + 1]);
-                    if (j + 2 < NB) b1 = fmax3f(b1, x[j + 2], x[j + 3]);
+                for (int c = 4; c < 32; c += 4) {
+                    b0 = fmax3f(b0, x[c], x[c + 1]);
+                    b1 = fmax3f(b1, x[c + 2], x[c + 3]);
                 }
-                const float bm = fmaxf(b0, b1);
+                // the row's maximum over both halves; their barrier also puts every load of S
+                // before the stores of P' below
+                float* xch = s_xch + (j & 1) * 256;
+                xch[hf * 128 + row] = fmaxf(b0, b1);
+                named_barrier_sync(2 + quad, 64);
+                const float bm = fmaxf(fmaxf(b0, b1), xch[(1 - hf) * 128 + row]);
                 const float ev = C::kScaled ? s_ev[blk % C::kScaleSlots] : 0.f;
+                const float m = w ? m_ref[1] : m_ref[0];
                 const float want = bm == kNegMax ? kNegMax : fmaf(bm, c2, ev - 10.f);
-                if (want > m_ref + 4.f) nref = want;
-            }
-            if (!idle) {
-                const float corr = fast_exp2(m_ref - nref);
-                if (__any_sync(0xffffffffu, nref != m_ref)) {
-                    l_sum *= corr;
-                    if (k > 0) {
+                const float nref = want > m + 4.f ? want : m;
+                float l = w ? l_sum[1] : l_sum[0];
+                if (__any_sync(0xffffffffu, nref != m)) {
+                    const float corr = fast_exp2(m - nref);
+                    l *= corr;
+                    if (k > 0) {  // this half of the row's O
 #pragma unroll 1
-                        for (int cb = 0; cb < D; cb += 32) {
+                        for (int cb = 0; cb < D / 2; cb += 32) {
                             float o[32];
-                            tmem_ld32(tO + cb, o);
+                            tmem_ld32(tO + hf * (D / 2) + cb, o);
 #pragma unroll
                             for (int i = 0; i < 32; ++i) o[i] *= corr;
-                            tmem_st32(tO + cb, o);
+                            tmem_st32(tO + hf * (D / 2) + cb, o);
                         }
-                        tmem_wait_st();
                     }
                 }
-                m_ref = nref;
                 float2 sum = make_float2(0.f, 0.f);
                 // (two instantiations: only blocks with drafted rows or the end select)
                 const auto weights = [&](auto is_tail) {
+                    constexpr bool kTail = decltype(is_tail)::value;
                     const float2 sc2 = make_float2(c2, c2), nm = make_float2(-nref, -nref);
 #pragma unroll
-                    for (int jj = 0; jj < NB; jj += 16) {
-                        uint32_t h[SG][8];  // P' of 16 positions, fp16 pairs
-#pragma unroll
-                        for (int j = jj; j < jj + 16; j += 4) {
-                            float2 e[2];
-#pragma unroll
-                            for (int i = 0; i < 2; ++i) {
-                                const float2 y = ffma2(make_float2(x[j + 2 * i], x[j + 2 * i + 1]), sc2, nm);
-                                e[i] = make_float2(fast_exp2(y.x), fast_exp2(y.y));
-                                if constexpr (decltype(is_tail)::value) {
-                                    if (!(vis >> (j + 2 * i) & 1ull)) e[i].x = 0.f;
-                                    if (!(vis >> (j + 2 * i + 1) & 1ull)) e[i].y = 0.f;
-                                }
-                                sum = fadd2(sum, e[i]);
-                            }
-#pragma unroll
-                            for (int g = 0; g < SG; ++g) {
-                                float2 v[2] = {e[0], e[1]};
-                                if constexpr (C::kScaled) {
-                                    const float4 v0 = lds_f4(sc + 4 * ((NG + g) * NB + j));
-                                    v[0] = fmul2(e[0], make_float2(v0.x, v0.y));
-                                    v[1] = fmul2(e[1], make_float2(v0.z, v0.w));
-                                }
-#pragma unroll
-                                for (int i = 0; i < 2; ++i) {
-                                    if constexpr (C::kScaled && decltype(is_tail)::value) {  // an unseen row's scale may be nan
-                                        if (!(vis >> (j + 2 * i) & 1ull)) v[i].x = 0.f;
-                                        if (!(vis >> (j + 2 * i + 1) & 1ull)) v[i].y = 0.f;
-                                    }
-                                    h[g][(j - jj) / 2 + i] = h2_bits(__floats2half2_rn(v[i].x, v[i].y));
-                                }
-                            }
+                    for (int c = 0; c < 32; c += 2) {
+                        const float2 y = ffma2(make_float2(x[c], x[c + 1]), sc2, nm);
+                        float2 e = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+                        if constexpr (kTail) {
+                            if (!(vis >> c & 1u)) e.x = 0.f;
+                            if (!(vis >> (c + 1) & 1u)) e.y = 0.f;
                         }
+                        sum = fadd2(sum, e);
+                        x[c] = e.x;
+                        x[c + 1] = e.y;
+                    }
 #pragma unroll
-                        for (int g = 0; g < SG; ++g) tmem_st8_u(tS + 32 * g + jj / 2, h[g]);
+                    for (int g = 0; g < SG; ++g) {
+                        uint32_t h[16];  // P'_g, pairs of positions
+#pragma unroll
+                        for (int c = 0; c < 32; c += 4) {
+                            float2 u = make_float2(x[c], x[c + 1]), v = make_float2(x[c + 2], x[c + 3]);
+                            if constexpr (C::kScaled) {
+                                const float4 f = lds_f4(sc + C::kScaleV + 4 * (g * NB + 32 * hf + c));
+                                u = fmul2(u, make_float2(f.x, f.y));
+                                v = fmul2(v, make_float2(f.z, f.w));
+                                if constexpr (kTail) {  // an unseen row's scale may be nan
+                                    if (!(vis >> c & 1u)) u.x = 0.f;
+                                    if (!(vis >> (c + 1) & 1u)) u.y = 0.f;
+                                    if (!(vis >> (c + 2) & 1u)) v.x = 0.f;
+                                    if (!(vis >> (c + 3) & 1u)) v.y = 0.f;
+                                }
+                            }
+                            h[c / 2] = h2_bits(__floats2half2_rn(u.x, u.y));
+                            h[c / 2 + 1] = h2_bits(__floats2half2_rn(v.x, v.y));
+                        }
+                        tmem_st16_u(tS + 32 * g + 16 * hf, h);
                     }
                 };
                 if (tail) weights(std::true_type{});
                 else weights(std::false_type{});
-                l_sum += sum.x + sum.y;
+                l += sum.x + sum.y;
+                if (w) m_ref[1] = nref, l_sum[1] = l;
+                else m_ref[0] = nref, l_sum[0] = l;
                 tmem_wait_st();
             }
             tc05_fence_before();
@@ -513,7 +523,9 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
             *fail = 1;
         }
         tc05_fence_after();
-    } else if (warp < 12) {
+    } else if (C::kDirect && warp < 12) {
+        tree_tc_fix_v<C>(p0, len, ctx, nblk, smem, vraw, vfull, special, fail);
+    } else if (!C::kDirect && warp < 12) {
         // ---- producers: K of block i + 1 before V of block i, so the next scores never
         // wait for this block's PV. A thread takes two slices (row, quarter of the dims) -----
         const int pw = warp - 8;
@@ -533,7 +545,8 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
             const uint8_t* raw = raw_of(i);
             if (u > 0 && !mbar_wait_bounded(kempty + i % KS, (uint32_t)(u - 1) & 1u)) return false;
             if (C::kScaled && pw == (i & 3)) {  // the block's scales: two positions a lane
-                float* sc = reinterpret_cast<float*>(smem + C::kOffScales) + (i % C::kScaleSlots) * 2 * NG * NB;
+                float* sk = reinterpret_cast<float*>(smem + C::kOffScales + (i % C::kScaleSlots) * C::kScaleSlot);
+                float* sv = sk + C::kScaleV / 4;
                 __half2 big = __float2half2_rn(0.f);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
@@ -546,13 +559,11 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                         ks = reinterpret_cast<const uint16_t*>(raw + C::kRawSK)[at];
                         vs = reinterpret_cast<const uint16_t*>(raw + C::kRawSV)[at];
                     }
-                    const float2 fk = __half22float2(bits_h2(ks)), fv = __half22float2(bits_h2(vs));
-                    sc[at] = fk.x;
-                    sc[NG * NB + at] = fv.x;
-                    if constexpr (NG == 2) {
-                        sc[NB + at] = fk.y;
-                        sc[3 * NB + at] = fv.y;
-                    }
+                    const float2 fk = __half22float2(bits_h2(ks));
+                    sk[at] = fk.x;
+                    const float2 fv = __half22float2(bits_h2(vs));
+                    sv[at] = fv.x;
+                    if constexpr (NG == 2) sk[NB + at] = fk.y, sv[NB + at] = fv.y;
                     // rows past the end and scales that are not finite are no measure
                     uint32_t a = vs & 0x7FFF7FFFu;
                     if (p0 + i * NB + at >= len) a = 0u;
@@ -561,11 +572,11 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                     big = __hmax2(big, bits_h2(a));
                 }
                 const float vm = fmaxf(__low2float(big), __high2float(big));
-                __syncwarp();
                 const unsigned vb = __reduce_max_sync(0xffffffffu, __float_as_uint(vm));
+                __syncwarp();
                 if (lane == 0) {
                     s_ev[i % C::kScaleSlots] = vb ? (float)((int)(vb >> 23) - 127) : 0.f;
-                    mbar_arrive(scfull + i % C::kScaleSlots);  // (the reduction came after all lanes' stores)
+                    mbar_arrive(scfull + i % C::kScaleSlots);
                 }
             }
             uint8_t* kt = smem + C::kOffK + (i % KS) * C::kTile;
@@ -620,7 +631,43 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
             if (lane == 0) report_error(kErrEmptyWait);
             *fail = 1;
         }
-    } else if (warp == 13) {
+    } else if (C::kDirect && warp == 13) {
+        // ---- copies of fp16 rows: tensor copies of 64 dims by the block's rows inside a
+        // page (boxes of 64 or 8 rows) into the swizzled tiles; lane = run + 8 * group
+        const int run = p.page_rows % NB == 0 ? NB : 8, at = (lane & 7) * run, g = lane >> 3;
+        const bool copies = at < NB && g < NG;
+        int i = 0;
+        bool ok = true;
+        for (; ok && i < nblk; ++i) {
+            int off = 0, pg = 0;
+            if (copies) pg = page_of(p0 + i * NB + at, off);
+            const int y = (int)(((long long)pg * p.Hkv + hk) * p.page_rows + off);
+            const uint32_t o = g * (NB * 128) + at * 128;
+            const int ks = i % KS, vs = i % VS;
+            ok = i < KS || mbar_wait_bounded(kempty + ks, (uint32_t)(i / KS - 1) & 1u);
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(kfull + ks, C::kTile);
+            __syncwarp();
+            if (copies) pf_tma_2d(sbase + C::kOffK + ks * C::kTile + o, &tmK, 64 * g, y, kfull + ks);
+            ok = i < VS || mbar_wait_bounded(vempty + vs, (uint32_t)(i / VS - 1) & 1u);
+            if (!ok) {
+                (void)mbar_wait_bounded(kfull + ks, (uint32_t)(i / KS) & 1u);
+                break;
+            }
+            if (lane == 0) mbar_arrive_expect_tx(vraw + vs, C::kTile);
+            __syncwarp();
+            if (copies) pf_tma_2d(sbase + C::kOffV + vs * C::kTile + o, &tmV, 64 * g, y, vraw + vs);
+        }
+        if (!ok) {
+            if (lane == 0) report_error(kErrEmptyWait);
+            *fail = 1;
+        }
+        // the copies in flight land (bounded) before the shared memory is given back
+        for (int k = max(0, i - VS); k < i; ++k)
+            if (!mbar_wait_bounded(kfull + k % KS, (uint32_t)(k / KS) & 1u) ||
+                !mbar_wait_bounded(vraw + k % VS, (uint32_t)(k / VS) & 1u))
+                *fail = 1;
+    } else if (!C::kDirect && warp == 13) {
         // ---- copies: lane 4 r + k brings run r of buffer k (K, V, their scales): the
         // whole block when it lies inside a page, else runs of 8 rows
         const bool whole = p.page_rows % NB == 0;
@@ -725,55 +772,46 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     }
     grid_launch_dependents();
 
-    // ---- epilogue: a thread's row, its half of the dims (one tile) or all of them ------
+    // ---- epilogue: a thread's row (of each tile), its half of the dims ------------------
     const bool direct = nsplit == 1;
     if (warp < 8) {
-        const int w = warp >> 2, row = tid & 127, qrow = C::kTwo ? w * 128 + row : row, r = r0 + qrow;
-        const uint32_t tO = tbase + w * 256 + 128 + ((uint32_t)((warp & 3) * 32) << 16);
-        const bool idle = (C::kTwo ? w * 128 : 0) + (warp & 3) * 32 >= live;
-        float mx = m_ref, sum = l_sum, a0 = 1.f, a1 = 0.f;
-        float* xch = reinterpret_cast<float*>(smem + C::kOffK);  // [D][128]: the other warpgroup's half
-        constexpr int kCols = C::kTwo ? D : D / 2;               // dims this thread finishes
-        const int c0 = C::kTwo ? 0 : w * kCols;
-        const bool has = C::kTwo || w == 0 || nblk > 1;          // (one block: warpgroup 1 had no job)
-        if constexpr (!C::kTwo) {
-            s_ml[w * 128 + row] = make_float2(m_ref, l_sum);
-            if (!idle && has) {
-                const int o0 = (1 - w) * kCols;
+        s_xch[hf * 128 + row] = l_sum[0];
+        s_xch[256 + hf * 128 + row] = l_sum[1];
+        named_barrier_sync(1, 256);
+        const float l0 = l_sum[0] + s_xch[(1 - hf) * 128 + row], l1 = l_sum[1] + s_xch[256 + (1 - hf) * 128 + row];
+        const int c0 = hf * (D / 2);
 #pragma unroll 1
-                for (int cb = 0; cb < kCols; cb += 32) {
-                    float o[32];
-                    tmem_ld32(tO + o0 + cb, o);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) xch[(o0 + cb + i) * 128 + row] = o[i];
-                }
+        for (int w = 0; w < (C::kTwo ? 2 : 1); ++w) {
+            const int qr = w * 128 + row, r = r0 + qr;
+            const bool on = w * 128 + quad * 32 < live;  // (the same for the whole warp)
+            const bool both = !C::kTwo && nblk > 1;      // odd blocks' set has something
+            float mx = C::kTwo && w ? m_ref[1] : m_ref[0], sum = C::kTwo ? (w ? l1 : l0) : l0, a0 = 1.f, a1 = 0.f;
+            if (both) {
+                mx = fmaxf(m_ref[0], m_ref[1]);
+                a0 = fast_exp2(m_ref[0] - mx);
+                a1 = fast_exp2(m_ref[1] - mx);
+                sum = l0 * a0 + l1 * a1;
             }
-            named_barrier_sync(1, 256);
-            const float2 other = s_ml[(1 - w) * 128 + row];
-            mx = fmaxf(m_ref, other.x);
-            a0 = has ? fast_exp2(m_ref - mx) : 0.f;
-            a1 = (w == 1 || nblk > 1) ? fast_exp2(other.x - mx) : 0.f;
-            sum = l_sum * a0 + other.y * a1;
-        }
-        if (!idle) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
             const size_t slot = ((size_t)stream * p.R + r) * p.S + split;
-            const unsigned long long mk = s_mask[qrow];
+            const unsigned long long mk = s_mask[qr];
 #pragma unroll 1
-            for (int cb = 0; cb < kCols; cb += 32) {
+            for (int cb = c0; cb < c0 + D / 2; cb += 32) {
+                __syncwarp();
                 float o[32];
-                if (has) {
-                    tmem_ld32(tO + c0 + cb, o);
-                } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = 0.f;
-                }
-                if constexpr (!C::kTwo) {
+                for (int i = 0; i < 32; ++i) o[i] = 0.f;
+                if (on) {
+                    tmem_ld32(tbase + w * 256 + 128 + lane_addr + cb, o);
+                    if (both) {
+                        float o1[32];
+                        tmem_ld32(tbase + 256 + 128 + lane_addr + cb, o1);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        o[i] = a1 != 0.f ? fmaf(xch[(c0 + cb + i) * 128 + row], a1, o[i] * a0) : o[i] * a0;
+                        for (int i = 0; i < 32; ++i) o[i] = fmaf(o1[i], a1, o[i] * a0);
+                    }
                 }
                 if constexpr (C::kFloat) {
-                    if (*special && qrow < live) {
+                    if (*special && qr < live) {
                         for (int j = max(0, p0 - ctx); j < n && ctx + j < p1; ++j) {
                             if (!(mk >> j & 1ull)) continue;
                             int off;
@@ -781,13 +819,13 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                             const uint8_t* vr = p.V + (((size_t)pg * p.Hkv + hk) * p.page_rows + off) * C::kRb;
 #pragma unroll
                             for (int i = 0; i < 32; ++i) {
-                                const float v = v_one<KK>(vr, c0 + cb + i);
+                                const float v = v_one<KK>(vr, cb + i);
                                 if (!(fabsf(v) <= 65504.f)) o[i] += v;
                             }
                         }
                     }
                 }
-                if (qrow >= rows_here) continue;
+                if (qr >= rows_here) continue;
 #pragma unroll
                 for (int i = 0; i < 32; i += 8) {
                     float v[8];
@@ -795,27 +833,19 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                     for (int d = 0; d < 8; ++d)
                         v[d] = C::kPairs4 ? o[i + 2 * (d & 3) + (d >> 2)] * tc_v_step<KK>(d & 3) : o[i + d];
                     const float4 lo = make_float4(v[0], v[1], v[2], v[3]), hi = make_float4(v[4], v[5], v[6], v[7]);
-                    const int c = (c0 + cb + i) / 4;
+                    const int c = (cb + i) / 4;
                     if (direct) {
-                        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                        store_out(r, c, lo, inv);
-                        store_out(r, c + 1, hi, inv);
-                    } else {
+                        store_out(r, c, lo, on ? inv : 0.f);
+                        store_out(r, c + 1, hi, on ? inv : 0.f);
+                    } else if (on) {
                         float4* dst = reinterpret_cast<float4*>(p.ws_o + slot * D) + c;
                         __stcg(dst, lo);
                         __stcg(dst + 1, hi);
                     }
                 }
             }
-            if (!direct && qrow < rows_here && (C::kTwo || w == 0))
+            if (!direct && on && hf == 0 && qr < rows_here)
                 __stcg(reinterpret_cast<float2*>(p.ws_ml) + slot, make_float2(mx, sum));
-        } else if (qrow < rows_here && (C::kTwo || w == 0)) {
-            // rows past the sequence's nodes
-            if (direct) {
-                for (int c = 0; c < D / 4; ++c) store_out(r, c, make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
-            } else {
-                __stcg(reinterpret_cast<float2*>(p.ws_ml) + ((size_t)stream * p.R + r) * p.S + split, make_float2(kNegMax, 0.f));
-            }
         }
     }
     tc05_fence_before();

@@ -81,8 +81,8 @@ int launch_append_packed(int fmt, int in_type, const AppendParams& p, cudaStream
 int launch_accept_tree(const AcceptParams& p, int B, int layers, cudaStream_t st);
 int launch_fork_pages(const ForkParams& p, cudaStream_t st);
 int launch_compact_pages(const CompactParams& p, cudaStream_t st);
-// fp16 [rows][128] tensor map, 64-element x box_rows boxes, 128-byte swizzle.
-int encode_f16_rows_map(CUtensorMap* m, const void* base, long long rows, int box_rows);
+// fp16 [rows][dims] tensor map, 64-element x box_rows boxes, 128-byte swizzle.
+int encode_f16_rows_map(CUtensorMap* m, const void* base, long long rows, int box_rows, int dims = 128);
 
 }  // namespace host
 }  // namespace va

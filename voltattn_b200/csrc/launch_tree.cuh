@@ -12,8 +12,8 @@
 namespace va {
 namespace host {
 
-template <class C>
-int launch_tree_cfg(void (*kernel)(const TreeParams), const TreeParams& p, cudaStream_t st) {
+template <class C, class... Maps>
+int launch_tree_cfg(void (*kernel)(const TreeParams, const Maps...), const TreeParams& p, cudaStream_t st, const Maps&... maps) {
     int dev;
     int rc = current_device(&dev);
     if (rc) return rc;
@@ -36,19 +36,32 @@ int launch_tree_cfg(void (*kernel)(const TreeParams), const TreeParams& p, cudaS
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    VA_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+    VA_CUDA(cudaLaunchKernelEx(&cfg, kernel, p, maps...));
     return VA_OK;
+}
+
+template <class C>
+int launch_tree_tc(const TreeParams& p, cudaStream_t st) {
+    CUtensorMap tmK = {}, tmV = {};
+    if constexpr (C::kDirect) {  // boxes of a block's rows inside a page
+        const long long rows = (long long)p.num_pages * p.Hkv * p.page_rows;
+        if (rows >= (1ll << 31)) return VA_ERR_TOO_LARGE;
+        const int box = p.page_rows % C::kNb == 0 ? C::kNb : 8;
+        int rc = encode_f16_rows_map(&tmK, p.K, rows, box, C::kD);
+        if (!rc) rc = encode_f16_rows_map(&tmV, p.V, rows, box, C::kD);
+        if (rc) return rc;
+    }
+    return launch_tree_cfg<C>(decode_tree_tc_kernel<C>, p, st, tmK, tmV);
 }
 
 template <int D>
 int launch_tree_dim(int fmt, const TreeParams& p, int rows, cudaStream_t st) {
-#define VA_TREE_CFG(kernel, ...) return launch_tree_cfg<__VA_ARGS__>(kernel<__VA_ARGS__>, p, st)
-#define VA_TREE_KIND(kind)                                                                       \
-    do {                                                                                         \
-        if (rows == 16) VA_TREE_CFG(decode_tree_kernel, TreeCfg<kind, D, 1>);                    \
-        if (rows == 32) VA_TREE_CFG(decode_tree_kernel, TreeCfg<kind, D, 2>);                    \
-        if (rows == 128) VA_TREE_CFG(decode_tree_tc_kernel, TreeTcCfg<kind, D, false>);          \
-        VA_TREE_CFG(decode_tree_tc_kernel, TreeTcCfg<kind, D, true>);                            \
+#define VA_TREE_KIND(kind)                                                                               \
+    do {                                                                                                 \
+        if (rows == 16) return launch_tree_cfg<TreeCfg<kind, D, 1>>(decode_tree_kernel<TreeCfg<kind, D, 1>>, p, st); \
+        if (rows == 32) return launch_tree_cfg<TreeCfg<kind, D, 2>>(decode_tree_kernel<TreeCfg<kind, D, 2>>, p, st); \
+        if (rows == 128) return launch_tree_tc<TreeTcCfg<kind, D, false>>(p, st);                        \
+        return launch_tree_tc<TreeTcCfg<kind, D, true>>(p, st);                                          \
     } while (0)
     switch (fmt) {
         case VA_F16P: VA_TREE_KIND(Kind::F16);
@@ -60,7 +73,6 @@ int launch_tree_dim(int fmt, const TreeParams& p, int rows, cudaStream_t st) {
         default: return VA_ERR_UNSUPPORTED;
     }
 #undef VA_TREE_KIND
-#undef VA_TREE_CFG
 }
 
 }  // namespace host
