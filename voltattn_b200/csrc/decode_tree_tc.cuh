@@ -3,15 +3,16 @@
 // query rows, with tcgen05.mma and accumulators in tensor memory.
 //
 // One CTA per (sequence, KV head, tile of query rows, range of positions), one
-// per SM, 14 warps (4 on an SM sub-partition at most: 128 registers a thread):
-//   warps 0-7    softmax: thread (half hf, row r) has 32 of a job's 64 positions of
-//                query row r (TMEM lane r);
-//   warps 8-11   producers: codes -> exact fp16 codes in swizzled tiles;
-//   warp 12      one elected lane issues every tcgen05.mma;
-//   warp 13      copies: blocks of codes and scales into a ring, several ahead (fp16
+// per SM, 22 warps:
+//   warps 0-15   softmax: thread (set w, half hf, row r) has 32 of the 64 positions of
+//                query row r (TMEM lane r) in the jobs of set w;
+//   warps 16-19  producers: codes -> exact fp16 codes in swizzled tiles;
+//   warp 20      one elected lane issues every tcgen05.mma;
+//   warp 21      copies: blocks of codes and scales into a ring, several ahead (fp16
 //                rows by tensor copies straight into the swizzled tiles).
 // A job is one block of 64 positions against 128 query rows; the jobs alternate
-// between two sets w of TMEM columns (S_w, O_w, 256 each). kTwo = false (up to 128
+// between two sets w of TMEM columns (S_w, O_w, 256 each) and of softmax warps, so
+// one set's exponentials run under the other's loads, exchange and MMAs. kTwo = false (up to 128
 // query rows): job j is block j, and O_0, O_1 (even and odd blocks) merge at the end.
 // kTwo = true (up to 256): jobs 2 i, 2 i + 1 are block i against rows 0..127 and
 // 128..255, so a decoded tile serves twice.
@@ -53,7 +54,7 @@ struct TreeTcCfg {
     static constexpr int kRb = kDim * KindTraits<K>::kBits / 8;
     static constexpr int kNb = 64;                 // positions of a block
     static constexpr int kProducers = 128;
-    static constexpr int kThreads = 14 * 32;
+    static constexpr int kThreads = 22 * 32;
     static constexpr int kQTile = 128 * kDim * 2;
     static constexpr int kTile = kNb * kDim * 2;   // one K or V tile
     static constexpr bool kDirect = K == Kind::F16;  // tiles by tensor copies
@@ -67,18 +68,18 @@ struct TreeTcCfg {
     static constexpr int kRawTx = kRawSV + kNb * kSb;
     static constexpr int kRawStage = (kRawTx + 127) / 128 * 128;
     // what follows the ring: scales as floats [4 slots][K, V][kNG][64], masks,
-    // [2][2][128] maxima or sums, barriers, ev[4], TMEM slot, fail, special, ticket
+    // [2][2][2][128] maxima or sums, barriers, ev[4], TMEM slot, fail, special, ticket
     static constexpr int kScaleSlots = 4;
     static constexpr int kScaleSlot = 2 * kNG * kNb * 4;
     static constexpr int kScaleV = kNG * kNb * 4;  // where a slot's V scales begin
     static constexpr int kScaleBytes = kScaled ? kScaleSlots * kScaleSlot : 0;
-    static constexpr int kRest = kScaleBytes + kRows * 8 + 2 * 128 * 8 + 512 + 64;
+    static constexpr int kRest = kScaleBytes + kRows * 8 + 4096 + 512 + 64;
     static constexpr int kRoom = (227 * 1024 - 1024 - kOffRaw - kRest) / kRawStage;
     static constexpr int kRawStages = kDirect ? 1 : kRoom < 8 ? kRoom : 8;
     static constexpr int kOffScales = kOffRaw + (kDirect ? 0 : kRawStages * kRawStage);
     static constexpr int kOffMask = kOffScales + kScaleBytes;
     static constexpr int kOffMl = kOffMask + kRows * 8;
-    static constexpr int kOffBars = kOffMl + 2 * 128 * 8;
+    static constexpr int kOffBars = kOffMl + 4096;
     static constexpr int kBars = 2 * kKS + 3 * kVS + 2 * 2 + 2 + kScaleSlots + 2 * kRawStages;
     static constexpr int kOffMisc = kOffBars + kBars * 8;
     static constexpr int kSmemBytes = 1024 + kOffMisc + 64;
@@ -203,6 +204,24 @@ __device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
     return d;
 }
 
+// 16 consecutive fp32 columns of this thread's TMEM lane, without the wait (as
+// tmem_ld32_nowait), and the tie to it.
+__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_tie16(uint32_t* r) {
+    asm volatile(""
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15]));
+}
+
 // True in one lane of the (converged) warp. The values around it stay warp-uniform,
 // so the operands of the MMAs need no move from vector to uniform registers.
 __device__ __forceinline__ bool elect_one() {
@@ -238,7 +257,7 @@ __device__ __forceinline__ bool clear_not_finite(uint4& v) {
 template <class C>
 __device__ __forceinline__ void tree_tc_fix_v(int p0, int len, int ctx, int nblk, uint8_t* smem, uint64_t* vraw,
                                               uint64_t* vfull, volatile int* special, volatile int* fail) {
-    const int t = (int)threadIdx.x - 256, lane = t & 31, row = t >> 1;
+    const int t = (int)threadIdx.x - 512, lane = t & 31, row = t >> 1;
     for (int i = 0; i < nblk; ++i) {
         const int s = i % C::kVS, pb = p0 + i * C::kNb;
         if (!mbar_wait_bounded(vraw + s, (uint32_t)(i / C::kVS) & 1u)) {
@@ -271,7 +290,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     constexpr int D = C::kD, NG = C::kNG, NB = C::kNb, KS = C::kKS, VS = C::kVS, SG = C::kSG;
     constexpr Kind KK = C::kKind;
     unsigned long long* s_mask = reinterpret_cast<unsigned long long*>(smem + C::kOffMask);
-    float* s_xch = reinterpret_cast<float*>(smem + C::kOffMl);  // [2][2][128]
+    float* s_xch = reinterpret_cast<float*>(smem + C::kOffMl);  // [2][2][2][128]
     uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
     uint64_t *kempty = kfull + KS, *vfull = kempty + KS, *vempty = vfull + VS, *sfull = vempty + VS;
     uint64_t *pfull = sfull + 2, *odone = pfull + 2, *fin = odone + 1, *scfull = fin + 1;
@@ -318,7 +337,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
 
     const int nblk = (p1 - p0 + NB - 1) / NB;
     const int njobs = C::kTwo ? 2 * nblk : nblk;
-    if (warp == 12) tmem_alloc(tslot, 512);
+    if (warp == 20) tmem_alloc(tslot, 512);
     if (tid == 0) {
         for (int i = 0; i < KS; ++i) mbar_init(kfull + i, C::kDirect ? 1 : C::kProducers / 32), mbar_init(kempty + i, 1);
         for (int i = 0; i < VS; ++i) mbar_init(vfull + i, C::kProducers / 32), mbar_init(vempty + i, 1);
@@ -368,15 +387,16 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     const uint32_t tbase = *tslot;
     const uint32_t sbase = smem_u32(smem);
 
-    // softmax threads: the reference (log2 units) and their half's sum of each set
-    float m_ref[2] = {kNegMax, kNegMax}, l_sum[2] = {0.f, 0.f};
-    const int hf = warp >> 2, row = tid & 127, quad = warp & 3;
+    // softmax threads: the reference (log2 units) and their half's sum
+    float m_ref = kNegMax, l_sum = 0.f;
+    const int set = warp >> 3, hf = (warp >> 2) & 1, row = tid & 127, quad = warp & 3;
     const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
-    if (warp < 8) {
+    if (warp < 16) {
         // ---- softmax -------------------------------------------------------------
         const float c2 = rsqrtf((float)D) * kLog2e * tc_k_inv_step<KK>();
-        for (int j = 0; j < njobs; ++j) {
-            const int w = j & 1, k = j >> 1, blk = C::kTwo ? k : j;
+        const int w = set;
+        for (int j = w; j < njobs; j += 2) {
+            const int k = j >> 1, blk = C::kTwo ? k : j;
             const int pb = p0 + blk * NB;
             bool ok = mbar_wait_fast(sfull + w, (uint32_t)k & 1u);
             // (a slot of scales is written again only after this block's PV, so this phase
@@ -395,33 +415,34 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                 asm volatile("" : "+r"(sc));  // the loads of scales come after the waits
                 const uint32_t tS = tbase + w * 256 + lane_addr, tO = tS + 128;
                 float x[32];
-                {
-                    uint32_t s0[32], s1[32];
-                    tmem_ld32_nowait(tS + 32 * hf, s0);
-                    if constexpr (SG == 2) tmem_ld32_nowait(tS + 64 + 32 * hf, s1);
-                    tmem_wait_ld_only();
-                    tmem_tie32(s0);
-                    if constexpr (SG == 2) tmem_tie32(s1);
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4) {
+                for (int cb = 0; cb < 32; cb += 16) {
+                    uint32_t s0[16], s1[16];
+                    tmem_ld16_nowait(tS + 32 * hf + cb, s0);
+                    if constexpr (SG == 2) tmem_ld16_nowait(tS + 64 + 32 * hf + cb, s1);
+                    tmem_wait_ld_only();
+                    tmem_tie16(s0);
+                    if constexpr (SG == 2) tmem_tie16(s1);
+#pragma unroll
+                    for (int c = 0; c < 16; c += 4) {
                         float2 u = make_float2(__uint_as_float(s0[c]), __uint_as_float(s0[c + 1]));
                         float2 v = make_float2(__uint_as_float(s0[c + 2]), __uint_as_float(s0[c + 3]));
                         if constexpr (C::kScaled) {
-                            const float4 k0 = lds_f4(sc + 4 * (32 * hf + c));
+                            const float4 k0 = lds_f4(sc + 4 * (32 * hf + cb + c));
                             u = fmul2(u, make_float2(k0.x, k0.y));
                             v = fmul2(v, make_float2(k0.z, k0.w));
                             if constexpr (SG == 2) {
-                                const float4 k1 = lds_f4(sc + 4 * (NB + 32 * hf + c));
+                                const float4 k1 = lds_f4(sc + 4 * (NB + 32 * hf + cb + c));
                                 u = ffma2(make_float2(__uint_as_float(s1[c]), __uint_as_float(s1[c + 1])),
                                           make_float2(k1.x, k1.y), u);
                                 v = ffma2(make_float2(__uint_as_float(s1[c + 2]), __uint_as_float(s1[c + 3])),
                                           make_float2(k1.z, k1.w), v);
                             }
                         }
-                        x[c] = u.x;
-                        x[c + 1] = u.y;
-                        x[c + 2] = v.x;
-                        x[c + 3] = v.y;
+                        x[cb + c] = u.x;
+                        x[cb + c + 1] = u.y;
+                        x[cb + c + 2] = v.x;
+                        x[cb + c + 3] = v.y;
                     }
                 }
                 // which of its 32 columns the row sees
@@ -444,26 +465,27 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                 }
                 // the row's maximum over both halves; their barrier also puts every load of S
                 // before the stores of P' below
-                float* xch = s_xch + (j & 1) * 256;
+                float* xch = s_xch + w * 512 + (k & 1) * 256;
                 xch[hf * 128 + row] = fmaxf(b0, b1);
-                named_barrier_sync(2 + quad, 64);
+                named_barrier_sync(2 + w * 4 + quad, 64);
                 const float bm = fmaxf(fmaxf(b0, b1), xch[(1 - hf) * 128 + row]);
                 const float ev = C::kScaled ? s_ev[blk % C::kScaleSlots] : 0.f;
-                const float m = w ? m_ref[1] : m_ref[0];
                 const float want = bm == kNegMax ? kNegMax : fmaf(bm, c2, ev - 10.f);
-                const float nref = want > m + 4.f ? want : m;
-                float l = w ? l_sum[1] : l_sum[0];
-                if (__any_sync(0xffffffffu, nref != m)) {
-                    const float corr = fast_exp2(m - nref);
-                    l *= corr;
+                const float nref = want > m_ref + 4.f ? want : m_ref;
+                if (__any_sync(0xffffffffu, nref != m_ref)) {
+                    const float corr = fast_exp2(m_ref - nref);
+                    l_sum *= corr;
+                    m_ref = nref;
                     if (k > 0) {  // this half of the row's O
 #pragma unroll 1
-                        for (int cb = 0; cb < D / 2; cb += 32) {
-                            float o[32];
-                            tmem_ld32(tO + hf * (D / 2) + cb, o);
+                        for (int cb = 0; cb < D / 2; cb += 16) {
+                            uint32_t o[16];
+                            tmem_ld16_nowait(tO + hf * (D / 2) + cb, o);
+                            tmem_wait_ld_only();
+                            tmem_tie16(o);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] *= corr;
-                            tmem_st32(tO + hf * (D / 2) + cb, o);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                            tmem_st16_u(tO + hf * (D / 2) + cb, o);
                         }
                     }
                 }
@@ -509,9 +531,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                 };
                 if (tail) weights(std::true_type{});
                 else weights(std::false_type{});
-                l += sum.x + sum.y;
-                if (w) m_ref[1] = nref, l_sum[1] = l;
-                else m_ref[0] = nref, l_sum[0] = l;
+                l_sum += sum.x + sum.y;
                 tmem_wait_st();
             }
             tc05_fence_before();
@@ -523,12 +543,12 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
             *fail = 1;
         }
         tc05_fence_after();
-    } else if (C::kDirect && warp < 12) {
+    } else if (C::kDirect && warp < 20) {
         tree_tc_fix_v<C>(p0, len, ctx, nblk, smem, vraw, vfull, special, fail);
-    } else if (!C::kDirect && warp < 12) {
+    } else if (!C::kDirect && warp < 20) {
         // ---- producers: K of block i + 1 before V of block i, so the next scores never
         // wait for this block's PV. A thread takes two slices (row, quarter of the dims) -----
-        const int pw = warp - 8;
+        const int pw = warp - 16;
         // lane bits: quarter bit 0, row bits 0..1, quarter bit 1, row bit 2: eight
         // neighbouring lanes store to eight different 16-byte banks
         const int q = (lane & 1) | ((lane >> 2) & 2), row0 = pw * 16 + ((lane >> 1) & 3) + ((lane >> 4) << 2);
@@ -631,7 +651,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
             if (lane == 0) report_error(kErrEmptyWait);
             *fail = 1;
         }
-    } else if (C::kDirect && warp == 13) {
+    } else if (C::kDirect && warp == 21) {
         // ---- copies of fp16 rows: tensor copies of 64 dims by the block's rows inside a
         // page (boxes of 64 or 8 rows) into the swizzled tiles; lane = run + 8 * group
         const int run = p.page_rows % NB == 0 ? NB : 8, at = (lane & 7) * run, g = lane >> 3;
@@ -667,7 +687,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
             if (!mbar_wait_bounded(kfull + k % KS, (uint32_t)(k / KS) & 1u) ||
                 !mbar_wait_bounded(vraw + k % VS, (uint32_t)(k / VS) & 1u))
                 *fail = 1;
-    } else if (!C::kDirect && warp == 13) {
+    } else if (!C::kDirect && warp == 21) {
         // ---- copies: lane 4 r + k brings run r of buffer k (K, V, their scales): the
         // whole block when it lies inside a page, else runs of 8 rows
         const bool whole = p.page_rows % NB == 0;
@@ -767,90 +787,95 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     __syncthreads();
     tc05_fence_after();
     if (*fail) {
-        if (warp == 12) tmem_dealloc(tbase, 512);
+        if (warp == 20) tmem_dealloc(tbase, 512);
         return;
     }
     grid_launch_dependents();
 
-    // ---- epilogue: a thread's row (of each tile), its half of the dims ------------------
+    // ---- epilogue: a thread's row, its part of the dims: half of them (two tiles: of its
+    // set's tile) or a quarter (one tile: both sets' outputs merged)
     const bool direct = nsplit == 1;
-    if (warp < 8) {
-        s_xch[hf * 128 + row] = l_sum[0];
-        s_xch[256 + hf * 128 + row] = l_sum[1];
-        named_barrier_sync(1, 256);
-        const float l0 = l_sum[0] + s_xch[(1 - hf) * 128 + row], l1 = l_sum[1] + s_xch[256 + (1 - hf) * 128 + row];
-        const int c0 = hf * (D / 2);
+    if (warp < 16) {
+        s_xch[(set * 2 + hf) * 128 + row] = l_sum;
+        if (hf == 0) s_xch[512 + set * 128 + row] = m_ref;
+        named_barrier_sync(1, 512);
+        const auto sum_of = [&](int w) { return s_xch[w * 256 + row] + s_xch[w * 256 + 128 + row]; };
+        const int qr = (C::kTwo ? set * 128 : 0) + row, r = r0 + qr;
+        const bool on = (C::kTwo ? set * 128 : 0) + quad * 32 < live;  // (the same for the whole warp)
+        const bool both = !C::kTwo && nblk > 1;                        // the odd blocks' set has something
+        const int w0 = C::kTwo ? set : 0;
+        float mx = s_xch[512 + w0 * 128 + row], sum = sum_of(w0), a0 = 1.f, a1 = 0.f;
+        if (both) {
+            const float m0 = mx, m1 = s_xch[512 + 128 + row];
+            mx = fmaxf(m0, m1);
+            a0 = fast_exp2(m0 - mx);
+            a1 = fast_exp2(m1 - mx);
+            sum = sum * a0 + sum_of(1) * a1;
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const size_t slot = ((size_t)stream * p.R + r) * p.S + split;
+        constexpr int kCols = C::kTwo ? D / 2 : D / 4;
+        const int c0 = C::kTwo ? hf * kCols : (set * 2 + hf) * kCols;
 #pragma unroll 1
-        for (int w = 0; w < (C::kTwo ? 2 : 1); ++w) {
-            const int qr = w * 128 + row, r = r0 + qr;
-            const bool on = w * 128 + quad * 32 < live;  // (the same for the whole warp)
-            const bool both = !C::kTwo && nblk > 1;      // odd blocks' set has something
-            float mx = C::kTwo && w ? m_ref[1] : m_ref[0], sum = C::kTwo ? (w ? l1 : l0) : l0, a0 = 1.f, a1 = 0.f;
-            if (both) {
-                mx = fmaxf(m_ref[0], m_ref[1]);
-                a0 = fast_exp2(m_ref[0] - mx);
-                a1 = fast_exp2(m_ref[1] - mx);
-                sum = l0 * a0 + l1 * a1;
-            }
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            const size_t slot = ((size_t)stream * p.R + r) * p.S + split;
-            const unsigned long long mk = s_mask[qr];
-#pragma unroll 1
-            for (int cb = c0; cb < c0 + D / 2; cb += 32) {
-                __syncwarp();
-                float o[32];
+        for (int cb = c0; cb < c0 + kCols; cb += 16) {
+            __syncwarp();
+            float o[16];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = 0.f;
-                if (on) {
-                    tmem_ld32(tbase + w * 256 + 128 + lane_addr + cb, o);
-                    if (both) {
-                        float o1[32];
-                        tmem_ld32(tbase + 256 + 128 + lane_addr + cb, o1);
+            for (int i = 0; i < 16; ++i) o[i] = 0.f;
+            if (on) {
+                uint32_t u[16], v[16];
+                tmem_ld16_nowait(tbase + w0 * 256 + 128 + lane_addr + cb, u);
+                if (both) tmem_ld16_nowait(tbase + 256 + 128 + lane_addr + cb, v);
+                tmem_wait_ld_only();
+                tmem_tie16(u);
+                tmem_tie16(v);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = fmaf(o1[i], a1, o[i] * a0);
-                    }
+                for (int i = 0; i < 16; ++i) {
+                    o[i] = __uint_as_float(u[i]);
+                    if (both) o[i] = fmaf(__uint_as_float(v[i]), a1, o[i] * a0);
                 }
-                if constexpr (C::kFloat) {
-                    if (*special && qr < live) {
-                        for (int j = max(0, p0 - ctx); j < n && ctx + j < p1; ++j) {
-                            if (!(mk >> j & 1ull)) continue;
-                            int off;
-                            const int pg = page_of(ctx + j, off);
-                            const uint8_t* vr = p.V + (((size_t)pg * p.Hkv + hk) * p.page_rows + off) * C::kRb;
+            }
+            if constexpr (C::kFloat) {
+                if (*special && qr < live) {
+                    const unsigned long long mk = s_mask[qr];
+                    for (int j = max(0, p0 - ctx); j < n && ctx + j < p1; ++j) {
+                        if (!(mk >> j & 1ull)) continue;
+                        int off;
+                        const int pg = page_of(ctx + j, off);
+                        const uint8_t* vr = p.V + (((size_t)pg * p.Hkv + hk) * p.page_rows + off) * C::kRb;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                const float v = v_one<KK>(vr, cb + i);
-                                if (!(fabsf(v) <= 65504.f)) o[i] += v;
-                            }
+                        for (int i = 0; i < 16; ++i) {
+                            const float x = v_one<KK>(vr, cb + i);
+                            if (!(fabsf(x) <= 65504.f)) o[i] += x;
                         }
                     }
                 }
-                if (qr >= rows_here) continue;
+            }
+            if (qr >= rows_here) continue;
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    float v[8];
+            for (int i = 0; i < 16; i += 8) {
+                float v[8];
 #pragma unroll
-                    for (int d = 0; d < 8; ++d)
-                        v[d] = C::kPairs4 ? o[i + 2 * (d & 3) + (d >> 2)] * tc_v_step<KK>(d & 3) : o[i + d];
-                    const float4 lo = make_float4(v[0], v[1], v[2], v[3]), hi = make_float4(v[4], v[5], v[6], v[7]);
-                    const int c = (cb + i) / 4;
-                    if (direct) {
-                        store_out(r, c, lo, on ? inv : 0.f);
-                        store_out(r, c + 1, hi, on ? inv : 0.f);
-                    } else if (on) {
-                        float4* dst = reinterpret_cast<float4*>(p.ws_o + slot * D) + c;
-                        __stcg(dst, lo);
-                        __stcg(dst + 1, hi);
-                    }
+                for (int d = 0; d < 8; ++d)
+                    v[d] = C::kPairs4 ? o[i + 2 * (d & 3) + (d >> 2)] * tc_v_step<KK>(d & 3) : o[i + d];
+                const float4 lo = make_float4(v[0], v[1], v[2], v[3]), hi = make_float4(v[4], v[5], v[6], v[7]);
+                const int c = (cb + i) / 4;
+                if (direct) {
+                    store_out(r, c, lo, on ? inv : 0.f);
+                    store_out(r, c + 1, hi, on ? inv : 0.f);
+                } else if (on) {
+                    float4* dst = reinterpret_cast<float4*>(p.ws_o + slot * D) + c;
+                    __stcg(dst, lo);
+                    __stcg(dst + 1, hi);
                 }
             }
-            if (!direct && on && hf == 0 && qr < rows_here)
-                __stcg(reinterpret_cast<float2*>(p.ws_ml) + slot, make_float2(mx, sum));
         }
+        if (!direct && on && c0 == 0 && qr < rows_here)
+            __stcg(reinterpret_cast<float2*>(p.ws_ml) + slot, make_float2(mx, sum));
     }
     tc05_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 20) {
         tc05_fence_after();
         tmem_dealloc(tbase, 512);
     }
