@@ -2,7 +2,6 @@
 // in include/voltattn.h): argument checks, workspace layout and launch.
 #include <algorithm>
 #include <climits>
-#include <cstdlib>
 
 #include "../../include/voltattn.h"
 #include "cache_rows.cuh"
@@ -39,16 +38,11 @@ int check_pool(int fmt, const va_bufs* b, int B, int max_pages, int Hkv, int pag
     return VA_OK;
 }
 
-// Rows of a CTA's tile of query rows: 16 or 32 (decode_tree.cuh), 128 or 256
-// (decode_tree_tc.cuh). VOLTATTN_TREE_ROWS overrides for measurements.
-int tree_rows(int R) {
-    static const int forced = [] {
-        const char* e = std::getenv("VOLTATTN_TREE_ROWS");
-        return e ? std::atoi(e) : 0;
-    }();
-    if (forced) return forced;
-    return R <= 16 ? 16 : R <= 128 ? 128 : 256;
-}
+// Rows of a CTA's tile of query rows: 16 (decode_tree.cuh), 128 or 256
+// (decode_tree_tc.cuh). Measured on B200 at 64 rows: 113 us in four tiles of 16
+// against 137 in one of 128 (8-bit cache, 590000 positions x heads); at 128 rows 598
+// against 313 (4-bit, 1.6 million).
+int tree_rows(int R) { return R <= 64 ? 16 : R <= 128 ? 128 : 256; }
 
 // Completion counters, one per (sequence, KV head, row tile), at the front of the
 // workspace: a fixed number, so the slots of a call never lie where a call of
@@ -64,8 +58,8 @@ int tree_splits(int nsm, int B, int Hkv, int R, int Lmax) {
     const int rows = tree_rows(R);
     const double ctas = (double)B * Hkv * ((R + rows - 1) / rows);
     if (ctas > (double)kCounters) return 1;
-    const double cap = (double)nsm * (rows == 16 ? 3 : rows == 32 ? 2 : 1);
-    const double fixed = rows <= 32 ? 128.0 : 384.0;
+    const double cap = (double)nsm * (rows == 16 ? 3 : 1);
+    const double fixed = rows == 16 ? 128.0 : 384.0;
     const int units = (Lmax + kTreeUnit - 1) / kTreeUnit;
     double best = 1e300;
     int S = 1;

@@ -10,7 +10,7 @@
 // in the running form of a softmax; a row that sees nothing gives 0.
 //
 // All G * Q query rows of a (sequence, KV head) read the same cache rows, so
-// a CTA takes a tile of 16 or 32 query rows (row r: node r / G, query head
+// a CTA takes a tile of 16 query rows (row r: node r / G, query head
 // r % G of the group) over a range of the sequence's positions, and streams
 // the codes once. Its four warps take blocks of positions in turn, each with
 // its own running statistics and its own ring of shared-memory stages that one
@@ -27,8 +27,8 @@
 //     fp16 (P' = fp16(w * scale), one P' per group).
 // The rounding of P' is the only one below 32 bits: it is relative (2^-11)
 // because the exponent's reference is kept so that P' of the largest weight
-// lies in [2^13, 2^15): ref = max over blocks of (row maximum + exponent of
-// the block's largest V scale - 13), in log2 units.
+// lies in [2^9, 2^15): ref follows (row maximum + exponent of the largest V scale
+// - 12), in log2 units, and is left while that grows by no more than 2.
 //
 // Rows that a query row does not see have no influence at all on it: their
 // scores are replaced, their weights selected to 0 before the scale (which may
@@ -43,6 +43,7 @@
 
 #include "common.cuh"
 #include "formats.cuh"
+#include "prefill_tc.cuh"
 
 namespace va {
 
@@ -76,12 +77,11 @@ __device__ __forceinline__ int tree_chunk(int len, int S) {
     return max(1, (units + S - 1) / S) * kTreeUnit;
 }
 
-template <Kind K, int kDim, int kMTiles>
+template <Kind K, int kDim>
 struct TreeCfg {
     static constexpr Kind kKind = K;
     static constexpr int kD = kDim;
-    static constexpr int kMT = kMTiles;           // 16-row tiles of query rows
-    static constexpr int kRows = 16 * kMTiles;    // query rows of a CTA
+    static constexpr int kRows = 16;              // query rows of a CTA
     static constexpr int kNG = kDim / 64;         // scale groups
     static constexpr bool kScaled = !(K == Kind::F16 || K == Kind::BF16);
     static constexpr bool kFloat = is_float_kind(K);  // rows that can hold inf / nan
@@ -104,7 +104,7 @@ struct TreeCfg {
     static constexpr int kBig = kRing > kMerge ? kRing : kMerge;
     // + barriers, masks, (ref, l) of every warp and row, the ticket
     static constexpr int kSmemBytes = kBig + kWarps * kStages * 8 + kRows * 8 + kWarps * kRows * 8 + 16;
-    static constexpr int kMinCtas = kMTiles == 1 ? 3 : 2;
+    static constexpr int kMinCtas = 3;
 };
 
 __device__ __forceinline__ void mma_f16_16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -305,8 +305,12 @@ __device__ __forceinline__ float v_one(const uint8_t* row, int d) {
     else return __low2float(bits_h2(f8x2_to_h2(row[d])));
 }
 
-__device__ __forceinline__ bool h2_not_finite(uint32_t u) {
-    return (u & 0x7C00u) == 0x7C00u || (u & 0x7C000000u) == 0x7C000000u;
+// Clears the halves of an fp16 pair that are not finite; true if there were any.
+__device__ __forceinline__ bool clear_not_finite(uint32_t& u) {
+    bool any = false;
+    if ((u & 0x7C00u) == 0x7C00u) u &= 0xFFFF0000u, any = true;
+    if ((u & 0x7C000000u) == 0x7C000000u) u &= 0xFFFFu, any = true;
+    return any;
 }
 
 // The last range of a row tile merges all of them, in order: first the weights of
@@ -374,7 +378,7 @@ __device__ __forceinline__ void tree_merge(const TreeParams& p, int stream, int 
 template <class C>
 __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(const TreeParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
-    constexpr int D = C::kD, NG = C::kNG, MT = C::kMT, PB = C::kPb;
+    constexpr int D = C::kD, NG = C::kNG, PB = C::kPb;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBig);
     unsigned long long* s_mask = reinterpret_cast<unsigned long long*>(bars + C::kWarps * C::kStages);
     float2* s_ml = reinterpret_cast<float2*>(s_mask + C::kRows);
@@ -451,13 +455,11 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
 
     // the query rows as A fragments, 16 dims (64 gr + 16 t ..) of rows g and
     // g + 8 per lane, in the order of k_chunk's pairs; sums of q per group
-    uint32_t qa[MT][NG][4][4];
-    float qsum[MT][NG][2];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
+    uint32_t qa[NG][4][4];
+    float qsum[NG][2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const int r = r0 + 16 * m + g + 8 * e;
+            const int r = r0 + g + 8 * e;
             const int node = r / p.G;
             const bool ok = r < p.R && node < n;
             const __half* src = p.q + b * p.qs_b + (ok ? node : 0) * p.qs_t + (long long)(hk * p.G + (ok ? r - node * p.G : 0)) * p.qs_h;
@@ -476,29 +478,24 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
                     constexpr Kind KK = C::kKind;
                     const int d0 = k_dim<KK>(i, 0), d1 = k_dim<KK>(i, 1);
                     const uint32_t sel = ((d0 & 1) ? 0x32u : 0x10u) | ((d1 & 1) ? 0x7600u : 0x5400u);
-                    qa[m][gr][i >> 1][e + 2 * (i & 1)] = __byte_perm(w[d0 >> 1], w[d1 >> 1], sel);
+                    qa[gr][i >> 1][e + 2 * (i & 1)] = __byte_perm(w[d0 >> 1], w[d1 >> 1], sel);
                     const float2 f = __half22float2(bits_h2(w[i]));
                     sum += f.x + f.y;
                 }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                qsum[m][gr][e] = -TreeCode<C::kKind>::kOffset * sum;
+                qsum[gr][e] = -TreeCode<C::kKind>::kOffset * sum;
             }
         }
-    }
 
-    float o[MT][NG][8][4];
+    float o[NG][8][4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int gr = 0; gr < NG; ++gr)
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr)
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) o[m][gr][i][k] = 0.f;
-    float ref[MT][2], l[MT][2];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) ref[m][0] = ref[m][1] = kNegMax, l[m][0] = l[m][1] = 0.f;
+            for (int k = 0; k < 4; ++k) o[gr][i][k] = 0.f;
+    float ref[2] = {kNegMax, kNegMax}, l[2] = {0.f, 0.f};  // rows g and g + 8
     // scores in log2 units per unit of the raw product
     const float c2 = rsqrtf((float)D) * kLog2e * TreeCode<C::kKind>::kInvStep;
 
@@ -507,153 +504,143 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
     const auto block = [&](auto is_tail, const uint8_t* st, int pb) {
         constexpr bool tail = decltype(is_tail)::value;
         constexpr int NT = PB / 8;  // 8-position tiles of S
-        float x[MT][NT][4];         // scores, then weights
+        // scores, then weights: row g + 8 r, this lane's positions t + 8 (nt & 1) (.x) and + 4 (.y) of
+        // the 16 of tiles nt, nt ^ 1
+        float2 x[NT][2];
         __half2 vmax = __float2half2_rn(0.f);
-        uint32_t vsc[NT][2];        // V scales of this lane's positions (both groups)
+        uint32_t vsc[NT][2];  // V scales of the two positions (both groups)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             // S of 8 positions: lane g decodes row (g >> 1) + 4 (g & 1) (+ 8 for odd tiles) of the 16
             const uint8_t* krow = st + (16 * (nt >> 1) + (g >> 1) + 4 * (g & 1) + 8 * (nt & 1)) * C::kRb;
-            float acc[MT][NG][4];
+            float acc[NG][4];
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
                 uint32_t h[8];
                 k_chunk<C::kKind>(krow, gr, t, h);
+                float* a = acc[C::kScaled ? gr : 0];
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    float* a = acc[m][C::kScaled ? gr : 0];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        if (k == 0 && (C::kScaled || gr == 0))
-                            mma_f16_16816_init(a, qa[m][gr][k], h[0], h[1], C::kFloat ? 0.f : qsum[m][gr][0],
-                                               C::kFloat ? 0.f : qsum[m][gr][1]);
-                        else mma_f16_16816(a, qa[m][gr][k], h[2 * k], h[2 * k + 1]);
-                    }
+                for (int k = 0; k < 4; ++k) {
+                    if (k == 0 && (C::kScaled || gr == 0))
+                        mma_f16_16816_init(a, qa[gr][k], h[0], h[1], C::kFloat ? 0.f : qsum[gr][0],
+                                           C::kFloat ? 0.f : qsum[gr][1]);
+                    else mma_f16_16816(a, qa[gr][k], h[2 * k], h[2 * k + 1]);
                 }
             }
-            // this lane's columns: positions t and t + 4 (+ 8) of the 16
+            float2 ks[NG];
+            if constexpr (C::kScaled) {
+                float2 f[2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int pr = 16 * (nt >> 1) + t + 4 * e + 8 * (nt & 1);
-                if constexpr (C::kScaled) {
-                    float ks[NG];
+                for (int e = 0; e < 2; ++e) {
+                    const int pr = 16 * (nt >> 1) + t + 4 * e + 8 * (nt & 1);
+                    uint32_t k;
                     if constexpr (NG == 2) {
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(st + C::kOffSK + 4 * pr));
-                        ks[0] = f.x;
-                        ks[1] = f.y;
+                        k = *reinterpret_cast<const uint32_t*>(st + C::kOffSK + 4 * pr);
                         vsc[nt][e] = *reinterpret_cast<const uint32_t*>(st + C::kOffSV + 4 * pr);
                     } else {
-                        ks[0] = __half2float(*reinterpret_cast<const __half*>(st + C::kOffSK + 2 * pr));
+                        k = *reinterpret_cast<const uint16_t*>(st + C::kOffSK + 2 * pr);
                         vsc[nt][e] = *reinterpret_cast<const uint16_t*>(st + C::kOffSV + 2 * pr);
                     }
-                    uint32_t va = vsc[nt][e] & 0x7FFF7FFFu;
+                    f[e] = __half22float2(bits_h2(k));
+                    uint32_t va = vsc[nt][e];
                     if constexpr (tail) {
                         if (pb + pr >= len) vsc[nt][e] = va = 0u;
                         // an infinite scale of a row that not all rows see is no measure
+                        va &= 0x7FFF7FFFu;
                         if ((va & 0x7FFFu) >= 0x7C00u) va &= 0x7FFF0000u;
                         if ((va >> 16) >= 0x7C00u) va &= 0x7FFFu;
                     }
-                    vmax = __hmax2(vmax, bits_h2(va));
-#pragma unroll
-                    for (int m = 0; m < MT; ++m)
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            float v = acc[m][0][2 * r + e] * ks[0];
-                            if constexpr (NG == 2) v = fmaf(acc[m][1][2 * r + e], ks[1], v);
-                            x[m][nt][2 * r + e] = v;
-                        }
-                } else {
-#pragma unroll
-                    for (int m = 0; m < MT; ++m)
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) x[m][nt][2 * r + e] = acc[m][0][2 * r + e];
+                    vmax = __hmax2(vmax, __habs2(bits_h2(va)));
                 }
+                ks[0] = make_float2(f[0].x, f[1].x);
+                if constexpr (NG == 2) ks[NG - 1] = make_float2(f[0].y, f[1].y);
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float2 v = make_float2(acc[0][2 * r], acc[0][2 * r + 1]);
+                if constexpr (C::kScaled) {
+                    v = fmul2(v, ks[0]);
+                    if constexpr (NG == 2) v = ffma2(make_float2(acc[NG - 1][2 * r], acc[NG - 1][2 * r + 1]), ks[NG - 1], v);
+                }
+                x[nt][r] = v;
             }
         }
-        uint32_t seen[MT][2];  // which of this lane's columns a row sees (bit 2 nt + e)
+        uint32_t seen[2];  // which of this lane's columns a row sees (bit 2 nt + e)
         if constexpr (tail) {
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const unsigned long long mk = s_mask[16 * m + g + 8 * r];
-                    uint32_t bits = 0;
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int j = pb + 16 * (nt >> 1) + t + 4 * e + 8 * (nt & 1) - ctx;
-                            const bool v = j < 0 || (j < n && ((mk >> (j & 63)) & 1ull));
-                            bits |= (v ? 1u : 0u) << (2 * nt + e);
-                            if (!v) x[m][nt][2 * r + e] = kNegMax;
-                        }
-                    seen[m][r] = bits;
-                }
-        }
-        // running reference: the block's row maximum and its largest V scale
-        float ev = -13.f;
-        if constexpr (C::kScaled) {
-            float vm = fmaxf(__low2float(vmax), __high2float(vmax));
-            vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 1));
-            vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 2));
-            // floor(log2 vm) from the exponent field; 0, inf (and an all-zero block) need no shift
-            const int ex = (int)(__float_as_uint(vm) >> 23);
-            ev += (ex == 0 || ex == 255) ? 0.f : (float)(ex - 127);
-        }
-        bool moved = false;
-        float want[MT][2];
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
             for (int r = 0; r < 2; ++r) {
-                float bm = fmaxf(x[m][0][2 * r], x[m][0][2 * r + 1]);
-#pragma unroll
-                for (int nt = 1; nt < NT; ++nt) bm = fmaxf(bm, fmaxf(x[m][nt][2 * r], x[m][nt][2 * r + 1]));
-                bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
-                bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
-                want[m][r] = fmaf(bm, c2, ev);
-                // (a block that the row does not see at all leaves the reference)
-                if (tail && bm == kNegMax) want[m][r] = kNegMax;
-                moved |= want[m][r] > ref[m][r];
-            }
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                float corr[2];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float nr = fmaxf(ref[m][r], want[m][r]);
-                    corr[r] = fast_exp2(ref[m][r] - nr);
-                    ref[m][r] = nr;
-                    l[m][r] *= corr[r];
-                }
-#pragma unroll
-                for (int gr = 0; gr < NG; ++gr)
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        o[m][gr][k][0] *= corr[0];
-                        o[m][gr][k][1] *= corr[0];
-                        o[m][gr][k][2] *= corr[1];
-                        o[m][gr][k][3] *= corr[1];
-                    }
-            }
-        }
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                float sum = 0.f;
+                const unsigned long long mk = s_mask[g + 8 * r];
+                uint32_t bits = 0;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float w = fast_exp2(fmaf(x[m][nt][2 * r + e], c2, -ref[m][r]));
-                        if constexpr (tail) w = (seen[m][r] >> (2 * nt + e)) & 1u ? w : 0.f;
-                        x[m][nt][2 * r + e] = w;
-                        sum += w;
+                        const int j = pb + 16 * (nt >> 1) + t + 4 * e + 8 * (nt & 1) - ctx;
+                        const bool v = j < 0 || (j < n && ((mk >> (j & 63)) & 1ull));
+                        bits |= (v ? 1u : 0u) << (2 * nt + e);
+                        if (!v) (e ? x[nt][r].y : x[nt][r].x) = kNegMax;
                     }
-                l[m][r] += sum;
+                seen[r] = bits;
             }
+        }
+        // running reference, from this lane's columns alone: its largest score and its
+        // largest V scale bound its P'. Only where one exceeds the row's reference by more
+        // than 2 (log2) do the row's lanes agree on a new one.
+        float ev = -12.f;
+        if constexpr (C::kScaled) {
+            // floor(log2) of the largest scale from its exponent field; 0 and inf need no shift
+            const float vm = fmaxf(__low2float(vmax), __high2float(vmax));
+            const int ex = (int)(__float_as_uint(vm) >> 23);
+            ev += (ex == 0 || ex == 255) ? 0.f : (float)(ex - 127);
+        }
+        float want[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float bm = fmaxf(x[0][r].x, x[0][r].y);
+#pragma unroll
+            for (int nt = 1; nt < NT; ++nt) bm = fmax3f(bm, x[nt][r].x, x[nt][r].y);
+            want[r] = fmaf(bm, c2, ev);
+            // (columns that the row does not see at all leave the reference)
+            if (tail && bm == kNegMax) want[r] = kNegMax;
+        }
+        if (__any_sync(0xffffffffu, want[0] > ref[0] + 2.f || want[1] > ref[1] + 2.f)) {
+            float corr[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                want[r] = fmaxf(want[r], __shfl_xor_sync(0xffffffffu, want[r], 1));
+                want[r] = fmaxf(want[r], __shfl_xor_sync(0xffffffffu, want[r], 2));
+                const float nr = fmaxf(ref[r], want[r]);
+                corr[r] = fast_exp2(ref[r] - nr);
+                ref[r] = nr;
+                l[r] *= corr[r];
+            }
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    o[gr][k][0] *= corr[0];
+                    o[gr][k][1] *= corr[0];
+                    o[gr][k][2] *= corr[1];
+                    o[gr][k][3] *= corr[1];
+                }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const float2 cc = make_float2(c2, c2), nr = make_float2(-ref[r], -ref[r]);
+            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float2 y = ffma2(x[nt][r], cc, nr);
+                float2 w = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+                if constexpr (tail) {
+                    w.x = (seen[r] >> (2 * nt)) & 1u ? w.x : 0.f;
+                    w.y = (seen[r] >> (2 * nt + 1)) & 1u ? w.y : 0.f;
+                }
+                x[nt][r] = w;
+                sum = fadd2(sum, w);
+            }
+            l[r] += sum.x + sum.y;
+        }
         // O += P' V, 16 positions at a time
         bool special = false;
 #pragma unroll
@@ -661,60 +648,43 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
             const uint8_t* vb = st + C::kOffV + (16 * j + t) * C::kRb;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
-                uint32_t pa[MT][4];
+                uint32_t pa[4];
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
                     const int nt = 2 * j + hf;
-                    float s0 = 1.f, s1 = 1.f;
-                    if constexpr (C::kScaled) {
-                        s0 = __half2float(gr ? __high2half(bits_h2(vsc[nt][0])) : __low2half(bits_h2(vsc[nt][0])));
-                        s1 = __half2float(gr ? __high2half(bits_h2(vsc[nt][1])) : __low2half(bits_h2(vsc[nt][1])));
-                    }
+                    float2 s = make_float2(1.f, 1.f);
+                    if constexpr (C::kScaled)
+                        s = make_float2(__half2float(gr ? __high2half(bits_h2(vsc[nt][0])) : __low2half(bits_h2(vsc[nt][0]))),
+                                        __half2float(gr ? __high2half(bits_h2(vsc[nt][1])) : __low2half(bits_h2(vsc[nt][1]))));
 #pragma unroll
-                    for (int m = 0; m < MT; ++m)
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            float w0 = x[m][nt][2 * r], w1 = x[m][nt][2 * r + 1];
-                            if constexpr (C::kScaled) {
-                                w0 *= s0;
-                                w1 *= s1;
-                                if constexpr (tail) {  // an unseen row's scale may be nan
-                                    if (!((seen[m][r] >> (2 * nt)) & 1u)) w0 = 0.f;
-                                    if (!((seen[m][r] >> (2 * nt + 1)) & 1u)) w1 = 0.f;
-                                }
+                    for (int r = 0; r < 2; ++r) {
+                        float2 w = x[nt][r];
+                        if constexpr (C::kScaled) {
+                            w = fmul2(w, s);
+                            if constexpr (tail) {  // an unseen row's scale may be nan
+                                if (!((seen[r] >> (2 * nt)) & 1u)) w.x = 0.f;
+                                if (!((seen[r] >> (2 * nt + 1)) & 1u)) w.y = 0.f;
                             }
-                            pa[m][2 * hf + r] = h2_bits(__floats2half2_rn(w0, w1));
                         }
+                        pa[2 * hf + r] = h2_bits(__floats2half2_rn(w.x, w.y));
+                    }
                 }
                 uint32_t h0[8], h1[8];
                 v_pairs<C::kKind>(vb, vb + 4 * C::kRb, gr, g, h0);
                 v_pairs<C::kKind>(vb + 8 * C::kRb, vb + 12 * C::kRb, gr, g, h1);
                 if constexpr (C::kFloat && tail) {
-                    {
-                        const int q0 = pb + 16 * j + t;
-                        const uint32_t k0 = (q0 < len ? 0xFFFFu : 0u) | (q0 + 4 < len ? 0xFFFF0000u : 0u);
-                        const uint32_t k1 = (q0 + 8 < len ? 0xFFFFu : 0u) | (q0 + 12 < len ? 0xFFFF0000u : 0u);
+                    const int q0 = pb + 16 * j + t;
+                    const uint32_t k0 = (q0 < len ? 0xFFFFu : 0u) | (q0 + 4 < len ? 0xFFFF0000u : 0u);
+                    const uint32_t k1 = (q0 + 8 < len ? 0xFFFFu : 0u) | (q0 + 12 < len ? 0xFFFF0000u : 0u);
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            h0[k] &= k0;
-                            h1[k] &= k1;
-                            if (h2_not_finite(h0[k])) {  // left to `special`
-                                special = true;
-                                if ((h0[k] & 0x7C00u) == 0x7C00u) h0[k] &= 0xFFFF0000u;
-                                if ((h0[k] & 0x7C000000u) == 0x7C000000u) h0[k] &= 0xFFFFu;
-                            }
-                            if (h2_not_finite(h1[k])) {
-                                special = true;
-                                if ((h1[k] & 0x7C00u) == 0x7C00u) h1[k] &= 0xFFFF0000u;
-                                if ((h1[k] & 0x7C000000u) == 0x7C000000u) h1[k] &= 0xFFFFu;
-                            }
-                        }
+                    for (int k = 0; k < 8; ++k) {  // entries that are not finite are left to `special`
+                        h0[k] &= k0;
+                        h1[k] &= k1;
+                        special |= clear_not_finite(h0[k]) | clear_not_finite(h1[k]);
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) mma_f16_16816(o[m][gr][k], pa[m], h0[k], h1[k]);
+                for (int k = 0; k < 8; ++k) mma_f16_16816(o[gr][k], pa, h0[k], h1[k]);
             }
         }
         if constexpr (C::kFloat && tail) {
@@ -726,20 +696,18 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
                     if (j >= n) break;
                     const uint8_t* vr = st + C::kOffV + pr * C::kRb;
 #pragma unroll
-                    for (int m = 0; m < MT; ++m)
+                    for (int r = 0; r < 2; ++r) {
+                        if (!(j < 0 || ((s_mask[g + 8 * r] >> (j & 63)) & 1ull))) continue;
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            if (!(j < 0 || ((s_mask[16 * m + g + 8 * r] >> (j & 63)) & 1ull))) continue;
+                        for (int gr = 0; gr < NG; ++gr)
 #pragma unroll
-                            for (int gr = 0; gr < NG; ++gr)
+                            for (int k = 0; k < 8; ++k)
 #pragma unroll
-                                for (int k = 0; k < 8; ++k)
-#pragma unroll
-                                    for (int e = 0; e < 2; ++e) {
-                                        const float v = v_one<C::kKind>(vr, 64 * gr + 16 * t + 8 * e + k);
-                                        if (!(fabsf(v) <= 65504.f)) o[m][gr][k][2 * r + e] += v;
-                                    }
-                        }
+                                for (int e = 0; e < 2; ++e) {
+                                    const float v = v_one<C::kKind>(vr, 64 * gr + 16 * t + 8 * e + k);
+                                    if (!(fabsf(v) <= 65504.f)) o[gr][k][2 * r + e] += v;
+                                }
+                    }
                 }
             }
         }
@@ -771,14 +739,12 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
     // merge the four warps: o and (ref, l) through shared memory
     float* so = reinterpret_cast<float*>(smem);
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
         for (int r = 0; r < 2; ++r) {
-            float sum = l[m][r];
+            float sum = l[r];
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            const int row = 16 * m + g + 8 * r;
-            if (t == 0) s_ml[warp * C::kRows + row] = make_float2(ref[m][r], sum);
+            const int row = g + 8 * r;
+            if (t == 0) s_ml[warp * C::kRows + row] = make_float2(ref[r], sum);
             float* dst = so + (size_t)(warp * C::kRows + row) * C::kOStride;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr)
@@ -787,10 +753,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
 #pragma unroll
                     for (int k = 0; k < 8; k += 4)
                         *reinterpret_cast<float4*>(dst + 64 * gr + 16 * t + 8 * e + k) =
-                            make_float4(o[m][gr][k][2 * r + e] * v_step<C::kKind>(k),
-                                        o[m][gr][k + 1][2 * r + e] * v_step<C::kKind>(k + 1),
-                                        o[m][gr][k + 2][2 * r + e] * v_step<C::kKind>(k + 2),
-                                        o[m][gr][k + 3][2 * r + e] * v_step<C::kKind>(k + 3));
+                            make_float4(o[gr][k][2 * r + e] * v_step<C::kKind>(k),
+                                        o[gr][k + 1][2 * r + e] * v_step<C::kKind>(k + 1),
+                                        o[gr][k + 2][2 * r + e] * v_step<C::kKind>(k + 2),
+                                        o[gr][k + 3][2 * r + e] * v_step<C::kKind>(k + 3));
         }
     __syncthreads();
     grid_launch_dependents();

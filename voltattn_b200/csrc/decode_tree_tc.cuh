@@ -194,16 +194,6 @@ __device__ __forceinline__ uint4 tc_convert(const TcRaw<K, kDim>& r, int j) {
     return make_uint4(h[0], h[1], h[2], h[3]);
 }
 
-__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
-        "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
-        "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-
 // 16 consecutive fp32 columns of this thread's TMEM lane, without the wait (as
 // tmem_ld32_nowait), and the tie to it.
 __device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t* r) {
@@ -238,17 +228,9 @@ __device__ __forceinline__ float4 lds_f4(uint32_t addr) {
     return v;
 }
 
-// Clears the entries of eight fp16 values that are not finite; true if there were any.
+// The same for eight fp16 values.
 __device__ __forceinline__ bool clear_not_finite(uint4& v) {
-    uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if ((w[i] & 0x7C00u) == 0x7C00u) w[i] &= 0xFFFF0000u, any = true;
-        if ((w[i] & 0x7C000000u) == 0x7C000000u) w[i] &= 0xFFFFu, any = true;
-    }
-    v = make_uint4(w[0], w[1], w[2], w[3]);
-    return any;
+    return clear_not_finite(v.x) | clear_not_finite(v.y) | clear_not_finite(v.z) | clear_not_finite(v.w);
 }
 
 // fp16 rows: the V tiles of blocks that hold drafted rows or the end are mended where

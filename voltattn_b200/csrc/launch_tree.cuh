@@ -58,8 +58,7 @@ template <int D>
 int launch_tree_dim(int fmt, const TreeParams& p, int rows, cudaStream_t st) {
 #define VA_TREE_KIND(kind)                                                                               \
     do {                                                                                                 \
-        if (rows == 16) return launch_tree_cfg<TreeCfg<kind, D, 1>>(decode_tree_kernel<TreeCfg<kind, D, 1>>, p, st); \
-        if (rows == 32) return launch_tree_cfg<TreeCfg<kind, D, 2>>(decode_tree_kernel<TreeCfg<kind, D, 2>>, p, st); \
+        if (rows == 16) return launch_tree_cfg<TreeCfg<kind, D>>(decode_tree_kernel<TreeCfg<kind, D>>, p, st); \
         if (rows == 128) return launch_tree_tc<TreeTcCfg<kind, D, false>>(p, st);                        \
         return launch_tree_tc<TreeTcCfg<kind, D, true>>(p, st);                                          \
     } while (0)
