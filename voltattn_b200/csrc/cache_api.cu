@@ -59,7 +59,7 @@ int tree_splits(int nsm, int B, int Hkv, int R, int Lmax) {
     const double ctas = (double)B * Hkv * ((R + rows - 1) / rows);
     if (ctas > (double)kCounters) return 1;
     const double cap = (double)nsm * (rows == 16 ? 3 : 1);
-    const double fixed = rows == 16 ? 128.0 : 384.0;
+    const double fixed = rows == 16 ? 192.0 : 768.0;
     const int units = (Lmax + kTreeUnit - 1) / kTreeUnit;
     double best = 1e300;
     int S = 1;

@@ -80,7 +80,7 @@ struct TreeTcCfg {
     static constexpr int kOffMask = kOffScales + kScaleBytes;
     static constexpr int kOffMl = kOffMask + kRows * 8;
     static constexpr int kOffBars = kOffMl + 4096;
-    static constexpr int kBars = 2 * kKS + 3 * kVS + 2 * 2 + 2 + kScaleSlots + 2 * kRawStages;
+    static constexpr int kBars = 2 * kKS + 3 * kVS + 2 * 2 + 3 + kScaleSlots + 2 * kRawStages;
     static constexpr int kOffMisc = kOffBars + kBars * 8;
     static constexpr int kSmemBytes = 1024 + kOffMisc + 64;
     static_assert((kDirect || kRawStages >= 2) && kBars * 8 <= 512, "two blocks in flight");
@@ -277,6 +277,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     uint64_t *kempty = kfull + KS, *vfull = kempty + KS, *vempty = vfull + VS, *sfull = vempty + VS;
     uint64_t *pfull = sfull + 2, *odone = pfull + 2, *fin = odone + 1, *scfull = fin + 1;
     uint64_t *rfull = scfull + C::kScaleSlots, *rempty = rfull + C::kRawStages, *vraw = rempty + C::kRawStages;
+    uint64_t* qfull = vraw + VS;
     float* s_ev = reinterpret_cast<float*>(smem + C::kOffMisc);
     uint32_t* tslot = reinterpret_cast<uint32_t*>(s_ev + 4);
     volatile int* fail = reinterpret_cast<volatile int*>(tslot + 1);
@@ -327,6 +328,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
             mbar_init(sfull + i, 1), mbar_init(pfull + i, 8);
         mbar_init(odone, 1);
         mbar_init(fin, 1);
+        mbar_init(qfull, 1);
         for (int i = 0; i < C::kScaleSlots; ++i) mbar_init(scfull + i, 1);
         for (int i = 0; i < C::kRawStages; ++i) mbar_init(rfull + i, 1), mbar_init(rempty + i, C::kProducers / 32);
         if constexpr (C::kDirect)
@@ -342,27 +344,6 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
         const int pg = pi < p.max_pages ? __ldg(trow + pi) : 0;
         return (unsigned)pg < (unsigned)p.num_pages ? pg : 0;
     };
-    // the query rows into shared memory in the tiles' order of dims, and their masks
-    for (int i = tid; i < C::kRows * (D / 8); i += C::kThreads) {
-        const int row = i / (D / 8), c = i - row * (D / 8);
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (row < live) {
-            const int r = r0 + row, node = r / p.G;
-            v = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.qs_b + node * p.qs_t +
-                                                     (long long)(hk * p.G + (r - node * p.G)) * p.qs_h) + c);
-            if constexpr (C::kPairs4)
-                v = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
-                               __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
-        }
-        const int rr = row & 127;
-        *reinterpret_cast<uint4*>(smem + (row >> 7) * C::kQTile + (c >> 3) * 16384 + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
-    }
-    const unsigned long long nodes_mask = n >= 64 ? ~0ull : (1ull << n) - 1ull;
-    for (int i = tid; i < C::kRows; i += C::kThreads) {
-        const int node = (r0 + i) / p.G;
-        s_mask[i] = i < live ? __ldg(p.mask + (size_t)b * p.Q + node) & nodes_mask : 0ull;
-    }
-    fence_proxy_async_smem();
     tc05_fence_before();
     __syncthreads();
     tc05_fence_after();
@@ -375,6 +356,36 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
     if (warp < 16) {
         // ---- softmax -------------------------------------------------------------
+        // first the query rows into shared memory in the tiles' order of dims (all loads of a
+        // thread before its stores), and their masks
+        {
+            constexpr int kPer = C::kRows * (D / 8) / 512;
+            uint4 v[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int x = tid + 512 * i, qr = x / (D / 8), c = x - qr * (D / 8);
+                v[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (qr < live) {
+                    const int r = r0 + qr, node = r / p.G;
+                    v[i] = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.qs_b + node * p.qs_t +
+                                                                (long long)(hk * p.G + (r - node * p.G)) * p.qs_h) + c);
+                }
+            }
+            const unsigned long long in_tree = n >= 64 ? ~0ull : (1ull << n) - 1ull;
+            if (tid < C::kRows) s_mask[tid] = tid < live ? __ldg(p.mask + (size_t)b * p.Q + (r0 + tid) / p.G) & in_tree : 0ull;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int x = tid + 512 * i, qr = x / (D / 8), c = x - qr * (D / 8), rr = qr & 127;
+                if constexpr (C::kPairs4)
+                    v[i] = make_uint4(__byte_perm(v[i].x, v[i].z, 0x5410), __byte_perm(v[i].x, v[i].z, 0x7632),
+                                      __byte_perm(v[i].y, v[i].w, 0x5410), __byte_perm(v[i].y, v[i].w, 0x7632));
+                *reinterpret_cast<uint4*>(smem + (qr >> 7) * C::kQTile + (c >> 3) * 16384 + rr * 128 +
+                                          (((c & 7) ^ (rr & 7)) << 4)) = v[i];
+            }
+            fence_proxy_async_smem();
+            named_barrier_sync(1, 512);
+            if (tid == 0) mbar_arrive(qfull);
+        }
         const float c2 = rsqrtf((float)D) * kLog2e * tc_k_inv_step<KK>();
         const int w = set;
         for (int j = w; j < njobs; j += 2) {
@@ -749,7 +760,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
             __syncwarp();
             return true;
         };
-        bool ok = issue_s(0);
+        bool ok = mbar_wait_fast(qfull, 0) && issue_s(0);
         if (njobs > 1) ok = ok && issue_s(1);
         for (int j = 0; ok && j < njobs; ++j) {
             ok = issue_pv(j);
@@ -796,6 +807,10 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
         }
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const size_t slot = ((size_t)stream * p.R + r) * p.S + split;
+        const int node = r / p.G;
+        __half* orow = p.out + b * p.os_b + node * p.os_t + (long long)(hk * p.G + (r - node * p.G)) * p.os_h;
+        const float scale = on && node < n ? inv : 0.f;  // (0: rows of no node, or that see nothing)
+        const bool wide = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
         constexpr int kCols = C::kTwo ? D / 2 : D / 4;
         const int c0 = C::kTwo ? hf * kCols : (set * 2 + hf) * kCols;
 #pragma unroll 1
@@ -840,15 +855,21 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
 #pragma unroll
                 for (int d = 0; d < 8; ++d)
                     v[d] = C::kPairs4 ? o[i + 2 * (d & 3) + (d >> 2)] * tc_v_step<KK>(d & 3) : o[i + d];
-                const float4 lo = make_float4(v[0], v[1], v[2], v[3]), hi = make_float4(v[4], v[5], v[6], v[7]);
-                const int c = (cb + i) / 4;
                 if (direct) {
-                    store_out(r, c, lo, on ? inv : 0.f);
-                    store_out(r, c + 1, hi, on ? inv : 0.f);
+                    uint32_t h[4];
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+                        h[d] = scale != 0.f ? h2_bits(__floats2half2_rn(v[2 * d] * scale, v[2 * d + 1] * scale)) : 0u;
+                    if (wide) {
+                        *reinterpret_cast<uint4*>(orow + cb + i) = make_uint4(h[0], h[1], h[2], h[3]);
+                    } else {
+                        reinterpret_cast<uint2*>(orow + cb + i)[0] = make_uint2(h[0], h[1]);
+                        reinterpret_cast<uint2*>(orow + cb + i)[1] = make_uint2(h[2], h[3]);
+                    }
                 } else if (on) {
-                    float4* dst = reinterpret_cast<float4*>(p.ws_o + slot * D) + c;
-                    __stcg(dst, lo);
-                    __stcg(dst + 1, hi);
+                    float4* dst = reinterpret_cast<float4*>(p.ws_o + slot * D + cb + i);
+                    __stcg(dst, make_float4(v[0], v[1], v[2], v[3]));
+                    __stcg(dst + 1, make_float4(v[4], v[5], v[6], v[7]));
                 }
             }
         }
