@@ -196,10 +196,13 @@ def _ptr(t) -> Optional[int]:
 
 
 def _stream_ptr(stream) -> Optional[int]:
+    if stream is not None:
+        return stream.cuda_stream
     import torch
-    if stream is None:
-        stream = torch.cuda.current_stream()
-    return stream.cuda_stream
+    try:  # the handle of torch's current stream without building a Stream object (1.6 us a call)
+        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    except AttributeError:
+        return torch.cuda.current_stream().cuda_stream
 
 
 @dataclass
@@ -418,20 +421,32 @@ def decode_paged(fmt, b: DeviceBufs, block_table, max_pages: int, lens, B: int, 
 
 # ---- speculative decoding over a paged cache (no reference counterpart) ----
 
+_fmt_codes: dict = {}
+
+
+def _fmt(f) -> int:
+    """int(Fmt.parse(f)), remembered per name: the calls below serve small batches, where the
+    host's time counts."""
+    code = _fmt_codes.get(f)
+    if code is None:
+        code = _fmt_codes[f] = int(Fmt.parse(f))
+    return code
+
 
 def _nbytes(t) -> int:
-    return 0 if t is None else t.numel() * t.element_size()
+    return 0 if t is None else t.nbytes
 
 
 def _strides(t, n: int):
     """The strides of a tensor's first n dimensions (its last one dense), None for a flat or contiguous one."""
-    if t.dim() != n + 1 or t.is_contiguous():
-        if not t.is_contiguous():
-            raise ValueError(f"expected a contiguous tensor or one of {n + 1} dimensions")
+    if t.is_contiguous():
         return None
-    if t.stride(-1) != 1:
+    st = t.stride()
+    if len(st) != n + 1:
+        raise ValueError(f"expected a contiguous tensor or one of {n + 1} dimensions")
+    if st[-1] != 1:
         raise ValueError("the last dimension must be dense")
-    return (C.c_longlong * n)(*t.stride()[:n])
+    return (C.c_longlong * n)(*st[:n])
 
 
 def tree_workspace_bytes(B: int, Hq: int, Hkv: int, Q: int, D: int, S: int) -> int:
@@ -440,7 +455,7 @@ def tree_workspace_bytes(B: int, Hq: int, Hkv: int, Q: int, D: int, S: int) -> i
 
 def suggest_tree_splits(f, B: int, Hq: int, Hkv: int, Q: int, Lmax: int, D: int) -> int:
     s = C.c_int(0)
-    _check(_lib.va_suggest_tree_splits(int(Fmt.parse(f)), B, Hq, Hkv, Q, Lmax, D, C.byref(s)), "suggest_tree_splits")
+    _check(_lib.va_suggest_tree_splits(_fmt(f), B, Hq, Hkv, Q, Lmax, D, C.byref(s)), "suggest_tree_splits")
     return s.value
 
 
@@ -454,7 +469,7 @@ def decode_tree(fmt, b: DeviceBufs, tree_mask, lens, nodes, block_table, max_pag
     (nodes None: Q each), block_table int32 [B][max_pages]. S = 0: the library
     splits the rows as the workspace b.ws (zeroed once, tree_workspace_bytes) allows."""
     vb = b.va()
-    _check(_lib.va_decode_tree(int(Fmt.parse(fmt)), C.byref(vb), _strides(b.q, 3), _strides(b.out, 3),
+    _check(_lib.va_decode_tree(_fmt(fmt), C.byref(vb), _strides(b.q, 3), _strides(b.out, 3),
                                _ptr(tree_mask), _ptr(lens), _ptr(nodes), _ptr(block_table), max_pages, B, Hq, Hkv, Q,
                                page_rows, num_pages, D, S, _ptr(b.ws), _nbytes(b.ws), _stream_ptr(stream)),
            "decode_tree")
@@ -474,7 +489,7 @@ def append_packed(fmt, k, v, b: DeviceBufs, block_table, max_pages: int, cu_toke
     if T * Hkv * D != k.numel():
         raise ValueError("append_packed: k and v must hold T * Hkv * D elements")
     vb = b.va()
-    _check(_lib.va_append_packed(int(Fmt.parse(fmt)), _ptr(k), _ptr(v), kinds[k.dtype], _strides(k, 2), _strides(v, 2),
+    _check(_lib.va_append_packed(_fmt(fmt), _ptr(k), _ptr(v), kinds[k.dtype], _strides(k, 2), _strides(v, 2),
                                  C.byref(vb), _ptr(block_table), max_pages, _ptr(cu_tokens), _ptr(pos), T, B, Hkv,
                                  page_rows, num_pages, D, _stream_ptr(stream)), "append_packed")
 
@@ -486,7 +501,7 @@ def accept_tree(fmt, b: DeviceBufs, block_table, max_pages: int, lens, nodes, pa
     every layer of the pool; new_lens[b] = lens[b] - nodes[b] + accepted. path:
     int32 [B][P] ascending node indices (P <= 64)."""
     vb = b.va()
-    _check(_lib.va_accept_tree(int(Fmt.parse(fmt)), C.byref(vb), _ptr(block_table), max_pages, _ptr(lens), _ptr(nodes),
+    _check(_lib.va_accept_tree(_fmt(fmt), C.byref(vb), _ptr(block_table), max_pages, _ptr(lens), _ptr(nodes),
                                _ptr(path), _ptr(accepted), _ptr(new_lens), B, P, Hkv, page_rows, num_pages, D, layers,
                                _stream_ptr(stream)), "accept_tree")
 
@@ -504,7 +519,7 @@ def fork_pages(fmt, b: DeviceBufs, refs, block_table, lens, parent, new_refs, ne
     All tensors int32 CUDA; refs counts a page's table entries (0: free). b.ws:
     scratch of pages_workspace_bytes(Bout, max_pages, num_pages)."""
     vb = b.va()
-    _check(_lib.va_fork_pages(int(Fmt.parse(fmt)), C.byref(vb), _ptr(refs), _ptr(block_table), _ptr(lens), _ptr(parent),
+    _check(_lib.va_fork_pages(_fmt(fmt), C.byref(vb), _ptr(refs), _ptr(block_table), _ptr(lens), _ptr(parent),
                               _ptr(new_refs), _ptr(new_table), _ptr(new_lens), _ptr(shortage), Bin, Bout, max_pages,
                               reserve, Hkv, page_rows, num_pages, D, layers, _ptr(b.ws), _nbytes(b.ws),
                               _stream_ptr(stream)), "fork_pages")
@@ -516,7 +531,7 @@ def compact_pages(fmt, b: DeviceBufs, refs, block_table, new_refs, new_table, us
     renumbers refs and block_table into new_refs and new_table; used[0] = their
     number. b.ws: scratch of pages_workspace_bytes(B, max_pages, num_pages)."""
     vb = b.va()
-    _check(_lib.va_compact_pages(int(Fmt.parse(fmt)), C.byref(vb), _ptr(refs), _ptr(block_table), _ptr(new_refs),
+    _check(_lib.va_compact_pages(_fmt(fmt), C.byref(vb), _ptr(refs), _ptr(block_table), _ptr(new_refs),
                                  _ptr(new_table), _ptr(used), B, max_pages, Hkv, page_rows, num_pages, D, layers,
                                  _ptr(b.ws), _nbytes(b.ws), _stream_ptr(stream)), "compact_pages")
 

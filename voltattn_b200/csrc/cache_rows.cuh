@@ -26,18 +26,29 @@ struct AppendParams {
     const int* cu;   // [B + 1] first token of each sequence
     const int* pos;  // [B] row of a sequence's first token
     int T, B, Hkv, D, max_pages, page_rows, num_pages;
+    int split;  // warps to a token
 };
 
+// Eight consecutive elements of a token's row as they lie in memory, and in fp32.
 template <class T>
-__device__ __forceinline__ void load8(const T* src, float (&v)[8]) {
+struct Raw8 {
+    uint4 w[sizeof(T) / 2];
+};
+template <class T>
+__device__ __forceinline__ Raw8<T> load8(const T* src) {
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+    return r;
+}
+template <class T>
+__device__ __forceinline__ void to_fp32(const Raw8<T>& r, float (&v)[8]) {
     if constexpr (sizeof(T) == 4) {
-        const float4* p = reinterpret_cast<const float4*>(src);
-        const float4 a = __ldg(p), b = __ldg(p + 1);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        const uint32_t w[8] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w, r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
     } else {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(src));
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+        const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float2 f;
@@ -62,55 +73,172 @@ __device__ __forceinline__ int token_sequence(const int* cu, int B, int token, i
     return seq;
 }
 
-// A warp quantizes four 64-element groups of one token at a time (8 lanes a
-// group), K's groups of all heads before V's; its sequence and page are looked
-// up once per token.
+// The code of va_quantize, by its division: a real call, so that the rare elements that
+// need it cost the others a branch and not 25 predicated instructions each.
+static __device__ __noinline__ int quantize_exact(float x, float s, int lim) {
+    return max(-lim, min(lim, lrint_narrow(__fdiv_rn(x, s))));
+}
+
+// The larger of two values, nan if either is.
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// bits[i] = the fp32 pattern of 1.5 * 2^23 + kBias + code i, code = rint(x / s) clamped to
+// [-kLim, kLim] as va_quantize has it, without a division per element: inv = 1 / s to one
+// ulp (2^-23) once a group, y = x * inv, and adding 1.5 * 2^23 (+ an even bias) rounds y to an
+// integer, half to even. y is within 1.6 * 2^-23 |y| of x / s and the rounded quotient within
+// 2^-24 |y|: below 2.6e-7 * (kLim + 1) together, kMargin; so the nearest integer is the
+// same unless y is that close to a half. With |y| < kLim + 0.49 in the whole group no
+// clamp acts. An element that is close to a half or nan, and groups of other sizes (scales
+// that under- or overflowed fp16), take the division.
+template <int kLim, int kBias>
+__device__ __forceinline__ void quantize_codes(const float (&x)[8], float amax, float s, float inv, uint32_t (&bits)[8]) {
+    constexpr float kRound = 12582912.f + (float)kBias, kMargin = 2.6e-7f * (float)(kLim + 1);
+    float far = 0.f, y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        y[i] = x[i] * inv;
+        const float t = __fadd_rn(y[i], kRound);
+        far = fmax_nan(far, fabsf(y[i] - __fadd_rn(t, -kRound)));
+        bits[i] = __float_as_uint(t);
+    }
+    const bool plain = amax * inv < (float)kLim + 0.49f;
+    if (!(plain && far < 0.5f - kMargin)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float d = fabsf(y[i] - __fadd_rn(__uint_as_float(bits[i]), -kRound));
+            if (!(plain && d < 0.5f - kMargin))
+                bits[i] = 0x4B400000u + (uint32_t)(kBias + quantize_exact(x[i], s, kLim));
+        }
+    }
+}
+
+// The group scale of va_quantize, amax > 0 ? amax / lim : 1 rounded to fp32, then to
+// fp16. The product with 1 / lim is within 2 fp32 ulps of the quotient, so both round to the
+// same fp16 unless it lies that close to the middle of two of them: those (about one in
+// 1000), and results outside fp16's normal range, take the division.
+template <int kLim>
+__device__ __forceinline__ __half group_scale(float amax) {
+    const float q = amax * (1.f / (float)kLim);
+    const uint32_t low = __float_as_uint(q) & 0x1FFFu;
+    if (low - 0xFF8u <= 16u || !(q > 6.2e-5f && q < 65000.f))
+        return __float2half_rn(amax > 0.f ? __fdiv_rn(amax, (float)kLim) : 1.f);
+    return __float2half_rn(q);
+}
+
+// One 64-element group from registers, eight consecutive elements per thread (8 lanes a
+// group, lane-aligned): scale and codes as quantize_group_values, at `codes` + the
+// group's bytes and *scale. All 32 lanes call it.
+template <int BITS>
+__device__ __forceinline__ void quantize_group_packed(const float (&v)[8], bool active, int part, uint8_t* codes,
+                                                      __half* scale) {
+    constexpr int lim = BITS == 8 ? 127 : BITS == 4 ? 7 : 3;
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));  // fmaxf drops nan operands
+#pragma unroll
+    for (int off = 1; off < 8; off <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+    const __half hs = group_scale<lim>(amax);
+    const float sh = __half2float(hs);
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sh));
+    uint32_t c[8];
+    quantize_codes<lim, BITS == 8 ? 0 : lim + 1>(v, amax, sh, inv, c);
+    if constexpr (BITS == 8) {
+        uint32_t w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            w[i] = __byte_perm(__byte_perm(c[4 * i], c[4 * i + 1], 0x0040), __byte_perm(c[4 * i + 2], c[4 * i + 3], 0x0040), 0x5410);
+        if (active) reinterpret_cast<uint2*>(codes)[part] = make_uint2(w[0], w[1]);
+    } else {
+        // sum of 2^(BITS i) * (field + the pattern of 1.5 * 2^23), less the patterns' share
+        uint32_t w = 0, base = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            w += c[i] * (1u << (BITS * i));
+            base += 0x4B400000u * (1u << (BITS * i));
+        }
+        w -= base;
+        if constexpr (BITS == 4) {
+            if (active) reinterpret_cast<uint32_t*>(codes)[part] = w;
+        } else {
+            // eight 24-bit pieces as six words: word i begins s bits into piece a
+            const int a = (4 * part) / 3, s = 32 * part - 24 * a, lane0 = (threadIdx.x & 31) - part;
+            const uint32_t lo = __shfl_sync(0xffffffffu, w, lane0 + (a & 7));
+            const uint32_t hi = __shfl_sync(0xffffffffu, w, lane0 + ((a + 1) & 7));
+            if (active && part < 6) reinterpret_cast<uint32_t*>(codes)[part] = (lo >> s) | (hi << (24 - s));
+        }
+    }
+    if (active && part == 0) *scale = hs;
+}
+
+// A warp takes quads of one token's 64-element groups of K or V (blockIdx.y), 8 lanes a
+// group, `split` warps to a token; its sequence and page are looked up once. kBatch
+// quads are loaded before the first is quantized.
 template <int BITS, class T>
-__global__ void __launch_bounds__(256) append_packed_kernel(const AppendParams p) {
-    const int lane = threadIdx.x & 31;
-    const int ng = p.D / kGroup, side_groups = p.Hkv * ng;
-    const int quads = (2 * side_groups + 3) / 4;
-    const long long w = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+__global__ void __launch_bounds__(256, 3) append_packed_kernel(const AppendParams p) {
+    constexpr int kBatch = 2;
+    const int lane = threadIdx.x & 31, part = lane & 7;
+    const int ng = p.D / kGroup, groups = p.Hkv * ng, quads = (groups + 3) / 4;
+    const unsigned w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     grid_dependency_wait();
     grid_launch_dependents();
-    if (w >= (long long)p.T * quads) return;
-    const int token = (int)(w / quads), quad = (int)(w - (long long)token * quads);
+    if (w >= (unsigned)p.T * p.split) return;
+    const int token = (int)(w / (unsigned)p.split);
     const int seq = token_sequence(p.cu, p.B, token, lane);
     if (seq >= p.B) return;
     const int i = token - __ldg(p.cu + seq), at = __ldg(p.pos + seq);
     const long long row = (long long)at + i;
     if (i < 0 || at < 0 || row >= (long long)p.max_pages * p.page_rows) return;
-    const int pi = (int)(row / p.page_rows);
+    const int pi = (int)row / p.page_rows;  // (rows fit 31 bits)
     const int pg = __ldg(p.table + (size_t)seq * p.max_pages + pi);
     if (pg < 0 || pg >= p.num_pages) return;
-    const int grp = quad * 4 + (lane >> 3), part = lane & 7;
-    const bool active = grp < 2 * side_groups;
-    const bool is_v = grp >= side_groups;
-    const int sg = active ? grp - (is_v ? side_groups : 0) : 0;
-    const int h = sg / ng, gi = sg - h * ng;
-    const T* src = is_v ? static_cast<const T*>(p.v) + token * p.vt + h * p.vh
-                        : static_cast<const T*>(p.k) + token * p.kt + h * p.kh;
-    float v[8];
-    load8(src + gi * kGroup + part * 8, v);
-    const long long r = ((long long)pg * p.Hkv + h) * p.page_rows + (row - (long long)pi * p.page_rows);
-    uint8_t* codes = is_v ? p.V : p.K;
-    const long long e0 = r * p.D + gi * kGroup + part * 8;
-    if constexpr (BITS == 16 || BITS == kBitsBf16) {
-        if (!active) return;
-        uint32_t o[4];
+    const bool is_v = blockIdx.y != 0;
+    constexpr int kBytes = kGroup * (BITS == kBitsF8 ? 8 : BITS == kBitsBf16 ? 16 : BITS) / 8;  // of a group's codes
+    const size_t g0 = ((size_t)pg * p.Hkv * p.page_rows + ((int)row - pi * p.page_rows)) * ng;
+    uint8_t* codes = (is_v ? p.V : p.K) + g0 * kBytes;
+    __half* scales = (is_v ? p.scV : p.scK) + g0;
+    const T* src = is_v ? static_cast<const T*>(p.v) + token * p.vt : static_cast<const T*>(p.k) + token * p.kt;
+    src += part * 8;
+    const long long head = is_v ? p.vh : p.kh, head_groups = (long long)p.page_rows * ng;
+    for (int q0 = (int)(w - (unsigned)token * p.split); q0 < quads; q0 += kBatch * p.split) {
+        Raw8<T> raw[kBatch];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            if constexpr (BITS == 16) {
-                const __half2 x = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
-                o[k] = *reinterpret_cast<const uint32_t*>(&x);
+        for (int k = 0; k < kBatch; ++k) {
+            const int grp = (q0 + k * p.split) * 4 + (lane >> 3), h = ng == 2 ? grp >> 1 : grp;
+            raw[k] = Raw8<T>{};
+            if (grp < groups) raw[k] = load8(src + h * head + (grp - h * ng) * kGroup);
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const int grp = (q0 + k * p.split) * 4 + (lane >> 3), h = ng == 2 ? grp >> 1 : grp;
+            if (q0 + k * p.split >= quads) break;
+            const bool active = grp < groups;
+            const size_t at_g = (size_t)(h * head_groups + (grp - h * ng));  // past g0
+            float v[8];
+            to_fp32(raw[k], v);
+            if constexpr (BITS == 16 || BITS == kBitsBf16) {
+                uint32_t o[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (BITS == 16) {
+                        const __half2 x = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+                        o[e] = *reinterpret_cast<const uint32_t*>(&x);
+                    } else {
+                        const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+                        o[e] = *reinterpret_cast<const uint32_t*>(&x);
+                    }
+                }
+                if (active) reinterpret_cast<uint4*>(codes + at_g * kBytes)[part] = make_uint4(o[0], o[1], o[2], o[3]);
+            } else if constexpr (BITS == kBitsF8) {
+                quantize_group_values<BITS>(v, active, part, (long long)at_g * kGroup + part * 8, (long long)at_g, codes, scales);
             } else {
-                const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
-                o[k] = *reinterpret_cast<const uint32_t*>(&x);
+                quantize_group_packed<BITS>(v, active, part, codes + at_g * kBytes, scales + at_g);
             }
         }
-        *reinterpret_cast<uint4*>(codes + e0 * 2) = make_uint4(o[0], o[1], o[2], o[3]);
-    } else {
-        quantize_group_values<BITS>(v, active, part, e0, r * ng + gi, codes, is_v ? p.scV : p.scK);
     }
 }
 
