@@ -26,7 +26,7 @@ struct AppendParams {
     const int* cu;   // [B + 1] first token of each sequence
     const int* pos;  // [B] row of a sequence's first token
     int T, B, Hkv, D, max_pages, page_rows, num_pages;
-    int split;  // warps to a token
+    unsigned page_mul, page_shift;  // as TreeParams
 };
 
 // Eight consecutive elements of a token's row as they lie in memory, and in fp32.
@@ -175,70 +175,89 @@ __device__ __forceinline__ void quantize_group_packed(const float (&v)[8], bool 
     if (active && part == 0) *scale = hs;
 }
 
-// A warp takes quads of one token's 64-element groups of K or V (blockIdx.y), 8 lanes a
-// group, `split` warps to a token; its sequence and page are looked up once. kBatch
-// quads are loaded before the first is quantized.
+// A work item is two quads of one token's 64-element groups of K or V (blockIdx.y), 8
+// lanes a group. A warp takes items w, w + W, ... and loads the next one (its sequence, its
+// page, its elements: four dependent loads) before it quantizes the current one.
 template <int BITS, class T>
 __global__ void __launch_bounds__(256, 3) append_packed_kernel(const AppendParams p) {
     constexpr int kBatch = 2;
+    constexpr int kBytes = kGroup * (BITS == kBitsF8 ? 8 : BITS == kBitsBf16 ? 16 : BITS) / 8;  // of a group's codes
     const int lane = threadIdx.x & 31, part = lane & 7;
-    const int ng = p.D / kGroup, groups = p.Hkv * ng, quads = (groups + 3) / 4;
-    const unsigned w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    const int ng = p.D / kGroup, groups = p.Hkv * ng;
+    const unsigned per = (unsigned)(groups + 4 * kBatch - 1) / (4 * kBatch);  // items of a token
+    const unsigned warps = gridDim.x * (blockDim.x >> 5), step_t = warps / per, step_s = warps - step_t * per;
+    const bool is_v = blockIdx.y != 0;
+    const long long head = is_v ? p.vh : p.kh, token_step = is_v ? p.vt : p.kt;
+    const long long head_groups = (long long)p.page_rows * ng;
+    const T* x = static_cast<const T*>(is_v ? p.v : p.k) + part * 8;
+    uint8_t* const codes = is_v ? p.V : p.K;
+    __half* const scales = is_v ? p.scV : p.scK;
+    struct Item {
+        Raw8<T> raw[kBatch];
+        long long g0;  // the row's first group in the pool; < 0: nothing to do
+        int grp;       // this lane's first group of the row
+    };
+    const auto load = [&](unsigned token, unsigned sub) {
+        Item m;
+        m.g0 = -1;
+        if (token >= (unsigned)p.T) return m;
+        m.grp = (int)sub * 4 * kBatch + (lane >> 3);
+        const int seq = token_sequence(p.cu, p.B, (int)token, lane);
+        if (seq >= p.B) return m;
+        const int i = (int)token - __ldg(p.cu + seq), at = __ldg(p.pos + seq);
+        const long long row = (long long)at + i;
+        if (i < 0 || at < 0 || row >= (long long)p.max_pages * p.page_rows) return m;
+        const int pi = (int)((__umulhi((unsigned)row, p.page_mul) + (unsigned)row) >> p.page_shift);  // (rows fit 31 bits)
+        const int pg = __ldg(p.table + (size_t)seq * p.max_pages + pi);
+        if (pg < 0 || pg >= p.num_pages) return m;
+        m.g0 = ((long long)pg * p.Hkv * p.page_rows + ((int)row - pi * p.page_rows)) * ng;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const int grp = m.grp + 4 * k, h = ng == 2 ? grp >> 1 : grp;
+            m.raw[k] = Raw8<T>{};
+            if (grp < groups) m.raw[k] = load8(x + token * token_step + h * head + (grp - h * ng) * kGroup);
+        }
+        return m;
+    };
     grid_dependency_wait();
     grid_launch_dependents();
-    if (w >= (unsigned)p.T * p.split) return;
-    const int token = (int)(w / (unsigned)p.split);
-    const int seq = token_sequence(p.cu, p.B, token, lane);
-    if (seq >= p.B) return;
-    const int i = token - __ldg(p.cu + seq), at = __ldg(p.pos + seq);
-    const long long row = (long long)at + i;
-    if (i < 0 || at < 0 || row >= (long long)p.max_pages * p.page_rows) return;
-    const int pi = (int)row / p.page_rows;  // (rows fit 31 bits)
-    const int pg = __ldg(p.table + (size_t)seq * p.max_pages + pi);
-    if (pg < 0 || pg >= p.num_pages) return;
-    const bool is_v = blockIdx.y != 0;
-    constexpr int kBytes = kGroup * (BITS == kBitsF8 ? 8 : BITS == kBitsBf16 ? 16 : BITS) / 8;  // of a group's codes
-    const size_t g0 = ((size_t)pg * p.Hkv * p.page_rows + ((int)row - pi * p.page_rows)) * ng;
-    uint8_t* codes = (is_v ? p.V : p.K) + g0 * kBytes;
-    __half* scales = (is_v ? p.scV : p.scK) + g0;
-    const T* src = is_v ? static_cast<const T*>(p.v) + token * p.vt : static_cast<const T*>(p.k) + token * p.kt;
-    src += part * 8;
-    const long long head = is_v ? p.vh : p.kh, head_groups = (long long)p.page_rows * ng;
-    for (int q0 = (int)(w - (unsigned)token * p.split); q0 < quads; q0 += kBatch * p.split) {
-        Raw8<T> raw[kBatch];
+    const unsigned w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    unsigned token = w / per, sub = w - token * per;
+    Item cur = load(token, sub);
+    while (token < (unsigned)p.T) {
+        token += step_t;
+        sub += step_s;
+        if (sub >= per) sub -= per, ++token;
+        const Item next = load(token, sub);
+        if (cur.g0 >= 0) {
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-            const int grp = (q0 + k * p.split) * 4 + (lane >> 3), h = ng == 2 ? grp >> 1 : grp;
-            raw[k] = Raw8<T>{};
-            if (grp < groups) raw[k] = load8(src + h * head + (grp - h * ng) * kGroup);
-        }
+            for (int k = 0; k < kBatch; ++k) {
+                const int grp = cur.grp + 4 * k, h = ng == 2 ? grp >> 1 : grp;
+                const bool active = grp < groups;
+                const long long g = cur.g0 + h * head_groups + (grp - h * ng);
+                float v[8];
+                to_fp32(cur.raw[k], v);
+                if constexpr (BITS == 16 || BITS == kBitsBf16) {
+                    uint32_t o[4];
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-            const int grp = (q0 + k * p.split) * 4 + (lane >> 3), h = ng == 2 ? grp >> 1 : grp;
-            if (q0 + k * p.split >= quads) break;
-            const bool active = grp < groups;
-            const size_t at_g = (size_t)(h * head_groups + (grp - h * ng));  // past g0
-            float v[8];
-            to_fp32(raw[k], v);
-            if constexpr (BITS == 16 || BITS == kBitsBf16) {
-                uint32_t o[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (BITS == 16) {
-                        const __half2 x = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
-                        o[e] = *reinterpret_cast<const uint32_t*>(&x);
-                    } else {
-                        const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-                        o[e] = *reinterpret_cast<const uint32_t*>(&x);
+                    for (int e = 0; e < 4; ++e) {
+                        if constexpr (BITS == 16) {
+                            const __half2 y = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+                            o[e] = *reinterpret_cast<const uint32_t*>(&y);
+                        } else {
+                            const __nv_bfloat162 y = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+                            o[e] = *reinterpret_cast<const uint32_t*>(&y);
+                        }
                     }
+                    if (active) reinterpret_cast<uint4*>(codes + g * kBytes)[part] = make_uint4(o[0], o[1], o[2], o[3]);
+                } else if constexpr (BITS == kBitsF8) {
+                    quantize_group_values<BITS>(v, active, part, g * kGroup + part * 8, g, codes, scales);
+                } else {
+                    quantize_group_packed<BITS>(v, active, part, codes + g * kBytes, scales + g);
                 }
-                if (active) reinterpret_cast<uint4*>(codes + at_g * kBytes)[part] = make_uint4(o[0], o[1], o[2], o[3]);
-            } else if constexpr (BITS == kBitsF8) {
-                quantize_group_values<BITS>(v, active, part, (long long)at_g * kGroup + part * 8, (long long)at_g, codes, scales);
-            } else {
-                quantize_group_packed<BITS>(v, active, part, codes + at_g * kBytes, scales + at_g);
             }
         }
+        cur = next;
     }
 }
 

@@ -333,18 +333,14 @@ int launch_pdl(void (*kernel)(const P), dim3 grid, int threads, size_t smem, cud
 }
 
 template <class T>
-int launch_append_in(int bits, AppendParams p, cudaStream_t st) {
-    const int quads = (p.Hkv * (p.D / kGroup) + 3) / 4;
-    // one warp to a token's K or V where the tokens alone fill the device (32 warps an SM),
-    // a warp to every quad of groups where they are few
+int launch_append_in(int bits, const AppendParams& p, cudaStream_t st) {
+    // a warp to every item (half of a 16-group token's K or V) up to three 8-warp CTAs an SM
+    // for each side twice over; beyond that the warps loop
     int dev;
     const int rc = current_device(&dev);
     if (rc) return rc;
-    const long long want = (long long)sm_count(dev) * 16;
-    p.split = (int)std::max<long long>(1, std::min<long long>(quads, (want + p.T - 1) / p.T));
-    const long long warps = (long long)p.T * p.split;
-    if (warps + 7 > INT_MAX) return VA_ERR_TOO_LARGE;  // (split > 1 only for few tokens)
-    const dim3 grid((unsigned)((warps + 7) / 8), 2);
+    const long long items = (long long)p.T * ((p.Hkv * (p.D / kGroup) + 7) / 8);
+    const dim3 grid((unsigned)std::min<long long>((items + 7) / 8, (long long)sm_count(dev) * 3), 2);
     switch (bits) {
         case 16: return launch_pdl(append_packed_kernel<16, T>, grid, 256, 0, st, p);
         case kBitsBf16: return launch_pdl(append_packed_kernel<kBitsBf16, T>, grid, 256, 0, st, p);
