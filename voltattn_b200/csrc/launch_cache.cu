@@ -68,30 +68,46 @@ __global__ void __launch_bounds__(kAcceptThreads) accept_tree_kernel(const Accep
 }
 
 // The plan of a fork: tables, lengths, counts, and which rows are to be copied
-// (copied by fork_copy_kernel). One CTA: the work is a pass over refs and two
-// over the tables.
+// (copied by fork_copy_kernel). One CTA: the work is a pass over refs and two over the
+// tables, each bound by the latency of its loads, so parents and lengths are kept in
+// shared memory and a warp has the first 32 entries of kAhead sequences in flight.
+constexpr int kAhead = 2;
+constexpr int kFreeHere = 1024;  // pages of the free list kept in shared memory as well
 __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParams p) {
     extern __shared__ int sm[];
-    int* kids = sm;             // [Bin]
-    int* first = kids + p.Bin;  // [Bin]
-    int* base = first + p.Bin;  // [Bout]
-    __shared__ int scan[33];
+    int* kids = sm;              // [Bin]
+    int* first = kids + p.Bin;   // [Bin]
+    int* lens = first + p.Bin;   // [Bin]
+    int* full = lens + p.Bin;    // [Bin] full pages
+    int* need = full + p.Bin;    // [Bin] pages of lens + reserve rows
+    int* base = need + p.Bin;    // [Bout]
+    int* from_seq = base + p.Bout;  // [Bout] parent, or -1
+    __shared__ int scan[33], free_here[kFreeHere];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int kWarps = kPlanThreads / 32;
     const int num_pages = p.pool.num_pages, pr = p.pool.page_rows;
     grid_dependency_wait();
+    const long long cap = (long long)p.max_pages * pr;
     for (int s = tid; s < p.Bin; s += kPlanThreads) {
         kids[s] = 0;
         first[s] = INT_MAX;
+        const int len = (int)max(0ll, min((long long)__ldg(p.lens + s), cap));
+        lens[s] = len;
+        full[s] = len / pr;
+        // (the rest of a page, a page and a reserve below 2^31: 32 bits)
+        need[s] = (int)min((unsigned)p.max_pages, (unsigned)full[s] + ((unsigned)(len - full[s] * pr) + p.reserve + pr - 1) / pr);
+    }
+    for (int i = tid; i < p.Bout; i += kPlanThreads) {
+        const int s = __ldg(p.parent + i);
+        from_seq[i] = s >= 0 && s < p.Bin ? s : -1;
     }
     for (int i = tid; i < num_pages; i += kPlanThreads) p.new_refs[i] = __ldg(p.refs + i);
     __syncthreads();
-    for (int i = tid; i < p.Bout; i += kPlanThreads) {
-        const int s = __ldg(p.parent + i);
-        if (s >= 0 && s < p.Bin) {
-            atomicAdd(kids + s, 1);
-            atomicMin(first + s, i);
+    for (int i = tid; i < p.Bout; i += kPlanThreads)
+        if (from_seq[i] >= 0) {
+            atomicAdd(kids + from_seq[i], 1);
+            atomicMin(first + from_seq[i], i);
         }
-    }
     __syncthreads();
     // a new sequence: its parent, its length, how many pages it shares and needs
     struct Child {
@@ -100,30 +116,52 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
     };
     const auto child = [&](int i) {
         Child c;
-        c.s = __ldg(p.parent + i);
-        c.len = c.full = c.need = 0;
-        c.keep = false;
-        if (c.s < 0 || c.s >= p.Bin) {
-            c.s = -1;
-            return c;
-        }
-        const long long cap = (long long)p.max_pages * pr;
-        c.len = (int)max(0ll, min((long long)__ldg(p.lens + c.s), cap));
-        c.full = c.len / pr;
-        c.need = (int)min((long long)p.max_pages, ((long long)c.len + p.reserve + pr - 1) / pr);
-        c.keep = first[c.s] == i;
+        c.s = i < p.Bout ? from_seq[i] : -1;
+        c.len = c.s >= 0 ? lens[c.s] : 0;
+        c.full = c.s >= 0 ? full[c.s] : 0;
+        c.need = c.s >= 0 ? need[c.s] : 0;
+        c.keep = c.s >= 0 && first[c.s] == i;
         return c;
     };
     const auto held = [&](const Child& c, int j) {
         if (c.s < 0 || j >= p.max_pages || !(c.keep || j < c.full)) return -1;
         return valid_page(__ldg(p.table + (size_t)c.s * p.max_pages + j), num_pages);
     };
-    for (int i = warp; i < p.Bout; i += kPlanThreads / 32) {
-        const Child c = child(i);
-        int n = 0;
-        for (int j = lane; j - lane < c.need; j += 32)
-            n += __popc(__ballot_sync(0xffffffffu, j < c.need && held(c, j) < 0));
-        if (lane == 0) base[i] = n;
+    for (int i0 = warp; i0 < p.Bout; i0 += kWarps * kAhead) {
+        Child c[kAhead];
+        int e[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            c[u] = child(i0 + u * kWarps);
+            e[u] = held(c[u], lane);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            int n = 0;
+            for (int j = lane; j - lane < c[u].need; j += 32)
+                n += __popc(__ballot_sync(0xffffffffu, j < c[u].need && (j < 32 ? e[u] : held(c[u], j)) < 0));
+            if (lane == 0 && i0 + u * kWarps < p.Bout) base[i0 + u * kWarps] = n;
+        }
+    }
+    // counts of the pages that the old tables hold
+    for (int s0 = warp; s0 < p.Bin; s0 += kWarps * kAhead) {
+        int e[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int s = s0 + u * kWarps;
+            e[u] = s < p.Bin && lane < p.max_pages ? __ldg(p.table + (size_t)s * p.max_pages + lane) : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int s = s0 + u * kWarps;
+            if (s >= p.Bin) break;
+            const int shared = kids[s] - 1, own = kids[s] > 0 ? 0 : -1;
+            for (int j = lane; j < p.max_pages; j += 32) {
+                const int pg = valid_page(j < 32 ? e[u] : __ldg(p.table + (size_t)s * p.max_pages + j), num_pages);
+                const int d = j < full[s] ? shared : own;
+                if (pg >= 0 && d != 0) atomicAdd(p.new_refs + pg, d);
+            }
+        }
     }
     __syncthreads();
     int total = 0;
@@ -149,7 +187,8 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             if (f >> k & 1u) {
-                if (at < total) p.free_list[at] = c0 + 4 * tid + k;
+                if (at < kFreeHere) free_here[at] = c0 + 4 * tid + k;
+                else if (at < total) p.free_list[at] = c0 + 4 * tid + k;
                 ++at;
             }
         found += sum;
@@ -157,60 +196,63 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
     found = min(found, total);
     __syncthreads();
     if (tid == 0) *p.shortage = total - found;
-    for (int i = warp; i < p.Bout; i += kPlanThreads / 32) {
-        const Child c = child(i);
-        const int part = c.len / pr, rest = c.len - part * pr;
-        int at = base[i];
-        bool lost = false;
-        int from = -1, to = -1;
-        for (int j = lane; j - lane < p.max_pages; j += 32) {
-            const int h = held(c, j);
-            const bool ask = j < c.need && h < 0;
-            const unsigned m = __ballot_sync(0xffffffffu, ask);
-            const int rank = at + __popc(m & ((1u << lane) - 1u));
-            at += __popc(m);
-            int e = h;
-            if (ask && rank < found) {
-                e = p.free_list[rank];
-                atomicAdd(p.new_refs + e, 1);
-                if (j == part && rest > 0 && !c.keep) {
-                    from = valid_page(__ldg(p.table + (size_t)c.s * p.max_pages + j), num_pages);
-                    to = e;
+    for (int i0 = warp; i0 < p.Bout; i0 += kWarps * kAhead) {
+        Child cs[kAhead];
+        int es[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            cs[u] = child(i0 + u * kWarps);
+            es[u] = held(cs[u], lane);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = i0 + u * kWarps;
+            if (i >= p.Bout) break;
+            const Child& c = cs[u];
+            const int part = c.full, rest = c.len - part * pr;
+            int at = base[i];
+            bool lost = false;
+            int from = -1, to = -1;
+            for (int j = lane; j - lane < p.max_pages; j += 32) {
+                const int h = j < 32 ? es[u] : held(c, j);
+                const bool ask = j < c.need && h < 0;
+                const unsigned m = __ballot_sync(0xffffffffu, ask);
+                const int rank = at + __popc(m & ((1u << lane) - 1u));
+                at += __popc(m);
+                int e = h;
+                if (ask && rank < found) {
+                    e = rank < kFreeHere ? free_here[rank] : p.free_list[rank];
+                    atomicAdd(p.new_refs + e, 1);
+                    if (j == part && rest > 0 && !c.keep) {
+                        from = valid_page(__ldg(p.table + (size_t)c.s * p.max_pages + j), num_pages);
+                        to = e;
+                    }
+                } else if (ask && j == part && rest > 0) {
+                    lost = true;
                 }
-            } else if (ask && j == part && rest > 0) {
-                lost = true;
+                if (j < p.max_pages) p.new_table[(size_t)i * p.max_pages + j] = e;
             }
-            if (j < p.max_pages) p.new_table[(size_t)i * p.max_pages + j] = e;
-        }
-        lost = __any_sync(0xffffffffu, lost);
-        const unsigned who = __ballot_sync(0xffffffffu, to >= 0);
-        if (who) {
-            from = __shfl_sync(0xffffffffu, from, __ffs(who) - 1);
-            to = __shfl_sync(0xffffffffu, to, __ffs(who) - 1);
-        }
-        if (lane == 0) {
-            p.new_lens[i] = lost ? part * pr : c.len;
-            p.copy[i] = from;
-            p.copy[p.Bout + i] = to;
-            p.copy[2 * p.Bout + i] = from >= 0 && to >= 0 ? (rest + 7) & ~7 : 0;
-        }
-    }
-    // counts of the pages that the old tables hold
-    for (int s = warp; s < p.Bin; s += kPlanThreads / 32) {
-        const long long cap = (long long)p.max_pages * pr;
-        const int full = (int)(max(0ll, min((long long)__ldg(p.lens + s), cap)) / pr);
-        const int shared = kids[s] - 1, own = kids[s] > 0 ? 0 : -1;
-        for (int j = lane; j < p.max_pages; j += 32) {
-            const int e = valid_page(__ldg(p.table + (size_t)s * p.max_pages + j), num_pages);
-            const int d = j < full ? shared : own;
-            if (e >= 0 && d != 0) atomicAdd(p.new_refs + e, d);
+            lost = __any_sync(0xffffffffu, lost);
+            const unsigned who = __ballot_sync(0xffffffffu, to >= 0);
+            if (who) {
+                from = __shfl_sync(0xffffffffu, from, __ffs(who) - 1);
+                to = __shfl_sync(0xffffffffu, to, __ffs(who) - 1);
+            }
+            if (lane == 0) {
+                p.new_lens[i] = lost ? part * pr : c.len;
+                p.copy[i] = from;
+                p.copy[p.Bout + i] = to;
+                p.copy[2 * p.Bout + i] = from >= 0 && to >= 0 ? (rest + 7) & ~7 : 0;
+            }
         }
     }
 }
 
 // CTA (new sequence, layer, KV head): the used rows of its parent's last page
-// into its own, in blocks of eight (16-byte words in every format).
-__global__ void __launch_bounds__(128) fork_copy_kernel(const ForkParams p) {
+// into its own, in blocks of eight (16-byte words in every format), K and V with four
+// loads in flight a thread.
+constexpr int kCopyThreads = 256;
+__global__ void __launch_bounds__(kCopyThreads) fork_copy_kernel(const ForkParams p) {
     grid_dependency_wait();
     const int i = blockIdx.x;
     const int rows = p.copy[2 * p.Bout + i];
@@ -224,7 +266,15 @@ __global__ void __launch_bounds__(128) fork_copy_kernel(const ForkParams p) {
         const uint4* src = reinterpret_cast<const uint4*>(p.pool.base[k] + ((layer + from) * p.pool.Hkv + blockIdx.z) * head);
         uint4* dst = reinterpret_cast<uint4*>(p.pool.base[k] + ((layer + to) * p.pool.Hkv + blockIdx.z) * head);
         const int n = rows * p.pool.row_bytes[k] / 16;
-        for (int x = threadIdx.x; x < n; x += 128) dst[x] = __ldg(src + x);
+        for (int x = threadIdx.x; x < n; x += 4 * kCopyThreads) {
+            uint4 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (x + j * kCopyThreads < n) v[j] = __ldg(src + x + j * kCopyThreads);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (x + j * kCopyThreads < n) dst[x + j * kCopyThreads] = v[j];
+        }
     }
 }
 
@@ -364,10 +414,16 @@ int launch_accept_tree(const AcceptParams& p, int B, int layers, cudaStream_t st
 }
 
 int launch_fork_pages(const ForkParams& p, cudaStream_t st) {
-    const size_t smem = sizeof(int) * (2 * (size_t)p.Bin + p.Bout);
-    int rc = launch_pdl(fork_plan_kernel, dim3(1), kPlanThreads, smem, st, p);
+    int dev;
+    int rc = current_device(&dev);
     if (rc) return rc;
-    return launch_pdl(fork_copy_kernel, dim3((unsigned)p.Bout, (unsigned)p.pool.layers, (unsigned)p.pool.Hkv), 128, 0, st, p);
+    const size_t smem = sizeof(int) * (5 * (size_t)p.Bin + 2 * p.Bout);
+    if (smem > 40 * 1024)  // (4 KB more are static; at most 7 * 4000 entries)
+        VA_CUDA(cudaFuncSetAttribute(fork_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024));
+    rc = launch_pdl(fork_plan_kernel, dim3(1), kPlanThreads, smem, st, p);
+    if (rc) return rc;
+    return launch_pdl(fork_copy_kernel, dim3((unsigned)p.Bout, (unsigned)p.pool.layers, (unsigned)p.pool.Hkv),
+                      kCopyThreads, 0, st, p);
 }
 
 int launch_compact_pages(const CompactParams& p, cudaStream_t st) {
