@@ -4,28 +4,28 @@
 //
 // One CTA per (sequence, KV head, tile of query rows, range of positions), one
 // per SM, 22 warps:
-//   warps 0-15   softmax: thread (set w, half hf, row r) has 32 of the 64 positions of
-//                query row r (TMEM lane r) in the jobs of set w;
+//   warps 0-15   softmax: thread (group w, half hf, row r) has 32 of the 64 positions of
+//                query row r (TMEM lane r) in the jobs of group w;
 //   warps 16-19  producers: codes -> exact fp16 codes in swizzled tiles;
 //   warp 20      one elected lane issues every tcgen05.mma;
 //   warp 21      copies: blocks of codes and scales into a ring, several ahead (fp16
 //                rows by tensor copies straight into the swizzled tiles).
-// A job is one block of 64 positions against 128 query rows; the jobs alternate
-// between two sets w of TMEM columns (S_w, O_w, 256 each) and of softmax warps, so
-// one set's exponentials run under the other's loads, exchange and MMAs. kTwo = false (up to 128
-// query rows): job j is block j, and O_0, O_1 (even and odd blocks) merge at the end.
-// kTwo = true (up to 256): jobs 2 i, 2 i + 1 are block i against rows 0..127 and
-// 128..255, so a decoded tile serves twice.
+// A job is one block of 64 positions against 128 query rows; the groups take the jobs in
+// turn, so one group's exponentials run under the other's loads and exchange. kTwo = false
+// (up to 128 query rows): job j is block j, one O, and the groups hand the rows' references
+// on from job to job. kTwo = true (up to 256): jobs 2 i, 2 i + 1 are block i against
+// rows 0..127 and 128..255, group w has rows and O of its own, and a decoded tile serves
+// twice. TMEM holds the O's and kNS buffers of scores, job j's in buffer j % kNS.
 //
-// Per job j (MMA order S(0) S(1), then PV(j) S(j + 2)):
+// Per job j (MMA order S(0) .. S(kNS - 1), then PV(j) S(j + kNS)):
 //   S_g = Q_g K_g^T (M = 128 rows, N = 64 positions) for each 64-dim group g, in
 //     TMEM. The K tile holds the exact codes (times a power of two), so the group
 //     scales multiply fp32 scores, as in decode_tree.cuh;
 //   the softmax threads load their scores, x = S_0 k_0 + S_1 k_1, exchange the row's
 //     maximum, and write P'_g = fp16(w v_g) over the scores;
 //   O_g += P'_g V_g (A = P' read from TMEM, B = the V tile read MN-major).
-// The MMAs of one thread execute in issue order, so S(j + 2) follows PV(j) into the
-// same columns, and a completed S implies every earlier PV into its set.
+// The MMAs of one thread execute in issue order, so S(j + kNS) follows PV(j) into the
+// same columns, and a completed PV(j) implies every earlier one.
 // O is rescaled only when a row's reference grows by more than 4 (log2): P' of the
 // largest weight stays in [2^6, 2^15), its one rounding relative.
 //
@@ -53,6 +53,10 @@ struct TreeTcCfg {
     static constexpr int kSG = kScaled ? kNG : 1;  // score accumulators, weight copies
     static constexpr int kRb = kDim * KindTraits<K>::kBits / 8;
     static constexpr int kNb = 64;                 // positions of a block
+    static constexpr int kSw = 64 * kSG;           // TMEM columns of a buffer of scores
+    static constexpr int kNS = kSG == 2 ? (kTwoTiles ? 2 : 3) : 4;
+    static constexpr int kOCols = kTwoTiles ? 256 : 128;  // TMEM: O, then the scores
+    static_assert(kOCols + kNS * kSw <= 512, "tensor memory");
     static constexpr int kProducers = 128;
     static constexpr int kThreads = 22 * 32;
     static constexpr int kQTile = 128 * kDim * 2;
@@ -68,19 +72,19 @@ struct TreeTcCfg {
     static constexpr int kRawTx = kRawSV + kNb * kSb;
     static constexpr int kRawStage = (kRawTx + 127) / 128 * 128;
     // what follows the ring: scales as floats [4 slots][K, V][kNG][64], masks,
-    // [2][2][2][128] maxima or sums, barriers, ev[4], TMEM slot, fail, special, ticket
+    // [2][2][2][128] maxima or sums, [2][128] references, barriers, ev[4], TMEM slot, fail, special, ticket
     static constexpr int kScaleSlots = 4;
     static constexpr int kScaleSlot = 2 * kNG * kNb * 4;
     static constexpr int kScaleV = kNG * kNb * 4;  // where a slot's V scales begin
     static constexpr int kScaleBytes = kScaled ? kScaleSlots * kScaleSlot : 0;
-    static constexpr int kRest = kScaleBytes + kRows * 8 + 4096 + 512 + 64;
+    static constexpr int kRest = kScaleBytes + kRows * 8 + 5120 + 512 + 64;
     static constexpr int kRoom = (227 * 1024 - 1024 - kOffRaw - kRest) / kRawStage;
     static constexpr int kRawStages = kDirect ? 1 : kRoom < 8 ? kRoom : 8;
     static constexpr int kOffScales = kOffRaw + (kDirect ? 0 : kRawStages * kRawStage);
     static constexpr int kOffMask = kOffScales + kScaleBytes;
     static constexpr int kOffMl = kOffMask + kRows * 8;
-    static constexpr int kOffBars = kOffMl + 4096;
-    static constexpr int kBars = 2 * kKS + 3 * kVS + 2 * 2 + 3 + kScaleSlots + 2 * kRawStages;
+    static constexpr int kOffBars = kOffMl + 5120;
+    static constexpr int kBars = 2 * kKS + 3 * kVS + 3 * kNS + 4 + 2 + kScaleSlots + 2 * kRawStages;
     static constexpr int kOffMisc = kOffBars + kBars * 8;
     static constexpr int kSmemBytes = 1024 + kOffMisc + 64;
     static_assert((kDirect || kRawStages >= 2) && kBars * 8 <= 512, "two blocks in flight");
@@ -269,13 +273,14 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     extern __shared__ __align__(128) uint8_t smem_raw[];
     // (an offset, not a rounded address: the compiler keeps seeing shared memory)
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    constexpr int D = C::kD, NG = C::kNG, NB = C::kNb, KS = C::kKS, VS = C::kVS, SG = C::kSG;
+    constexpr int D = C::kD, NG = C::kNG, NB = C::kNb, KS = C::kKS, VS = C::kVS, SG = C::kSG, NS = C::kNS;
     constexpr Kind KK = C::kKind;
     unsigned long long* s_mask = reinterpret_cast<unsigned long long*>(smem + C::kOffMask);
     float* s_xch = reinterpret_cast<float*>(smem + C::kOffMl);  // [2][2][2][128]
+    float* s_ref = s_xch + 1024;                                // [2][128]
     uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
     uint64_t *kempty = kfull + KS, *vfull = kempty + KS, *vempty = vfull + VS, *sfull = vempty + VS;
-    uint64_t *pfull = sfull + 2, *odone = pfull + 2, *fin = odone + 1, *scfull = fin + 1;
+    uint64_t *pfull = sfull + NS, *pvdone = pfull + NS, *refbar = pvdone + NS, *fin = refbar + 4, *scfull = fin + 1;
     uint64_t *rfull = scfull + C::kScaleSlots, *rempty = rfull + C::kRawStages, *vraw = rempty + C::kRawStages;
     uint64_t* qfull = vraw + VS;
     float* s_ev = reinterpret_cast<float*>(smem + C::kOffMisc);
@@ -324,9 +329,8 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     if (tid == 0) {
         for (int i = 0; i < KS; ++i) mbar_init(kfull + i, C::kDirect ? 1 : C::kProducers / 32), mbar_init(kempty + i, 1);
         for (int i = 0; i < VS; ++i) mbar_init(vfull + i, C::kProducers / 32), mbar_init(vempty + i, 1);
-        for (int i = 0; i < 2; ++i)
-            mbar_init(sfull + i, 1), mbar_init(pfull + i, 8);
-        mbar_init(odone, 1);
+        for (int i = 0; i < NS; ++i) mbar_init(sfull + i, 1), mbar_init(pfull + i, 8), mbar_init(pvdone + i, 1);
+        for (int i = 0; i < 4; ++i) mbar_init(refbar + i, 2);
         mbar_init(fin, 1);
         mbar_init(qfull, 1);
         for (int i = 0; i < C::kScaleSlots; ++i) mbar_init(scfull + i, 1);
@@ -389,9 +393,10 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
         const float c2 = rsqrtf((float)D) * kLog2e * tc_k_inv_step<KK>();
         const int w = set;
         for (int j = w; j < njobs; j += 2) {
-            const int k = j >> 1, blk = C::kTwo ? k : j;
+            const int blk = C::kTwo ? j >> 1 : j, sb = j % NS;
+            const uint32_t ph = (uint32_t)(j / NS) & 1u;
             const int pb = p0 + blk * NB;
-            bool ok = mbar_wait_fast(sfull + w, (uint32_t)k & 1u);
+            bool ok = mbar_wait_fast(sfull + sb, ph);
             // (a slot of scales is written again only after this block's PV, so this phase
             // cannot be passed twice before it is seen here)
             if constexpr (C::kScaled)
@@ -406,7 +411,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
             if ((C::kTwo ? w * 128 : 0) + quad * 32 < live) {
                 uint32_t sc = sbase + C::kOffScales + (blk % C::kScaleSlots) * C::kScaleSlot;
                 asm volatile("" : "+r"(sc));  // the loads of scales come after the waits
-                const uint32_t tS = tbase + w * 256 + lane_addr, tO = tS + 128;
+                const uint32_t tS = tbase + C::kOCols + sb * C::kSw + lane_addr, tO = tbase + (C::kTwo ? w * 128 : 0) + lane_addr;
                 float x[32];
 #pragma unroll
                 for (int cb = 0; cb < 32; cb += 16) {
@@ -458,29 +463,51 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                 }
                 // the row's maximum over both halves; their barrier also puts every load of S
                 // before the stores of P' below
-                float* xch = s_xch + w * 512 + (k & 1) * 256;
+                float* xch = s_xch + w * 512 + (j >> 1 & 1) * 256;
                 xch[hf * 128 + row] = fmaxf(b0, b1);
                 named_barrier_sync(2 + w * 4 + quad, 64);
                 const float bm = fmaxf(fmaxf(b0, b1), xch[(1 - hf) * 128 + row]);
                 const float ev = C::kScaled ? s_ev[blk % C::kScaleSlots] : 0.f;
                 const float want = bm == kNegMax ? kNegMax : fmaf(bm, c2, ev - 10.f);
-                const float nref = want > m_ref + 4.f ? want : m_ref;
-                if (__any_sync(0xffffffffu, nref != m_ref)) {
-                    const float corr = fast_exp2(m_ref - nref);
-                    l_sum *= corr;
-                    m_ref = nref;
-                    if (k > 0) {  // this half of the row's O
-#pragma unroll 1
-                        for (int cb = 0; cb < D / 2; cb += 16) {
-                            uint32_t o[16];
-                            tmem_ld16_nowait(tO + hf * (D / 2) + cb, o);
-                            tmem_wait_ld_only();
-                            tmem_tie16(o);
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-                            tmem_st16_u(tO + hf * (D / 2) + cb, o);
-                        }
+                // the reference that O has so far: the row's own (two tiles), or what the other
+                // group left after job j - 1 (two slots, each rewritten two jobs on, after both
+                // halves have read it)
+                float oref = m_ref;
+                if constexpr (!C::kTwo) {
+                    if (j > 0) {
+                        ok = mbar_wait_fast(refbar + quad, (uint32_t)(j - 1) & 1u);
+                        oref = s_ref[((j - 1) & 1) * 128 + row];
                     }
+                }
+                const float nref = want > oref + 4.f ? want : oref;
+                if constexpr (!C::kTwo) {
+                    if (hf == 0) s_ref[(j & 1) * 128 + row] = nref;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(refbar + quad);
+                }
+                l_sum *= fast_exp2(m_ref - nref);
+                m_ref = nref;
+                const int prev = j - (C::kTwo ? 2 : 1);  // the last job into this O
+                if (__any_sync(0xffffffffu, nref != oref) && prev >= 0) {
+                    // this half of the row's O, once its earlier products are in
+                    ok = ok && mbar_wait_fast(pvdone + prev % NS, (uint32_t)(prev / NS) & 1u);
+                    tc05_fence_after();
+                    const float corr = fast_exp2(oref - nref);
+#pragma unroll 1
+                    for (int cb = 0; cb < D / 2; cb += 16) {
+                        uint32_t o[16];
+                        tmem_ld16_nowait(tO + hf * (D / 2) + cb, o);
+                        tmem_wait_ld_only();
+                        tmem_tie16(o);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                        tmem_st16_u(tO + hf * (D / 2) + cb, o);
+                    }
+                }
+                if (!ok) {
+                    if (lane == 0) report_error(kErrFullWait);
+                    *fail = 1;
+                    break;
                 }
                 float2 sum = make_float2(0.f, 0.f);
                 // (two instantiations: only blocks with drafted rows or the end select)
@@ -529,9 +556,9 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
             }
             tc05_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(pfull + w);
+            if (lane == 0) mbar_arrive(pfull + sb);
         }
-        if (!*fail && !mbar_wait_fast(odone, 0)) {  // every MMA of the CTA
+        if (!*fail && !mbar_wait_fast(pvdone + (njobs - 1) % NS, (uint32_t)((njobs - 1) / NS) & 1u)) {  // every MMA of the CTA
             if (lane == 0) report_error(kErrFullWait);
             *fail = 1;
         }
@@ -723,11 +750,11 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
         const uint64_t dq = umma_desc_sw128(ub, 16, 1024), dk = umma_desc_sw128(ub + C::kOffK, 16, 1024);
         const uint64_t dv = umma_desc_sw128(ub + C::kOffV, NB * 128, 1024);
         const auto issue_s = [&](int j) {
-            const int w = j & 1, i = C::kTwo ? j >> 1 : j, s = i % KS;
+            const int w = j & 1, i = C::kTwo ? j >> 1 : j, s = i % KS, sb = j % NS;
             if (!mbar_wait_fast(kfull + s, (uint32_t)(i / KS) & 1u)) return false;
             tc05_fence_after();
             const uint64_t qa = dq + (C::kTwo ? w * (C::kQTile / 16) : 0), ka = dk + s * (C::kTile / 16);
-            const uint32_t d = ut + w * 256;
+            const uint32_t d = ut + C::kOCols + sb * C::kSw;
             if (elect_one()) {
 #pragma unroll
                 for (int g = 0; g < NG; ++g)
@@ -735,40 +762,40 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                     for (int kk = 0; kk < 4; ++kk)
                         umma_f16(d + (C::kScaled ? 64 * g : 0), qa + (g * 16384 + kk * 32) / 16, ka + (g * (NB * 128) + kk * 32) / 16,
                                  kIdescS, kk > 0 || (!C::kScaled && g > 0));
-                umma_commit(sfull + w);
+                umma_commit(sfull + sb);
                 if (!C::kTwo || w == 1) umma_commit(kempty + s);
             }
             __syncwarp();
             return true;
         };
         const auto issue_pv = [&](int j) {
-            const int w = j & 1, k = j >> 1, i = C::kTwo ? j >> 1 : j, s = i % VS;
+            const int w = j & 1, i = C::kTwo ? j >> 1 : j, s = i % VS, sb = j % NS;
             if (!mbar_wait_fast(vfull + s, (uint32_t)(i / VS) & 1u)) return false;
-            if (!mbar_wait_fast(pfull + w, (uint32_t)k & 1u)) return false;
+            if (!mbar_wait_fast(pfull + sb, (uint32_t)(j / NS) & 1u)) return false;
             tc05_fence_after();
             const uint64_t va = dv + s * (C::kTile / 16);
-            const uint32_t d = ut + w * 256;
+            const uint32_t o = ut + (C::kTwo ? w * 128 : 0), a = ut + C::kOCols + sb * C::kSw;
+            const bool more = j >= (C::kTwo ? 2 : 1);  // O holds earlier products
             if (elect_one()) {
 #pragma unroll
                 for (int g = 0; g < SG; ++g)
 #pragma unroll
                     for (int kk = 0; kk < NB / 16; ++kk)
-                        umma_f16_ts(d + 128 + 64 * g, d + 32 * g + 8 * kk, va + (g * (NB * 128) + kk * 2048) / 16, kIdescO,
-                                    k > 0 || kk > 0);
+                        umma_f16_ts(o + 64 * g, a + 32 * g + 8 * kk, va + (g * (NB * 128) + kk * 2048) / 16, kIdescO,
+                                    more || kk > 0);
                 if (!C::kTwo || w == 1) umma_commit(vempty + s);
+                umma_commit(pvdone + sb);
             }
             __syncwarp();
             return true;
         };
-        bool ok = mbar_wait_fast(qfull, 0) && issue_s(0);
-        if (njobs > 1) ok = ok && issue_s(1);
+        bool ok = mbar_wait_fast(qfull, 0);
+        for (int j = 0; j < min(NS, njobs); ++j) ok = ok && issue_s(j);
         for (int j = 0; ok && j < njobs; ++j) {
             ok = issue_pv(j);
-            if (j + 2 < njobs) ok = ok && issue_s(j + 2);
+            if (j + NS < njobs) ok = ok && issue_s(j + NS);
         }
-        if (ok) {
-            if (elect_one()) umma_commit(odone);
-        } else {  // every MMA issued so far ends before the tensor memory is given back
+        if (!ok) {  // every MMA issued so far ends before the tensor memory is given back
             if (lane == 0) report_error(kErrFullWait);
             *fail = 1;
             if (elect_one()) umma_commit(fin);
@@ -786,7 +813,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     grid_launch_dependents();
 
     // ---- epilogue: a thread's row, its part of the dims: half of them (two tiles: of its
-    // set's tile) or a quarter (one tile: both sets' outputs merged)
+    // group's tile) or a quarter
     const bool direct = nsplit == 1;
     if (warp < 16) {
         s_xch[(set * 2 + hf) * 128 + row] = l_sum;
@@ -795,15 +822,12 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
         const auto sum_of = [&](int w) { return s_xch[w * 256 + row] + s_xch[w * 256 + 128 + row]; };
         const int qr = (C::kTwo ? set * 128 : 0) + row, r = r0 + qr;
         const bool on = (C::kTwo ? set * 128 : 0) + quad * 32 < live;  // (the same for the whole warp)
-        const bool both = !C::kTwo && nblk > 1;                        // the odd blocks' set has something
         const int w0 = C::kTwo ? set : 0;
-        float mx = s_xch[512 + w0 * 128 + row], sum = sum_of(w0), a0 = 1.f, a1 = 0.f;
-        if (both) {
+        float mx = s_xch[512 + w0 * 128 + row], sum = sum_of(w0);
+        if constexpr (!C::kTwo) {  // O has the last reference, the larger; the sums each group's own
             const float m0 = mx, m1 = s_xch[512 + 128 + row];
             mx = fmaxf(m0, m1);
-            a0 = fast_exp2(m0 - mx);
-            a1 = fast_exp2(m1 - mx);
-            sum = sum * a0 + sum_of(1) * a1;
+            sum = sum * fast_exp2(m0 - mx) + sum_of(1) * fast_exp2(m1 - mx);
         }
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const size_t slot = ((size_t)stream * p.R + r) * p.S + split;
@@ -820,17 +844,12 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[i] = 0.f;
             if (on) {
-                uint32_t u[16], v[16];
-                tmem_ld16_nowait(tbase + w0 * 256 + 128 + lane_addr + cb, u);
-                if (both) tmem_ld16_nowait(tbase + 256 + 128 + lane_addr + cb, v);
+                uint32_t u[16];
+                tmem_ld16_nowait(tbase + w0 * 128 + lane_addr + cb, u);
                 tmem_wait_ld_only();
                 tmem_tie16(u);
-                tmem_tie16(v);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    o[i] = __uint_as_float(u[i]);
-                    if (both) o[i] = fmaf(__uint_as_float(v[i]), a1, o[i] * a0);
-                }
+                for (int i = 0; i < 16; ++i) o[i] = __uint_as_float(u[i]);
             }
             if constexpr (C::kFloat) {
                 if (*special && qr < live) {
