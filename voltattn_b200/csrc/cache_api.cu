@@ -74,13 +74,13 @@ int tree_splits(int nsm, int B, int Hkv, int R, int Lmax) {
     return S;
 }
 
-// Division by the page size as a multiplication (round-up method): with 2^(l-1) < d <=
+// Division by d >= 1 as a multiplication (round-up method): with 2^(l-1) < d <=
 // 2^l and m = floor(2^32 (2^l - d) / d) + 1, floor(n / d) = (mulhi(n, m) + n) >> l for
 // every n < 2^31.
-void page_divisor(int page_rows, unsigned& mul, unsigned& shift) {
+void divisor(int d, unsigned& mul, unsigned& shift) {
     shift = 0;
-    while ((1ll << shift) < page_rows) ++shift;
-    mul = (unsigned)((((unsigned long long)1 << 32) * ((1ull << shift) - (unsigned)page_rows)) / (unsigned)page_rows + 1);
+    while ((1ll << shift) < d) ++shift;
+    mul = (unsigned)((((unsigned long long)1 << 32) * ((1ull << shift) - (unsigned)d)) / (unsigned)d + 1);
 }
 
 int check_layers(int fmt, int Hkv, int page_rows, int num_pages, int layers) {
@@ -183,7 +183,8 @@ int va_decode_tree(int fmt, const va_bufs* b, const long long* q_strides, const 
     p.max_pages = max_pages;
     p.page_rows = page_rows;
     p.num_pages = num_pages;
-    page_divisor(page_rows, p.page_mul, p.page_shift);
+    divisor(page_rows, p.page_mul, p.page_shift);
+    divisor(p.G, p.g_mul, p.g_shift);
     uint8_t* w = static_cast<uint8_t*>(ws);
     p.counters = reinterpret_cast<unsigned*>(w);
     w += kCounterBytes;
@@ -231,7 +232,7 @@ int va_append_packed(int fmt, const void* k, const void* v, int in_type, const l
     p.max_pages = max_pages;
     p.page_rows = page_rows;
     p.num_pages = num_pages;
-    page_divisor(page_rows, p.page_mul, p.page_shift);
+    divisor(page_rows, p.page_mul, p.page_shift);
     return launch_append_packed(fmt, in_type, p, static_cast<cudaStream_t>(stream));
 }
 

@@ -67,6 +67,9 @@ struct TreeParams {
     int max_pages, page_rows, num_pages;
     // pos / page_rows = (umulhi(pos, page_mul) + pos) >> page_shift for 0 <= pos < 2^31
     unsigned page_mul, page_shift;
+    unsigned g_mul, g_shift;  // r / G likewise
+    // node of query row r
+    __device__ __forceinline__ int node_of(int r) const { return (int)((__umulhi((unsigned)r, g_mul) + (unsigned)r) >> g_shift); }
 };
 
 // Splits of a sequence of len rows: whole units of kTreeUnit rows, at most S.
@@ -323,21 +326,17 @@ __device__ __forceinline__ void tree_merge(const TreeParams& p, int stream, int 
     float* sl = sw + kRows * kTreeMaxSplits;  // [kRows] sums
     for (int row = tid >> 5; row < rows; row += kThreads / 32) {
         const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + ((size_t)stream * p.R + r0 + row) * p.S;
-        float2 w[kTreeMaxSplits / 32];
         float mx = kNegMax, sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < kTreeMaxSplits / 32; ++k) {
-            const int s = 32 * k + lane;
-            w[k] = s < nsplit ? __ldcg(ml + s) : make_float2(kNegMax, 0.f);
-            mx = fmaxf(mx, w[k].x);
-        }
+#pragma unroll 1
+        for (int i = lane; i < nsplit; i += 32) mx = fmaxf(mx, __ldcg(ml + i).x);
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-#pragma unroll
-        for (int k = 0; k < kTreeMaxSplits / 32; ++k) {
-            const float a = fast_exp2(w[k].x - mx);
-            sum = fmaf(w[k].y, a, sum);
-            if (32 * k + lane < nsplit) sw[row * kTreeMaxSplits + 32 * k + lane] = a;
+#pragma unroll 1
+        for (int i = lane; i < nsplit; i += 32) {
+            const float2 w = __ldcg(ml + i);
+            const float a = fast_exp2(w.x - mx);
+            sum = fmaf(w.y, a, sum);
+            sw[row * kTreeMaxSplits + i] = a;
         }
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
@@ -385,9 +384,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
     unsigned* s_ticket = reinterpret_cast<unsigned*>(s_ml + C::kWarps * C::kRows);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int split = (int)(blockIdx.x % p.S);
-    const int rest = (int)(blockIdx.x / p.S);
-    const int tile = rest % p.tiles, stream = rest / p.tiles;
+    const int tile = (int)blockIdx.x / p.S, split = (int)blockIdx.x - tile * p.S;
+    const int stream = (int)(blockIdx.y + blockIdx.z * gridDim.y);
+    if (stream >= p.B * p.Hkv) return;
     const int b = stream / p.Hkv, hk = stream - b * p.Hkv;
     const int r0 = tile * C::kRows;
 
@@ -400,7 +399,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
     const int nsplit = max(1, (len + chunk - 1) / chunk);
     if (split >= nsplit) return;
     const int p0 = split * chunk, p1 = min(len, p0 + chunk);
-    const bool dead = r0 / p.G >= n;  // every row of the tile is past the sequence's nodes
+    const bool dead = p.node_of(r0) >= n;  // every row of the tile is past the sequence's nodes
     if (dead && split > 0) return;
 
     uint8_t* ring = smem + warp * (C::kStages * C::kStageBytes);
@@ -411,7 +410,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
         fence_mbar_init();
     }
     if (tid < C::kRows) {
-        const int r = r0 + tid, node = r / p.G;
+        const int r = r0 + tid, node = p.node_of(r);
         s_mask[tid] = (r < p.R && node < n) ? __ldg(p.mask + (size_t)b * p.Q + node) : 0ull;
     }
     __syncthreads();
@@ -449,9 +448,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
                      lane_bytes, bar + s, policy);
         }
     };
-#pragma unroll
-    for (int i = 0; i < C::kStages; ++i)
-        if (i < mine) issue(i, i);
+#pragma unroll 1
+    for (int i = 0; i < min(C::kStages, mine); ++i) issue(i, i);
 
     // the query rows as A fragments, 16 dims (64 gr + 16 t ..) of rows g and
     // g + 8 per lane, in the order of k_chunk's pairs; sums of q per group
@@ -460,7 +458,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int r = r0 + g + 8 * e;
-            const int node = r / p.G;
+            const int node = p.node_of(r);
             const bool ok = r < p.R && node < n;
             const __half* src = p.q + b * p.qs_b + (ok ? node : 0) * p.qs_t + (long long)(hk * p.G + (ok ? r - node * p.G : 0)) * p.qs_h;
 #pragma unroll
@@ -499,11 +497,12 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
     // scores in log2 units per unit of the raw product
     const float c2 = rsqrtf((float)D) * kLog2e * TreeCode<C::kKind>::kInvStep;
 
-    // One block of positions in stage st. tail: it holds drafted rows or the end
-    // of the sequence (two instantiations: the others spend nothing on masks).
-    const auto block = [&](auto is_tail, const uint8_t* st, int pb) {
+    // kStep positions from row row0 of stage st on. tail: they hold drafted rows or the
+    // end of the sequence (two instantiations: the others spend nothing on masks).
+    constexpr int kStep = 16;
+    const auto block = [&](auto is_tail, const uint8_t* st, int row0, int pb) {
         constexpr bool tail = decltype(is_tail)::value;
-        constexpr int NT = PB / 8;  // 8-position tiles of S
+        constexpr int NT = kStep / 8;  // 8-position tiles of S
         // scores, then weights: row g + 8 r, this lane's positions t + 8 (nt & 1) (.x) and + 4 (.y) of
         // the 16 of tiles nt, nt ^ 1
         float2 x[NT][2];
@@ -512,7 +511,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             // S of 8 positions: lane g decodes row (g >> 1) + 4 (g & 1) (+ 8 for odd tiles) of the 16
-            const uint8_t* krow = st + (16 * (nt >> 1) + (g >> 1) + 4 * (g & 1) + 8 * (nt & 1)) * C::kRb;
+            const uint8_t* krow = st + (row0 + 16 * (nt >> 1) + (g >> 1) + 4 * (g & 1) + 8 * (nt & 1)) * C::kRb;
             float acc[NG][4];
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
@@ -535,11 +534,11 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
                     const int pr = 16 * (nt >> 1) + t + 4 * e + 8 * (nt & 1);
                     uint32_t k;
                     if constexpr (NG == 2) {
-                        k = *reinterpret_cast<const uint32_t*>(st + C::kOffSK + 4 * pr);
-                        vsc[nt][e] = *reinterpret_cast<const uint32_t*>(st + C::kOffSV + 4 * pr);
+                        k = *reinterpret_cast<const uint32_t*>(st + C::kOffSK + 4 * (row0 + pr));
+                        vsc[nt][e] = *reinterpret_cast<const uint32_t*>(st + C::kOffSV + 4 * (row0 + pr));
                     } else {
-                        k = *reinterpret_cast<const uint16_t*>(st + C::kOffSK + 2 * pr);
-                        vsc[nt][e] = *reinterpret_cast<const uint16_t*>(st + C::kOffSV + 2 * pr);
+                        k = *reinterpret_cast<const uint16_t*>(st + C::kOffSK + 2 * (row0 + pr));
+                        vsc[nt][e] = *reinterpret_cast<const uint16_t*>(st + C::kOffSV + 2 * (row0 + pr));
                     }
                     f[e] = __half22float2(bits_h2(k));
                     uint32_t va = vsc[nt][e];
@@ -644,8 +643,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
         // O += P' V, 16 positions at a time
         bool special = false;
 #pragma unroll
-        for (int j = 0; j < PB / 16; ++j) {
-            const uint8_t* vb = st + C::kOffV + (16 * j + t) * C::kRb;
+        for (int j = 0; j < kStep / 16; ++j) {
+            const uint8_t* vb = st + C::kOffV + (row0 + 16 * j + t) * C::kRb;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
                 uint32_t pa[4];
@@ -691,10 +690,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
             // inf and nan entries of the block's rows, added to the rows that see them: what a
             // positive weight times such an entry gives
             if (__any_sync(0xffffffffu, special)) {
-                for (int pr = 0; pr < PB; ++pr) {
+                for (int pr = 0; pr < kStep; ++pr) {
                     const int j = pb + pr - ctx;
                     if (j >= n) break;
-                    const uint8_t* vr = st + C::kOffV + pr * C::kRb;
+                    const uint8_t* vr = st + C::kOffV + (row0 + pr) * C::kRb;
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         if (!(j < 0 || ((s_mask[g + 8 * r] >> (j & 63)) & 1ull))) continue;
@@ -723,8 +722,11 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
             break;
         }
         const int pb = p0 + (warp + i * C::kWarps) * PB;
-        if (pb + PB > ctx) block(std::true_type{}, ring + s * C::kStageBytes, pb);
-        else block(std::false_type{}, ring + s * C::kStageBytes, pb);
+#pragma unroll 1
+        for (int h = 0; h < PB; h += kStep) {
+            if (pb + h + kStep > ctx) block(std::true_type{}, ring + s * C::kStageBytes, h, pb + h);
+            else block(std::false_type{}, ring + s * C::kStageBytes, h, pb + h);
+        }
         __syncwarp();
         if (i + C::kStages < mine) issue(i + C::kStages, s);
         if (++s == C::kStages) s = 0, phase ^= 1u;
@@ -763,13 +765,14 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
     constexpr int Q4 = D / 4;  // float4 columns of a row
     const bool direct = nsplit == 1 || dead;
     const auto store_out = [&](int r, int c, float4 v, float inv) {
-        const int node = r / p.G;
+        const int node = p.node_of(r);
         __half* dst = p.out + b * p.os_b + node * p.os_t + (long long)(hk * p.G + (r - node * p.G)) * p.os_h + 4 * c;
         const bool live = node < n && inv != 0.f;
         const __half2 a = __floats2half2_rn(live ? v.x * inv : 0.f, live ? v.y * inv : 0.f);
         const __half2 d = __floats2half2_rn(live ? v.z * inv : 0.f, live ? v.w * inv : 0.f);
         *reinterpret_cast<uint2*>(dst) = make_uint2(h2_bits(a), h2_bits(d));
     };
+#pragma unroll 1
     for (int i = tid; i < C::kRows * Q4; i += C::kThreads) {
         const int row = i / Q4, c = i - row * Q4, r = r0 + row;
         if (r >= p.R) break;

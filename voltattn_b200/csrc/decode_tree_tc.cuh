@@ -290,9 +290,9 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     unsigned* s_ticket = tslot + 3;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int split = (int)(blockIdx.x % p.S);
-    const int rest = (int)(blockIdx.x / p.S);
-    const int tile = rest % p.tiles, stream = rest / p.tiles;
+    const int tile = (int)blockIdx.x / p.S, split = (int)blockIdx.x - tile * p.S;
+    const int stream = (int)(blockIdx.y + blockIdx.z * gridDim.y);
+    if (stream >= p.B * p.Hkv) return;
     const int b = stream / p.Hkv, hk = stream - b * p.Hkv;
     const int r0 = tile * C::kRows;
 
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     const int rows_here = min(C::kRows, p.R - r0);
 
     const auto store_out = [&](int r, int c, float4 v, float inv) {
-        const int node = r / p.G;
+        const int node = p.node_of(r);
         __half* dst = p.out + b * p.os_b + node * p.os_t + (long long)(hk * p.G + (r - node * p.G)) * p.os_h + 4 * c;
         const bool on = node < n && inv != 0.f;
         const __half2 a = __floats2half2_rn(on ? v.x * inv : 0.f, on ? v.y * inv : 0.f);
@@ -370,13 +370,13 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
                 const int x = tid + 512 * i, qr = x / (D / 8), c = x - qr * (D / 8);
                 v[i] = make_uint4(0u, 0u, 0u, 0u);
                 if (qr < live) {
-                    const int r = r0 + qr, node = r / p.G;
+                    const int r = r0 + qr, node = p.node_of(r);
                     v[i] = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.qs_b + node * p.qs_t +
                                                                 (long long)(hk * p.G + (r - node * p.G)) * p.qs_h) + c);
                 }
             }
             const unsigned long long in_tree = n >= 64 ? ~0ull : (1ull << n) - 1ull;
-            if (tid < C::kRows) s_mask[tid] = tid < live ? __ldg(p.mask + (size_t)b * p.Q + (r0 + tid) / p.G) & in_tree : 0ull;
+            if (tid < C::kRows) s_mask[tid] = tid < live ? __ldg(p.mask + (size_t)b * p.Q + p.node_of(r0 + tid)) & in_tree : 0ull;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int x = tid + 512 * i, qr = x / (D / 8), c = x - qr * (D / 8), rr = qr & 127;
@@ -831,7 +831,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
         }
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         const size_t slot = ((size_t)stream * p.R + r) * p.S + split;
-        const int node = r / p.G;
+        const int node = p.node_of(r);
         __half* orow = p.out + b * p.os_b + node * p.os_t + (long long)(hk * p.G + (r - node * p.G)) * p.os_h;
         const float scale = on && node < n ? inv : 0.f;  // (0: rows of no node, or that see nothing)
         const bool wide = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;

@@ -30,7 +30,10 @@ int launch_tree_cfg(void (*kernel)(const TreeParams, const Maps...), const TreeP
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)((long long)p.B * p.Hkv * p.tiles * p.S));
+    // x: the splits and tiles of one (sequence, KV head), which read the same rows, next to
+    // one another; y, z: the (sequence, KV head) pairs
+    const unsigned streams = (unsigned)(p.B * p.Hkv), y = std::min(streams, 65535u);
+    cfg.gridDim = dim3((unsigned)(p.tiles * p.S), y, (streams + y - 1) / y);
     cfg.blockDim = dim3(C::kThreads);
     cfg.dynamicSmemBytes = C::kSmemBytes;
     cfg.stream = st;
