@@ -322,49 +322,70 @@ __device__ __forceinline__ bool clear_not_finite(uint32_t& u) {
 template <int D, int kRows, int kThreads, class Store>
 __device__ __forceinline__ void tree_merge(const TreeParams& p, int stream, int r0, int rows, int nsplit, float* sw,
                                            int tid, const Store& store_out) {
-    const int lane = tid & 31;
     float* sl = sw + kRows * kTreeMaxSplits;  // [kRows] sums
-    for (int row = tid >> 5; row < rows; row += kThreads / 32) {
+    // eight lanes a row, four ranges in flight a lane
+    const int l8 = tid & 7;
+#pragma unroll 1
+    for (int r8 = tid >> 3; r8 < (rows + 3 & ~3); r8 += kThreads / 8) {  // (whole warps: four rows)
+        const int row = min(r8, rows - 1);
         const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + ((size_t)stream * p.R + r0 + row) * p.S;
         float mx = kNegMax, sum = 0.f;
 #pragma unroll 1
-        for (int i = lane; i < nsplit; i += 32) mx = fmaxf(mx, __ldcg(ml + i).x);
+        for (int i = l8; i < nsplit; i += 32) {
+            float m[4];
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-#pragma unroll 1
-        for (int i = lane; i < nsplit; i += 32) {
-            const float2 w = __ldcg(ml + i);
-            const float a = fast_exp2(w.x - mx);
-            sum = fmaf(w.y, a, sum);
-            sw[row * kTreeMaxSplits + i] = a;
+            for (int k = 0; k < 4; ++k) m[k] = i + 8 * k < nsplit ? __ldcg(&ml[i + 8 * k].x) : kNegMax;
+            mx = fmaxf(mx, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
         }
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        if (lane == 0) sl[row] = sum;
+        for (int off = 4; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+#pragma unroll 1
+        for (int i = l8; i < nsplit; i += 32) {
+            float2 w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = i + 8 * k < nsplit ? __ldcg(ml + i + 8 * k) : make_float2(kNegMax, 0.f);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float a = fast_exp2(w[k].x - mx);
+                sum = fmaf(w[k].y, a, sum);
+                if (i + 8 * k < nsplit) sw[row * kTreeMaxSplits + i + 8 * k] = a;
+            }
+        }
+#pragma unroll
+        for (int off = 4; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (l8 == 0) sl[row] = sum;
     }
     named_barrier_sync(1, kThreads);
     constexpr int Q4 = D / 4;
     static_assert(kThreads % Q4 == 0, "a thread keeps its column");
-    constexpr int kRowStep = kThreads / Q4, kItems = 4;
+    constexpr int kRowStep = kThreads / Q4, kItems = kRows == 16 ? 4 : 2, kAhead = 4;
     const int c = tid % Q4;
     for (int rw = tid / Q4; rw < rows; rw += kItems * kRowStep) {
         float4 v[kItems];
 #pragma unroll
         for (int k = 0; k < kItems; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-        for (int s = 0; s < nsplit; ++s) {
+        const float4* src = reinterpret_cast<const float4*>(p.ws_o + ((size_t)stream * p.R + r0) * p.S * D) + c;
+#pragma unroll 1
+        for (int s0 = 0; s0 < nsplit; s0 += kAhead) {
+            float4 u[kAhead][kItems];
 #pragma unroll
-            for (int k = 0; k < kItems; ++k) {
-                const int row = rw + k * kRowStep;
-                if (row >= rows) break;
-                const float4 u = __ldcg(
-                    reinterpret_cast<const float4*>(p.ws_o + (((size_t)stream * p.R + r0 + row) * p.S + s) * D + 4 * c));
-                const float a = sw[row * kTreeMaxSplits + s];
-                v[k].x = fmaf(u.x, a, v[k].x);
-                v[k].y = fmaf(u.y, a, v[k].y);
-                v[k].z = fmaf(u.z, a, v[k].z);
-                v[k].w = fmaf(u.w, a, v[k].w);
-            }
+            for (int z = 0; z < kAhead; ++z)
+#pragma unroll
+                for (int k = 0; k < kItems; ++k) {
+                    const int row = min(rw + k * kRowStep, rows - 1), s = min(s0 + z, nsplit - 1);
+                    u[z][k] = __ldcg(src + ((size_t)row * p.S + s) * Q4);
+                }
+#pragma unroll
+            for (int z = 0; z < kAhead; ++z)
+#pragma unroll
+                for (int k = 0; k < kItems; ++k) {
+                    const int row = min(rw + k * kRowStep, rows - 1);
+                    const float a = s0 + z < nsplit ? sw[row * kTreeMaxSplits + s0 + z] : 0.f;
+                    v[k].x = fmaf(u[z][k].x, a, v[k].x);
+                    v[k].y = fmaf(u[z][k].y, a, v[k].y);
+                    v[k].z = fmaf(u[z][k].z, a, v[k].z);
+                    v[k].w = fmaf(u[z][k].w, a, v[k].w);
+                }
         }
 #pragma unroll
         for (int k = 0; k < kItems; ++k) {
