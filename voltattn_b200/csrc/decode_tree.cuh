@@ -108,6 +108,7 @@ struct TreeCfg {
     // + barriers, masks, (ref, l) of every warp and row, the ticket
     static constexpr int kSmemBytes = kBig + kWarps * kStages * 8 + kRows * 8 + kWarps * kRows * 8 + 16;
     static constexpr int kMinCtas = 3;
+    static_assert(kRows * (kTreeMaxSplits + 1) * 4 <= kBig, "the merge of the ranges fits before the barriers");
 };
 
 __device__ __forceinline__ void mma_f16_16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {

@@ -80,7 +80,10 @@ struct TreeTcCfg {
     static constexpr int kRest = kScaleBytes + kRows * 8 + 5120 + 512 + 64;
     static constexpr int kRoom = (227 * 1024 - 1024 - kOffRaw - kRest) / kRawStage;
     static constexpr int kRawStages = kDirect ? 1 : kRoom < 8 ? kRoom : 8;
-    static constexpr int kOffScales = kOffRaw + (kDirect ? 0 : kRawStages * kRawStage);
+    // (the merge of the ranges takes the front of shared memory: what follows stays past it)
+    static constexpr int kMergeBytes = (kRows * (kTreeMaxSplits + 1) * 4 + 127) / 128 * 128;
+    static constexpr int kRingEnd = kOffRaw + (kDirect ? 0 : kRawStages * kRawStage);
+    static constexpr int kOffScales = kRingEnd > kMergeBytes ? kRingEnd : kMergeBytes;
     static constexpr int kOffMask = kOffScales + kScaleBytes;
     static constexpr int kOffMl = kOffMask + kRows * 8;
     static constexpr int kOffBars = kOffMl + 5120;
