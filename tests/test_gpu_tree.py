@@ -316,3 +316,79 @@ def test_chain_matches_multiquery(va):
     va.decode_multiquery("q4+", va.DeviceBufs(*sides, *sc, q, out, ws), torch.from_numpy(c.lens).cuda(), B, Hq, Hkv, Q, Lmax, D, 2)
     torch.cuda.synchronize()
     assert np.abs(out.transpose(1, 2).cpu().numpy().astype(np.float64) - got).max() < 2e-2
+
+
+@pytest.mark.parametrize("fmt", R.FORMATS)
+@pytest.mark.parametrize("rows,D", [(64, 128), (65, 128), (66, 64), (96, 128), (128, 64), (128, 128), (129, 128), (130, 64), (256, 128),
+                                    (257, 128), (320, 64)])
+def test_row_tile_edges(va, fmt, rows, D):
+    """Query rows around each tile size of the kernels, with a full, a ragged and an unused sequence."""
+    Q = 64 if rows > 129 else 32 if rows % 32 == 0 else 13 if rows % 13 == 0 else 11 if rows % 11 == 0 else 3
+    G = -(-rows // Q)
+    c = Case(fmt, 3, G, 1, Q, D, 32, [Q + 300, Q // 2 + 65, 0], [Q, Q // 2, 0], seed=rows)
+    got = c.check(va, 3)
+    assert (got[2] == 0).all() and (got[1, Q // 2:] == 0).all()
+
+
+@pytest.mark.parametrize("fmt", R.FORMATS)
+@pytest.mark.parametrize("what", ["nan", "inf", "-inf"])
+def test_unseen_rows_in_tiles_of_128(va, fmt, what):
+    test_unseen_rows_have_no_influence(va, fmt, 8, what)
+
+
+@pytest.mark.parametrize("fmt", ["f16+", "bf16+", "f8+"])
+@pytest.mark.parametrize("Hq", [32, 96])
+def test_entry_of_nan_in_large_tiles(va, fmt, Hq):
+    """One nan entry of a drafted V row, tiles of 128 and 256 query rows."""
+    Q, D, j, d = 6, 128, 2, 77
+    c = Case(fmt, 1, Hq, 1 if Hq == 32 else 2, Q, D, 32, [200], seed=Hq)
+    want, mag = c.expect()
+    r = 200 - Q + j
+    row = c.sides[1][0][(c.table[0, r // 32], 0, r % 32)]
+    if fmt == "f8+":
+        row[d] = 0x7F
+    else:
+        row[2 * d:2 * d + 2] = np.array([0x7FFF if fmt == "f16+" else 0x7FC0], np.uint16).view(np.uint8)
+    got = c.run(va, 2).astype(np.float64)
+    G = Hq // c.Hkv
+    for i in range(Q):
+        hit = np.zeros((Hq, D), bool)
+        hit[:G, d] = bool(int(c.mask[0, i]) >> j & 1)
+        assert np.isnan(got[0, i][hit]).all()
+        assert (np.abs(got[0, i] - want[0, i]) <= bound(want[0, i], mag[0, i]))[~hit].all()
+
+
+@pytest.mark.parametrize("fmt", ["q8+", "f16+", "q3+", "bf16+"])
+@pytest.mark.parametrize("G,Q", [(4, 4), (4, 32), (8, 32)])
+def test_growing_scores(va, fmt, G, Q):
+    """Scores that rise along the cache: the running reference moves block after block, in every range."""
+    c = Case(fmt, 1, G, 1, Q, 128, 64, [1500], seed=Q)
+    kc, ks = c.sides[0]
+    for p in range(1500 - Q):  # keys grow from 1 / 40 to 10 times as large
+        at = (c.table[0, p // 64], 0, p % 64)
+        f = 0.025 * 400.0 ** (p / 1500)
+        if ks is not None:
+            ks[at] = (ks[at].astype(np.float32) * f).astype(np.float16)
+        elif fmt == "f16+":
+            kc[at] = (kc[at].view(np.float16).astype(np.float32) * f).astype(np.float16).view(np.uint8)
+        else:
+            x = (kc[at].view(np.uint16).astype(np.uint32) << 16).view(np.float32) * np.float32(f)
+            kc[at] = (x.view(np.uint32) >> 16).astype(np.uint16).view(np.uint8)
+    for S in (1, 4):
+        c.check(va, S)
+
+
+def test_many_sequences(va):
+    """More (sequence, KV head) pairs than a grid dimension holds; one row each."""
+    import torch
+    B, Hkv = 8200, 8
+    c = Case("q8+", 1, 8, 8, 1, 64, 8, [3], spare=0)
+    b = c.bufs(va)
+    b.q = b.q.expand(B, 1, 8, 64).contiguous()
+    b.out = torch.full((B, 1, 8, 64), float("nan"), dtype=torch.float16, device="cuda")
+    rep = lambda t, *s: t.expand(B, *s).contiguous()  # noqa: E731
+    m, lens, nodes, table = c.args()[:4]
+    va.decode_tree("q8+", b, rep(m, 1), rep(lens), rep(nodes), rep(table, 1), 1, B, 8, Hkv, 1, 8, c.pages, 64, S=1)
+    torch.cuda.synchronize()
+    want, mag = c.expect()
+    assert (np.abs(b.out.cpu().numpy().astype(np.float64) - want) <= bound(want, mag)).all()
