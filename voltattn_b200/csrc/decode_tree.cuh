@@ -519,12 +519,11 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
     // scores in log2 units per unit of the raw product
     const float c2 = rsqrtf((float)D) * kLog2e * TreeCode<C::kKind>::kInvStep;
 
-    // kStep positions from row row0 of stage st on. tail: they hold drafted rows or the
-    // end of the sequence (two instantiations: the others spend nothing on masks).
-    constexpr int kStep = 16;
-    const auto block = [&](auto is_tail, const uint8_t* st, int row0, int pb) {
+    // One block of positions in stage st. tail: it holds drafted rows or the end
+    // of the sequence (two instantiations: the others spend nothing on masks).
+    const auto block = [&](auto is_tail, const uint8_t* st, int pb) {
         constexpr bool tail = decltype(is_tail)::value;
-        constexpr int NT = kStep / 8;  // 8-position tiles of S
+        constexpr int NT = PB / 8;  // 8-position tiles of S
         // scores, then weights: row g + 8 r, this lane's positions t + 8 (nt & 1) (.x) and + 4 (.y) of
         // the 16 of tiles nt, nt ^ 1
         float2 x[NT][2];
@@ -533,7 +532,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             // S of 8 positions: lane g decodes row (g >> 1) + 4 (g & 1) (+ 8 for odd tiles) of the 16
-            const uint8_t* krow = st + (row0 + 16 * (nt >> 1) + (g >> 1) + 4 * (g & 1) + 8 * (nt & 1)) * C::kRb;
+            const uint8_t* krow = st + (16 * (nt >> 1) + (g >> 1) + 4 * (g & 1) + 8 * (nt & 1)) * C::kRb;
             float acc[NG][4];
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
@@ -556,11 +555,11 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
                     const int pr = 16 * (nt >> 1) + t + 4 * e + 8 * (nt & 1);
                     uint32_t k;
                     if constexpr (NG == 2) {
-                        k = *reinterpret_cast<const uint32_t*>(st + C::kOffSK + 4 * (row0 + pr));
-                        vsc[nt][e] = *reinterpret_cast<const uint32_t*>(st + C::kOffSV + 4 * (row0 + pr));
+                        k = *reinterpret_cast<const uint32_t*>(st + C::kOffSK + 4 * pr);
+                        vsc[nt][e] = *reinterpret_cast<const uint32_t*>(st + C::kOffSV + 4 * pr);
                     } else {
-                        k = *reinterpret_cast<const uint16_t*>(st + C::kOffSK + 2 * (row0 + pr));
-                        vsc[nt][e] = *reinterpret_cast<const uint16_t*>(st + C::kOffSV + 2 * (row0 + pr));
+                        k = *reinterpret_cast<const uint16_t*>(st + C::kOffSK + 2 * pr);
+                        vsc[nt][e] = *reinterpret_cast<const uint16_t*>(st + C::kOffSV + 2 * pr);
                     }
                     f[e] = __half22float2(bits_h2(k));
                     uint32_t va = vsc[nt][e];
@@ -665,8 +664,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
         // O += P' V, 16 positions at a time
         bool special = false;
 #pragma unroll
-        for (int j = 0; j < kStep / 16; ++j) {
-            const uint8_t* vb = st + C::kOffV + (row0 + 16 * j + t) * C::kRb;
+        for (int j = 0; j < PB / 16; ++j) {
+            const uint8_t* vb = st + C::kOffV + (16 * j + t) * C::kRb;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
                 uint32_t pa[4];
@@ -712,10 +711,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
             // inf and nan entries of the block's rows, added to the rows that see them: what a
             // positive weight times such an entry gives
             if (__any_sync(0xffffffffu, special)) {
-                for (int pr = 0; pr < kStep; ++pr) {
+                for (int pr = 0; pr < PB; ++pr) {
                     const int j = pb + pr - ctx;
                     if (j >= n) break;
-                    const uint8_t* vr = st + C::kOffV + (row0 + pr) * C::kRb;
+                    const uint8_t* vr = st + C::kOffV + pr * C::kRb;
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         if (!(j < 0 || ((s_mask[g + 8 * r] >> (j & 63)) & 1ull))) continue;
@@ -744,11 +743,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
             break;
         }
         const int pb = p0 + (warp + i * C::kWarps) * PB;
-#pragma unroll 1
-        for (int h = 0; h < PB; h += kStep) {
-            if (pb + h + kStep > ctx) block(std::true_type{}, ring + s * C::kStageBytes, h, pb + h);
-            else block(std::false_type{}, ring + s * C::kStageBytes, h, pb + h);
-        }
+        if (pb + PB > ctx) block(std::true_type{}, ring + s * C::kStageBytes, pb);
+        else block(std::false_type{}, ring + s * C::kStageBytes, pb);
         __syncwarp();
         if (i + C::kStages < mine) issue(i + C::kStages, s);
         if (++s == C::kStages) s = 0, phase ^= 1u;

@@ -3,11 +3,12 @@
 // query rows, with tcgen05.mma and accumulators in tensor memory.
 //
 // One CTA per (sequence, KV head, tile of query rows, range of positions), one
-// per SM, 22 warps:
+// per SM, 23 warps:
 //   warps 0-15   softmax: thread (group w, half hf, row r) has 32 of the 64 positions of
 //                query row r (TMEM lane r) in the jobs of group w;
 //   warps 16-19  producers: codes -> exact fp16 codes in swizzled tiles;
-//   warp 20      one elected lane issues every tcgen05.mma;
+//   warp 20      one elected lane issues the S products, warp 22 the P V products (one
+//                warp for both made each wait for the other's barriers);
 //   warp 21      copies: blocks of codes and scales into a ring, several ahead (fp16
 //                rows by tensor copies straight into the swizzled tiles).
 // A job is one block of 64 positions against 128 query rows; the groups take the jobs in
@@ -17,15 +18,15 @@
 // rows 0..127 and 128..255, group w has rows and O of its own, and a decoded tile serves
 // twice. TMEM holds the O's and kNS buffers of scores, job j's in buffer j % kNS.
 //
-// Per job j (MMA order S(0) .. S(kNS - 1), then PV(j) S(j + kNS)):
+// Per job j:
 //   S_g = Q_g K_g^T (M = 128 rows, N = 64 positions) for each 64-dim group g, in
 //     TMEM. The K tile holds the exact codes (times a power of two), so the group
 //     scales multiply fp32 scores, as in decode_tree.cuh;
 //   the softmax threads load their scores, x = S_0 k_0 + S_1 k_1, exchange the row's
 //     maximum, and write P'_g = fp16(w v_g) over the scores;
 //   O_g += P'_g V_g (A = P' read from TMEM, B = the V tile read MN-major).
-// The MMAs of one thread execute in issue order, so S(j + kNS) follows PV(j) into the
-// same columns, and a completed PV(j) implies every earlier one.
+// S(j + kNS) overwrites the buffer of job j once PV(j) has completed; the MMAs of one
+// thread complete in issue order, so a completed PV(j) implies every earlier one.
 // O is rescaled only when a row's reference grows by more than 4 (log2): P' of the
 // largest weight stays in [2^6, 2^15), its one rounding relative.
 //
@@ -58,7 +59,7 @@ struct TreeTcCfg {
     static constexpr int kOCols = kTwoTiles ? 256 : 128;  // TMEM: O, then the scores
     static_assert(kOCols + kNS * kSw <= 512, "tensor memory");
     static constexpr int kProducers = 128;
-    static constexpr int kThreads = 22 * 32;
+    static constexpr int kThreads = 23 * 32;
     static constexpr int kQTile = 128 * kDim * 2;
     static constexpr int kTile = kNb * kDim * 2;   // one K or V tile
     static constexpr bool kDirect = K == Kind::F16;  // tiles by tensor copies
@@ -87,7 +88,7 @@ struct TreeTcCfg {
     static constexpr int kOffMask = kOffScales + kScaleBytes;
     static constexpr int kOffMl = kOffMask + kRows * 8;
     static constexpr int kOffBars = kOffMl + 5120;
-    static constexpr int kBars = 2 * kKS + 3 * kVS + 3 * kNS + 4 + 2 + kScaleSlots + 2 * kRawStages;
+    static constexpr int kBars = 2 * kKS + 3 * kVS + 3 * kNS + 4 + 3 + kScaleSlots + 2 * kRawStages;
     static constexpr int kOffMisc = kOffBars + kBars * 8;
     static constexpr int kSmemBytes = 1024 + kOffMisc + 64;
     static_assert((kDirect || kRawStages >= 2) && kBars * 8 <= 512, "two blocks in flight");
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     float* s_ref = s_xch + 1024;                                // [2][128]
     uint64_t* kfull = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
     uint64_t *kempty = kfull + KS, *vfull = kempty + KS, *vempty = vfull + VS, *sfull = vempty + VS;
-    uint64_t *pfull = sfull + NS, *pvdone = pfull + NS, *refbar = pvdone + NS, *fin = refbar + 4, *scfull = fin + 1;
+    uint64_t *pfull = sfull + NS, *pvdone = pfull + NS, *refbar = pvdone + NS, *fin = refbar + 4, *scfull = fin + 2;
     uint64_t *rfull = scfull + C::kScaleSlots, *rempty = rfull + C::kRawStages, *vraw = rempty + C::kRawStages;
     uint64_t* qfull = vraw + VS;
     float* s_ev = reinterpret_cast<float*>(smem + C::kOffMisc);
@@ -335,6 +336,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
         for (int i = 0; i < NS; ++i) mbar_init(sfull + i, 1), mbar_init(pfull + i, 8), mbar_init(pvdone + i, 1);
         for (int i = 0; i < 4; ++i) mbar_init(refbar + i, 2);
         mbar_init(fin, 1);
+        mbar_init(fin + 1, 1);
         mbar_init(qfull, 1);
         for (int i = 0; i < C::kScaleSlots; ++i) mbar_init(scfull + i, 1);
         for (int i = 0; i < C::kRawStages; ++i) mbar_init(rfull + i, 1), mbar_init(rempty + i, C::kProducers / 32);
@@ -745,7 +747,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
         for (int k = max(0, i - C::kRawStages); k < i; ++k)
             if (!mbar_wait_bounded(rfull + k % C::kRawStages, (uint32_t)(k / C::kRawStages) & 1u)) *fail = 1;
     } else {
-        // ---- the MMA warp: one elected lane issues -----------------------------------
+        // ---- the MMA warps: one elected lane of each issues ---------------------------
         constexpr uint32_t kIdescS = umma_idesc_f16(128, NB, false);
         constexpr uint32_t kIdescO = umma_idesc_f16(128, C::kScaled ? 64 : D, true);
         const uint32_t ub = __shfl_sync(0xffffffffu, sbase, 0), ut = __shfl_sync(0xffffffffu, tbase, 0);
@@ -755,6 +757,8 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
         const auto issue_s = [&](int j) {
             const int w = j & 1, i = C::kTwo ? j >> 1 : j, s = i % KS, sb = j % NS;
             if (!mbar_wait_fast(kfull + s, (uint32_t)(i / KS) & 1u)) return false;
+            // (job j - NS, the buffer's last)
+            if (j >= NS && !mbar_wait_fast(pvdone + sb, (uint32_t)(j / NS - 1) & 1u)) return false;
             tc05_fence_after();
             const uint64_t qa = dq + (C::kTwo ? w * (C::kQTile / 16) : 0), ka = dk + s * (C::kTile / 16);
             const uint32_t d = ut + C::kOCols + sb * C::kSw;
@@ -792,17 +796,18 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
             __syncwarp();
             return true;
         };
-        bool ok = mbar_wait_fast(qfull, 0);
-        for (int j = 0; j < min(NS, njobs); ++j) ok = ok && issue_s(j);
-        for (int j = 0; ok && j < njobs; ++j) {
-            ok = issue_pv(j);
-            if (j + NS < njobs) ok = ok && issue_s(j + NS);
+        bool ok = true;
+        if (warp == 20) {
+            ok = mbar_wait_fast(qfull, 0);
+            for (int j = 0; ok && j < njobs; ++j) ok = issue_s(j);
+        } else {
+            for (int j = 0; ok && j < njobs; ++j) ok = issue_pv(j);
         }
         if (!ok) {  // every MMA issued so far ends before the tensor memory is given back
             if (lane == 0) report_error(kErrFullWait);
             *fail = 1;
-            if (elect_one()) umma_commit(fin);
-            (void)mbar_wait_bounded(fin, 0);
+            if (elect_one()) umma_commit(fin + (warp == 22));
+            (void)mbar_wait_bounded(fin + (warp == 22), 0);
         }
         __syncwarp();
     }
