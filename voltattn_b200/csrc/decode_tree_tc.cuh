@@ -6,7 +6,8 @@
 // per SM, 23 warps:
 //   warps 0-15   softmax: thread (group w, half hf, row r) has 32 of the 64 positions of
 //                query row r (TMEM lane r) in the jobs of group w;
-//   warps 16-19  producers: codes -> exact fp16 codes in swizzled tiles;
+//   warps 16, 17  producers of K tiles, 18, 19 of V tiles: codes -> exact fp16 codes in
+//                swizzled tiles (fp16 rows: warps 16-19 mend the V tiles of the last blocks);
 //   warp 20      one elected lane issues the S products, warp 22 the P V products (one
 //                warp for both made each wait for the other's barriers);
 //   warp 21      copies: blocks of codes and scales into a ring, several ahead (fp16
@@ -72,9 +73,9 @@ struct TreeTcCfg {
     static constexpr int kRawV = kNb * kRb, kRawSK = 2 * kNb * kRb, kRawSV = kRawSK + kNb * kSb;
     static constexpr int kRawTx = kRawSV + kNb * kSb;
     static constexpr int kRawStage = (kRawTx + 127) / 128 * 128;
-    // what follows the ring: scales as floats [4 slots][K, V][kNG][64], masks,
-    // [2][2][2][128] maxima or sums, [2][128] references, barriers, ev[4], TMEM slot, fail, special, ticket
-    static constexpr int kScaleSlots = 4;
+    // what follows the ring: scales as floats [8 slots][K, V][kNG][64], masks,
+    // [2][2][2][128] maxima or sums, [2][128] references, barriers, ev[8], TMEM slot, fail, special, ticket
+    static constexpr int kScaleSlots = 8;
     static constexpr int kScaleSlot = 2 * kNG * kNb * 4;
     static constexpr int kScaleV = kNG * kNb * 4;  // where a slot's V scales begin
     static constexpr int kScaleBytes = kScaled ? kScaleSlots * kScaleSlot : 0;
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     uint64_t *rfull = scfull + C::kScaleSlots, *rempty = rfull + C::kRawStages, *vraw = rempty + C::kRawStages;
     uint64_t* qfull = vraw + VS;
     float* s_ev = reinterpret_cast<float*>(smem + C::kOffMisc);
-    uint32_t* tslot = reinterpret_cast<uint32_t*>(s_ev + 4);
+    uint32_t* tslot = reinterpret_cast<uint32_t*>(s_ev + C::kScaleSlots);
     volatile int* fail = reinterpret_cast<volatile int*>(tslot + 1);
     volatile int* special = fail + 1;
     unsigned* s_ticket = tslot + 3;
@@ -331,8 +332,8 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     const int njobs = C::kTwo ? 2 * nblk : nblk;
     if (warp == 20) tmem_alloc(tslot, 512);
     if (tid == 0) {
-        for (int i = 0; i < KS; ++i) mbar_init(kfull + i, C::kDirect ? 1 : C::kProducers / 32), mbar_init(kempty + i, 1);
-        for (int i = 0; i < VS; ++i) mbar_init(vfull + i, C::kProducers / 32), mbar_init(vempty + i, 1);
+        for (int i = 0; i < KS; ++i) mbar_init(kfull + i, C::kDirect ? 1 : 2), mbar_init(kempty + i, 1);
+        for (int i = 0; i < VS; ++i) mbar_init(vfull + i, C::kDirect ? C::kProducers / 32 : 2), mbar_init(vempty + i, 1);
         for (int i = 0; i < NS; ++i) mbar_init(sfull + i, 1), mbar_init(pfull + i, 8), mbar_init(pvdone + i, 1);
         for (int i = 0; i < 4; ++i) mbar_init(refbar + i, 2);
         mbar_init(fin, 1);
@@ -402,8 +403,8 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
             const uint32_t ph = (uint32_t)(j / NS) & 1u;
             const int pb = p0 + blk * NB;
             bool ok = mbar_wait_fast(sfull + sb, ph);
-            // (a slot of scales is written again only after this block's PV, so this phase
-            // cannot be passed twice before it is seen here)
+            // (block i + 8's scales overwrite block i's: its K tile waits for S(i + 6), issued
+            // after block i + 2's products at the least, so this phase is not passed twice)
             if constexpr (C::kScaled)
                 ok = ok && mbar_wait_fast(scfull + blk % C::kScaleSlots, (uint32_t)(blk / C::kScaleSlots) & 1u);
             if (!ok) {
@@ -571,106 +572,117 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     } else if (C::kDirect && warp < 20) {
         tree_tc_fix_v<C>(p0, len, ctx, nblk, smem, vraw, vfull, special, fail);
     } else if (!C::kDirect && warp < 20) {
-        // ---- producers: K of block i + 1 before V of block i, so the next scores never
-        // wait for this block's PV. A thread takes two slices (row, quarter of the dims) -----
-        const int pw = warp - 16;
+        // ---- producers: a thread takes four slices (row, quarter of the dims) of a tile -------
+        const bool is_v = warp >= 18;
+        const int pw = warp & 1;
         // lane bits: quarter bit 0, row bits 0..1, quarter bit 1, row bit 2: eight
         // neighbouring lanes store to eight different 16-byte banks
-        const int q = (lane & 1) | ((lane >> 2) & 2), row0 = pw * 16 + ((lane >> 1) & 3) + ((lane >> 4) << 2);
+        const int q = (lane & 1) | ((lane >> 2) & 2), row0 = pw * 32 + ((lane >> 1) & 3) + ((lane >> 4) << 2);
         using Raw = TcRaw<KK, D>;
         constexpr int kChunks = Raw::kDims / 8;
-        const auto put = [&](uint8_t* dst, int row, int j, uint4 v) {
-            const int c = q * kChunks + j;
-            *reinterpret_cast<uint4*>(dst + (c >> 3) * (NB * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
-        };
-        const auto raw_of = [&](int i) { return smem + C::kOffRaw + (i % C::kRawStages) * C::kRawStage; };
-        const auto make_k = [&](int i) {
-            const int u = i / KS;
-            if (!mbar_wait_bounded(rfull + i % C::kRawStages, (uint32_t)(i / C::kRawStages) & 1u)) return false;
-            const uint8_t* raw = raw_of(i);
-            if (u > 0 && !mbar_wait_bounded(kempty + i % KS, (uint32_t)(u - 1) & 1u)) return false;
-            if (C::kScaled && pw == (i & 3)) {  // the block's scales: two positions a lane
-                float* sk = reinterpret_cast<float*>(smem + C::kOffScales + (i % C::kScaleSlots) * C::kScaleSlot);
-                float* sv = sk + C::kScaleV / 4;
-                __half2 big = __float2half2_rn(0.f);
+        // where its chunks of row row0 go in a tile (rows 8 apart: 1024 bytes, the same phase)
+        int to[kChunks];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int at = lane + 32 * e;
-                    uint32_t ks, vs;
-                    if constexpr (NG == 2) {
-                        ks = reinterpret_cast<const uint32_t*>(raw + C::kRawSK)[at];
-                        vs = reinterpret_cast<const uint32_t*>(raw + C::kRawSV)[at];
-                    } else {
-                        ks = reinterpret_cast<const uint16_t*>(raw + C::kRawSK)[at];
-                        vs = reinterpret_cast<const uint16_t*>(raw + C::kRawSV)[at];
+        for (int j = 0; j < kChunks; ++j) {
+            const int c = q * kChunks + j;
+            to[j] = (c >> 3) * (NB * 128) + row0 * 128 + (((c & 7) ^ (row0 & 7)) << 4);
+        }
+        bool ok = true;
+        for (int i = 0; i < nblk; ++i) {
+            const int rs = i % C::kRawStages;
+            ok = mbar_wait_bounded(rfull + rs, (uint32_t)(i / C::kRawStages) & 1u);
+            if (!ok) break;
+            const uint8_t* raw = smem + C::kOffRaw + rs * C::kRawStage;
+            if (!is_v) {
+                const int s = i % KS;
+                ok = i < KS || mbar_wait_bounded(kempty + s, (uint32_t)(i / KS - 1) & 1u);
+                if (!ok) break;
+                if (C::kScaled && pw == (i & 1)) {  // the block's scales: two positions a lane
+                    float* sk = reinterpret_cast<float*>(smem + C::kOffScales + (i % C::kScaleSlots) * C::kScaleSlot);
+                    float* sv = sk + C::kScaleV / 4;
+                    __half2 big = __float2half2_rn(0.f);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int at = lane + 32 * e;
+                        uint32_t ks, vs;
+                        if constexpr (NG == 2) {
+                            ks = reinterpret_cast<const uint32_t*>(raw + C::kRawSK)[at];
+                            vs = reinterpret_cast<const uint32_t*>(raw + C::kRawSV)[at];
+                        } else {
+                            ks = reinterpret_cast<const uint16_t*>(raw + C::kRawSK)[at];
+                            vs = reinterpret_cast<const uint16_t*>(raw + C::kRawSV)[at];
+                        }
+                        const float2 fk = __half22float2(bits_h2(ks)), fv = __half22float2(bits_h2(vs));
+                        sk[at] = fk.x;
+                        sv[at] = fv.x;
+                        if constexpr (NG == 2) sk[NB + at] = fk.y, sv[NB + at] = fv.y;
+                        // rows past the end and scales that are not finite are no measure
+                        uint32_t a = vs & 0x7FFF7FFFu;
+                        if (p0 + i * NB + at >= len) a = 0u;
+                        if ((a & 0x7FFFu) >= 0x7C00u) a &= 0x7FFF0000u;
+                        if ((a >> 16) >= 0x7C00u) a &= 0x7FFFu;
+                        big = __hmax2(big, bits_h2(a));
                     }
-                    const float2 fk = __half22float2(bits_h2(ks));
-                    sk[at] = fk.x;
-                    const float2 fv = __half22float2(bits_h2(vs));
-                    sv[at] = fv.x;
-                    if constexpr (NG == 2) sk[NB + at] = fk.y, sv[NB + at] = fv.y;
-                    // rows past the end and scales that are not finite are no measure
-                    uint32_t a = vs & 0x7FFF7FFFu;
-                    if (p0 + i * NB + at >= len) a = 0u;
-                    if ((a & 0x7FFFu) >= 0x7C00u) a &= 0x7FFF0000u;
-                    if ((a >> 16) >= 0x7C00u) a &= 0x7FFFu;
-                    big = __hmax2(big, bits_h2(a));
+                    const float vm = fmaxf(__low2float(big), __high2float(big));
+                    const unsigned vb = __reduce_max_sync(0xffffffffu, __float_as_uint(vm));
+                    __syncwarp();
+                    if (lane == 0) {
+                        s_ev[i % C::kScaleSlots] = vb ? (float)((int)(vb >> 23) - 127) : 0.f;
+                        mbar_arrive(scfull + i % C::kScaleSlots);
+                    }
                 }
-                const float vm = fmaxf(__low2float(big), __high2float(big));
-                const unsigned vb = __reduce_max_sync(0xffffffffu, __float_as_uint(vm));
+                uint8_t* tile_at = smem + C::kOffK + s * C::kTile;
+#pragma unroll
+                for (int h = 0; h < 4; h += 2) {
+                    Raw r[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) tc_load<KK, D>(r[e], raw + (row0 + 8 * (h + e)) * C::kRb, q);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int j = 0; j < kChunks; ++j)
+                            *reinterpret_cast<uint4*>(tile_at + to[j] + 1024 * (h + e)) = tc_convert<KK, D, false>(r[e], j);
+                }
+                fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {
-                    s_ev[i % C::kScaleSlots] = vb ? (float)((int)(vb >> 23) - 127) : 0.f;
-                    mbar_arrive(scfull + i % C::kScaleSlots);
+                    mbar_arrive(kfull + s);
+                    mbar_arrive(rempty + rs);
                 }
-            }
-            uint8_t* kt = smem + C::kOffK + (i % KS) * C::kTile;
-            Raw r[2];
+            } else {
+                const int s = i % VS;
+                ok = i < VS || mbar_wait_bounded(vempty + s, (uint32_t)(i / VS - 1) & 1u);
+                if (!ok) break;
+                uint8_t* tile_at = smem + C::kOffV + s * C::kTile;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) tc_load<KK, D>(r[h], raw + (row0 + 8 * h) * C::kRb, q);
+                for (int h = 0; h < 4; h += 2) {
+                    Raw r[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+                    for (int e = 0; e < 2; ++e)
+                        tc_load<KK, D>(r[e], raw + C::kRawV + (row0 + 8 * (h + e)) * C::kRb, q);
 #pragma unroll
-                for (int j = 0; j < kChunks; ++j) put(kt, row0 + 8 * h, j, tc_convert<KK, D, false>(r[h], j));
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(kfull + i % KS);
-            return true;
-        };
-        const auto make_v = [&](int i) {
-            const int x = i / VS;
-            const uint8_t* raw = raw_of(i) + C::kRawV;
-            Raw r[2];
+                    for (int e = 0; e < 2; ++e) {
+                        const int pos = p0 + i * NB + row0 + 8 * (h + e);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) tc_load<KK, D>(r[h], raw + (row0 + 8 * h) * C::kRb, q);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(rempty + i % C::kRawStages);
-            if (x > 0 && !mbar_wait_bounded(vempty + i % VS, (uint32_t)(x - 1) & 1u)) return false;
-            uint8_t* vt = smem + C::kOffV + (i % VS) * C::kTile;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int pos = p0 + i * NB + row0 + 8 * h;
-#pragma unroll
-                for (int j = 0; j < kChunks; ++j) {
-                    uint4 v = tc_convert<KK, D, true>(r[h], j);
-                    if constexpr (C::kFloat) {
-                        // rows past the end are cleared; entries of drafted rows that are not finite
-                        // are left to the epilogue, which adds them to the rows that see them
-                        if (pos >= len) v = make_uint4(0u, 0u, 0u, 0u);
-                        else if (pos >= ctx && clear_not_finite(v)) *special = 1;
+                        for (int j = 0; j < kChunks; ++j) {
+                            uint4 v = tc_convert<KK, D, true>(r[e], j);
+                            if constexpr (C::kFloat) {
+                                // rows past the end are cleared; entries of drafted rows that are not finite
+                                // are left to the epilogue, which adds them to the rows that see them
+                                if (pos >= len) v = make_uint4(0u, 0u, 0u, 0u);
+                                else if (pos >= ctx && clear_not_finite(v)) *special = 1;
+                            }
+                            *reinterpret_cast<uint4*>(tile_at + to[j] + 1024 * (h + e)) = v;
+                        }
                     }
-                    put(vt, row0 + 8 * h, j, v);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(vfull + s);
+                    mbar_arrive(rempty + rs);
                 }
             }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(vfull + i % VS);
-            return true;
-        };
-        bool ok = make_k(0);
-        for (int i = 0; ok && i < nblk; ++i) {
-            if (i + 1 < nblk) ok = make_k(i + 1);
-            ok = ok && make_v(i);
         }
         if (!ok) {
             if (lane == 0) report_error(kErrEmptyWait);
