@@ -1,6 +1,7 @@
 // C ABI of tree attention and of the rows and pages of a paged cache (declared
 // in include/voltattn.h): argument checks, workspace layout and launch.
 #include <algorithm>
+#include <cmath>
 #include <climits>
 
 #include "../../include/voltattn.h"
@@ -51,21 +52,23 @@ int tree_rows(int R) { return R <= 64 ? 16 : R <= 128 ? 128 : 256; }
 constexpr long long kCounters = 16384;
 constexpr size_t kCounterBytes = kCounters * sizeof(unsigned);
 
-// The splits with the least cost: the CTAs' rows (of sequences that fill 5/8 of
-// their tables on average, plus a CTA's fixed work in rows) shared by the device's
-// slots, and half of the longest range for the uneven end; smallest S first.
+// Tiles of 16 rows: the splits with the least cost: the CTAs' rows (of sequences that fill
+// 5/8 of their tables on average, plus a CTA's fixed work in rows) shared by the device's
+// slots, and half of the longest range for the uneven end; smallest S first. The larger
+// tiles' CTAs share the work evenly by themselves: S only has to let the longest
+// sequence spread, here one of 2.5 times the mean length.
 int tree_splits(int nsm, int B, int Hkv, int R, int Lmax) {
     const int rows = tree_rows(R);
     const double ctas = (double)B * Hkv * ((R + rows - 1) / rows);
     if (ctas > (double)kCounters) return 1;
-    const double cap = (double)nsm * (rows == 16 ? 3 : 1);
-    const double fixed = rows == 16 ? 192.0 : 768.0;
-    const int units = (Lmax + kTreeUnit - 1) / kTreeUnit;
+    const int units = (Lmax + kTreeUnit - 1) / kTreeUnit, most = std::min(kMaxSplits, units);
+    if (rows != 16) return std::max(1, std::min(most, (int)std::ceil(2.5 * nsm / ctas) + 1));
+    const double load = ctas / (3.0 * nsm), fixed = 320.0;
     double best = 1e300;
     int S = 1;
-    for (int s = 1; s <= std::min(kMaxSplits, units); ++s) {
+    for (int s = 1; s <= most && load * s * fixed < best; ++s) {
         const double chunk = (double)((units + s - 1) / s) * kTreeUnit;
-        const double cost = std::max(1.0, ctas * s / cap) * (0.625 * chunk + fixed) + 0.5 * chunk;
+        const double cost = std::max(1.0, load * s) * (0.625 * chunk + fixed) + 0.5 * chunk;
         if (cost < best - 1e-9) {
             best = cost;
             S = s;

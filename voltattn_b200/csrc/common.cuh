@@ -43,6 +43,10 @@ __device__ __forceinline__ uint64_t global_timer_ns() {
 
 // ---- mbarrier -------------------------------------------------------------
 
+// (before its memory, or the barrier itself, is set up anew; no thread or copy uses it any more)
+__device__ __forceinline__ void mbar_inval(uint64_t* bar) {
+    asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
 }

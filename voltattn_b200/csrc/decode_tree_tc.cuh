@@ -74,12 +74,12 @@ struct TreeTcCfg {
     static constexpr int kRawTx = kRawSV + kNb * kSb;
     static constexpr int kRawStage = (kRawTx + 127) / 128 * 128;
     // what follows the ring: scales as floats [8 slots][K, V][kNG][64], masks,
-    // [2][2][2][128] maxima or sums, [2][128] references, barriers, ev[8], TMEM slot, fail, special, ticket
+    // [2][2][2][128] maxima or sums, [2][128] references, barriers, ev[8], TMEM slot, fail, special, ticket, plan, range
     static constexpr int kScaleSlots = 8;
     static constexpr int kScaleSlot = 2 * kNG * kNb * 4;
     static constexpr int kScaleV = kNG * kNb * 4;  // where a slot's V scales begin
     static constexpr int kScaleBytes = kScaled ? kScaleSlots * kScaleSlot : 0;
-    static constexpr int kRest = kScaleBytes + kRows * 8 + 5120 + 512 + 64;
+    static constexpr int kRest = kScaleBytes + kRows * 8 + 5120 + 512 + 128;
     static constexpr int kRoom = (227 * 1024 - 1024 - kOffRaw - kRest) / kRawStage;
     static constexpr int kRawStages = kDirect ? 1 : kRoom < 8 ? kRoom : 8;
     // (the merge of the ranges takes the front of shared memory: what follows stays past it)
@@ -91,7 +91,7 @@ struct TreeTcCfg {
     static constexpr int kOffBars = kOffMl + 5120;
     static constexpr int kBars = 2 * kKS + 3 * kVS + 3 * kNS + 4 + 3 + kScaleSlots + 2 * kRawStages;
     static constexpr int kOffMisc = kOffBars + kBars * 8;
-    static constexpr int kSmemBytes = 1024 + kOffMisc + 64;
+    static constexpr int kSmemBytes = 1024 + kOffMisc + 128;
     static_assert((kDirect || kRawStages >= 2) && kBars * 8 <= 512, "two blocks in flight");
     static_assert(kSmemBytes <= 227 * 1024, "one CTA per SM");
 };
@@ -271,13 +271,120 @@ __device__ __forceinline__ void tree_tc_fix_v(int p0, int len, int ctx, int nblk
     }
 }
 
+// A CTA's share of the call (splits allowed), and the part of it that comes next.
+struct TreeTcPlan {
+    long long window, at, end;  // cost units
+};
+struct TreeTcRange {
+    int b, hk, tile, p0, p1, part, parts;  // positions [p0, p1): one of the tile's parts (parts = 0: no work)
+};
+
+// The work in a line: sequences, their KV heads, their tiles of query rows, each tile
+// its sequence's blocks of 64 positions. CTA i takes the i-th window of it, so every CTA
+// has the same number of blocks whatever the lengths (a range per CTA in proportion to its
+// sequence's length left the SMs idle for a third of the call). A tile counts kTcFixed blocks more
+// than it has, about what starting and writing it takes; one without live rows counts 1. Windows
+// are long enough that none of a tile's blocks need more than S of them.
+constexpr int kTcFixed = 8, kTcMinWindow = 12;
+
+struct TreeTcSeq {
+    int blocks, live_tiles;
+    long long cost;  // of one KV head
+};
 template <class C>
-__global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const TreeParams p,
-                                                                           const __grid_constant__ CUtensorMap tmK,
-                                                                           const __grid_constant__ CUtensorMap tmV) {
-    extern __shared__ __align__(128) uint8_t smem_raw[];
-    // (an offset, not a rounded address: the compiler keeps seeing shared memory)
-    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+__device__ __forceinline__ TreeTcSeq tree_tc_seq(const TreeParams& p, int b) {
+    const long long cap = (long long)p.max_pages * p.page_rows;
+    const int len = (int)max(0ll, min((long long)__ldg(p.lens + b), cap));
+    const int n = max(0, min(min(p.nodes ? __ldg(p.nodes + b) : p.Q, p.Q), len));
+    TreeTcSeq q;
+    q.blocks = (len + C::kNb - 1) / C::kNb;
+    q.live_tiles = (min(p.R, n * p.G) + C::kRows - 1) / C::kRows;
+    q.cost = (long long)q.live_tiles * (q.blocks + kTcFixed) + (p.tiles - q.live_tiles);
+    return q;
+}
+
+// (one warp) Whether the CTA has any work.
+template <class C>
+__device__ __forceinline__ bool tree_tc_plan(const TreeParams& p, int lane, TreeTcPlan* plan) {
+    long long total = 0;
+    int most = 0;
+    for (int b = lane; b < p.B; b += 32) {
+        const TreeTcSeq q = tree_tc_seq<C>(p, b);
+        total += q.cost;
+        most = max(most, q.blocks);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+    total *= p.Hkv;
+    most = __reduce_max_sync(0xffffffffu, most);
+    const long long window = max(max((total + gridDim.x - 1) / gridDim.x, (long long)((most + p.S - 2) / (p.S - 1))),
+                                 (long long)kTcMinWindow);
+    const long long at = blockIdx.x * window;
+    if (lane == 0) {
+        plan->window = window;
+        plan->at = at;
+        plan->end = min(total, at + window);
+    }
+    return at < total;
+}
+
+// (one warp) The next range of the CTA's window; false: the window is done.
+template <class C>
+__device__ __forceinline__ bool tree_tc_next(const TreeParams& p, int lane, TreeTcPlan* plan, TreeTcRange* range) {
+    const long long window = plan->window, at = plan->at, end = plan->end;
+    if (at >= end) return false;
+    // the sequence that position `at` of the line lies in
+    long long base = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+        TreeTcSeq q = {0, 0, 0};
+        if (b0 + lane < p.B) q = tree_tc_seq<C>(p, b0 + lane);
+        const long long mine = q.cost * p.Hkv;
+        long long upto = mine;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const long long up = __shfl_up_sync(0xffffffffu, upto, off);
+            if (lane >= off) upto += up;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, base + upto > at);
+        if (hit) {
+            if (lane == __ffs(hit) - 1) {
+                const long long y0 = at - (base + upto - mine), each = q.blocks + kTcFixed;
+                const int hk = (int)(y0 / q.cost);
+                const long long y = y0 - hk * q.cost, live = q.live_tiles * each;
+                TreeTcRange r;
+                r.b = b0 + lane;
+                r.hk = hk;
+                r.part = 0;
+                r.parts = 1;
+                r.p0 = r.p1 = 0;
+                long long next = at + 1;
+                if (y >= live) {
+                    r.tile = q.live_tiles + (int)(y - live);
+                } else {
+                    r.tile = (int)(y / each);
+                    const long long z = y - r.tile * each, first = at - z + kTcFixed;  // where its blocks begin
+                    next = min(end, first + q.blocks);
+                    r.p0 = (int)max(0ll, at - first) * C::kNb;
+                    r.p1 = (int)min(max(0ll, next - first) * C::kNb, 0x7FFFFFFFll);  // (may pass the sequence's end)
+                    r.part = (int)(blockIdx.x - first / window);
+                    // (a window that ends before the tile's blocks leaves it to the next)
+                    r.parts = next > first ? (int)((first + q.blocks - 1) / window - first / window) + 1 : 0;
+                }
+                *range = r;
+                plan->at = next;
+            }
+            break;
+        }
+        base += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    __syncwarp();
+    return true;
+}
+
+// One range of a tile's positions; false: a wait gave up.
+template <class C>
+__device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtensorMap& tmK, const CUtensorMap& tmV, uint8_t* smem,
+                                              const TreeTcRange& range, bool final) {
     constexpr int D = C::kD, NG = C::kNG, NB = C::kNb, KS = C::kKS, VS = C::kVS, SG = C::kSG, NS = C::kNS;
     constexpr Kind KK = C::kKind;
     unsigned long long* s_mask = reinterpret_cast<unsigned long long*>(smem + C::kOffMask);
@@ -295,23 +402,15 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     unsigned* s_ticket = tslot + 3;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int tile = (int)blockIdx.x / p.S, split = (int)blockIdx.x - tile * p.S;
-    const int stream = (int)(blockIdx.y + blockIdx.z * gridDim.y);
-    if (stream >= p.B * p.Hkv) return;
-    const int b = stream / p.Hkv, hk = stream - b * p.Hkv;
-    const int r0 = tile * C::kRows;
-
-    grid_dependency_wait();
+    const int b = range.b, hk = range.hk, split = range.part, nsplit = range.parts;
+    const int r0 = range.tile * C::kRows;
     const long long cap = (long long)p.max_pages * p.page_rows;
     const int len = (int)max(0ll, min((long long)__ldg(p.lens + b), cap));
     const int n = max(0, min(min(p.nodes ? __ldg(p.nodes + b) : p.Q, p.Q), len));
     const int ctx = len - n;
-    const int chunk = tree_chunk(len, p.S);
-    const int nsplit = max(1, (len + chunk - 1) / chunk);
-    if (split >= nsplit) return;
-    const int p0 = split * chunk, p1 = min(len, p0 + chunk);
+    const int p0 = range.p0, p1 = min(len, range.p1);
+    const int stream = b * p.Hkv + hk;
     const int live = min(p.R, n * p.G) - r0;  // rows of the tile that belong to a node; none: zeros
-    if (live <= 0 && split > 0) return;
     const int rows_here = min(C::kRows, p.R - r0);
 
     const auto store_out = [&](int r, int c, float4 v, float inv) {
@@ -325,12 +424,11 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     if (live <= 0) {
         for (int i = tid; i < rows_here * (D / 4); i += C::kThreads)
             store_out(r0 + i / (D / 4), i % (D / 4), make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
-        return;
+        return true;
     }
 
     const int nblk = (p1 - p0 + NB - 1) / NB;
     const int njobs = C::kTwo ? 2 * nblk : nblk;
-    if (warp == 20) tmem_alloc(tslot, 512);
     if (tid == 0) {
         for (int i = 0; i < KS; ++i) mbar_init(kfull + i, C::kDirect ? 1 : 2), mbar_init(kempty + i, 1);
         for (int i = 0; i < VS; ++i) mbar_init(vfull + i, C::kDirect ? C::kProducers / 32 : 2), mbar_init(vempty + i, 1);
@@ -341,9 +439,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
         mbar_init(qfull, 1);
         for (int i = 0; i < C::kScaleSlots; ++i) mbar_init(scfull + i, 1);
         for (int i = 0; i < C::kRawStages; ++i) mbar_init(rfull + i, 1), mbar_init(rempty + i, C::kProducers / 32);
-        if constexpr (C::kDirect)
-            for (int i = 0; i < VS; ++i) mbar_init(vraw + i, 1);
-        *fail = 0;
+        for (int i = 0; i < VS; ++i) mbar_init(vraw + i, 1);
         *special = 0;
         fence_mbar_init();
     }
@@ -354,9 +450,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
         const int pg = pi < p.max_pages ? __ldg(trow + pi) : 0;
         return (unsigned)pg < (unsigned)p.num_pages ? pg : 0;
     };
-    tc05_fence_before();
     __syncthreads();
-    tc05_fence_after();
     const uint32_t tbase = *tslot;
     const uint32_t sbase = smem_u32(smem);
 
@@ -812,8 +906,10 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
         if (warp == 20) {
             ok = mbar_wait_fast(qfull, 0);
             for (int j = 0; ok && j < njobs; ++j) ok = issue_s(j);
+            for (int i = max(0, nblk - KS); ok && i < nblk; ++i) ok = mbar_wait_fast(kempty + i % KS, (uint32_t)(i / KS) & 1u);
         } else {
             for (int j = 0; ok && j < njobs; ++j) ok = issue_pv(j);
+            for (int i = max(0, nblk - VS); ok && i < nblk; ++i) ok = mbar_wait_fast(vempty + i % VS, (uint32_t)(i / VS) & 1u);
         }
         if (!ok) {  // every MMA issued so far ends before the tensor memory is given back
             if (lane == 0) report_error(kErrFullWait);
@@ -826,11 +922,10 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     tc05_fence_before();
     __syncthreads();
     tc05_fence_after();
-    if (*fail) {
-        if (warp == 20) tmem_dealloc(tbase, 512);
-        return;
-    }
-    grid_launch_dependents();
+    if (*fail) return false;
+    // (every arrival has come: the warps above waited for the commits' as well)
+    if (tid < C::kBars) mbar_inval(kfull + tid);
+    if (final) grid_launch_dependents();
 
     // ---- epilogue: a thread's row, its part of the dims: half of them (two tiles: of its
     // group's tile) or a quarter
@@ -917,19 +1012,62 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     }
     tc05_fence_before();
     __syncthreads();
-    if (warp == 20) {
-        tc05_fence_after();
-        tmem_dealloc(tbase, 512);
-    }
-    if (direct) return;
-    unsigned* counter = p.counters + (size_t)stream * p.tiles + tile;
+    tc05_fence_after();
+    if (direct) return true;
+    unsigned* counter = p.counters + (size_t)stream * p.tiles + range.tile;
     if (tid == 0) *s_ticket = atomic_add_acq_rel_gpu(counter, 1u);
     __syncthreads();
-    if (*s_ticket != (unsigned)(nsplit - 1)) return;
+    if (*s_ticket != (unsigned)(nsplit - 1)) return true;
     if (tid == 0) store_relaxed_gpu(counter, 0u);
     tree_merge<D, C::kRows, C::kThreads>(p, stream, r0, min(rows_here, live), nsplit, reinterpret_cast<float*>(smem), tid, store_out);
     for (int i = tid; i < (rows_here - min(rows_here, live)) * (D / 4); i += C::kThreads)
         store_out(r0 + live + i / (D / 4), i % (D / 4), make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
+    return true;
+}
+
+template <class C>
+__global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const TreeParams p,
+                                                                           const __grid_constant__ CUtensorMap tmK,
+                                                                           const __grid_constant__ CUtensorMap tmV) {
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    // (an offset, not a rounded address: the compiler keeps seeing shared memory)
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint32_t* tslot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc + 4 * C::kScaleSlots);
+    TreeTcPlan* plan = reinterpret_cast<TreeTcPlan*>(smem + C::kOffMisc + 64);
+    TreeTcRange* range = reinterpret_cast<TreeTcRange*>(plan + 1);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (warp == 20) tmem_alloc(tslot, 512);
+    if (tid == 0) tslot[1] = 0u;  // no wait has given up
+    grid_dependency_wait();
+    bool more = true;
+    if (warp == 0) {
+        if (p.S > 1) {
+            more = tree_tc_plan<C>(p, lane, plan);
+            __syncwarp();
+            if (more) tree_tc_next<C>(p, lane, plan, range);
+        } else if (lane == 0) {  // a whole tile a CTA
+            const int stream = (int)(blockIdx.x / p.tiles), b = stream / p.Hkv;
+            *range = {b, stream - b * p.Hkv, (int)blockIdx.x - stream * p.tiles, 0, 0x7FFFFFFF, 0, 1};
+            plan->at = plan->end = 0;
+        }
+    }
+    more = __syncthreads_or(warp == 0 && more);
+    tc05_fence_before();
+    __syncthreads();
+    tc05_fence_after();
+    while (more) {
+        const TreeTcRange now = *range;
+        const bool final = plan->at >= plan->end;
+        if (now.parts > 0 && !tree_tc_range<C>(p, tmK, tmV, smem, now, final)) break;
+        if (final) break;
+        // what this range left in shared memory by plain stores comes before the next one's copies
+        fence_proxy_async_smem();
+        __syncthreads();
+        if (warp == 0) more = tree_tc_next<C>(p, lane, plan, range);
+        more = __syncthreads_or(warp == 0 && more);
+    }
+    __syncthreads();
+    if (warp == 20) tmem_dealloc(*tslot, 512);
 }
 
 }  // namespace va

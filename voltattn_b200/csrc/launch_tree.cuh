@@ -13,7 +13,8 @@ namespace va {
 namespace host {
 
 template <class C, class... Maps>
-int launch_tree_cfg(void (*kernel)(const TreeParams, const Maps...), const TreeParams& p, cudaStream_t st, const Maps&... maps) {
+int launch_tree_cfg(void (*kernel)(const TreeParams, const Maps...), const TreeParams& p, dim3 grid, cudaStream_t st,
+                    const Maps&... maps) {
     int dev;
     int rc = current_device(&dev);
     if (rc) return rc;
@@ -30,10 +31,7 @@ int launch_tree_cfg(void (*kernel)(const TreeParams, const Maps...), const TreeP
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    // x: the splits and tiles of one (sequence, KV head), which read the same rows, next to
-    // one another; y, z: the (sequence, KV head) pairs
-    const unsigned streams = (unsigned)(p.B * p.Hkv), y = std::min(streams, 65535u);
-    cfg.gridDim = dim3((unsigned)(p.tiles * p.S), y, (streams + y - 1) / y);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(C::kThreads);
     cfg.dynamicSmemBytes = C::kSmemBytes;
     cfg.stream = st;
@@ -41,6 +39,13 @@ int launch_tree_cfg(void (*kernel)(const TreeParams, const Maps...), const TreeP
     cfg.numAttrs = 1;
     VA_CUDA(cudaLaunchKernelEx(&cfg, kernel, p, maps...));
     return VA_OK;
+}
+
+// x: the splits and tiles of one (sequence, KV head), which read the same rows, next to
+// one another; y, z: the (sequence, KV head) pairs
+inline dim3 tree_grid(const TreeParams& p) {
+    const unsigned streams = (unsigned)(p.B * p.Hkv), y = std::min(streams, 65535u);
+    return dim3((unsigned)(p.tiles * p.S), y, (streams + y - 1) / y);
 }
 
 template <class C>
@@ -54,14 +59,21 @@ int launch_tree_tc(const TreeParams& p, cudaStream_t st) {
         if (!rc) rc = encode_f16_rows_map(&tmV, p.V, rows, box, C::kD);
         if (rc) return rc;
     }
-    return launch_tree_cfg<C>(decode_tree_tc_kernel<C>, p, st, tmK, tmV);
+    int dev;
+    const int rc = current_device(&dev);
+    if (rc) return rc;
+    // splits: one CTA per SM, each with a window of the work; without: a CTA per tile
+    const long long items = (long long)p.B * p.Hkv * p.tiles;
+    if (items > 0x7FFFFFFFll) return VA_ERR_TOO_LARGE;
+    const long long ctas = p.S > 1 ? std::min((long long)sm_count(dev), items * p.S) : items;
+    return launch_tree_cfg<C>(decode_tree_tc_kernel<C>, p, dim3((unsigned)ctas), st, tmK, tmV);
 }
 
 template <int D>
 int launch_tree_dim(int fmt, const TreeParams& p, int rows, cudaStream_t st) {
 #define VA_TREE_KIND(kind)                                                                               \
     do {                                                                                                 \
-        if (rows == 16) return launch_tree_cfg<TreeCfg<kind, D>>(decode_tree_kernel<TreeCfg<kind, D>>, p, st); \
+        if (rows == 16) return launch_tree_cfg<TreeCfg<kind, D>>(decode_tree_kernel<TreeCfg<kind, D>>, p, tree_grid(p), st); \
         if (rows == 128) return launch_tree_tc<TreeTcCfg<kind, D, false>>(p, st);                        \
         return launch_tree_tc<TreeTcCfg<kind, D, true>>(p, st);                                          \
     } while (0)
