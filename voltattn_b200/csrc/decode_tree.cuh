@@ -324,42 +324,47 @@ template <int D, int kRows, int kThreads, class Store>
 __device__ __forceinline__ void tree_merge(const TreeParams& p, int stream, int r0, int rows, int nsplit, float* sw,
                                            int tid, const Store& store_out) {
     float* sl = sw + kRows * kTreeMaxSplits;  // [kRows] sums
-    // eight lanes a row, four ranges in flight a lane
-    const int l8 = tid & 7;
+    // some lanes a row, four ranges in flight a lane; the first four are loaded once
+    constexpr int kPer = kThreads / kRows >= 8 ? 8 : kThreads / kRows >= 4 ? 4 : 2;
+    const int sub = tid % kPer;
 #pragma unroll 1
-    for (int r8 = tid >> 3; r8 < (rows + 3 & ~3); r8 += kThreads / 8) {  // (whole warps: four rows)
-        const int row = min(r8, rows - 1);
+    for (int at = tid / kPer; at < (rows + 15 & ~15); at += kThreads / kPer) {  // (whole warps)
+        const int row = min(at, rows - 1);
         const float2* ml = reinterpret_cast<const float2*>(p.ws_ml) + ((size_t)stream * p.R + r0 + row) * p.S;
+        float2 w[4];
+        const auto load = [&](int i) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                w[k] = i + kPer * k < nsplit ? __ldcg(ml + i + kPer * k) : make_float2(kNegMax, 0.f);
+        };
         float mx = kNegMax, sum = 0.f;
 #pragma unroll 1
-        for (int i = l8; i < nsplit; i += 32) {
-            float m[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) m[k] = i + 8 * k < nsplit ? __ldcg(&ml[i + 8 * k].x) : kNegMax;
-            mx = fmaxf(mx, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+        for (int i = sub + (nsplit - 1) / (4 * kPer) * (4 * kPer); i >= 0; i -= 4 * kPer) {
+            load(i);
+            mx = fmaxf(mx, fmaxf(fmaxf(w[0].x, w[1].x), fmaxf(w[2].x, w[3].x)));
         }
 #pragma unroll
-        for (int off = 4; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        for (int off = kPer / 2; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
 #pragma unroll 1
-        for (int i = l8; i < nsplit; i += 32) {
-            float2 w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = i + 8 * k < nsplit ? __ldcg(ml + i + 8 * k) : make_float2(kNegMax, 0.f);
+        for (int i = sub;;) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const float a = fast_exp2(w[k].x - mx);
                 sum = fmaf(w[k].y, a, sum);
-                if (i + 8 * k < nsplit) sw[row * kTreeMaxSplits + i + 8 * k] = a;
+                if (i + kPer * k < nsplit) sw[row * kTreeMaxSplits + i + kPer * k] = a;
             }
+            i += 4 * kPer;
+            if (i - sub >= nsplit) break;
+            load(i);
         }
 #pragma unroll
-        for (int off = 4; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        if (l8 == 0) sl[row] = sum;
+        for (int off = kPer / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (sub == 0) sl[row] = sum;
     }
     named_barrier_sync(1, kThreads);
     constexpr int Q4 = D / 4;
     static_assert(kThreads % Q4 == 0, "a thread keeps its column");
-    constexpr int kRowStep = kThreads / Q4, kItems = kRows == 16 ? 4 : 2, kAhead = 4;
+    constexpr int kRowStep = kThreads / Q4, kItems = 4, kAhead = kRows == 16 ? 4 : 2;
     const int c = tid % Q4;
     for (int rw = tid / Q4; rw < rows; rw += kItems * kRowStep) {
         float4 v[kItems];

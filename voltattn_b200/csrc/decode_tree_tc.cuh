@@ -74,16 +74,18 @@ struct TreeTcCfg {
     static constexpr int kRawTx = kRawSV + kNb * kSb;
     static constexpr int kRawStage = (kRawTx + 127) / 128 * 128;
     // what follows the ring: scales as floats [8 slots][K, V][kNG][64], masks,
-    // [2][2][2][128] maxima or sums, [2][128] references, barriers, ev[8], TMEM slot, fail, special, ticket, plan, range
+    // [2][2][2][128] maxima or sums, [2][128] references, barriers, ev[8], TMEM slot, fail, special, ticket, plan, two ranges
     static constexpr int kScaleSlots = 8;
     static constexpr int kScaleSlot = 2 * kNG * kNb * 4;
     static constexpr int kScaleV = kNG * kNb * 4;  // where a slot's V scales begin
     static constexpr int kScaleBytes = kScaled ? kScaleSlots * kScaleSlot : 0;
-    static constexpr int kRest = kScaleBytes + kRows * 8 + 5120 + 512 + 128;
+    static constexpr int kRest = kScaleBytes + kRows * 8 + 5120 + 512 + 192;
     static constexpr int kRoom = (227 * 1024 - 1024 - kOffRaw - kRest) / kRawStage;
     static constexpr int kRawStages = kDirect ? 1 : kRoom < 8 ? kRoom : 8;
     // (the merge of the ranges takes the front of shared memory: what follows stays past it)
-    static constexpr int kMergeBytes = (kRows * (kTreeMaxSplits + 1) * 4 + 127) / 128 * 128;
+    static constexpr int kStageRow = kDim + 4;  // floats of a row of the epilogue's stage, there as well
+    static constexpr int kMergeBytes =
+        (kRows * (kTreeMaxSplits + 1 > kStageRow ? kTreeMaxSplits + 1 : kStageRow) * 4 + 127) / 128 * 128;
     static constexpr int kRingEnd = kOffRaw + (kDirect ? 0 : kRawStages * kRawStage);
     static constexpr int kOffScales = kRingEnd > kMergeBytes ? kRingEnd : kMergeBytes;
     static constexpr int kOffMask = kOffScales + kScaleBytes;
@@ -91,7 +93,7 @@ struct TreeTcCfg {
     static constexpr int kOffBars = kOffMl + 5120;
     static constexpr int kBars = 2 * kKS + 3 * kVS + 3 * kNS + 4 + 3 + kScaleSlots + 2 * kRawStages;
     static constexpr int kOffMisc = kOffBars + kBars * 8;
-    static constexpr int kSmemBytes = 1024 + kOffMisc + 128;
+    static constexpr int kSmemBytes = 1024 + kOffMisc + 192;
     static_assert((kDirect || kRawStages >= 2) && kBars * 8 <= 512, "two blocks in flight");
     static_assert(kSmemBytes <= 227 * 1024, "one CTA per SM");
 };
@@ -273,10 +275,12 @@ __device__ __forceinline__ void tree_tc_fix_v(int p0, int len, int ctx, int nblk
 
 // A CTA's share of the call (splits allowed), and the part of it that comes next.
 struct TreeTcPlan {
-    long long window, at, end;  // cost units
+    int window, at, end;  // cost units
+    int more;             // whether `range` was found
 };
 struct TreeTcRange {
-    int b, hk, tile, p0, p1, part, parts;  // positions [p0, p1): one of the tile's parts (parts = 0: no work)
+    int b, hk, tile, len, n;    // rows of the sequence, drafted ones
+    int p0, p1, part, parts;    // positions [p0, p1): one of the tile's parts (parts = 0: no work)
 };
 
 // The work in a line: sequences, their KV heads, their tiles of query rows, each tile
@@ -288,103 +292,121 @@ struct TreeTcRange {
 constexpr int kTcFixed = 8, kTcMinWindow = 12;
 
 struct TreeTcSeq {
-    int blocks, live_tiles;
-    long long cost;  // of one KV head
+    int len, n, blocks, live_tiles;
+    int cost;  // of one KV head
 };
 template <class C>
 __device__ __forceinline__ TreeTcSeq tree_tc_seq(const TreeParams& p, int b) {
     const long long cap = (long long)p.max_pages * p.page_rows;
-    const int len = (int)max(0ll, min((long long)__ldg(p.lens + b), cap));
-    const int n = max(0, min(min(p.nodes ? __ldg(p.nodes + b) : p.Q, p.Q), len));
     TreeTcSeq q;
-    q.blocks = (len + C::kNb - 1) / C::kNb;
-    q.live_tiles = (min(p.R, n * p.G) + C::kRows - 1) / C::kRows;
-    q.cost = (long long)q.live_tiles * (q.blocks + kTcFixed) + (p.tiles - q.live_tiles);
+    q.len = (int)max(0ll, min((long long)__ldg(p.lens + b), cap));
+    q.n = max(0, min(min(p.nodes ? __ldg(p.nodes + b) : p.Q, p.Q), q.len));
+    q.blocks = (int)(((unsigned)q.len + C::kNb - 1) / C::kNb);
+    q.live_tiles = (min(p.R, q.n * p.G) + C::kRows - 1) / C::kRows;
+    q.cost = q.live_tiles * (q.blocks + kTcFixed) + (p.tiles - q.live_tiles);
     return q;
 }
 
-// (one warp) Whether the CTA has any work.
+// (one warp) The sequence that position `at` of the line lies in, and the range that the
+// CTA's window has of its tile from there on.
 template <class C>
-__device__ __forceinline__ bool tree_tc_plan(const TreeParams& p, int lane, TreeTcPlan* plan) {
-    long long total = 0;
-    int most = 0;
-    for (int b = lane; b < p.B; b += 32) {
-        const TreeTcSeq q = tree_tc_seq<C>(p, b);
-        total += q.cost;
+__device__ __forceinline__ void tree_tc_take(const TreeParams& p, const TreeTcSeq& q, int b, int upto, int at, int window, int end,
+                                             TreeTcPlan* plan, TreeTcRange* range) {
+    const int y0 = at - (upto - q.cost * p.Hkv);
+    if (y0 < 0 || upto <= at) return;  // one lane's sequence has it
+    const int each = q.blocks + kTcFixed, hk = y0 / q.cost, y = y0 - hk * q.cost, live = q.live_tiles * each;
+    TreeTcRange r = {b, hk, q.live_tiles + y - live, q.len, q.n, 0, 0, 0, 1};
+    int next = at + 1;
+    if (y < live) {
+        r.tile = y / each;
+        const int first = at - (y - r.tile * each) + kTcFixed;  // where its blocks begin
+        next = min(end, first + q.blocks);
+        r.p0 = max(0, at - first) * C::kNb;
+        r.p1 = (int)min((long long)max(0, next - first) * C::kNb, (long long)q.len);
+        // (a window that ends before the tile's blocks leaves it to the next)
+        const int w0 = first / window;
+        r.part = (int)blockIdx.x - w0;
+        r.parts = next > first ? (first + q.blocks - 1) / window - w0 + 1 : 0;
+    }
+    *range = r;
+    plan->at = next;
+}
+
+// inclusive sums over the lanes
+__device__ __forceinline__ int tree_tc_scan(int x, int lane) {
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, x, off);
+        if (lane >= off) x += up;
+    }
+    return x;
+}
+
+// (one warp) The next range of the CTA's window.
+template <class C>
+__device__ __forceinline__ void tree_tc_next(const TreeParams& p, int lane, TreeTcPlan* plan, TreeTcRange* range) {
+    const int window = plan->window, at = plan->at, end = plan->end;
+    __syncwarp();
+    if (lane == 0) plan->more = at < end;
+    int base = 0;
+    for (int b0 = 0; at < end && base <= at && b0 < p.B; b0 += 32) {
+        TreeTcSeq q = {0, 0, 0, 0, 0};
+        if (b0 + lane < p.B) q = tree_tc_seq<C>(p, b0 + lane);
+        const int upto = tree_tc_scan(q.cost * p.Hkv, lane) + base;
+        tree_tc_take<C>(p, q, b0 + lane, upto, at, window, end, plan, range);
+        base = __shfl_sync(0xffffffffu, upto, 31);
+    }
+}
+
+// (one warp) The CTA's window, and its first range.
+template <class C>
+__device__ __forceinline__ void tree_tc_plan(const TreeParams& p, int lane, TreeTcPlan* plan, TreeTcRange* range) {
+    int total = 0, most = 0;
+    TreeTcSeq q;
+    int upto;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+        q = {0, 0, 0, 0, 0};
+        if (b0 + lane < p.B) q = tree_tc_seq<C>(p, b0 + lane);
+        upto = tree_tc_scan(q.cost * p.Hkv, lane) + total;
+        total = __shfl_sync(0xffffffffu, upto, 31);
         most = max(most, q.blocks);
     }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
-    total *= p.Hkv;
     most = __reduce_max_sync(0xffffffffu, most);
-    const long long window = max(max((total + gridDim.x - 1) / gridDim.x, (long long)((most + p.S - 2) / (p.S - 1))),
-                                 (long long)kTcMinWindow);
-    const long long at = blockIdx.x * window;
+    const int grid = (int)gridDim.x;
+    const int window = max(max((total - 1) / grid + 1, (most + p.S - 2) / (p.S - 1)), kTcMinWindow);
+    // (the product fits: at least one CTA before this one had a window of its own, or it is past the end)
+    const bool some = (long long)blockIdx.x * window < total;
+    const int at = some ? (int)blockIdx.x * window : total, end = min((long long)total, (long long)at + window);
     if (lane == 0) {
         plan->window = window;
         plan->at = at;
-        plan->end = min(total, at + window);
-    }
-    return at < total;
-}
-
-// (one warp) The next range of the CTA's window; false: the window is done.
-template <class C>
-__device__ __forceinline__ bool tree_tc_next(const TreeParams& p, int lane, TreeTcPlan* plan, TreeTcRange* range) {
-    const long long window = plan->window, at = plan->at, end = plan->end;
-    if (at >= end) return false;
-    // the sequence that position `at` of the line lies in
-    long long base = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 32) {
-        TreeTcSeq q = {0, 0, 0};
-        if (b0 + lane < p.B) q = tree_tc_seq<C>(p, b0 + lane);
-        const long long mine = q.cost * p.Hkv;
-        long long upto = mine;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const long long up = __shfl_up_sync(0xffffffffu, upto, off);
-            if (lane >= off) upto += up;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, base + upto > at);
-        if (hit) {
-            if (lane == __ffs(hit) - 1) {
-                const long long y0 = at - (base + upto - mine), each = q.blocks + kTcFixed;
-                const int hk = (int)(y0 / q.cost);
-                const long long y = y0 - hk * q.cost, live = q.live_tiles * each;
-                TreeTcRange r;
-                r.b = b0 + lane;
-                r.hk = hk;
-                r.part = 0;
-                r.parts = 1;
-                r.p0 = r.p1 = 0;
-                long long next = at + 1;
-                if (y >= live) {
-                    r.tile = q.live_tiles + (int)(y - live);
-                } else {
-                    r.tile = (int)(y / each);
-                    const long long z = y - r.tile * each, first = at - z + kTcFixed;  // where its blocks begin
-                    next = min(end, first + q.blocks);
-                    r.p0 = (int)max(0ll, at - first) * C::kNb;
-                    r.p1 = (int)min(max(0ll, next - first) * C::kNb, 0x7FFFFFFFll);  // (may pass the sequence's end)
-                    r.part = (int)(blockIdx.x - first / window);
-                    // (a window that ends before the tile's blocks leaves it to the next)
-                    r.parts = next > first ? (int)((first + q.blocks - 1) / window - first / window) + 1 : 0;
-                }
-                *range = r;
-                plan->at = next;
-            }
-            break;
-        }
-        base += __shfl_sync(0xffffffffu, upto, 31);
+        plan->end = end;
+        plan->more = some;
     }
     __syncwarp();
-    return true;
+    if (!some) return;
+    if (p.B <= 32) tree_tc_take<C>(p, q, lane, upto, at, window, end, plan, range);
+    else tree_tc_next<C>(p, lane, plan, range);
 }
+
+// Four columns of query row r of a (sequence, KV head).
+struct TreeTcStore {
+    const TreeParams& p;
+    int b, hk, n;
+    __device__ __forceinline__ void operator()(int r, int c, float4 v, float inv) const {
+        const int node = p.node_of(r);
+        __half* dst = p.out + b * p.os_b + node * p.os_t + (long long)(hk * p.G + (r - node * p.G)) * p.os_h + 4 * c;
+        const bool on = node < n && inv != 0.f;
+        const __half2 x = __floats2half2_rn(on ? v.x * inv : 0.f, on ? v.y * inv : 0.f);
+        const __half2 y = __floats2half2_rn(on ? v.z * inv : 0.f, on ? v.w * inv : 0.f);
+        *reinterpret_cast<uint2*>(dst) = make_uint2(h2_bits(x), h2_bits(y));
+    }
+};
 
 // One range of a tile's positions; false: a wait gave up.
 template <class C>
 __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtensorMap& tmK, const CUtensorMap& tmV, uint8_t* smem,
-                                              const TreeTcRange& range, bool final) {
+                                              int slot, bool final) {
     constexpr int D = C::kD, NG = C::kNG, NB = C::kNb, KS = C::kKS, VS = C::kVS, SG = C::kSG, NS = C::kNS;
     constexpr Kind KK = C::kKind;
     unsigned long long* s_mask = reinterpret_cast<unsigned long long*>(smem + C::kOffMask);
@@ -402,28 +424,20 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
     unsigned* s_ticket = tslot + 3;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int b = range.b, hk = range.hk, split = range.part, nsplit = range.parts;
-    const int r0 = range.tile * C::kRows;
-    const long long cap = (long long)p.max_pages * p.page_rows;
-    const int len = (int)max(0ll, min((long long)__ldg(p.lens + b), cap));
-    const int n = max(0, min(min(p.nodes ? __ldg(p.nodes + b) : p.Q, p.Q), len));
-    const int ctx = len - n;
-    const int p0 = range.p0, p1 = min(len, range.p1);
-    const int stream = b * p.Hkv + hk;
+    TreeTcPlan* plan = reinterpret_cast<TreeTcPlan*>(smem + C::kOffMisc + 64);
+    TreeTcRange* ranges = reinterpret_cast<TreeTcRange*>(plan + 1);
+    const TreeTcRange now = ranges[slot];
+    const int b = now.b, hk = now.hk, r0 = now.tile * C::kRows, len = now.len, n = now.n, ctx = len - n;
+    const int p0 = now.p0, p1 = now.p1;
     const int live = min(p.R, n * p.G) - r0;  // rows of the tile that belong to a node; none: zeros
-    const int rows_here = min(C::kRows, p.R - r0);
+    __syncthreads();
 
-    const auto store_out = [&](int r, int c, float4 v, float inv) {
-        const int node = p.node_of(r);
-        __half* dst = p.out + b * p.os_b + node * p.os_t + (long long)(hk * p.G + (r - node * p.G)) * p.os_h + 4 * c;
-        const bool on = node < n && inv != 0.f;
-        const __half2 a = __floats2half2_rn(on ? v.x * inv : 0.f, on ? v.y * inv : 0.f);
-        const __half2 d = __floats2half2_rn(on ? v.z * inv : 0.f, on ? v.w * inv : 0.f);
-        *reinterpret_cast<uint2*>(dst) = make_uint2(h2_bits(a), h2_bits(d));
-    };
-    if (live <= 0) {
-        for (int i = tid; i < rows_here * (D / 4); i += C::kThreads)
+    if (live <= 0 || now.parts == 0) {  // (no rows of a node; or no blocks in this window)
+        const TreeTcStore store_out = {p, b, hk, n};
+        const int rows_here = min(C::kRows, p.R - r0);
+        for (int i = now.parts ? tid : rows_here * D; i < rows_here * (D / 4); i += C::kThreads)
             store_out(r0 + i / (D / 4), i % (D / 4), make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
+        if (warp == 21) tree_tc_next<C>(p, lane, plan, ranges + 1 - slot);
         return true;
     }
 
@@ -929,14 +943,20 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
 
     // ---- epilogue: a thread's row, its part of the dims: half of them (two tiles: of its
     // group's tile) or a quarter
+    // (read again: not held in registers over the loops)
+    const volatile TreeTcRange* was = ranges + slot;
+    const TreeTcStore store_out = {p, was->b, was->hk, was->n};
+    const int stream = store_out.b * p.Hkv + store_out.hk, tile0 = was->tile, r0e = tile0 * C::kRows, split = was->part, nsplit = was->parts;
+    const int rows_here = min(C::kRows, p.R - r0e), rows_live = min(p.R, store_out.n * p.G) - r0e;
     const bool direct = nsplit == 1;
+    float* stage = reinterpret_cast<float*>(smem);
     if (warp < 16) {
         s_xch[(set * 2 + hf) * 128 + row] = l_sum;
         if (hf == 0) s_xch[512 + set * 128 + row] = m_ref;
         named_barrier_sync(1, 512);
         const auto sum_of = [&](int w) { return s_xch[w * 256 + row] + s_xch[w * 256 + 128 + row]; };
-        const int qr = (C::kTwo ? set * 128 : 0) + row, r = r0 + qr;
-        const bool on = (C::kTwo ? set * 128 : 0) + quad * 32 < live;  // (the same for the whole warp)
+        const int qr = (C::kTwo ? set * 128 : 0) + row, r = r0e + qr;
+        const bool on = (C::kTwo ? set * 128 : 0) + quad * 32 < rows_live;  // (the same for the whole warp)
         const int w0 = C::kTwo ? set : 0;
         float mx = s_xch[512 + w0 * 128 + row], sum = sum_of(w0);
         if constexpr (!C::kTwo) {  // O has the last reference, the larger; the sums each group's own
@@ -945,11 +965,8 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
             sum = sum * fast_exp2(m0 - mx) + sum_of(1) * fast_exp2(m1 - mx);
         }
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const size_t slot = ((size_t)stream * p.R + r) * p.S + split;
-        const int node = p.node_of(r);
-        __half* orow = p.out + b * p.os_b + node * p.os_t + (long long)(hk * p.G + (r - node * p.G)) * p.os_h;
-        const float scale = on && node < n ? inv : 0.f;  // (0: rows of no node, or that see nothing)
-        const bool wide = (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
+        const float scale = direct ? on && qr < rows_live ? inv : 0.f : 1.f;  // (0: rows of no node, or that see nothing)
+        float* mine = stage + qr * C::kStageRow;
         constexpr int kCols = C::kTwo ? D / 2 : D / 4;
         const int c0 = C::kTwo ? hf * kCols : (set * 2 + hf) * kCols;
 #pragma unroll 1
@@ -967,7 +984,7 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
                 for (int i = 0; i < 16; ++i) o[i] = __uint_as_float(u[i]);
             }
             if constexpr (C::kFloat) {
-                if (*special && qr < live) {
+                if (*special && qr < rows_live) {
                     const unsigned long long mk = s_mask[qr];
                     for (int j = max(0, p0 - ctx); j < n && ctx + j < p1; ++j) {
                         if (!(mk >> j & 1ull)) continue;
@@ -989,39 +1006,38 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
 #pragma unroll
                 for (int d = 0; d < 8; ++d)
                     v[d] = C::kPairs4 ? o[i + 2 * (d & 3) + (d >> 2)] * tc_v_step<KK>(d & 3) : o[i + d];
-                if (direct) {
-                    uint32_t h[4];
 #pragma unroll
-                    for (int d = 0; d < 4; ++d)
-                        h[d] = scale != 0.f ? h2_bits(__floats2half2_rn(v[2 * d] * scale, v[2 * d + 1] * scale)) : 0u;
-                    if (wide) {
-                        *reinterpret_cast<uint4*>(orow + cb + i) = make_uint4(h[0], h[1], h[2], h[3]);
-                    } else {
-                        reinterpret_cast<uint2*>(orow + cb + i)[0] = make_uint2(h[0], h[1]);
-                        reinterpret_cast<uint2*>(orow + cb + i)[1] = make_uint2(h[2], h[3]);
-                    }
-                } else if (on) {
-                    float4* dst = reinterpret_cast<float4*>(p.ws_o + slot * D + cb + i);
-                    __stcg(dst, make_float4(v[0], v[1], v[2], v[3]));
-                    __stcg(dst + 1, make_float4(v[4], v[5], v[6], v[7]));
-                }
+                for (int d = 0; d < 8; ++d) v[d] = scale != 0.f ? v[d] * scale : 0.f;
+                *reinterpret_cast<float4*>(mine + cb + i) = make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4*>(mine + cb + i + 4) = make_float4(v[4], v[5], v[6], v[7]);
             }
         }
         if (!direct && on && c0 == 0 && qr < rows_here)
-            __stcg(reinterpret_cast<float2*>(p.ws_ml) + slot, make_float2(mx, sum));
+            __stcg(reinterpret_cast<float2*>(p.ws_ml) + ((size_t)stream * p.R + r) * p.S + split, make_float2(mx, sum));
+    } else if (warp == 21) {
+        tree_tc_next<C>(p, lane, plan, ranges + 1 - slot);
     }
     tc05_fence_before();
     __syncthreads();
     tc05_fence_after();
+    // a row at a time: rows' stores by the threads that hold them took 4 us more a range
+#pragma unroll 4
+    for (int i = tid; i < rows_here * (D / 4); i += C::kThreads) {
+        const int qr = i / (D / 4), c = i - qr * (D / 4);
+        const float4 v = *reinterpret_cast<const float4*>(stage + qr * C::kStageRow + 4 * c);
+        if (direct) store_out(r0e + qr, c, v, 1.f);
+        else if (qr < rows_live) __stcg(reinterpret_cast<float4*>(p.ws_o + (((size_t)stream * p.R + r0e + qr) * p.S + split) * D) + c, v);
+    }
     if (direct) return true;
-    unsigned* counter = p.counters + (size_t)stream * p.tiles + range.tile;
+    __syncthreads();
+    unsigned* counter = p.counters + (size_t)stream * p.tiles + tile0;
     if (tid == 0) *s_ticket = atomic_add_acq_rel_gpu(counter, 1u);
     __syncthreads();
     if (*s_ticket != (unsigned)(nsplit - 1)) return true;
     if (tid == 0) store_relaxed_gpu(counter, 0u);
-    tree_merge<D, C::kRows, C::kThreads>(p, stream, r0, min(rows_here, live), nsplit, reinterpret_cast<float*>(smem), tid, store_out);
-    for (int i = tid; i < (rows_here - min(rows_here, live)) * (D / 4); i += C::kThreads)
-        store_out(r0 + live + i / (D / 4), i % (D / 4), make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
+    tree_merge<D, C::kRows, C::kThreads>(p, stream, r0e, min(rows_here, rows_live), nsplit, reinterpret_cast<float*>(smem), tid, store_out);
+    for (int i = tid; i < (rows_here - min(rows_here, rows_live)) * (D / 4); i += C::kThreads)
+        store_out(r0e + rows_live + i / (D / 4), i % (D / 4), make_float4(0.f, 0.f, 0.f, 0.f), 0.f);
     return true;
 }
 
@@ -1039,32 +1055,24 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     if (warp == 20) tmem_alloc(tslot, 512);
     if (tid == 0) tslot[1] = 0u;  // no wait has given up
     grid_dependency_wait();
-    bool more = true;
     if (warp == 0) {
         if (p.S > 1) {
-            more = tree_tc_plan<C>(p, lane, plan);
-            __syncwarp();
-            if (more) tree_tc_next<C>(p, lane, plan, range);
+            tree_tc_plan<C>(p, lane, plan, range);
         } else if (lane == 0) {  // a whole tile a CTA
             const int stream = (int)(blockIdx.x / p.tiles), b = stream / p.Hkv;
-            *range = {b, stream - b * p.Hkv, (int)blockIdx.x - stream * p.tiles, 0, 0x7FFFFFFF, 0, 1};
-            plan->at = plan->end = 0;
+            const TreeTcSeq q = tree_tc_seq<C>(p, b);
+            *range = {b, stream - b * p.Hkv, (int)blockIdx.x - stream * p.tiles, q.len, q.n, 0, q.len, 0, 1};
+            *plan = {0, 0, 0, 1};
         }
     }
-    more = __syncthreads_or(warp == 0 && more);
     tc05_fence_before();
     __syncthreads();
     tc05_fence_after();
-    while (more) {
-        const TreeTcRange now = *range;
-        const bool final = plan->at >= plan->end;
-        if (now.parts > 0 && !tree_tc_range<C>(p, tmK, tmV, smem, now, final)) break;
-        if (final) break;
+    for (int slot = 0; plan->more; slot ^= 1) {
+        if (!tree_tc_range<C>(p, tmK, tmV, smem, slot, plan->at >= plan->end)) break;
         // what this range left in shared memory by plain stores comes before the next one's copies
         fence_proxy_async_smem();
         __syncthreads();
-        if (warp == 0) more = tree_tc_next<C>(p, lane, plan, range);
-        more = __syncthreads_or(warp == 0 && more);
     }
     __syncthreads();
     if (warp == 20) tmem_dealloc(*tslot, 512);

@@ -65,8 +65,10 @@ int launch_tree_tc(const TreeParams& p, cudaStream_t st) {
     // splits: one CTA per SM, each with a window of the work; without: a CTA per tile
     const long long items = (long long)p.B * p.Hkv * p.tiles;
     if (items > 0x7FFFFFFFll) return VA_ERR_TOO_LARGE;
-    const long long ctas = p.S > 1 ? std::min((long long)sm_count(dev), items * p.S) : items;
-    return launch_tree_cfg<C>(decode_tree_tc_kernel<C>, p, dim3((unsigned)ctas), st, tmK, tmV);
+    TreeParams q = p;
+    if (items * ((long long)p.max_pages * p.page_rows / C::kNb + 1 + kTcFixed) > 0x7FFFFFFFll) q.S = 1;  // (32-bit windows)
+    const long long ctas = q.S > 1 ? std::min((long long)sm_count(dev), items * q.S) : items;
+    return launch_tree_cfg<C>(decode_tree_tc_kernel<C>, q, dim3((unsigned)ctas), st, tmK, tmV);
 }
 
 template <int D>
