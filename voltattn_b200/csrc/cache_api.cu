@@ -56,13 +56,15 @@ constexpr size_t kCounterBytes = kCounters * sizeof(unsigned);
 // 5/8 of their tables on average, plus a CTA's fixed work in rows) shared by the device's
 // slots, and half of the longest range for the uneven end; smallest S first. The larger
 // tiles' CTAs share the work evenly by themselves: S only has to let the longest
-// sequence spread, here one of 2.5 times the mean length.
+// sequence spread, here one of 2.5 times the mean length. Tables of up to 640 rows are
+// not split there: merging two parts takes longer than 5 blocks (2 x 300 rows, f16+, 256
+// query rows: 17 us whole, 23 us in parts).
 int tree_splits(int nsm, int B, int Hkv, int R, int Lmax) {
     const int rows = tree_rows(R);
     const double ctas = (double)B * Hkv * ((R + rows - 1) / rows);
     if (ctas > (double)kCounters) return 1;
     const int units = (Lmax + kTreeUnit - 1) / kTreeUnit, most = std::min(kMaxSplits, units);
-    if (rows != 16) return std::max(1, std::min(most, (int)std::ceil(2.5 * nsm / ctas) + 1));
+    if (rows != 16) return most <= 5 ? 1 : std::min(most, (int)std::ceil(2.5 * nsm / ctas) + 1);
     const double load = ctas / (3.0 * nsm), fixed = 320.0;
     double best = 1e300;
     int S = 1;

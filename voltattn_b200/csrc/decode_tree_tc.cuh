@@ -289,7 +289,7 @@ struct TreeTcRange {
 // sequence's length left the SMs idle for a third of the call). A tile counts kTcFixed blocks more
 // than it has, about what starting and writing it takes; one without live rows counts 1. Windows
 // are long enough that none of a tile's blocks need more than S of them.
-constexpr int kTcFixed = 8, kTcMinWindow = 12;
+constexpr int kTcFixed = 6, kTcMinWindow = 8;
 
 struct TreeTcSeq {
     int len, n, blocks, live_tiles;
