@@ -392,13 +392,15 @@ VA_API int va_device_error(int* code);
  * [B][Q][Hq][D]); q 16-byte, out 8-byte aligned. Any Hq / Hkv. Formats f16+ / bf16+ /
  * f8+ / q8+ / q4+ / q3+ at D = 64 or 128, page_rows a multiple of 8 (else
  * VA_ERR_UNSUPPORTED). bf16 rows are taken as fp16 values (beyond fp16's range:
- * infinite). Table entries outside [0, num_pages) read page 0.
- * S: splits of a sequence's rows over CTAs (<= 128; 0: chosen by
- * va_suggest_tree_splits' rule and what ws holds). ws: 16-byte aligned,
+ * infinite; below 2^-14 with fewer bits). Table entries outside [0, num_pages) read page 0.
+ * S: the most parts that a sequence's rows are split into over CTAs (<= 128; 0:
+ * chosen by va_suggest_tree_splits' rule and what ws holds). ws: 16-byte aligned,
  * ws_bytes >= va_tree_workspace_bytes(B, Hq, Hkv, Q, D, max(S, 1)), zeroed before
  * first use (va_workspace_init). A completed call leaves the counters at its front
  * zero, so one workspace serves calls of any shape in order on one stream. Splits
- * (S > 1) take at most 16384 row tiles (B * Hkv * (Hq / Hkv * Q / 32, rounded up)). */
+ * (S > 1) take at most 16384 row tiles, one per (sequence, KV head, 16 to 256 of its
+ * Hq / Hkv * Q query rows, by the call's size). Results are the same from
+ * call to call; where a sequence is split depends on the batch's lengths as well. */
 VA_API size_t va_tree_workspace_bytes(int B, int Hq, int Hkv, int Q, int D, int S);
 VA_API int va_suggest_tree_splits(int fmt, int B, int Hq, int Hkv, int Q, int Lmax, int D, int* S);
 VA_API int va_decode_tree(int fmt, const va_bufs* bufs, const long long* q_strides, const long long* out_strides,

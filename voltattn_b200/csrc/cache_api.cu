@@ -39,11 +39,19 @@ int check_pool(int fmt, const va_bufs* b, int B, int max_pages, int Hkv, int pag
     return VA_OK;
 }
 
-// Rows of a CTA's tile of query rows: 16 (decode_tree.cuh), 128 or 256
-// (decode_tree_tc.cuh). Measured on B200 at 64 rows: 113 us in four tiles of 16
-// against 137 in one of 128 (8-bit cache, 590000 positions x heads); at 128 rows 598
-// against 313 (4-bit, 1.6 million).
-int tree_rows(int R) { return R <= 64 ? 16 : R <= 128 ? 128 : 256; }
+// Rows of a CTA's tile of query rows: 16 (decode_tree.cuh), 128 or 256 (decode_tree_tc.cuh).
+// The large tiles read the cache once for all their rows but cost more to start: 18 us in
+// tiles of 16 against 26 in one of 128 (128 query rows, 8 KV heads x 1024 rows, q4+), 43
+// against 32 at 4 x 4000 rows. Few live rows leave them idle: 64 rows of q8+, 16
+// sequences up to 8192 rows, take 101 us in tiles of 16, 107 in one of 128. fp16 rows go to
+// the tensor cores without a conversion: 64 rows 132 against 74 us, 32 rows 88
+// against 70. The sizes are those of the tables, the lengths being on the device.
+int tree_rows(int fmt, int B, int Hkv, int R, int Lmax) {
+    const bool f16 = fmt == VA_F16P;
+    const double work = (double)B * Hkv * Lmax * R;
+    if (R <= (f16 ? 16 : 64) || work <= (f16 ? 1 << 21 : 1 << 23)) return 16;
+    return R <= 128 ? 128 : 256;
+}
 
 // Completion counters, one per (sequence, KV head, row tile), at the front of the
 // workspace: a fixed number, so the slots of a call never lie where a call of
@@ -59,8 +67,7 @@ constexpr size_t kCounterBytes = kCounters * sizeof(unsigned);
 // sequence spread, here one of 2.5 times the mean length. Tables of up to 640 rows are
 // not split there: merging two parts takes longer than 5 blocks (2 x 300 rows, f16+, 256
 // query rows: 17 us whole, 23 us in parts).
-int tree_splits(int nsm, int B, int Hkv, int R, int Lmax) {
-    const int rows = tree_rows(R);
+int tree_splits(int nsm, int rows, int B, int Hkv, int R, int Lmax) {
     const double ctas = (double)B * Hkv * ((R + rows - 1) / rows);
     if (ctas > (double)kCounters) return 1;
     const int units = (Lmax + kTreeUnit - 1) / kTreeUnit, most = std::min(kMaxSplits, units);
@@ -88,8 +95,7 @@ void divisor(int d, unsigned& mul, unsigned& shift) {
     mul = (unsigned)((((unsigned long long)1 << 32) * ((1ull << shift) - (unsigned)d)) / (unsigned)d + 1);
 }
 
-int check_layers(int fmt, int Hkv, int page_rows, int num_pages, int layers) {
-    (void)fmt;
+int check_layers(int Hkv, int page_rows, int num_pages, int layers) {
     if (layers < 1) return VA_ERR_INVALID;
     if (layers > 65535 || Hkv > 65535) return VA_ERR_TOO_LARGE;
     if ((long long)layers * num_pages > (1ll << 31) || (long long)Hkv * page_rows > (1ll << 24)) return VA_ERR_TOO_LARGE;
@@ -128,7 +134,8 @@ int va_suggest_tree_splits(int fmt, int B, int Hq, int Hkv, int Q, int Lmax, int
     int dev;
     const int rc = current_device(&dev);
     if (rc) return rc;
-    *S = tree_splits(sm_count(dev), B, Hkv, Hq / Hkv * Q, Lmax);
+    const int R = Hq / Hkv * Q;
+    *S = tree_splits(sm_count(dev), tree_rows(fmt, B, Hkv, R, Lmax), B, Hkv, R, Lmax);
     return VA_OK;
 }
 
@@ -148,18 +155,17 @@ int va_decode_tree(int fmt, const va_bufs* b, const long long* q_strides, const 
     const long long* os = out_strides ? out_strides : dense;
     for (int i = 0; i < 3; ++i)
         if (qs[i] % 8 || os[i] % 8) return VA_ERR_ALIGN;
-    const int R = Hq / Hkv * Q;
+    const int R = Hq / Hkv * Q, rows = tree_rows(fmt, B, Hkv, R, max_pages * page_rows);
     if ((long long)B * Hq * Q > INT_MAX / kMaxSplits) return VA_ERR_TOO_LARGE;
     if (!ws || !aligned16(ws)) return VA_ERR_WORKSPACE;
     if (S == 0) {
         int dev;
         rc = current_device(&dev);
         if (rc) return rc;
-        S = tree_splits(sm_count(dev), B, Hkv, R, max_pages * page_rows);
+        S = tree_splits(sm_count(dev), rows, B, Hkv, R, max_pages * page_rows);
         while (S > 1 && ws_bytes < va_tree_workspace_bytes(B, Hq, Hkv, Q, D, S)) --S;
     }
     if (ws_bytes < va_tree_workspace_bytes(B, Hq, Hkv, Q, D, S)) return VA_ERR_WORKSPACE;
-    const int rows = tree_rows(R);
     if (S > 1 && (long long)B * Hkv * ((R + rows - 1) / rows) > kCounters) return VA_ERR_TOO_LARGE;
     TreeParams p = {};
     p.K = static_cast<const uint8_t*>(b->K);
@@ -245,7 +251,7 @@ int va_accept_tree(int fmt, const va_bufs* b, const int* block_table, int max_pa
                    const int* path, const int* accepted, int* new_lens, int B, int P, int Hkv, int page_rows,
                    int num_pages, int D, int layers, void* stream) {
     int rc = check_pool(fmt, b, B, max_pages, Hkv, page_rows, num_pages, D);
-    if (!rc) rc = check_layers(fmt, Hkv, page_rows, num_pages, layers);
+    if (!rc) rc = check_layers(Hkv, page_rows, num_pages, layers);
     if (rc) return rc;
     if (!block_table || !lens || !nodes || !path || !accepted || !new_lens || new_lens == lens || P < 1) return VA_ERR_INVALID;
     if (P > kAcceptMax || B > 65535) return VA_ERR_TOO_LARGE;
@@ -285,7 +291,7 @@ int va_fork_pages(int fmt, const va_bufs* b, const int* refs, const int* block_t
                   int max_pages, int reserve, int Hkv, int page_rows, int num_pages, int D, int layers, void* ws,
                   size_t ws_bytes, void* stream) {
     int rc = check_pool(fmt, b, std::max(Bin, Bout), max_pages, Hkv, page_rows, num_pages, D);
-    if (!rc) rc = check_layers(fmt, Hkv, page_rows, num_pages, layers);
+    if (!rc) rc = check_layers(Hkv, page_rows, num_pages, layers);
     if (rc) return rc;
     if (page_rows % 8) return VA_ERR_UNSUPPORTED;
     if (Bin < 1 || Bout < 1 || reserve < 0) return VA_ERR_INVALID;
@@ -316,7 +322,7 @@ int va_compact_pages(int fmt, const va_bufs* b, const int* refs, const int* bloc
                      int* used, int B, int max_pages, int Hkv, int page_rows, int num_pages, int D, int layers,
                      void* ws, size_t ws_bytes, void* stream) {
     int rc = check_pool(fmt, b, B, max_pages, Hkv, page_rows, num_pages, D);
-    if (!rc) rc = check_layers(fmt, Hkv, page_rows, num_pages, layers);
+    if (!rc) rc = check_layers(Hkv, page_rows, num_pages, layers);
     if (rc) return rc;
     if (page_rows % 8) return VA_ERR_UNSUPPORTED;
     if (!refs || !block_table || !new_refs || !new_table || !used) return VA_ERR_INVALID;

@@ -533,7 +533,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
         // the 16 of tiles nt, nt ^ 1
         float2 x[NT][2];
         __half2 vmax = __float2half2_rn(0.f);
-        uint32_t vsc[NT][2];  // V scales of the two positions (both groups)
+        [[maybe_unused]] uint32_t vsc[NT][2];  // V scales of the two positions (both groups)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             // S of 8 positions: lane g decodes row (g >> 1) + 4 (g & 1) (+ 8 for odd tiles) of the 16
@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
                     else mma_f16_16816(a, qa[gr][k], h[2 * k], h[2 * k + 1]);
                 }
             }
-            float2 ks[NG];
+            [[maybe_unused]] float2 ks[NG];
             if constexpr (C::kScaled) {
                 float2 f[2];
 #pragma unroll

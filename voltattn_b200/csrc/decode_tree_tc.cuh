@@ -152,7 +152,7 @@ __device__ __forceinline__ void tc_load(TcRaw<K, kDim>& r, const uint8_t* row, i
 template <Kind K, int kDim, bool kIsV>
 __device__ __forceinline__ uint4 tc_convert(const TcRaw<K, kDim>& r, int j) {
     constexpr uint32_t kOne = 0x3C003C00u;
-    uint32_t h[4];
+    uint32_t h[4] = {};
     if constexpr (K == Kind::F16) {
         return make_uint4(r.w[4 * j], r.w[4 * j + 1], r.w[4 * j + 2], r.w[4 * j + 3]);
     } else if constexpr (K == Kind::BF16) {

@@ -73,7 +73,7 @@ int launch_prefill_fmt(int fmt, const PrefillParams& p, cudaStream_t st);
 int prefill_stage_rows(int L);
 size_t prefill_stage_bytes(int Hkv, int L, int D);
 int launch_prefill_staged_fmt(int fmt, const PrefillParams& p, void* ws, cudaStream_t st);
-// Tree attention (launch_tree_d*.cu): rows = query rows of a CTA (16 or 32).
+// Tree attention (launch_tree_d*.cu): rows = query rows of a CTA (16, 128 or 256).
 int launch_tree_d64(int fmt, const TreeParams& p, int rows, cudaStream_t st);
 int launch_tree_d128(int fmt, const TreeParams& p, int rows, cudaStream_t st);
 // Rows and pages of a paged cache (launch_cache.cu).
