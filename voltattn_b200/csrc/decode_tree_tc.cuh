@@ -279,6 +279,12 @@ __device__ __forceinline__ void tree_tc_fix_v(int p0, int len, int ctx, int nblk
     }
 }
 
+// Rows of a block's copies: the most of 64, 32, 16 and 8 that divide a page's, so that no
+// copy leaves its page.
+__host__ __device__ constexpr int tree_tc_run(int page_rows) {
+    return page_rows % 64 == 0 ? 64 : page_rows % 32 == 0 ? 32 : page_rows % 16 == 0 ? 16 : 8;
+}
+
 // A CTA's share of the call (splits allowed), and the part of it that comes next.
 struct TreeTcPlan {
     int window, at, end;  // cost units
@@ -804,8 +810,8 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
         }
     } else if (C::kDirect && warp == 21) {
         // ---- copies of fp16 rows: tensor copies of 64 dims by the block's rows inside a
-        // page (boxes of 64 or 8 rows) into the swizzled tiles; lane = run + 8 * group
-        const int run = p.page_rows % NB == 0 ? NB : 8, at = (lane & 7) * run, g = lane >> 3;
+        // page into the swizzled tiles; lane = run + 8 * group
+        const int run = tree_tc_run(p.page_rows), at = (lane & 7) * run, g = lane >> 3;
         const bool copies = at < NB && g < NG;
         int i = 0;
         bool ok = true;
@@ -839,10 +845,8 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
                 !mbar_wait_bounded(vraw + k % VS, (uint32_t)(k / VS) & 1u))
                 *fail = 1;
     } else if (!C::kDirect && warp == 21) {
-        // ---- copies: lane 4 r + k brings run r of buffer k (K, V, their scales): the
-        // whole block when it lies inside a page, else runs of 8 rows
-        const bool whole = p.page_rows % NB == 0;
-        const int run = whole ? NB : 8, nrun = NB / run, buf = lane & 3, at = (lane >> 2) * run;
+        // ---- copies: lane 4 r + k brings run r of buffer k (K, V, their scales)
+        const int run = tree_tc_run(p.page_rows), nrun = NB / run, buf = lane & 3, at = (lane >> 2) * run;
         const int rb = buf < 2 ? C::kRb : C::kSb;
         const uint32_t bytes = (uint32_t)(run * rb);
         const bool copies = lane < 4 * nrun && bytes > 0;

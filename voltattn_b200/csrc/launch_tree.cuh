@@ -54,7 +54,7 @@ int launch_tree_tc(const TreeParams& p, cudaStream_t st) {
     if constexpr (C::kDirect) {  // boxes of a block's rows inside a page
         const long long rows = (long long)p.num_pages * p.Hkv * p.page_rows;
         if (rows >= (1ll << 31)) return VA_ERR_TOO_LARGE;
-        const int box = p.page_rows % C::kNb == 0 ? C::kNb : 8;
+        const int box = tree_tc_run(p.page_rows);
         int rc = encode_f16_rows_map(&tmK, p.K, rows, box, C::kD);
         if (!rc) rc = encode_f16_rows_map(&tmV, p.V, rows, box, C::kD);
         if (rc) return rc;
