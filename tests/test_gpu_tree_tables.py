@@ -94,3 +94,12 @@ def test_more_sequences_than_lanes(va, B):
     c = Wide("q8+", B, 8, 1, 16, 64, 16, lens, nodes, seed=B)
     for S in (1, 2, 7):
         c.check(va, S)
+
+
+def test_window_across_many_sequences(va):
+    """More sequences than a window of a few CTAs' lanes: every window spans groups of 32 sequences."""
+    B = 700
+    rng = np.random.default_rng(3)
+    lens = rng.integers(1, 40, B)
+    c = Wide("q4+", B, 8, 1, 16, 64, 8, lens, np.minimum(16, lens), seed=1)
+    c.check(va, 2)

@@ -288,7 +288,8 @@ __host__ __device__ constexpr int tree_tc_run(int page_rows) {
 // A CTA's share of the call (splits allowed), and the part of it that comes next.
 struct TreeTcPlan {
     int window, at, end;  // cost units
-    int more;             // whether `range` was found
+    int more;             // whether there is a range at `at`
+    int b0, base;         // the 32 sequences that held the last one, and the units before them
 };
 struct TreeTcRange {
     int b, hk, tile, len, n;    // rows of the sequence, drafted ones
@@ -322,8 +323,8 @@ __device__ __forceinline__ TreeTcSeq tree_tc_seq(const TreeParams& p, int b) {
 // (one warp) The sequence that position `at` of the line lies in, and the range that the
 // CTA's window has of its tile from there on.
 template <class C>
-__device__ __forceinline__ void tree_tc_take(const TreeParams& p, const TreeTcSeq& q, int b, int upto, int at, int window, int end,
-                                             TreeTcPlan* plan, TreeTcRange* range) {
+__device__ __forceinline__ void tree_tc_take(const TreeParams& p, const TreeTcSeq& q, int b, int base, int upto, int at, int window,
+                                             int end, TreeTcPlan* plan, TreeTcRange* range) {
     const int y0 = at - (upto - q.cost * p.Hkv);
     if (y0 < 0 || upto <= at) return;  // one lane's sequence has it
     const int each = q.blocks + kTcFixed, hk = y0 / q.cost, y = y0 - hk * q.cost, live = q.live_tiles * each;
@@ -342,6 +343,8 @@ __device__ __forceinline__ void tree_tc_take(const TreeParams& p, const TreeTcSe
     }
     *range = r;
     plan->at = next;
+    plan->b0 = b & ~31;
+    plan->base = base;
 }
 
 // inclusive sums over the lanes
@@ -358,14 +361,14 @@ __device__ __forceinline__ int tree_tc_scan(int x, int lane) {
 template <class C>
 __device__ __forceinline__ void tree_tc_next(const TreeParams& p, int lane, TreeTcPlan* plan, TreeTcRange* range) {
     const int window = plan->window, at = plan->at, end = plan->end;
+    int base = plan->base, b0 = plan->b0;
     __syncwarp();
     if (lane == 0) plan->more = at < end;
-    int base = 0;
-    for (int b0 = 0; at < end && base <= at && b0 < p.B; b0 += 32) {
+    for (; at < end && base <= at && b0 < p.B; b0 += 32) {
         TreeTcSeq q = {0, 0, 0, 0, 0};
         if (b0 + lane < p.B) q = tree_tc_seq<C>(p, b0 + lane);
         const int upto = tree_tc_scan(q.cost * p.Hkv, lane) + base;
-        tree_tc_take<C>(p, q, b0 + lane, upto, at, window, end, plan, range);
+        tree_tc_take<C>(p, q, b0 + lane, base, upto, at, window, end, plan, range);
         base = __shfl_sync(0xffffffffu, upto, 31);
     }
 }
@@ -394,10 +397,11 @@ __device__ __forceinline__ void tree_tc_plan(const TreeParams& p, int lane, Tree
         plan->at = at;
         plan->end = end;
         plan->more = some;
+        plan->b0 = plan->base = 0;
     }
     __syncwarp();
     if (!some) return;
-    if (p.B <= 32) tree_tc_take<C>(p, q, lane, upto, at, window, end, plan, range);
+    if (p.B <= 32) tree_tc_take<C>(p, q, lane, 0, upto, at, window, end, plan, range);
     else tree_tc_next<C>(p, lane, plan, range);
 }
 
@@ -1072,7 +1076,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
             const int stream = (int)(blockIdx.x / p.tiles), b = stream / p.Hkv;
             const TreeTcSeq q = tree_tc_seq<C>(p, b);
             *range = {b, stream - b * p.Hkv, (int)blockIdx.x - stream * p.tiles, q.len, q.n, 0, q.len, 0, 1};
-            *plan = {0, 0, 0, 1};
+            *plan = {0, 0, 0, 1, 0, 0};
         }
     }
     tc05_fence_before();
