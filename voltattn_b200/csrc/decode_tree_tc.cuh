@@ -40,7 +40,7 @@
 // positions against 128 rows takes 1.27 us and 5600 warp-instructions. In copies with parts cut out (303 us then): no loads of scales 270, no stores of decoded tiles 261, a
 // quarter of the MMAs 293, no exponentials 295. Measured: 8 sequences of 16384 to 32768 rows, q4+,
 // 32 nodes, 32 query / 8 KV heads, 231 us, 470 TFLOP/s (598 us in tiles of 16); 16 of 2048
-// to 8192, f16+, 64 nodes, 32 / 4 heads, 144 us, 630 TFLOP/s.
+// to 8192, f16+, 64 nodes, 32 / 4 heads, 120 us, 760 TFLOP/s.
 #pragma once
 
 #include "decode_tree.cuh"
@@ -300,9 +300,10 @@ struct TreeTcRange {
 // its sequence's blocks of 64 positions. CTA i takes the i-th window of it, so every CTA
 // has the same number of blocks whatever the lengths (a range per CTA in proportion to its
 // sequence's length left the SMs idle for a third of the call). A tile counts kTcFixed blocks more
-// than it has, about what starting and writing it takes; one without live rows counts 1. Windows
-// are long enough that none of a tile's blocks need more than S of them.
-constexpr int kTcFixed = 6, kTcMinWindow = 8;
+// than it has, about what starting and writing it takes (6 to 14 measure the same); one
+// without live rows counts 1. Windows are long enough that none of a tile's blocks need more
+// than S of them.
+constexpr int kTcFixed = 8, kTcMinWindow = 8;
 
 struct TreeTcSeq {
     int len, n, blocks, live_tiles;
