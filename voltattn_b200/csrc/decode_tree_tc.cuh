@@ -37,11 +37,12 @@
 // stored in the same order and the output's are put back.
 //
 // Bound by what the roles share: issue slots (58 % busy) and shared memory. A block of 64
-// positions against 128 rows takes 1.27 us and 5600 warp-instructions. In copies with parts cut out (303 us then): no loads of scales 270, no stores of decoded tiles 261, a
-// quarter of the MMAs 293, no exponentials 295. Measured: 8 sequences of 16384 to 32768 rows, q4+,
+// positions against 128 rows takes 1.27 us and 5600 warp-instructions. In copies with parts
+// cut out (303 us then): no loads of scales 270, no stores of decoded tiles 261, a quarter of
+// the MMAs 293, no exponentials 295. Measured: 8 sequences of 16384 to 32768 rows, q4+,
 // 32 nodes, 32 query / 8 KV heads, 231 us, 470 TFLOP/s (598 us in tiles of 16); 16 of 2048
-// to 8192, f16+, 64 nodes, 32 / 4 heads, 120 us, 760 TFLOP/s
-// (144 in a loop of seconds, at the 1000 W power cap).
+// to 8192, f16+, 64 nodes, 32 / 4 heads, 120 us, 760 TFLOP/s (144 in a loop of seconds, at
+// the 1000 W power cap).
 #pragma once
 
 #include "decode_tree.cuh"
