@@ -25,10 +25,11 @@
 //     is taken off as -offset * sum(q) in the accumulator's initial value.
 //   O += P V: the V scale multiplies the fp32 weight before its one rounding to
 //     fp16 (P' = fp16(w * scale), one P' per group).
-// The rounding of P' is the only one below 32 bits: it is relative (2^-11)
-// because the exponent's reference is kept so that P' of the largest weight
-// lies in [2^9, 2^15): ref follows (row maximum + exponent of the largest V scale
-// - 12), in log2 units, and is left while that grows by no more than 2.
+// The rounding of P' is the only one below 32 bits: it is relative (2^-11) down to 2^-14. The
+// exponent's reference of a query row is the most of score + log2 of the position's own (larger) V scale
+// over the positions that it sees, set where P' of that position is 2^11, and left while that
+// grows by no more than kTreeLag (log2): a row's largest P' lies in [2^11, 2^16). P' of the other
+// positions, and of the group of smaller scales, lie below it by the ratio of weights and scales.
 //
 // Rows that a query row does not see have no influence at all on it: their
 // scores are replaced, their weights selected to 0 before the scale (which may
@@ -324,6 +325,18 @@ __device__ __forceinline__ bool clear_not_finite(uint32_t& u) {
     return any;
 }
 
+// log2 of a position's V scales (one, or two and the larger counts) for the exponents' reference.
+// Infinite and nan ones, which make what they scale infinite or nan whatever the reference is, count as
+// fp16's largest; 0, which gives no P' at all, as less than its least.
+__device__ __forceinline__ float tree_scale_log2(__half2 v) {
+    const float2 f = __half22float2(__habs2(v));
+    return fmaxf(__log2f(fminf(fmaxf(f.x, f.y), 65504.f)), -25.f);
+}
+// A row's reference is set where its largest P' is 2^kTreeBase, and left while that stays below
+// 2^(kTreeBase + kTreeLag): fp16 ends just below 2^16, and the approximate log2 and exp2 take less
+// than the remaining 0.1.
+constexpr float kTreeBase = 11.f, kTreeLag = 4.9f;
+
 // The last range of a row tile merges all of them, in order: first the weights of
 // every (row, range) into shared memory (kRows * (kTreeMaxSplits + 1) floats), then the
 // outputs with the loads of several rows in flight. kThreads threads take part.
@@ -574,15 +587,10 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
                         vsc[nt][e] = *reinterpret_cast<const uint16_t*>(st + C::kOffSV + 2 * pr);
                     }
                     f[e] = __half22float2(bits_h2(k));
-                    uint32_t va = vsc[nt][e];
                     if constexpr (tail) {
-                        if (pb + pr >= len) vsc[nt][e] = va = 0u;
-                        // an infinite scale of a row that not all rows see is no measure
-                        va &= 0x7FFF7FFFu;
-                        if ((va & 0x7FFFu) >= 0x7C00u) va &= 0x7FFF0000u;
-                        if ((va >> 16) >= 0x7C00u) va &= 0x7FFFu;
+                        if (pb + pr >= len) vsc[nt][e] = 0u;
                     }
-                    vmax = __hmax2(vmax, __habs2(bits_h2(va)));
+                    vmax = __hmax2(vmax, __habs2(bits_h2(vsc[nt][e])));
                 }
                 ks[0] = make_float2(f[0].x, f[1].x);
                 if constexpr (NG == 2) ks[NG - 1] = make_float2(f[0].y, f[1].y);
@@ -615,15 +623,13 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
                 seen[r] = bits;
             }
         }
-        // running reference, from this lane's columns alone: its largest score and its
-        // largest V scale bound its P'. Only where one exceeds the row's reference by more
-        // than 2 (log2) do the row's lanes agree on a new one.
-        float ev = -12.f;
+        // running reference: the most of score + own V scale's exponent over the columns that the row
+        // sees. This lane's largest score with its largest scale is no less; only where one exceeds
+        // a row's reference by more than kTreeLag are the row's columns looked at one by one. Nothing of
+        // other rows, or of columns that the row does not see, enters a reference.
+        float ev = -kTreeBase;
         if constexpr (C::kScaled) {
-            // floor(log2) of the largest scale from its exponent field; 0 and inf need no shift
-            const float vm = fmaxf(__low2float(vmax), __high2float(vmax));
-            const int ex = (int)(__float_as_uint(vm) >> 23);
-            ev += (ex == 0 || ex == 255) ? 0.f : (float)(ex - 127);
+            ev += tree_scale_log2(vmax);
         }
         float want[2];
 #pragma unroll
@@ -635,13 +641,33 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
             // (columns that the row does not see at all leave the reference)
             if (tail && bm == kNegMax) want[r] = kNegMax;
         }
-        if (__any_sync(0xffffffffu, want[0] > ref[0] + 2.f || want[1] > ref[1] + 2.f)) {
+        if (__any_sync(0xffffffffu, want[0] > ref[0] + kTreeLag || want[1] > ref[1] + kTreeLag)) {
+            const auto row_max = [](float v) {
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+                return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+            };
+            float own[2] = {want[0], want[1]};
+            if constexpr (C::kScaled) {
+                own[0] = own[1] = kNegMax;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float le = tree_scale_log2(bits_h2(vsc[nt][e])) - kTreeBase;
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const float y = fmaf(e ? x[nt][r].y : x[nt][r].x, c2, le);
+                            if (!tail || ((seen[r] >> (2 * nt + e)) & 1u)) own[r] = fmaxf(own[r], y);
+                        }
+                    }
+            }
             float corr[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                want[r] = fmaxf(want[r], __shfl_xor_sync(0xffffffffu, want[r], 1));
-                want[r] = fmaxf(want[r], __shfl_xor_sync(0xffffffffu, want[r], 2));
-                const float nr = fmaxf(ref[r], want[r]);
+                own[r] = row_max(own[r]);
+                // (in the last blocks the bound has scales of columns that the row does not see)
+                const float bound = tail ? own[r] : row_max(want[r]);
+                const float nr = bound > ref[r] + kTreeLag ? fmaxf(ref[r], own[r]) : ref[r];
                 corr[r] = fast_exp2(ref[r] - nr);
                 ref[r] = nr;
                 l[r] *= corr[r];

@@ -28,8 +28,9 @@
 //   O_g += P'_g V_g (A = P' read from TMEM, B = the V tile read MN-major).
 // S(j + kNS) overwrites the buffer of job j once PV(j) has completed; the MMAs of one
 // thread complete in issue order, so a completed PV(j) implies every earlier one.
-// O is rescaled only when a row's reference grows by more than 4 (log2): P' of the
-// largest weight stays in [2^6, 2^15), its one rounding relative.
+// O is rescaled only when a row's reference, the most of score + own V scale (log2) that it
+// sees, grows by more than kTcLag: a row's largest P' stays in [2^10, 2^16), its one rounding
+// relative (with two groups, that of the group with the larger scale).
 //
 // The K and V tiles are the canonical 128-byte-swizzled layout, one panel of 64
 // rows per 64-dim group. Packed codes are placed two dims apart by 4 in each
@@ -81,11 +82,12 @@ struct TreeTcCfg {
     static constexpr int kRawV = kNb * kRb, kRawSK = 2 * kNb * kRb, kRawSV = kRawSK + kNb * kSb;
     static constexpr int kRawTx = kRawSV + kNb * kSb;
     static constexpr int kRawStage = (kRawTx + 127) / 128 * 128;
-    // what follows the ring: scales as floats [8 slots][K, V][kNG][64], masks,
-    // [2][2][2][128] maxima or sums, [2][128] references, barriers, ev[8], TMEM slot, fail, special, ticket, plan, two ranges
+    // what follows the ring: scales as floats [8 slots][K, V][kNG][64] and log2 [64], masks,
+    // [2][2][2][128] maxima or sums, [2][128] references, barriers, TMEM slot, fail, special, ticket, plan, two ranges
     static constexpr int kScaleSlots = 8;
-    static constexpr int kScaleSlot = 2 * kNG * kNb * 4;
-    static constexpr int kScaleV = kNG * kNb * 4;  // where a slot's V scales begin
+    static constexpr int kScaleSlot = (2 * kNG + 1) * kNb * 4;
+    static constexpr int kScaleV = kNG * kNb * 4;  // where a slot's V scales begin, and their log2
+    static constexpr int kScaleLog = 2 * kScaleV;
     static constexpr int kScaleBytes = kScaled ? kScaleSlots * kScaleSlot : 0;
     static constexpr int kRest = kScaleBytes + kRows * 8 + 5120 + 512 + 192;
     static constexpr int kRoom = (227 * 1024 - 1024 - kOffRaw - kRest) / kRawStage;
@@ -408,6 +410,9 @@ __device__ __forceinline__ void tree_tc_plan(const TreeParams& p, int lane, Tree
     else tree_tc_next<C>(p, lane, plan, range);
 }
 
+// As kTreeBase and kTreeLag: a move costs more here, O's way through registers.
+constexpr float kTcBase = 10.f, kTcLag = 5.9f;
+
 // Four columns of query row r of a (sequence, KV head).
 struct TreeTcStore {
     const TreeParams& p;
@@ -436,8 +441,7 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
     uint64_t *pfull = sfull + NS, *pvdone = pfull + NS, *refbar = pvdone + NS, *fin = refbar + 4, *scfull = fin + 2;
     uint64_t *rfull = scfull + C::kScaleSlots, *rempty = rfull + C::kRawStages, *vraw = rempty + C::kRawStages;
     uint64_t* qfull = vraw + VS;
-    float* s_ev = reinterpret_cast<float*>(smem + C::kOffMisc);
-    uint32_t* tslot = reinterpret_cast<uint32_t*>(s_ev + C::kScaleSlots);
+    uint32_t* tslot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
     volatile int* fail = reinterpret_cast<volatile int*>(tslot + 1);
     volatile int* special = fail + 1;
     unsigned* s_ticket = tslot + 3;
@@ -546,6 +550,21 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
                 asm volatile("" : "+r"(sc));  // the loads of scales come after the waits
                 const uint32_t tS = tbase + C::kOCols + sb * C::kSw + lane_addr, tO = tbase + (C::kTwo ? w * 128 : 0) + lane_addr;
                 float x[32];
+                // their maximum; with scales, of score (log2 units) + the log2 of the position's V
+                // scale. One tile takes it as the scores come, two in a pass of its own: spills decide
+                // (16 sequences of 1000 to 4000 rows, q8+, 128 query rows: 76 us against 89; 256: 145
+                // against 135)
+                constexpr bool kWithLoads = C::kScaled && !C::kTwo;
+                float b0 = kNegMax, b1 = kNegMax;
+                const auto raise = [&](uint32_t scales, int c, float2 u, float2 v) {
+                    if constexpr (C::kScaled) {
+                        const float4 lv = lds_f4(scales + C::kScaleLog + 4 * (32 * hf + c));
+                        u = ffma2(u, make_float2(c2, c2), make_float2(lv.x, lv.y));
+                        v = ffma2(v, make_float2(c2, c2), make_float2(lv.z, lv.w));
+                    }
+                    b0 = fmax3f(b0, u.x, u.y);
+                    b1 = fmax3f(b1, v.x, v.y);
+                };
 #pragma unroll
                 for (int cb = 0; cb < 32; cb += 16) {
                     uint32_t s0[16], s1[16];
@@ -574,6 +593,7 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
                         x[cb + c + 1] = u.y;
                         x[cb + c + 2] = v.x;
                         x[cb + c + 3] = v.y;
+                        if constexpr (kWithLoads) raise(sc, cb + c, u, v);
                     }
                 }
                 // which of its 32 columns the row sees
@@ -588,11 +608,13 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
                     for (int c = 0; c < 32; ++c)
                         if (!(vis >> c & 1u)) x[c] = kNegMax;
                 }
-                float b0 = fmaxf(x[0], x[1]), b1 = fmaxf(x[2], x[3]);
+                if (tail || !kWithLoads) {
+                    b0 = b1 = kNegMax;
+                    // (sc once more: the compiler would hold all log2 loaded above until here)
+                    uint32_t again = sbase + C::kOffScales + (blk % C::kScaleSlots) * C::kScaleSlot;
+                    asm volatile("" : "+r"(again));
 #pragma unroll
-                for (int c = 4; c < 32; c += 4) {
-                    b0 = fmax3f(b0, x[c], x[c + 1]);
-                    b1 = fmax3f(b1, x[c + 2], x[c + 3]);
+                    for (int c = 0; c < 32; c += 4) raise(again, c, make_float2(x[c], x[c + 1]), make_float2(x[c + 2], x[c + 3]));
                 }
                 // the row's maximum over both halves; their barrier also puts every load of S
                 // before the stores of P' below
@@ -600,8 +622,8 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
                 xch[hf * 128 + row] = fmaxf(b0, b1);
                 named_barrier_sync(2 + w * 4 + quad, 64);
                 const float bm = fmaxf(fmaxf(b0, b1), xch[(1 - hf) * 128 + row]);
-                const float ev = C::kScaled ? s_ev[blk % C::kScaleSlots] : 0.f;
-                const float want = bm == kNegMax ? kNegMax : fmaf(bm, c2, ev - 10.f);
+                // (a score far below any product of finite numbers: the row sees none of the block)
+                const float want = bm < -1e37f ? kNegMax : C::kScaled ? bm - kTcBase : fmaf(bm, c2, -kTcBase);
                 // the reference that O has so far: the row's own (two tiles), or what the other
                 // group left after job j - 1 (two slots, each rewritten two jobs on, after both
                 // halves have read it)
@@ -612,7 +634,7 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
                         oref = s_ref[((j - 1) & 1) * 128 + row];
                     }
                 }
-                const float nref = want > oref + 4.f ? want : oref;
+                const float nref = want > oref + kTcLag ? want : oref;
                 if constexpr (!C::kTwo) {
                     if (hf == 0) s_ref[(j & 1) * 128 + row] = nref;
                     __syncwarp();
@@ -727,7 +749,6 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
                 if (C::kScaled && pw == (i & 1)) {  // the block's scales: two positions a lane
                     float* sk = reinterpret_cast<float*>(smem + C::kOffScales + (i % C::kScaleSlots) * C::kScaleSlot);
                     float* sv = sk + C::kScaleV / 4;
-                    __half2 big = __float2half2_rn(0.f);
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const int at = lane + 32 * e;
@@ -743,20 +764,10 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
                         sk[at] = fk.x;
                         sv[at] = fv.x;
                         if constexpr (NG == 2) sk[NB + at] = fk.y, sv[NB + at] = fv.y;
-                        // rows past the end and scales that are not finite are no measure
-                        uint32_t a = vs & 0x7FFF7FFFu;
-                        if (p0 + i * NB + at >= len) a = 0u;
-                        if ((a & 0x7FFFu) >= 0x7C00u) a &= 0x7FFF0000u;
-                        if ((a >> 16) >= 0x7C00u) a &= 0x7FFFu;
-                        big = __hmax2(big, bits_h2(a));
+                        sk[C::kScaleLog / 4 + at] = tree_scale_log2(bits_h2(vs));
                     }
-                    const float vm = fmaxf(__low2float(big), __high2float(big));
-                    const unsigned vb = __reduce_max_sync(0xffffffffu, __float_as_uint(vm));
                     __syncwarp();
-                    if (lane == 0) {
-                        s_ev[i % C::kScaleSlots] = vb ? (float)((int)(vb >> 23) - 127) : 0.f;
-                        mbar_arrive(scfull + i % C::kScaleSlots);
-                    }
+                    if (lane == 0) mbar_arrive(scfull + i % C::kScaleSlots);
                 }
                 uint8_t* tile_at = smem + C::kOffK + s * C::kTile;
 #pragma unroll
@@ -1065,7 +1076,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) decode_tree_tc_kernel(const Tr
     extern __shared__ __align__(128) uint8_t smem_raw[];
     // (an offset, not a rounded address: the compiler keeps seeing shared memory)
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    uint32_t* tslot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc + 4 * C::kScaleSlots);
+    uint32_t* tslot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
     TreeTcPlan* plan = reinterpret_cast<TreeTcPlan*>(smem + C::kOffMisc + 64);
     TreeTcRange* range = reinterpret_cast<TreeTcRange*>(plan + 1);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
