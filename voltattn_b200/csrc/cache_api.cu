@@ -18,6 +18,9 @@ namespace {
 constexpr int kMaxNodes = 64;
 constexpr int kMaxSplits = kTreeMaxSplits;
 constexpr int kMaxForks = 4000;
+// Rows of a table in decode_tree: positions are 32-bit, and rounding a range up to whole blocks and
+// parts adds less than 2^16 to them.
+constexpr long long kMaxTreeRows = (long long)INT_MAX - (1 << 16);
 
 bool pool_fmt(int f) { return f >= VA_F16 && f < VA_Q4CP; }
 bool tree_fmt(int f) {
@@ -155,8 +158,9 @@ int va_decode_tree(int fmt, const va_bufs* b, const long long* q_strides, const 
     const long long* os = out_strides ? out_strides : dense;
     for (int i = 0; i < 3; ++i)
         if (qs[i] % 8 || os[i] % 8) return VA_ERR_ALIGN;
-    const int R = Hq / Hkv * Q, rows = tree_rows(fmt, B, Hkv, R, max_pages * page_rows);
+    if ((long long)max_pages * page_rows > kMaxTreeRows) return VA_ERR_TOO_LARGE;
     if ((long long)B * Hq * Q > INT_MAX / kMaxSplits) return VA_ERR_TOO_LARGE;
+    const int R = Hq / Hkv * Q, rows = tree_rows(fmt, B, Hkv, R, max_pages * page_rows);
     if (!ws || !aligned16(ws)) return VA_ERR_WORKSPACE;
     if (S == 0) {
         int dev;

@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
             const int pi = (int)((__umulhi((unsigned)pos, p.page_mul) + (unsigned)pos) >> p.page_shift);
             int pg = pi < p.max_pages ? __ldg(trow + pi) : 0;
             pg = (unsigned)pg < (unsigned)p.num_pages ? pg : 0;
-            bulk_g2s(lane_dst + s * C::kStageBytes, lane_src + pg * lane_page + (pos - pi * p.page_rows) * lane_row,
+            bulk_g2s(lane_dst + s * C::kStageBytes, lane_src + pg * lane_page + (long long)(pos - pi * p.page_rows) * lane_row,
                      lane_bytes, bar + s, policy);
         }
     };
