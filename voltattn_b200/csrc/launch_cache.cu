@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(kCopyThreads) fork_copy_kernel(const ForkParam
         const size_t head = (size_t)p.pool.page_rows * p.pool.row_bytes[k];
         const uint4* src = reinterpret_cast<const uint4*>(p.pool.base[k] + ((layer + from) * p.pool.Hkv + blockIdx.z) * head);
         uint4* dst = reinterpret_cast<uint4*>(p.pool.base[k] + ((layer + to) * p.pool.Hkv + blockIdx.z) * head);
-        const int n = rows * p.pool.row_bytes[k] / 16;
+        const int n = rows / 8 * (p.pool.row_bytes[k] / 2);  // (rows: a multiple of 8; their bytes may pass 2^31)
         for (int x = threadIdx.x; x < n; x += 4 * kCopyThreads) {
             uint4 v[4];
 #pragma unroll
