@@ -430,7 +430,7 @@ VA_API int va_append_packed(int fmt, const void* k, const void* v, int in_type, 
  * ascending; the first accepted[b] of sequence b's are accepted (the path ends
  * at the first entry that does not ascend inside [0, nodes[b])). Row ctx + path[i]
  * becomes row ctx + i, ctx = lens[b] - nodes[b], in every KV head of every layer;
- * new_lens[b] = ctx + accepted (device int32 [B], not lens itself). Pool
+ * new_lens[b] = ctx + accepted (device int32 [B] that overlaps no input: else VA_ERR_INVALID). Pool
  * of `layers` layers, each [num_pages][Hkv][page_rows] rows, one after the other, that
  * share the table (layers of separate allocations: one call each). Every
  * format but q4c+. */
@@ -451,7 +451,7 @@ VA_API int va_accept_tree(int fmt, const va_bufs* bufs, const int* block_table, 
  * next one). *shortage (device int32) = how many it did not find: their entries
  * are -1, and a sequence that got none for its copied rows ends at its last full
  * page. Outputs new_refs [num_pages], new_table [Bout][max_pages], new_lens
- * [Bout]: separate buffers from the inputs. Bin, Bout <= 4000; page_rows a
+ * [Bout]: separate buffers from the inputs (what overlaps gives VA_ERR_INVALID). Bin, Bout <= 4000; page_rows a
  * multiple of 8; every format but q4c+; layers as va_accept_tree. ws: 4-byte
  * aligned scratch of va_pages_workspace_bytes(Bout, max_pages, num_pages)
  * (not one that va_decode_tree uses: it does not stay zero). */

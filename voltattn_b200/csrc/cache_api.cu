@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cmath>
 #include <climits>
+#include <initializer_list>
 
 #include "../../include/voltattn.h"
 #include "cache_rows.cuh"
@@ -96,6 +97,21 @@ void divisor(int d, unsigned& mul, unsigned& shift) {
     shift = 0;
     while ((1ll << shift) < d) ++shift;
     mul = (unsigned)((((unsigned long long)1 << 32) * ((1ull << shift) - (unsigned)d)) / (unsigned)d + 1);
+}
+
+// A buffer of int32, and whether the first `outs` of some (the outputs) lie in any other of them.
+struct Span {
+    const int* p;
+    long long n;
+};
+bool outputs_overlap(std::initializer_list<Span> spans, int outs) {
+    const Span* s = spans.begin();
+    for (int i = 0; i < outs; ++i)
+        for (int j = 0; j < (int)spans.size(); ++j) {
+            const uintptr_t a = reinterpret_cast<uintptr_t>(s[i].p), b = reinterpret_cast<uintptr_t>(s[j].p);
+            if (j != i && a < b + 4 * (uintptr_t)s[j].n && b < a + 4 * (uintptr_t)s[i].n) return true;
+        }
+    return false;
 }
 
 int check_layers(int Hkv, int page_rows, int num_pages, int layers) {
@@ -257,8 +273,11 @@ int va_accept_tree(int fmt, const va_bufs* b, const int* block_table, int max_pa
     int rc = check_pool(fmt, b, B, max_pages, Hkv, page_rows, num_pages, D);
     if (!rc) rc = check_layers(Hkv, page_rows, num_pages, layers);
     if (rc) return rc;
-    if (!block_table || !lens || !nodes || !path || !accepted || !new_lens || new_lens == lens || P < 1) return VA_ERR_INVALID;
+    if (!block_table || !lens || !nodes || !path || !accepted || !new_lens || P < 1) return VA_ERR_INVALID;
     if (P > kAcceptMax || B > 65535) return VA_ERR_TOO_LARGE;
+    // (one CTA of a sequence writes its new length while the others still read)
+    if (outputs_overlap({{new_lens, B}, {block_table, (long long)B * max_pages}, {lens, B}, {nodes, B}, {path, (long long)B * P}, {accepted, B}}, 1))
+        return VA_ERR_INVALID;
     const PoolView pool = make_pool(fmt, b, Hkv, page_rows, num_pages, D, layers);
     AcceptParams p = {};
     p.K = pool.base[0];
@@ -300,9 +319,13 @@ int va_fork_pages(int fmt, const va_bufs* b, const int* refs, const int* block_t
     if (page_rows % 8) return VA_ERR_UNSUPPORTED;
     if (Bin < 1 || Bout < 1 || reserve < 0) return VA_ERR_INVALID;
     if (!refs || !block_table || !lens || !parent || !new_refs || !new_table || !new_lens || !shortage) return VA_ERR_INVALID;
-    if (new_refs == refs || new_table == block_table || new_lens == lens || new_lens == parent) return VA_ERR_INVALID;
     if (Bin > kMaxForks || Bout > kMaxForks) return VA_ERR_TOO_LARGE;
+    const Span outs[4] = {{new_refs, num_pages}, {new_table, (long long)Bout * max_pages}, {new_lens, Bout}, {shortage, 1}};
+    const Span ins[4] = {{refs, num_pages}, {block_table, (long long)Bin * max_pages}, {lens, Bin}, {parent, Bout}};
+    if (outputs_overlap({outs[0], outs[1], outs[2], outs[3], ins[0], ins[1], ins[2], ins[3]}, 4)) return VA_ERR_INVALID;
     if (!ws || !aligned_to(ws, 4) || ws_bytes < va_pages_workspace_bytes(Bout, max_pages, num_pages)) return VA_ERR_WORKSPACE;
+    const Span scratch = {static_cast<int*>(ws), (long long)num_pages + 3ll * Bout};
+    if (outputs_overlap({scratch, outs[0], outs[1], outs[2], outs[3], ins[0], ins[1], ins[2], ins[3]}, 1)) return VA_ERR_INVALID;
     ForkParams p = {};
     p.pool = make_pool(fmt, b, Hkv, page_rows, num_pages, D, layers);
     p.refs = refs;
@@ -330,8 +353,12 @@ int va_compact_pages(int fmt, const va_bufs* b, const int* refs, const int* bloc
     if (rc) return rc;
     if (page_rows % 8) return VA_ERR_UNSUPPORTED;
     if (!refs || !block_table || !new_refs || !new_table || !used) return VA_ERR_INVALID;
-    if (new_refs == refs || new_table == block_table) return VA_ERR_INVALID;
+    const long long entries = (long long)B * max_pages;
+    const Span outs[3] = {{new_refs, num_pages}, {new_table, entries}, {used, 1}};
+    const Span ins[2] = {{refs, num_pages}, {block_table, entries}};
+    if (outputs_overlap({outs[0], outs[1], outs[2], ins[0], ins[1]}, 3)) return VA_ERR_INVALID;
     if (!ws || !aligned_to(ws, 4) || ws_bytes < va_pages_workspace_bytes(B, max_pages, num_pages)) return VA_ERR_WORKSPACE;
+    if (outputs_overlap({{static_cast<int*>(ws), 3ll * num_pages + 1}, outs[0], outs[1], outs[2], ins[0], ins[1]}, 1)) return VA_ERR_INVALID;
     CompactParams p = {};
     p.pool = make_pool(fmt, b, Hkv, page_rows, num_pages, D, layers);
     p.refs = refs;
@@ -343,7 +370,7 @@ int va_compact_pages(int fmt, const va_bufs* b, const int* refs, const int* bloc
     p.map = p.count + 1;
     p.from = p.map + num_pages;
     p.to = p.from + num_pages;
-    p.entries = (long long)B * max_pages;
+    p.entries = entries;
     return launch_compact_pages(p, static_cast<cudaStream_t>(stream));
 }
 
