@@ -376,7 +376,8 @@ VA_API int va_device_error(int* code);
  * The cache is the pool of va_decode_paged: K/V [num_pages][Hkv][page_rows] rows,
  * scales alike, row j of a sequence in page block_table[b * max_pages +
  * j / page_rows]. Lengths and tables live on the device; nothing is read back,
- * so a whole step can be captured in a CUDA graph. */
+ * so a whole step can be captured in a CUDA graph. Integer arrays are aligned to
+ * their elements (else VA_ERR_ALIGN). */
 
 /* Tree attention: sequence b's cache holds lens[b] rows (device int32 [B]; 0 is
  * an unused slot), of which the last n = nodes[b] (device int32 [B], or NULL: Q

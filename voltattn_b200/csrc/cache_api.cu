@@ -29,6 +29,9 @@ bool tree_fmt(int f) {
 }
 bool has_scales(int f) { return f != VA_F16 && f != VA_F16P && f != VA_BF16P; }
 bool aligned_to(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+bool all_aligned4(std::initializer_list<const void*> ps) {
+    return std::all_of(ps.begin(), ps.end(), [](const void* p) { return aligned_to(p, 4); });
+}
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Checks of what every entry point here takes: the pool's shape and its buffers.
@@ -169,6 +172,7 @@ int va_decode_tree(int fmt, const va_bufs* b, const long long* q_strides, const 
     if (Hq < 1 || Hq % Hkv || Q < 1 || S < 0) return VA_ERR_INVALID;
     if (Q > kMaxNodes || S > kMaxSplits) return VA_ERR_TOO_LARGE;
     if (!aligned16(b->q) || !aligned_to(b->out, 8)) return VA_ERR_ALIGN;
+    if (!aligned_to(tree_mask, 8) || !all_aligned4({lens, nodes, block_table})) return VA_ERR_ALIGN;
     const long long dense[3] = {(long long)Q * Hq * D, (long long)Hq * D, D};
     const long long* qs = q_strides ? q_strides : dense;
     const long long* os = out_strides ? out_strides : dense;
@@ -233,7 +237,7 @@ int va_append_packed(int fmt, const void* k, const void* v, int in_type, const l
     if (rc) return rc;
     if (in_type < VA_FP32 || in_type > VA_BF16 || T < 0) return VA_ERR_INVALID;
     if (!block_table || !cu_tokens || !pos || (T > 0 && (!k || !v))) return VA_ERR_INVALID;
-    if (!aligned16(k) || !aligned16(v)) return VA_ERR_ALIGN;
+    if (!aligned16(k) || !aligned16(v) || !all_aligned4({block_table, cu_tokens, pos})) return VA_ERR_ALIGN;
     const long long dense[2] = {(long long)Hkv * D, D};
     const long long* ks = k_strides ? k_strides : dense;
     const long long* vs = v_strides ? v_strides : dense;
@@ -275,6 +279,7 @@ int va_accept_tree(int fmt, const va_bufs* b, const int* block_table, int max_pa
     if (rc) return rc;
     if (!block_table || !lens || !nodes || !path || !accepted || !new_lens || P < 1) return VA_ERR_INVALID;
     if (P > kAcceptMax || B > 65535) return VA_ERR_TOO_LARGE;
+    if (!all_aligned4({block_table, lens, nodes, path, accepted, new_lens})) return VA_ERR_ALIGN;
     // (one CTA of a sequence writes its new length while the others still read)
     if (outputs_overlap({{new_lens, B}, {block_table, (long long)B * max_pages}, {lens, B}, {nodes, B}, {path, (long long)B * P}, {accepted, B}}, 1))
         return VA_ERR_INVALID;
@@ -320,6 +325,7 @@ int va_fork_pages(int fmt, const va_bufs* b, const int* refs, const int* block_t
     if (Bin < 1 || Bout < 1 || reserve < 0) return VA_ERR_INVALID;
     if (!refs || !block_table || !lens || !parent || !new_refs || !new_table || !new_lens || !shortage) return VA_ERR_INVALID;
     if (Bin > kMaxForks || Bout > kMaxForks) return VA_ERR_TOO_LARGE;
+    if (!all_aligned4({refs, block_table, lens, parent, new_refs, new_table, new_lens, shortage})) return VA_ERR_ALIGN;
     const Span outs[4] = {{new_refs, num_pages}, {new_table, (long long)Bout * max_pages}, {new_lens, Bout}, {shortage, 1}};
     const Span ins[4] = {{refs, num_pages}, {block_table, (long long)Bin * max_pages}, {lens, Bin}, {parent, Bout}};
     if (outputs_overlap({outs[0], outs[1], outs[2], outs[3], ins[0], ins[1], ins[2], ins[3]}, 4)) return VA_ERR_INVALID;
@@ -353,6 +359,7 @@ int va_compact_pages(int fmt, const va_bufs* b, const int* refs, const int* bloc
     if (rc) return rc;
     if (page_rows % 8) return VA_ERR_UNSUPPORTED;
     if (!refs || !block_table || !new_refs || !new_table || !used) return VA_ERR_INVALID;
+    if (!all_aligned4({refs, block_table, new_refs, new_table, used})) return VA_ERR_ALIGN;
     const long long entries = (long long)B * max_pages;
     const Span outs[3] = {{new_refs, num_pages}, {new_table, entries}, {used, 1}};
     const Span ins[2] = {{refs, num_pages}, {block_table, entries}};
