@@ -529,6 +529,15 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
         }
         const float c2 = rsqrtf((float)D) * kLog2e * tc_k_inv_step<KK>();
         const int w = set;
+        // A quadrant's two warps meet at a barrier in every job, which has no limit of its own: one that
+        // gives up a wait still comes to it for the jobs from `from` on, so that the other one ends too
+        const bool live_quad = (C::kTwo ? w * 128 : 0) + quad * 32 < live;
+        const auto give_up = [&](int from) {
+            if (lane == 0) report_error(kErrFullWait);
+            *fail = 1;
+            if (live_quad)
+                for (int k = from; k < njobs; k += 2) named_barrier_sync(2 + w * 4 + quad, 64);
+        };
         for (int j = w; j < njobs; j += 2) {
             const int blk = C::kTwo ? j >> 1 : j, sb = j % NS;
             const uint32_t ph = (uint32_t)(j / NS) & 1u;
@@ -538,23 +547,20 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
             // after block i + 2's products at the least, so this phase is not passed twice)
             if constexpr (C::kScaled)
                 ok = ok && mbar_wait_fast(scfull + blk % C::kScaleSlots, (uint32_t)(blk / C::kScaleSlots) & 1u);
-            if (!ok) {
-                if (lane == 0) report_error(kErrFullWait);
-                *fail = 1;
+            if (__any_sync(0xffffffffu, !ok)) {
+                give_up(j);
                 break;
             }
             tc05_fence_after();
             // a quadrant without live rows only keeps the barriers' count
-            if ((C::kTwo ? w * 128 : 0) + quad * 32 < live) {
+            if (live_quad) {
                 uint32_t sc = sbase + C::kOffScales + (blk % C::kScaleSlots) * C::kScaleSlot;
                 asm volatile("" : "+r"(sc));  // the loads of scales come after the waits
                 const uint32_t tS = tbase + C::kOCols + sb * C::kSw + lane_addr, tO = tbase + (C::kTwo ? w * 128 : 0) + lane_addr;
                 float x[32];
                 // their maximum; with scales, of score (log2 units) + the log2 of the position's V
-                // scale. One tile takes it as the scores come, two in a pass of its own: spills decide
-                // (16 sequences of 1000 to 4000 rows, q8+, 128 query rows: 76 us against 89; 256: 145
-                // against 135)
-                constexpr bool kWithLoads = C::kScaled && !C::kTwo;
+                // scale, taken as the scores come: in a pass of its own it held more registers (16
+                // sequences of 1000 to 4000 rows, q8+, 256 query rows: 166 us against 136)
                 float b0 = kNegMax, b1 = kNegMax;
                 const auto raise = [&](uint32_t scales, int c, float2 u, float2 v) {
                     if constexpr (C::kScaled) {
@@ -593,7 +599,7 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
                         x[cb + c + 1] = u.y;
                         x[cb + c + 2] = v.x;
                         x[cb + c + 3] = v.y;
-                        if constexpr (kWithLoads) raise(sc, cb + c, u, v);
+                        raise(sc, cb + c, u, v);
                     }
                 }
                 // which of its 32 columns the row sees
@@ -608,7 +614,7 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
                     for (int c = 0; c < 32; ++c)
                         if (!(vis >> c & 1u)) x[c] = kNegMax;
                 }
-                if (tail || !kWithLoads) {
+                if (tail) {
                     b0 = b1 = kNegMax;
                     // (sc once more: the compiler would hold all log2 loaded above until here)
                     uint32_t again = sbase + C::kOffScales + (blk % C::kScaleSlots) * C::kScaleSlot;
@@ -659,9 +665,8 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
                         tmem_st16_u(tO + hf * (D / 2) + cb, o);
                     }
                 }
-                if (!ok) {
-                    if (lane == 0) report_error(kErrFullWait);
-                    *fail = 1;
+                if (__any_sync(0xffffffffu, !ok)) {
+                    give_up(j + 2);
                     break;
                 }
                 float2 sum = make_float2(0.f, 0.f);
