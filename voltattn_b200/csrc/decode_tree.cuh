@@ -329,8 +329,9 @@ __device__ __forceinline__ bool clear_not_finite(uint32_t& u) {
 // Infinite and nan ones, which make what they scale infinite or nan whatever the reference is, count as
 // fp16's largest; 0, which gives no P' at all, as less than its least.
 __device__ __forceinline__ float tree_scale_log2(__half2 v) {
-    const float2 f = __half22float2(__habs2(v));
-    return fmaxf(__log2f(fminf(fmaxf(f.x, f.y), 65504.f)), -25.f);
+    v = __habs2(v);
+    const __half m = __hmin(__hmax(__low2half(v), __high2half(v)), __ushort_as_half((unsigned short)0x7BFF));
+    return fmaxf(__log2f(__half2float(m)), -25.f);
 }
 // A row's reference is set where its largest P' is 2^kTreeBase, and left while that stays below
 // 2^(kTreeBase + kTreeLag): fp16 ends just below 2^16, and the approximate log2 and exp2 take less
@@ -642,10 +643,6 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
             if (tail && bm == kNegMax) want[r] = kNegMax;
         }
         if (__any_sync(0xffffffffu, want[0] > ref[0] + kTreeLag || want[1] > ref[1] + kTreeLag)) {
-            const auto row_max = [](float v) {
-                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-                return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-            };
             float own[2] = {want[0], want[1]};
             if constexpr (C::kScaled) {
                 own[0] = own[1] = kNegMax;
@@ -664,10 +661,9 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
             float corr[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                own[r] = row_max(own[r]);
-                // (in the last blocks the bound has scales of columns that the row does not see)
-                const float bound = tail ? own[r] : row_max(want[r]);
-                const float nr = bound > ref[r] + kTreeLag ? fmaxf(ref[r], own[r]) : ref[r];
+                own[r] = fmaxf(own[r], __shfl_xor_sync(0xffffffffu, own[r], 1));
+                own[r] = fmaxf(own[r], __shfl_xor_sync(0xffffffffu, own[r], 2));
+                const float nr = own[r] > ref[r] + kTreeLag ? own[r] : ref[r];
                 corr[r] = fast_exp2(ref[r] - nr);
                 ref[r] = nr;
                 l[r] *= corr[r];
