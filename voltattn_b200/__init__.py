@@ -219,7 +219,9 @@ class DeviceBufs:
     ws: object = None
 
     def va(self) -> VaBufs:
-        return VaBufs(_ptr(self.K), _ptr(self.V), _ptr(self.scK), _ptr(self.scV), _ptr(self.q), _ptr(self.out))
+        scK, scV, q, out = self.scK, self.scV, self.q, self.out
+        return VaBufs(_ptr(self.K), _ptr(self.V), None if scK is None else scK.data_ptr(), None if scV is None else scV.data_ptr(),
+                      None if q is None else q.data_ptr(), None if out is None else out.data_ptr())
 
 
 def new_workspace(H: int, D: int, S: int, device=None):
@@ -449,6 +451,47 @@ def _strides(t, n: int):
     return (C.c_longlong * n)(*st[:n])
 
 
+_f16 = _i32 = _words = None  # torch.float16, torch.int32, the types of mask words (torch is imported on the first call)
+
+
+def _types():
+    global _f16, _i32, _words
+    import torch
+    _f16, _i32, _words = torch.float16, (torch.int32,), (torch.int64, torch.uint64)
+
+
+def _tree_strides(what: str, t, shape):
+    """Strides of fp16 rows of `shape` [B][Q][Hq][D]: None for a dense tensor of that size, else those of
+    a four-dimensional one that holds them as its first sequences and nodes."""
+    if t is None:
+        return None
+    sh = t.shape
+    if t.dtype is _f16:
+        if sh == shape and t.is_contiguous():
+            return None
+        if len(sh) == 4:
+            st = t.stride()
+            if sh[0] >= shape[0] and sh[1] >= shape[1] and sh[2:] == shape[2:] and st[3] == 1:
+                return (C.c_longlong * 3)(*st[:3])
+        elif t.is_contiguous() and t.numel() == shape[0] * shape[1] * shape[2] * shape[3]:
+            return None
+    raise ValueError(f"decode_tree: {what} must be float16 {list(shape)}, its last dimension dense, not {str(t.dtype)[6:]} {list(sh)} "
+                     f"of strides {list(t.stride())}")
+
+
+def _array(what: str, t, kinds, n: int, width: int = 0):
+    """Pointer to a dense array [n], or [n][width], or the front of a longer one, of one of the types `kinds`."""
+    if t is None:
+        return None
+    if t.dtype in kinds and t.is_contiguous():
+        if t.shape == (n, width) if width else t.numel() >= n:
+            return t.data_ptr()
+        if width and t.numel() >= n * width and (t.dim() == 1 or t.shape[-1] == width):
+            return t.data_ptr()
+    raise ValueError(f"{what} must be dense, " + " or ".join(str(k)[6:] for k in kinds) + f" [{n}]"
+                     + (f"[{width}]" if width else "") + f", not {str(t.dtype)[6:]} {list(t.shape)} of strides {list(t.stride())}")
+
+
 def tree_workspace_bytes(B: int, Hq: int, Hkv: int, Q: int, D: int, S: int) -> int:
     return int(_lib.va_tree_workspace_bytes(B, Hq, Hkv, Q, D, S))
 
@@ -465,14 +508,19 @@ def decode_tree(fmt, b: DeviceBufs, tree_mask, lens, nodes, block_table, max_pag
     node i of sequence b sees the lens[b] - nodes[b] rows before the drafted ones
     and the drafted rows j whose bit is set in tree_mask[b][i] (int64 or uint64
     CUDA tensor [B][Q], Q <= 64). b.q, b.out: fp16 [B][Q][Hq][D] (four-dimensional
-    tensors may be strided, the last dimension dense); lens, nodes int32 [B]
-    (nodes None: Q each), block_table int32 [B][max_pages]. S = 0: the library
+    tensors may be strided, the last dimension dense, and may hold more sequences
+    and nodes, of which the first are used); lens, nodes int32 [B] (nodes None: Q
+    each), block_table int32 [B][max_pages]. Other types and shapes: ValueError. S = 0: the library
     splits the rows as the workspace b.ws (zeroed once, tree_workspace_bytes) allows."""
-    vb = b.va()
-    _check(_lib.va_decode_tree(_fmt(fmt), C.byref(vb), _strides(b.q, 3), _strides(b.out, 3),
-                               _ptr(tree_mask), _ptr(lens), _ptr(nodes), _ptr(block_table), max_pages, B, Hq, Hkv, Q,
-                               page_rows, num_pages, D, S, _ptr(b.ws), _nbytes(b.ws), _stream_ptr(stream)),
-           "decode_tree")
+    code = _fmt(fmt)
+    if _i32 is None:
+        _types()
+    rows = (B, Q, Hq, D)
+    _check(_lib.va_decode_tree(code, C.byref(b.va()), _tree_strides("q", b.q, rows), _tree_strides("out", b.out, rows),
+                               _array("tree_mask", tree_mask, _words, B, Q), _array("lens", lens, _i32, B),
+                               _array("nodes", nodes, _i32, B), _array("block_table", block_table, _i32, B, max_pages),
+                               max_pages, B, Hq, Hkv, Q, page_rows, num_pages, D, S, _ptr(b.ws), _nbytes(b.ws),
+                               _stream_ptr(stream)), "decode_tree")
 
 
 def append_packed(fmt, k, v, b: DeviceBufs, block_table, max_pages: int, cu_tokens, pos, B: int, Hkv: int,
