@@ -195,14 +195,20 @@ def _ptr(t) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+_torch = None
+
+
 def _stream_ptr(stream) -> Optional[int]:
+    global _torch
     if stream is not None:
         return stream.cuda_stream
-    import torch
+    if _torch is None:
+        import torch
+        _torch = torch
     try:  # the handle of torch's current stream without building a Stream object (1.6 us a call)
-        return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+        return _torch._C._cuda_getCurrentRawStream(_torch._C._cuda_getDevice())
     except AttributeError:
-        return torch.cuda.current_stream().cuda_stream
+        return _torch.cuda.current_stream().cuda_stream
 
 
 @dataclass
@@ -451,13 +457,15 @@ def _strides(t, n: int):
     return (C.c_longlong * n)(*st[:n])
 
 
-_f16 = _i32 = _words = None  # torch.float16, torch.int32, the types of mask words (torch is imported on the first call)
+# torch.float16, int32, the types of mask words, VA_FP32 .. VA_BF16 (torch is imported on the first call)
+_f16 = _i32 = _words = _row_types = None
 
 
 def _types():
-    global _f16, _i32, _words
+    global _f16, _i32, _words, _row_types
     import torch
     _f16, _i32, _words = torch.float16, (torch.int32,), (torch.int64, torch.uint64)
+    _row_types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
 def _tree_strides(what: str, t, shape):
@@ -528,17 +536,24 @@ def append_packed(fmt, k, v, b: DeviceBufs, block_table, max_pages: int, cu_toke
     """K/V rows of packed tokens (k, v [T][Hkv][D], fp32 / fp16 / bf16, three-dimensional
     tensors may be strided as slices of one projection are) quantized into the
     pages of the pool in b: sequence b's tokens cu_tokens[b] .. cu_tokens[b+1] go
-    to its rows from pos[b] on (int32 CUDA tensors [B+1], [B])."""
-    import torch
-    kinds = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-    if k.dtype != v.dtype or k.dtype not in kinds or k.shape != v.shape:
+    to its rows from pos[b] on (int32 CUDA tensors [B+1], [B]). Other types and
+    shapes: ValueError, here and in the calls below."""
+    if _i32 is None:
+        _types()
+    kind, shape = _row_types.get(k.dtype), k.shape
+    if kind is None or k.dtype is not v.dtype or shape != v.shape:
         raise ValueError("append_packed: k and v must be float32, float16 or bfloat16 tensors of one shape")
-    T = k.shape[0] if k.dim() == 3 else k.numel() // (Hkv * D)
-    if T * Hkv * D != k.numel():
-        raise ValueError("append_packed: k and v must hold T * Hkv * D elements")
-    vb = b.va()
-    _check(_lib.va_append_packed(_fmt(fmt), _ptr(k), _ptr(v), kinds[k.dtype], _strides(k, 2), _strides(v, 2),
-                                 C.byref(vb), _ptr(block_table), max_pages, _ptr(cu_tokens), _ptr(pos), T, B, Hkv,
+    if len(shape) == 3:
+        T = shape[0]
+        if shape[1] != Hkv or shape[2] != D:
+            raise ValueError(f"append_packed: k and v must be [T][{Hkv}][{D}], not {list(shape)}")
+    else:
+        T = k.numel() // (Hkv * D)
+        if T * Hkv * D != k.numel():
+            raise ValueError("append_packed: k and v must hold T * Hkv * D elements")
+    _check(_lib.va_append_packed(_fmt(fmt), _ptr(k), _ptr(v), kind, _strides(k, 2), _strides(v, 2), C.byref(b.va()),
+                                 _array("block_table", block_table, _i32, B, max_pages), max_pages,
+                                 _array("cu_tokens", cu_tokens, _i32, B + 1), _array("pos", pos, _i32, B), T, B, Hkv,
                                  page_rows, num_pages, D, _stream_ptr(stream)), "append_packed")
 
 
@@ -548,10 +563,12 @@ def accept_tree(fmt, b: DeviceBufs, block_table, max_pages: int, lens, nodes, pa
     lens - nodes + path[b][i] becomes row lens - nodes + i for i < accepted[b], in
     every layer of the pool; new_lens[b] = lens[b] - nodes[b] + accepted. path:
     int32 [B][P] ascending node indices (P <= 64)."""
-    vb = b.va()
-    _check(_lib.va_accept_tree(_fmt(fmt), C.byref(vb), _ptr(block_table), max_pages, _ptr(lens), _ptr(nodes),
-                               _ptr(path), _ptr(accepted), _ptr(new_lens), B, P, Hkv, page_rows, num_pages, D, layers,
-                               _stream_ptr(stream)), "accept_tree")
+    if _i32 is None:
+        _types()
+    _check(_lib.va_accept_tree(_fmt(fmt), C.byref(b.va()), _array("block_table", block_table, _i32, B, max_pages), max_pages,
+                               _array("lens", lens, _i32, B), _array("nodes", nodes, _i32, B), _array("path", path, _i32, B, P),
+                               _array("accepted", accepted, _i32, B), _array("new_lens", new_lens, _i32, B), B, P, Hkv,
+                               page_rows, num_pages, D, layers, _stream_ptr(stream)), "accept_tree")
 
 
 def pages_workspace_bytes(B: int, max_pages: int, num_pages: int) -> int:
@@ -566,11 +583,14 @@ def fork_pages(fmt, b: DeviceBufs, refs, block_table, lens, parent, new_refs, ne
     pages and getting a copy of its last one, then pages for `reserve` more rows.
     All tensors int32 CUDA; refs counts a page's table entries (0: free). b.ws:
     scratch of pages_workspace_bytes(Bout, max_pages, num_pages)."""
-    vb = b.va()
-    _check(_lib.va_fork_pages(_fmt(fmt), C.byref(vb), _ptr(refs), _ptr(block_table), _ptr(lens), _ptr(parent),
-                              _ptr(new_refs), _ptr(new_table), _ptr(new_lens), _ptr(shortage), Bin, Bout, max_pages,
-                              reserve, Hkv, page_rows, num_pages, D, layers, _ptr(b.ws), _nbytes(b.ws),
-                              _stream_ptr(stream)), "fork_pages")
+    if _i32 is None:
+        _types()
+    _check(_lib.va_fork_pages(_fmt(fmt), C.byref(b.va()), _array("refs", refs, _i32, num_pages),
+                              _array("block_table", block_table, _i32, Bin, max_pages), _array("lens", lens, _i32, Bin),
+                              _array("parent", parent, _i32, Bout), _array("new_refs", new_refs, _i32, num_pages),
+                              _array("new_table", new_table, _i32, Bout, max_pages), _array("new_lens", new_lens, _i32, Bout),
+                              _array("shortage", shortage, _i32, 1), Bin, Bout, max_pages, reserve, Hkv, page_rows,
+                              num_pages, D, layers, _ptr(b.ws), _nbytes(b.ws), _stream_ptr(stream)), "fork_pages")
 
 
 def compact_pages(fmt, b: DeviceBufs, refs, block_table, new_refs, new_table, used, B: int, max_pages: int, Hkv: int,
@@ -578,10 +598,12 @@ def compact_pages(fmt, b: DeviceBufs, refs, block_table, new_refs, new_table, us
     """Moves the pages in use to the front of the pool (va_compact_pages) and
     renumbers refs and block_table into new_refs and new_table; used[0] = their
     number. b.ws: scratch of pages_workspace_bytes(B, max_pages, num_pages)."""
-    vb = b.va()
-    _check(_lib.va_compact_pages(_fmt(fmt), C.byref(vb), _ptr(refs), _ptr(block_table), _ptr(new_refs),
-                                 _ptr(new_table), _ptr(used), B, max_pages, Hkv, page_rows, num_pages, D, layers,
-                                 _ptr(b.ws), _nbytes(b.ws), _stream_ptr(stream)), "compact_pages")
+    if _i32 is None:
+        _types()
+    _check(_lib.va_compact_pages(_fmt(fmt), C.byref(b.va()), _array("refs", refs, _i32, num_pages),
+                                 _array("block_table", block_table, _i32, B, max_pages), _array("new_refs", new_refs, _i32, num_pages),
+                                 _array("new_table", new_table, _i32, B, max_pages), _array("used", used, _i32, 1), B, max_pages,
+                                 Hkv, page_rows, num_pages, D, layers, _ptr(b.ws), _nbytes(b.ws), _stream_ptr(stream)), "compact_pages")
 
 
 def probe_ceiling(device: int = 0, nbytes: int = 0, reps: int = 0, method: Optional[int] = None) -> float:
