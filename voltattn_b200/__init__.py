@@ -441,8 +441,18 @@ def _fmt(f) -> int:
     return code
 
 
-def _nbytes(t) -> int:
-    return 0 if t is None else t.nbytes
+# The C functions of the calls below once more, with argtypes for the pointers before their ints only: ctypes
+# converts what comes behind by its own type (ints as int) at a sixth of the time, so the pointers and
+# sizes there are passed as c_void_p.
+_vp = C.c_void_p
+_short = C.CDLL(LIB_PATH)
+for _name, _n in (("va_decode_tree", 8), ("va_append_packed", 11), ("va_accept_tree", 9), ("va_fork_pages", 10), ("va_compact_pages", 7)):
+    getattr(_short, _name).argtypes = getattr(_lib, _name).argtypes[:_n]
+
+
+def _scratch(t):
+    """Address and bytes of a workspace."""
+    return (None, _vp(0)) if t is None else (_vp(t.data_ptr()), _vp(t.nbytes))
 
 
 def _strides(t, n: int):
@@ -464,8 +474,43 @@ _f16 = _i32 = _words = _row_types = None
 def _types():
     global _f16, _i32, _words, _row_types
     import torch
-    _f16, _i32, _words = torch.float16, (torch.int32,), (torch.int64, torch.uint64)
+    _f16, _i32, _words = torch.float16, torch.int32, (torch.int64, torch.uint64)
     _row_types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _refuse(what: str, kind: str, t, *shape: int):
+    raise ValueError(f"{what} must be dense, {kind} {list(shape)}, not {str(t.dtype)[6:]} {list(t.shape)} of strides {list(t.stride())}")
+
+
+def _ints(what: str, t, n: int):
+    """Pointer to a dense int32 array of n elements, or the front of a longer one."""
+    if t is None:
+        return None
+    if t.dtype is _i32 and t.numel() >= n and t.is_contiguous():
+        return t.data_ptr()
+    _refuse(what, "int32", t, n)
+
+
+def _rows(what: str, t, n: int, width: int):
+    """The same of a dense [n][width] array, or the front of a longer one."""
+    if t is None:
+        return None
+    if t.dtype is _i32 and t.is_contiguous():
+        sh = t.shape
+        if sh == (n, width) or (t.numel() >= n * width and (len(sh) == 1 or sh[-1] == width)):
+            return t.data_ptr()
+    _refuse(what, "int32", t, n, width)
+
+
+def _masks(t, n: int, width: int):
+    """The same of 64-bit words."""
+    if t is None:
+        return None
+    if t.dtype in _words and t.is_contiguous():
+        sh = t.shape
+        if sh == (n, width) or (t.numel() >= n * width and (len(sh) == 1 or sh[-1] == width)):
+            return t.data_ptr()
+    _refuse("tree_mask", "int64 or uint64", t, n, width)
 
 
 def _tree_strides(what: str, t, shape):
@@ -485,19 +530,6 @@ def _tree_strides(what: str, t, shape):
             return None
     raise ValueError(f"decode_tree: {what} must be float16 {list(shape)}, its last dimension dense, not {str(t.dtype)[6:]} {list(sh)} "
                      f"of strides {list(t.stride())}")
-
-
-def _array(what: str, t, kinds, n: int, width: int = 0):
-    """Pointer to a dense array [n], or [n][width], or the front of a longer one, of one of the types `kinds`."""
-    if t is None:
-        return None
-    if t.dtype in kinds and t.is_contiguous():
-        if t.shape == (n, width) if width else t.numel() >= n:
-            return t.data_ptr()
-        if width and t.numel() >= n * width and (t.dim() == 1 or t.shape[-1] == width):
-            return t.data_ptr()
-    raise ValueError(f"{what} must be dense, " + " or ".join(str(k)[6:] for k in kinds) + f" [{n}]"
-                     + (f"[{width}]" if width else "") + f", not {str(t.dtype)[6:]} {list(t.shape)} of strides {list(t.stride())}")
 
 
 def tree_workspace_bytes(B: int, Hq: int, Hkv: int, Q: int, D: int, S: int) -> int:
@@ -524,11 +556,11 @@ def decode_tree(fmt, b: DeviceBufs, tree_mask, lens, nodes, block_table, max_pag
     if _i32 is None:
         _types()
     rows = (B, Q, Hq, D)
-    _check(_lib.va_decode_tree(code, C.byref(b.va()), _tree_strides("q", b.q, rows), _tree_strides("out", b.out, rows),
-                               _array("tree_mask", tree_mask, _words, B, Q), _array("lens", lens, _i32, B),
-                               _array("nodes", nodes, _i32, B), _array("block_table", block_table, _i32, B, max_pages),
-                               max_pages, B, Hq, Hkv, Q, page_rows, num_pages, D, S, _ptr(b.ws), _nbytes(b.ws),
-                               _stream_ptr(stream)), "decode_tree")
+    _check(_short.va_decode_tree(code, C.byref(b.va()), _tree_strides("q", b.q, rows), _tree_strides("out", b.out, rows),
+                               _masks(tree_mask, B, Q), _ints("lens", lens, B),
+                               _ints("nodes", nodes, B), _rows("block_table", block_table, B, max_pages),
+                               max_pages, B, Hq, Hkv, Q, page_rows, num_pages, D, S, *_scratch(b.ws),
+                               _vp(_stream_ptr(stream))), "decode_tree")
 
 
 def append_packed(fmt, k, v, b: DeviceBufs, block_table, max_pages: int, cu_tokens, pos, B: int, Hkv: int,
@@ -551,10 +583,10 @@ def append_packed(fmt, k, v, b: DeviceBufs, block_table, max_pages: int, cu_toke
         T = k.numel() // (Hkv * D)
         if T * Hkv * D != k.numel():
             raise ValueError("append_packed: k and v must hold T * Hkv * D elements")
-    _check(_lib.va_append_packed(_fmt(fmt), _ptr(k), _ptr(v), kind, _strides(k, 2), _strides(v, 2), C.byref(b.va()),
-                                 _array("block_table", block_table, _i32, B, max_pages), max_pages,
-                                 _array("cu_tokens", cu_tokens, _i32, B + 1), _array("pos", pos, _i32, B), T, B, Hkv,
-                                 page_rows, num_pages, D, _stream_ptr(stream)), "append_packed")
+    _check(_short.va_append_packed(_fmt(fmt), _ptr(k), _ptr(v), kind, _strides(k, 2), _strides(v, 2), C.byref(b.va()),
+                                 _rows("block_table", block_table, B, max_pages), max_pages,
+                                 _ints("cu_tokens", cu_tokens, B + 1), _ints("pos", pos, B), T, B, Hkv,
+                                 page_rows, num_pages, D, _vp(_stream_ptr(stream))), "append_packed")
 
 
 def accept_tree(fmt, b: DeviceBufs, block_table, max_pages: int, lens, nodes, path, accepted, new_lens, B: int, P: int,
@@ -565,10 +597,10 @@ def accept_tree(fmt, b: DeviceBufs, block_table, max_pages: int, lens, nodes, pa
     int32 [B][P] ascending node indices (P <= 64)."""
     if _i32 is None:
         _types()
-    _check(_lib.va_accept_tree(_fmt(fmt), C.byref(b.va()), _array("block_table", block_table, _i32, B, max_pages), max_pages,
-                               _array("lens", lens, _i32, B), _array("nodes", nodes, _i32, B), _array("path", path, _i32, B, P),
-                               _array("accepted", accepted, _i32, B), _array("new_lens", new_lens, _i32, B), B, P, Hkv,
-                               page_rows, num_pages, D, layers, _stream_ptr(stream)), "accept_tree")
+    _check(_short.va_accept_tree(_fmt(fmt), C.byref(b.va()), _rows("block_table", block_table, B, max_pages), max_pages,
+                               _ints("lens", lens, B), _ints("nodes", nodes, B), _rows("path", path, B, P),
+                               _ints("accepted", accepted, B), _ints("new_lens", new_lens, B), B, P, Hkv,
+                               page_rows, num_pages, D, layers, _vp(_stream_ptr(stream))), "accept_tree")
 
 
 def pages_workspace_bytes(B: int, max_pages: int, num_pages: int) -> int:
@@ -585,12 +617,12 @@ def fork_pages(fmt, b: DeviceBufs, refs, block_table, lens, parent, new_refs, ne
     scratch of pages_workspace_bytes(Bout, max_pages, num_pages)."""
     if _i32 is None:
         _types()
-    _check(_lib.va_fork_pages(_fmt(fmt), C.byref(b.va()), _array("refs", refs, _i32, num_pages),
-                              _array("block_table", block_table, _i32, Bin, max_pages), _array("lens", lens, _i32, Bin),
-                              _array("parent", parent, _i32, Bout), _array("new_refs", new_refs, _i32, num_pages),
-                              _array("new_table", new_table, _i32, Bout, max_pages), _array("new_lens", new_lens, _i32, Bout),
-                              _array("shortage", shortage, _i32, 1), Bin, Bout, max_pages, reserve, Hkv, page_rows,
-                              num_pages, D, layers, _ptr(b.ws), _nbytes(b.ws), _stream_ptr(stream)), "fork_pages")
+    _check(_short.va_fork_pages(_fmt(fmt), C.byref(b.va()), _ints("refs", refs, num_pages),
+                              _rows("block_table", block_table, Bin, max_pages), _ints("lens", lens, Bin),
+                              _ints("parent", parent, Bout), _ints("new_refs", new_refs, num_pages),
+                              _rows("new_table", new_table, Bout, max_pages), _ints("new_lens", new_lens, Bout),
+                              _ints("shortage", shortage, 1), Bin, Bout, max_pages, reserve, Hkv, page_rows,
+                              num_pages, D, layers, *_scratch(b.ws), _vp(_stream_ptr(stream))), "fork_pages")
 
 
 def compact_pages(fmt, b: DeviceBufs, refs, block_table, new_refs, new_table, used, B: int, max_pages: int, Hkv: int,
@@ -600,10 +632,10 @@ def compact_pages(fmt, b: DeviceBufs, refs, block_table, new_refs, new_table, us
     number. b.ws: scratch of pages_workspace_bytes(B, max_pages, num_pages)."""
     if _i32 is None:
         _types()
-    _check(_lib.va_compact_pages(_fmt(fmt), C.byref(b.va()), _array("refs", refs, _i32, num_pages),
-                                 _array("block_table", block_table, _i32, B, max_pages), _array("new_refs", new_refs, _i32, num_pages),
-                                 _array("new_table", new_table, _i32, B, max_pages), _array("used", used, _i32, 1), B, max_pages,
-                                 Hkv, page_rows, num_pages, D, layers, _ptr(b.ws), _nbytes(b.ws), _stream_ptr(stream)), "compact_pages")
+    _check(_short.va_compact_pages(_fmt(fmt), C.byref(b.va()), _ints("refs", refs, num_pages),
+                                 _rows("block_table", block_table, B, max_pages), _ints("new_refs", new_refs, num_pages),
+                                 _rows("new_table", new_table, B, max_pages), _ints("used", used, 1), B, max_pages,
+                                 Hkv, page_rows, num_pages, D, layers, *_scratch(b.ws), _vp(_stream_ptr(stream))), "compact_pages")
 
 
 def probe_ceiling(device: int = 0, nbytes: int = 0, reps: int = 0, method: Optional[int] = None) -> float:
