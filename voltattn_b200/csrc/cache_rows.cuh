@@ -38,7 +38,7 @@ template <class T>
 __device__ __forceinline__ Raw8<T> load8(const T* src) {
     Raw8<T> r;
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = load_global(reinterpret_cast<const uint4*>(src) + i);
     return r;
 }
 template <class T>
@@ -65,7 +65,7 @@ __device__ __forceinline__ void to_fp32(const Raw8<T>& r, float (&v)[8]) {
 __device__ __forceinline__ int token_sequence(const int* cu, int B, int token, int lane) {
     int seq = 0;
     for (int k = 0; k < B; k += 32) {
-        const bool past = k + lane < B && __ldg(cu + k + lane + 1) <= token;
+        const bool past = k + lane < B && load_global(cu + k + lane + 1) <= token;
         const int c = __popc(__ballot_sync(0xffffffffu, past));
         seq += c;
         if (c < 32) break;
@@ -207,11 +207,11 @@ __global__ void __launch_bounds__(256, 3) append_packed_kernel(const AppendParam
         m.grp = (int)sub * 4 * kBatch + (lane >> 3);
         const int seq = token_sequence(p.cu, p.B, (int)token, lane);
         if (seq >= p.B) return m;
-        const int i = (int)token - __ldg(p.cu + seq), at = __ldg(p.pos + seq);
+        const int i = (int)token - load_global(p.cu + seq), at = load_global(p.pos + seq);
         const long long row = (long long)at + i;
         if (i < 0 || at < 0 || row >= (long long)p.max_pages * p.page_rows) return m;
         const int pi = (int)((__umulhi((unsigned)row, p.page_mul) + (unsigned)row) >> p.page_shift);  // (rows fit 31 bits)
-        const int pg = __ldg(p.table + (size_t)seq * p.max_pages + pi);
+        const int pg = load_global(p.table + (size_t)seq * p.max_pages + pi);
         if (pg < 0 || pg >= p.num_pages) return m;
         m.g0 = ((long long)pg * p.Hkv * p.page_rows + ((int)row - pi * p.page_rows)) * ng;
 #pragma unroll

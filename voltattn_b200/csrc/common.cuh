@@ -171,6 +171,14 @@ __device__ __forceinline__ void grid_launch_dependents() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// Data that the preceding grid may have written, after grid_dependency_wait(): an ordinary load. The
+// read-only path (__ldg) is for data that nobody writes while the kernel is there, and a kernel that
+// was launched programmatically is there before its predecessor has ended.
+template <class T>
+__device__ __forceinline__ T load_global(const T* p) {
+    return *p;
+}
+
 // ---- misc -----------------------------------------------------------------
 
 __device__ __forceinline__ float fast_exp2(float x) {

@@ -142,7 +142,7 @@ __device__ __forceinline__ UnitGeom unit_geom(const DecodeParams& p, int u) {
     UnitGeom g;
     g.h = u / p.S;
     g.s = u - g.h * p.S;
-    const long long len = p.lens ? (long long)min(max(__ldg(p.lens + g.h / p.Hkv), 0), p.L) : (long long)p.L;
+    const long long len = p.lens ? (long long)min(max(load_global(p.lens + g.h / p.Hkv), 0), p.L) : (long long)p.L;
     const long long j0 = min(len, (long long)g.s * p.chunk);
     const long long j1 = min(len, j0 + p.chunk);
     g.r0 = (long long)g.h * p.L + j0;
@@ -330,7 +330,7 @@ __device__ void stream_producer(const DecodeParams& p, uint8_t* smem, uint64_t* 
                     for (int dr = 0; dr < brows;) {
                         const int pi = j / p.page_rows, in = j - pi * p.page_rows;
                         const int n = min(brows - dr, p.page_rows - in);
-                        int pg = pi < p.max_pages ? __ldg(p.block_table + (size_t)b * p.max_pages + pi) : 0;
+                        int pg = pi < p.max_pages ? load_global(p.block_table + (size_t)b * p.max_pages + pi) : 0;
                         pg = (pg >= 0 && pg < p.num_pages) ? pg : 0;
                         const size_t ph = ((size_t)pg * p.Hkv + hk) * p.page_rows + in;
                         bulk_g2s(sK + (size_t)dr * C::kRb, p.K + ph * C::kRb, (uint32_t)n * C::kRb, &full[stage], pol);

@@ -250,7 +250,7 @@ __device__ __forceinline__ TcUnit tc_unit_geom(const DecodeParams& p, int u) {
     g.S = p.S;
     g.b = g.h / p.Hkv;
     g.hk = g.h - g.b * p.Hkv;
-    long long len = p.lens ? (long long)min(max(__ldg(p.lens + g.b), 0), p.L) : (long long)p.L;
+    long long len = p.lens ? (long long)min(max(load_global(p.lens + g.b), 0), p.L) : (long long)p.L;
     if (p.page_rows > 0) {
         g.r0 = 0;
     } else {
@@ -368,7 +368,7 @@ __device__ void tc_producer(const DecodeParams& p, const CUtensorMap* tmK, const
         // division, far cheaper than the emulated 64-bit one
         const int yl = (int)(pt0 + (long long)lane * C::kBox);
         const int pg = yl / p.page_rows;
-        int pp = pg < p.max_pages ? __ldg(p.block_table + (size_t)g.b * p.max_pages + pg) : 0;
+        int pp = pg < p.max_pages ? load_global(p.block_table + (size_t)g.b * p.max_pages + pg) : 0;
         pp = (pp >= 0 && pp < p.num_pages) ? pp : 0;
         return (pp * p.Hkv + g.hk) * p.page_rows + (yl - pg * p.page_rows);
     };

@@ -440,8 +440,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
 
     grid_dependency_wait();
     const long long cap = (long long)p.max_pages * p.page_rows;
-    const int len = (int)max(0ll, min((long long)__ldg(p.lens + b), cap));
-    const int n = max(0, min(min(p.nodes ? __ldg(p.nodes + b) : p.Q, p.Q), len));
+    const int len = (int)max(0ll, min((long long)load_global(p.lens + b), cap));
+    const int n = max(0, min(min(p.nodes ? load_global(p.nodes + b) : p.Q, p.Q), len));
     const int ctx = len - n;
     const int chunk = tree_chunk(len, p.S);
     const int nsplit = max(1, (len + chunk - 1) / chunk);
@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
     }
     if (tid < C::kRows) {
         const int r = r0 + tid, node = p.node_of(r);
-        s_mask[tid] = (r < p.R && node < n) ? __ldg(p.mask + (size_t)b * p.Q + node) : 0ull;
+        s_mask[tid] = (r < p.R && node < n) ? load_global(p.mask + (size_t)b * p.Q + node) : 0ull;
     }
     __syncthreads();
 
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
         if (copies) {
             const int pos = p0 + (warp + i * C::kWarps) * PB + run_at;
             const int pi = (int)((__umulhi((unsigned)pos, p.page_mul) + (unsigned)pos) >> p.page_shift);
-            int pg = pi < p.max_pages ? __ldg(trow + pi) : 0;
+            int pg = pi < p.max_pages ? load_global(trow + pi) : 0;
             pg = (unsigned)pg < (unsigned)p.num_pages ? pg : 0;
             bulk_g2s(lane_dst + s * C::kStageBytes, lane_src + pg * lane_page + (long long)(pos - pi * p.page_rows) * lane_row,
                      lane_bytes, bar + s, policy);
@@ -514,8 +514,8 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinCtas) decode_tree_kernel(c
                 uint4 v[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
                 if (ok) {
                     const uint4* s4 = reinterpret_cast<const uint4*>(src + 64 * gr + 16 * t);
-                    v[0] = __ldg(s4);
-                    v[1] = __ldg(s4 + 1);
+                    v[0] = load_global(s4);
+                    v[1] = load_global(s4 + 1);
                 }
                 const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
                 float sum = 0.f;

@@ -317,8 +317,8 @@ template <class C>
 __device__ __forceinline__ TreeTcSeq tree_tc_seq(const TreeParams& p, int b) {
     const long long cap = (long long)p.max_pages * p.page_rows;
     TreeTcSeq q;
-    q.len = (int)max(0ll, min((long long)__ldg(p.lens + b), cap));
-    q.n = max(0, min(min(p.nodes ? __ldg(p.nodes + b) : p.Q, p.Q), q.len));
+    q.len = (int)max(0ll, min((long long)load_global(p.lens + b), cap));
+    q.n = max(0, min(min(p.nodes ? load_global(p.nodes + b) : p.Q, p.Q), q.len));
     q.blocks = (int)(((unsigned)q.len + C::kNb - 1) / C::kNb);
     q.live_tiles = (min(p.R, q.n * p.G) + C::kRows - 1) / C::kRows;
     q.cost = q.live_tiles * (q.blocks + kTcFixed) + (p.tiles - q.live_tiles);
@@ -484,7 +484,7 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
     const auto page_of = [&](int pos, int& off) {
         const int pi = (int)((__umulhi((unsigned)pos, p.page_mul) + (unsigned)pos) >> p.page_shift);
         off = pos - pi * p.page_rows;
-        const int pg = pi < p.max_pages ? __ldg(trow + pi) : 0;
+        const int pg = pi < p.max_pages ? load_global(trow + pi) : 0;
         return (unsigned)pg < (unsigned)p.num_pages ? pg : 0;
     };
     __syncthreads();
@@ -508,12 +508,12 @@ __device__ __forceinline__ bool tree_tc_range(const TreeParams& p, const CUtenso
                 v[i] = make_uint4(0u, 0u, 0u, 0u);
                 if (qr < live) {
                     const int r = r0 + qr, node = p.node_of(r);
-                    v[i] = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.qs_b + node * p.qs_t +
+                    v[i] = load_global(reinterpret_cast<const uint4*>(p.q + b * p.qs_b + node * p.qs_t +
                                                                 (long long)(hk * p.G + (r - node * p.G)) * p.qs_h) + c);
                 }
             }
             const unsigned long long in_tree = n >= 64 ? ~0ull : (1ull << n) - 1ull;
-            if (tid < C::kRows) s_mask[tid] = tid < live ? __ldg(p.mask + (size_t)b * p.Q + p.node_of(r0 + tid)) & in_tree : 0ull;
+            if (tid < C::kRows) s_mask[tid] = tid < live ? load_global(p.mask + (size_t)b * p.Q + p.node_of(r0 + tid)) & in_tree : 0ull;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int x = tid + 512 * i, qr = x / (D / 8), c = x - qr * (D / 8), rr = qr & 127;

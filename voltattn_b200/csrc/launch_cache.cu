@@ -14,18 +14,18 @@ __global__ void __launch_bounds__(kAcceptThreads) accept_tree_kernel(const Accep
     grid_dependency_wait();
     const int hk = blockIdx.x, b = blockIdx.y;
     const long long cap = (long long)p.max_pages * p.page_rows;
-    const int len = (int)max(0ll, min((long long)__ldg(p.lens + b), cap));
-    const int nodes = max(0, min(__ldg(p.nodes + b), len));
+    const int len = (int)max(0ll, min((long long)load_global(p.lens + b), cap));
+    const int nodes = max(0, min(load_global(p.nodes + b), len));
     const int ctx = len - nodes;
     if (threadIdx.x < 32) {
-        const int want = max(0, min(__ldg(p.accepted + b), p.P));
+        const int want = max(0, min(load_global(p.accepted + b), p.P));
         int n = want;
         for (int c = 0; c < want; c += 32) {
             const int i = c + (int)threadIdx.x;
             bool bad = false;
             if (i < want) {
-                const int x = __ldg(p.path + (size_t)b * p.P + i);
-                bad = x < 0 || x >= nodes || (i > 0 && x <= __ldg(p.path + (size_t)b * p.P + i - 1));
+                const int x = load_global(p.path + (size_t)b * p.P + i);
+                bad = x < 0 || x >= nodes || (i > 0 && x <= load_global(p.path + (size_t)b * p.P + i - 1));
             }
             const unsigned m = __ballot_sync(0xffffffffu, bad);
             if (m) {
@@ -43,12 +43,12 @@ __global__ void __launch_bounds__(kAcceptThreads) accept_tree_kernel(const Accep
     const int* trow = p.table + (size_t)b * p.max_pages;
     const auto place = [&](int row) -> long long {
         const int pi = row / p.page_rows;
-        const int pg = pi < p.max_pages ? valid_page(__ldg(trow + pi), p.num_pages) : -1;
+        const int pg = pi < p.max_pages ? valid_page(load_global(trow + pi), p.num_pages) : -1;
         return pg < 0 ? -1
                       : blockIdx.z * p.layer_rows + ((long long)pg * p.Hkv + hk) * p.page_rows + (row - pi * p.page_rows);
     };
     for (int i = threadIdx.x; i < n; i += kAcceptThreads) {
-        const int x = __ldg(p.path + (size_t)b * p.P + i);
+        const int x = load_global(p.path + (size_t)b * p.P + i);
         const long long s = place(ctx + x), d = place(ctx + i);
         // a row in place, or one whose page does not exist, is left
         src[i] = (x == i || d < 0) ? -1 : s;
@@ -92,17 +92,17 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
     for (int s = tid; s < p.Bin; s += kPlanThreads) {
         kids[s] = 0;
         first[s] = INT_MAX;
-        const int len = (int)max(0ll, min((long long)__ldg(p.lens + s), cap));
+        const int len = (int)max(0ll, min((long long)load_global(p.lens + s), cap));
         lens[s] = len;
         full[s] = len / pr;
         // (the rest of a page, a page and a reserve below 2^31: 32 bits)
         need[s] = (int)min((unsigned)p.max_pages, (unsigned)full[s] + ((unsigned)(len - full[s] * pr) + p.reserve + pr - 1) / pr);
     }
     for (int i = tid; i < p.Bout; i += kPlanThreads) {
-        const int s = __ldg(p.parent + i);
+        const int s = load_global(p.parent + i);
         from_seq[i] = s >= 0 && s < p.Bin ? s : -1;
     }
-    for (int i = tid; i < num_pages; i += kPlanThreads) p.new_refs[i] = __ldg(p.refs + i);
+    for (int i = tid; i < num_pages; i += kPlanThreads) p.new_refs[i] = load_global(p.refs + i);
     __syncthreads();
     for (int i = tid; i < p.Bout; i += kPlanThreads)
         if (from_seq[i] >= 0) {
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
     };
     const auto held = [&](const Child& c, int j) {
         if (c.s < 0 || j >= p.max_pages || !(c.keep || j < c.full)) return -1;
-        return valid_page(__ldg(p.table + (size_t)c.s * p.max_pages + j), num_pages);
+        return valid_page(load_global(p.table + (size_t)c.s * p.max_pages + j), num_pages);
     };
     for (int i0 = warp; i0 < p.Bout; i0 += kWarps * kAhead) {
         Child c[kAhead];
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             const int s = s0 + u * kWarps;
-            e[u] = s < p.Bin && lane < p.max_pages ? __ldg(p.table + (size_t)s * p.max_pages + lane) : -1;
+            e[u] = s < p.Bin && lane < p.max_pages ? load_global(p.table + (size_t)s * p.max_pages + lane) : -1;
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
             if (s >= p.Bin) break;
             const int shared = kids[s] - 1, own = kids[s] > 0 ? 0 : -1;
             for (int j = lane; j < p.max_pages; j += 32) {
-                const int pg = valid_page(j < 32 ? e[u] : __ldg(p.table + (size_t)s * p.max_pages + j), num_pages);
+                const int pg = valid_page(j < 32 ? e[u] : load_global(p.table + (size_t)s * p.max_pages + j), num_pages);
                 const int d = j < full[s] ? shared : own;
                 if (pg >= 0 && d != 0) atomicAdd(p.new_refs + pg, d);
             }
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int pg = c0 + 4 * tid + k;
-            if (pg < num_pages && __ldg(p.refs + pg) == 0) f |= 1u << k;
+            if (pg < num_pages && load_global(p.refs + pg) == 0) f |= 1u << k;
         }
         int sum;
         int at = found + block_scan(__popc(f), scan, sum);
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParam
                     e = rank < kFreeHere ? free_here[rank] : p.free_list[rank];
                     atomicAdd(p.new_refs + e, 1);
                     if (j == part && rest > 0 && !c.keep) {
-                        from = valid_page(__ldg(p.table + (size_t)c.s * p.max_pages + j), num_pages);
+                        from = valid_page(load_global(p.table + (size_t)c.s * p.max_pages + j), num_pages);
                         to = e;
                     }
                 } else if (ask && j == part && rest > 0) {
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kCopyThreads) fork_copy_kernel(const ForkParam
             uint4 v[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (x + j * kCopyThreads < n) v[j] = __ldg(src + x + j * kCopyThreads);
+                if (x + j * kCopyThreads < n) v[j] = load_global(src + x + j * kCopyThreads);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (x + j * kCopyThreads < n) dst[x + j * kCopyThreads] = v[j];
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const Compac
     const int tid = threadIdx.x, num_pages = p.pool.num_pages;
     grid_dependency_wait();
     int mine = 0;
-    for (int i = tid; i < num_pages; i += kPlanThreads) mine += __ldg(p.refs + i) > 0;
+    for (int i = tid; i < num_pages; i += kPlanThreads) mine += load_global(p.refs + i) > 0;
     int n;
     block_scan(mine, scan, n);
     int holes = 0, movers = 0;
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const Compac
         for (int k = 0; k < 4; ++k) {
             const int pg = c0 + 4 * tid + k;
             if (pg < num_pages) {
-                const int r = __ldg(p.refs + pg);
+                const int r = load_global(p.refs + pg);
                 if (pg < n) {
                     if (r > 0) p.new_refs[pg] = r;
                     else hole |= 1u << k;
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const Compac
     __syncthreads();
     for (int i = tid; i < movers; i += kPlanThreads) {
         const int f = p.from[i], t = p.to[i];
-        p.new_refs[t] = __ldg(p.refs + f);
+        p.new_refs[t] = load_global(p.refs + f);
         p.map[f] = t;
     }
     if (tid == 0) {
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kMoveThreads) compact_move_kernel(const Compac
             uint4 x[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (w0 + j * kMoveThreads < words) x[j] = __ldg(src + w0 + j * kMoveThreads);
+                if (w0 + j * kMoveThreads < words) x[j] = load_global(src + w0 + j * kMoveThreads);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (w0 + j * kMoveThreads < words) dst[w0 + j * kMoveThreads] = x[j];
@@ -360,8 +360,8 @@ __global__ void __launch_bounds__(kMoveThreads) compact_move_kernel(const Compac
     }
     for (long long i = (long long)blockIdx.x * kMoveThreads + threadIdx.x; i < p.entries;
          i += (long long)gridDim.x * kMoveThreads) {
-        const int e = __ldg(p.table + i);
-        p.new_table[i] = e >= n && e < v.num_pages && __ldg(p.refs + e) > 0 ? p.map[e] : e;
+        const int e = load_global(p.table + i);
+        p.new_table[i] = e >= n && e < v.num_pages && load_global(p.refs + e) > 0 ? p.map[e] : e;
     }
 }
 
