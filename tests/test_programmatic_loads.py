@@ -24,3 +24,12 @@ def test_no_read_only_loads(name):
 def test_lengths_and_tables_of_the_decodes(name):
     """The single-token decodes read the same lengths and tables."""
     assert not re.findall(r"__ldg\s*\(\s*p\.(?:lens|block_table)[^;]*;", code(name))
+
+
+@pytest.mark.parametrize("name", ["decode_stream.cuh", "decode_tc.cuh", "decode_tcg.cuh", "decode_mma.cuh"])
+def test_the_decodes_wait_before_they_read_the_cache(name):
+    """No build reads K and V ahead of the wait: the kernels that write rows release the next one early."""
+    text = code(name)
+    waits = re.findall(r"[^;{}]*\bgrid_dependency_wait\(\)\s*;", text)
+    assert all(w.strip() == "grid_dependency_wait();" for w in waits), waits  # none under a condition
+    assert "EARLY" not in text.upper(), "a build that starts copies early"

@@ -269,12 +269,6 @@ __device__ __forceinline__ long long tc_tile_row(const TcUnit& g, int i) {
     return g.a0 + (long long)i * C::kTr;
 }
 
-#ifdef VA_TC_EARLY_KV
-constexpr bool kTcEarlyKv = true;
-#else
-constexpr bool kTcEarlyKv = false;
-#endif
-
 // Rows per tensor copy of a contiguous cache (the paged path copies kBox-row
 // boxes, each inside one page; q3 rows move as flat byte ranges).
 template <class C>
@@ -309,24 +303,13 @@ __device__ void tc_producer(const DecodeParams& p, const CUtensorMap* tmK, const
     };
     // split-L across GPUs: the step's epoch, read once (after the grid
     // dependency: the previous step's last CTA advanced the counter) and kept
-    // in shared memory for the ticket warp; the early-copy variant waits first
+    // in shared memory for the ticket warp
     const auto read_epoch = [&]() {
         if (p.xR > 0 && lane == 0)
             *shep = p.xepoch_ptr ? *reinterpret_cast<volatile unsigned*>(p.xepoch_ptr) + 1u : p.xepoch;
     };
-    bool waited = !kTcEarlyKv || p.xR > 0;
-    if (waited) {
-        read_epoch();
-        first_query();
-    }
-    const auto ensure_wait = [&]() {
-        if (!waited) {
-            grid_dependency_wait();
-            VA_TL(12, global_timer_ns());
-            first_query();
-            waited = true;
-        }
-    };
+    read_epoch();
+    first_query();
     if (lane == 0) VA_TL(11, global_timer_ns());
     const long long nr8 = p.total_rows & ~7ll;
     // q3 rows (48 bytes) are copied as flat byte ranges: a tensor copy issues
@@ -394,7 +377,6 @@ __device__ void tc_producer(const DecodeParams& p, const CUtensorMap* tmK, const
         int nxt = -1;
         int py_next = cur >= 0 ? paged_row(g, cur) : 0;
         if (cur < 0) {  // empty split: the header alone (slot and ticket still count)
-            if (!waited && (k >= C::kStages || !asked)) ensure_wait();
             if (!asked) {
                 if (lane == 0) unext = next_unit(sched, nunits);
                 asked = true;
@@ -411,7 +393,6 @@ __device__ void tc_producer(const DecodeParams& p, const CUtensorMap* tmK, const
             ++k;
         }
         for (int t = 0; cur >= 0; ++t, ++k) {
-            if (!waited && (k >= C::kStages || (!asked && t >= g.ntiles - 2))) ensure_wait();
             if (!asked && t >= g.ntiles - 2) {
                 if (lane == 0) unext = next_unit(sched, nunits);
                 asked = true;
@@ -550,7 +531,6 @@ __device__ void tc_producer(const DecodeParams& p, const CUtensorMap* tmK, const
         }
         u = __shfl_sync(0xffffffffu, unext, 0);
     }
-    ensure_wait();
     // this CTA's last grab is done: count it; the last CTA resets the schedule
     // (fences: this CTA's grabs are performed before its count, and the reset
     // after every CTA's count)
@@ -1122,17 +1102,9 @@ __global__ void __launch_bounds__(C::kThreads, 2)
         fence_mbar_init();
     }
     __syncthreads();
-    // Programmatic dependent launch: every warp but the producer waits here for
-    // the preceding grid (its ws, counters and out, and the query, which a
-    // preceding kernel may have written). With kTcEarlyKv the producer streams
-    // the first stages of K/V first, which no decode writes, and waits before
-    // it reads the query or touches the schedule counters.
-#ifdef VA_TC_TIMELINE
-    // timeline: 13 the first stage landed (seen by the idle ticket warp, before its grid wait)
-    if (kTcEarlyKv && warp == C::kWarps + 1 && lane == 0 && mbar_wait_bounded(&full[0], 0))
-        VA_TL(13, global_timer_ns());
-#endif
-    if (warp != C::kWarps || !kTcEarlyKv) grid_dependency_wait();
+    // Programmatic dependent launch: every warp waits here for the preceding grid (its ws, counters and
+    // out, and the query and the cache's rows, which a preceding kernel may have written).
+    grid_dependency_wait();
     if (threadIdx.x == 0) grid_launch_dependents();
     if (threadIdx.x == 0) {  // timeline: 0 start, 1 SM
         VA_TL(0, global_timer_ns());

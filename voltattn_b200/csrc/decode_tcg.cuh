@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(C::kThreads, C::kMinBlocks)
     }
     __syncthreads();
     // programmatic dependent launch: as in decode_tc_kernel
-    if (warp != C::kWarps || !kTcEarlyKv) grid_dependency_wait();
+    grid_dependency_wait();
     if (threadIdx.x == 0) grid_launch_dependents();
 
     const int h0 = (int)blockIdx.x / p.S;
