@@ -404,6 +404,9 @@ VA_API int va_device_error(int* code);
  * call to call; where a sequence is split depends on the batch's lengths as well. */
 VA_API size_t va_tree_workspace_bytes(int B, int Hq, int Hkv, int Q, int D, int S);
 VA_API int va_suggest_tree_splits(int fmt, int B, int Hq, int Hkv, int Q, int Lmax, int D, int* S);
+/* *rows = query rows of a CTA (16, 128 or 256) in va_decode_tree's call of this size, Lmax =
+ * max_pages * page_rows: the size of the table, not of the sequences in it, decides. */
+VA_API int va_tree_tile_rows(int fmt, int B, int Hq, int Hkv, int Q, int Lmax, int D, int* rows);
 VA_API int va_decode_tree(int fmt, const va_bufs* bufs, const long long* q_strides, const long long* out_strides,
                           const uint64_t* tree_mask, const int* lens, const int* nodes, const int* block_table,
                           int max_pages, int B, int Hq, int Hkv, int Q, int page_rows, int num_pages, int D, int S,

@@ -93,6 +93,7 @@ def _load():
     ll2 = C.POINTER(C.c_longlong)
     lib.va_tree_workspace_bytes.argtypes = [i] * 6; lib.va_tree_workspace_bytes.restype = sz
     lib.va_suggest_tree_splits.argtypes = [i] * 7 + [C.POINTER(i)]; lib.va_suggest_tree_splits.restype = i
+    lib.va_tree_tile_rows.argtypes = [i] * 7 + [C.POINTER(i)]; lib.va_tree_tile_rows.restype = i
     lib.va_decode_tree.argtypes = [i, C.POINTER(VaBufs), ll2, ll2, vp, vp, vp, vp] + [i] * 9 + [vp, sz, vp]
     lib.va_decode_tree.restype = i
     lib.va_append_packed.argtypes = ([i, vp, vp, i, ll2, ll2, C.POINTER(VaBufs), vp, i, vp, vp] + [i] * 6 + [vp])
@@ -540,6 +541,13 @@ def suggest_tree_splits(f, B: int, Hq: int, Hkv: int, Q: int, Lmax: int, D: int)
     s = C.c_int(0)
     _check(_lib.va_suggest_tree_splits(_fmt(f), B, Hq, Hkv, Q, Lmax, D, C.byref(s)), "suggest_tree_splits")
     return s.value
+
+
+def tree_tile_rows(f, B: int, Hq: int, Hkv: int, Q: int, Lmax: int, D: int) -> int:
+    """Query rows of a CTA (16, 128 or 256) in decode_tree's call of this size, Lmax = max_pages * page_rows."""
+    r = C.c_int(0)
+    _check(_lib.va_tree_tile_rows(_fmt(f), B, Hq, Hkv, Q, Lmax, D, C.byref(r)), "tree_tile_rows")
+    return r.value
 
 
 def decode_tree(fmt, b: DeviceBufs, tree_mask, lens, nodes, block_table, max_pages: int, B: int, Hq: int, Hkv: int,

@@ -52,11 +52,15 @@ int check_pool(int fmt, const va_bufs* b, int B, int max_pages, int Hkv, int pag
 // against 32 at 4 x 4000 rows. Few live rows leave them idle: 64 rows of q8+, 16
 // sequences up to 8192 rows, take 101 us in tiles of 16, 107 in one of 128. fp16 rows go to
 // the tensor cores without a conversion: 64 rows 132 against 74 us, 32 rows 88
-// against 70. The sizes are those of the tables, the lengths being on the device.
-int tree_rows(int fmt, int B, int Hkv, int R, int Lmax) {
+// against 70. fp8 rows of 128 dims take the longest to convert, so they need more query rows: 80 rows,
+// 16 sequences of 1000 to 4000, 127 against 138, 128 rows 185 against 140 (128 with half of them
+// live 128 against 138; of 64 dims 80 rows already gain). The sizes are those of the tables, the
+// lengths being on the device.
+int tree_rows(int fmt, int B, int Hkv, int R, int Lmax, int D) {
     const bool f16 = fmt == VA_F16P;
     const double work = (double)B * Hkv * Lmax * R;
-    if (R <= (f16 ? 16 : 64) || work <= (f16 ? 1 << 21 : 1 << 23)) return 16;
+    const int small = f16 ? 16 : fmt == VA_F8P && D == 128 ? 96 : 64;
+    if (R <= small || work <= (f16 ? 1 << 21 : 1 << 23)) return 16;
     return R <= 128 ? 128 : 256;
 }
 
@@ -157,7 +161,15 @@ int va_suggest_tree_splits(int fmt, int B, int Hq, int Hkv, int Q, int Lmax, int
     const int rc = current_device(&dev);
     if (rc) return rc;
     const int R = Hq / Hkv * Q;
-    *S = tree_splits(sm_count(dev), tree_rows(fmt, B, Hkv, R, Lmax), B, Hkv, R, Lmax);
+    *S = tree_splits(sm_count(dev), tree_rows(fmt, B, Hkv, R, Lmax, D), B, Hkv, R, Lmax);
+    return VA_OK;
+}
+
+int va_tree_tile_rows(int fmt, int B, int Hq, int Hkv, int Q, int Lmax, int D, int* rows) {
+    if (!rows || fmt < VA_F16 || fmt > VA_Q4CP || B < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv || Q < 1 || Q > kMaxNodes || Lmax < 1)
+        return VA_ERR_INVALID;
+    if (!tree_fmt(fmt) || (D != 64 && D != 128)) return VA_ERR_UNSUPPORTED;
+    *rows = tree_rows(fmt, B, Hkv, Hq / Hkv * Q, Lmax, D);
     return VA_OK;
 }
 
@@ -180,7 +192,7 @@ int va_decode_tree(int fmt, const va_bufs* b, const long long* q_strides, const 
         if (qs[i] % 8 || os[i] % 8) return VA_ERR_ALIGN;
     if ((long long)max_pages * page_rows > kMaxTreeRows) return VA_ERR_TOO_LARGE;
     if ((long long)B * Hq * Q > INT_MAX / kMaxSplits) return VA_ERR_TOO_LARGE;
-    const int R = Hq / Hkv * Q, rows = tree_rows(fmt, B, Hkv, R, max_pages * page_rows);
+    const int R = Hq / Hkv * Q, rows = tree_rows(fmt, B, Hkv, R, max_pages * page_rows, D);
     if (!ws || !aligned16(ws)) return VA_ERR_WORKSPACE;
     if (S == 0) {
         int dev;
