@@ -392,8 +392,8 @@ VA_API int va_device_error(int* code);
  * h * strides[2] + d (host arrays of 3, multiples of 8; NULL: contiguous
  * [B][Q][Hq][D]); q 16-byte, out 8-byte aligned. Any Hq / Hkv. Formats f16+ / bf16+ /
  * f8+ / q8+ / q4+ / q3+ at D = 64 or 128, page_rows a multiple of 8 (else
- * VA_ERR_UNSUPPORTED). bf16 rows are taken as fp16 values (beyond fp16's range:
- * infinite; below 2^-14 with fewer bits). Table entries outside [0, num_pages) read page 0.
+ * VA_ERR_UNSUPPORTED). bf16 rows are taken as fp16 values (65536 and beyond:
+ * infinite; exact down to 2^-17, fewer bits below). Table entries outside [0, num_pages) read page 0.
  * S: the most parts that a sequence's rows are split into over CTAs (<= 128; 0:
  * chosen by va_suggest_tree_splits' rule and what ws holds). ws: 16-byte aligned,
  * ws_bytes >= va_tree_workspace_bytes(B, Hq, Hkv, Q, D, max(S, 1)), zeroed before

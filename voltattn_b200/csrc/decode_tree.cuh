@@ -403,16 +403,18 @@ __device__ __forceinline__ void tree_merge(const TreeParams& p, int stream, int 
                     u[z][k] = __ldcg(src + ((size_t)row * p.S + s) * Q4);
                 }
 #pragma unroll
-            for (int z = 0; z < kAhead; ++z)
+            for (int z = 0; z < kAhead; ++z) {
+                const bool on = s0 + z < nsplit;  // (a weight of 0 is not enough: the values may be infinite)
 #pragma unroll
                 for (int k = 0; k < kItems; ++k) {
                     const int row = min(rw + k * kRowStep, rows - 1);
-                    const float a = s0 + z < nsplit ? sw[row * kTreeMaxSplits + s0 + z] : 0.f;
-                    v[k].x = fmaf(u[z][k].x, a, v[k].x);
-                    v[k].y = fmaf(u[z][k].y, a, v[k].y);
-                    v[k].z = fmaf(u[z][k].z, a, v[k].z);
-                    v[k].w = fmaf(u[z][k].w, a, v[k].w);
+                    const float a = on ? sw[row * kTreeMaxSplits + s0 + z] : 0.f;
+                    v[k].x = fmaf(on ? u[z][k].x : 0.f, a, v[k].x);
+                    v[k].y = fmaf(on ? u[z][k].y : 0.f, a, v[k].y);
+                    v[k].z = fmaf(on ? u[z][k].z : 0.f, a, v[k].z);
+                    v[k].w = fmaf(on ? u[z][k].w : 0.f, a, v[k].w);
                 }
+            }
         }
 #pragma unroll
         for (int k = 0; k < kItems; ++k) {
