@@ -38,8 +38,8 @@ class ToyModel:
     def inputs(self, tokens, places):
         """x, q [..., HQ, D] and k, v [..., HKV, D] of tokens at their places."""
         x = self.embed[tokens] + self.place[places]
-        shape = (*tokens.shape, -1, D)
-        return x, (x @ self.wq).half().view(shape), (x @ self.wk).half().view(shape), (x @ self.wv).half().view(shape)
+        heads = lambda w, n: (x @ w).half().view(*tokens.shape, n, D)  # noqa: E731
+        return x, heads(self.wq, HQ), heads(self.wk, HKV), heads(self.wv, HKV)
 
     def next_tokens(self, x, attended):
         return (attended.float().flatten(-2) @ self.wo + x @ self.skip).argmax(-1)
@@ -100,7 +100,7 @@ def prefill(model, cache, prompts, device):
     """All but the prompts' last tokens into the cache; the last ones start the decoding."""
     B = len(prompts)
     cache.reorder(torch.arange(B, dtype=torch.int32, device=device), max(map(len, prompts)))
-    packed = torch.cat([torch.tensor(p[:-1], device=device) for p in prompts])
+    packed = torch.cat([torch.tensor(p[:-1], dtype=torch.long, device=device) for p in prompts])
     places = torch.cat([torch.arange(len(p) - 1, device=device) for p in prompts])
     _, _, k, v = model.inputs(packed, places)
     cache.append(k, v, torch.tensor([len(p) - 1 for p in prompts], dtype=torch.int32, device=device))
