@@ -26,7 +26,7 @@
 //   O += P V: the V scale multiplies the fp32 weight before its one rounding to
 //     fp16 (P' = fp16(w * scale), one P' per group).
 // The rounding of P' is the only one below 32 bits: it is relative (2^-11) down to 2^-14. The
-// exponent's reference of a query row is the most of score + log2 of the position's own (larger) V scale
+// exponent's reference of a query row is the most of score + floor(log2) of the position's own (larger) V scale
 // over the positions that it sees, set where P' of that position is 2^11, and left while that
 // grows by no more than kTreeLag (log2): a row's largest P' lies in [2^11, 2^16). P' of the other
 // positions, and of the group of smaller scales, lie below it by the ratio of weights and scales.
@@ -325,18 +325,20 @@ __device__ __forceinline__ bool clear_not_finite(uint32_t& u) {
     return any;
 }
 
-// log2 of a position's V scales (one, or two and the larger counts) for the exponents' reference.
-// Infinite and nan ones, which make what they scale infinite or nan whatever the reference is, count as
-// fp16's largest; 0, which gives no P' at all, as less than its least.
+// floor(log2) of a position's V scales (one, or two and the larger counts) for the exponents'
+// reference: whole, so that the position that sets a reference has a power of two as its weight and
+// its P' (the scales, then) need no rounding. Infinite and nan ones, which make what they scale
+// infinite or nan whatever the reference is, count as fp16's largest; 0, which gives no P' at all, as
+// less than its least.
 __device__ __forceinline__ float tree_scale_log2(__half2 v) {
     v = __habs2(v);
     const __half m = __hmin(__hmax(__low2half(v), __high2half(v)), __ushort_as_half((unsigned short)0x7BFF));
-    return fmaxf(__log2f(__half2float(m)), -25.f);
+    return fmaxf((float)((int)(__float_as_uint(__half2float(m)) >> 23) - 127), -25.f);
 }
-// A row's reference is set where its largest P' is 2^kTreeBase, and left while that stays below
-// 2^(kTreeBase + kTreeLag): fp16 ends just below 2^16, and the approximate log2 and exp2 take less
-// than the remaining 0.1.
-constexpr float kTreeBase = 11.f, kTreeLag = 4.9f;
+// A row's reference is set where its largest P' is in [2^kTreeBase, 2^(kTreeBase + 1)), and left while
+// that stays below 2^(kTreeBase + kTreeLag + 1); fp16 ends just below 2^16. A shorter way to go keeps more of
+// the heaviest positions at exact weights, and moves O more often (kTreeLag 2: 103 us where this takes 101).
+constexpr float kTreeBase = 11.f, kTreeLag = 3.9f;
 
 // The last range of a row tile merges all of them, in order: first the weights of
 // every (row, range) into shared memory (kRows * (kTreeMaxSplits + 1) floats), then the

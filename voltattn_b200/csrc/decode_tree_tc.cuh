@@ -411,7 +411,7 @@ __device__ __forceinline__ void tree_tc_plan(const TreeParams& p, int lane, Tree
 }
 
 // As kTreeBase and kTreeLag: a move costs more here, O's way through registers.
-constexpr float kTcBase = 10.f, kTcLag = 5.9f;
+constexpr float kTcBase = 10.f, kTcLag = 4.9f;
 
 // Four columns of query row r of a (sequence, KV head).
 struct TreeTcStore {
