@@ -392,16 +392,22 @@ VA_API int va_device_error(int* code);
  * h * strides[2] + d (host arrays of 3, multiples of 8; NULL: contiguous
  * [B][Q][Hq][D]); q 16-byte, out 8-byte aligned. Any Hq / Hkv. Formats f16+ / bf16+ /
  * f8+ / q8+ / q4+ / q3+ at D = 64 or 128, page_rows a multiple of 8 (else
- * VA_ERR_UNSUPPORTED). bf16 rows are taken as fp16 values (65536 and beyond:
- * infinite; exact down to 2^-17, fewer bits below). Table entries outside [0, num_pages) read page 0.
+ * VA_ERR_UNSUPPORTED), max_pages * page_rows below 2^31 - 2^16 (else
+ * VA_ERR_TOO_LARGE). bf16 rows are taken as fp16 values (exact from 2^-17 to 65280;
+ * fewer bits below, infinite from 65536 on). Table entries outside [0, num_pages)
+ * read page 0.
  * S: the most parts that a sequence's rows are split into over CTAs (<= 128; 0:
  * chosen by va_suggest_tree_splits' rule and what ws holds). ws: 16-byte aligned,
  * ws_bytes >= va_tree_workspace_bytes(B, Hq, Hkv, Q, D, max(S, 1)), zeroed before
  * first use (va_workspace_init). A completed call leaves the counters at its front
- * zero, so one workspace serves calls of any shape in order on one stream. Splits
+ * zero, so one workspace serves calls of any shape in order on one stream (zero it
+ * again after a call whose kernel reported an error, va_device_error). Splits
  * (S > 1) take at most 16384 row tiles, one per (sequence, KV head, 16 to 256 of its
  * Hq / Hkv * Q query rows, by the call's size). Results are the same from
- * call to call; where a sequence is split depends on the batch's lengths as well. */
+ * call to call; where a sequence is split depends on the batch's lengths as well.
+ * The table's size (max_pages * page_rows), not the lengths in it, chooses the tile of
+ * query rows and, with S = 0, the parts: tables much longer than the sequences take
+ * more time than tables of their length. */
 VA_API size_t va_tree_workspace_bytes(int B, int Hq, int Hkv, int Q, int D, int S);
 VA_API int va_suggest_tree_splits(int fmt, int B, int Hq, int Hkv, int Q, int Lmax, int D, int* S);
 /* *rows = query rows of a CTA (16, 128 or 256) in va_decode_tree's call of this size, Lmax =
@@ -449,6 +455,10 @@ VA_API int va_accept_tree(int fmt, const va_bufs* bufs, const int* block_table, 
  * free. The first new sequence of a parent keeps all of its pages; the others
  * share its full pages (lens / page_rows of them), and get a page of their own
  * for the rest, into which the rows are copied (in blocks of 8, in every layer).
+ * Shared pages are not copied when someone writes them later: lens has to be final
+ * for the rows that are there, so fork between accept_tree and the next append, not
+ * while drafted rows are in the cache, and do not take a length back into a full page
+ * that a fork has shared (two sequences would write one page).
  * Each new sequence then has pages for lens + reserve rows, as far as max_pages
  * go. Pages are given out lowest number first, in order of sequence and place,
  * from those with refs 0 before the call (pages that the call frees serve the

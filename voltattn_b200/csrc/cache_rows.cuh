@@ -180,7 +180,8 @@ __device__ __forceinline__ void quantize_group_packed(const float (&v)[8], bool 
 // page, its elements: four dependent loads) before it quantizes the current one. Bound by the
 // quantizer's instructions on prompts (issue slots 70 % busy, DRAM 27 %): 12 prompts of 301 to 4099
 // tokens, fp16 to q8+, 8 heads of 128: 55 us, 3.1 TB/s (a division an element: 108 us); 32
-// drafts of 7 to 16 tokens: 3.7 us, a launch's latency.
+// drafts of 7 to 16 tokens: 3.6 us, a launch's latency. (fp32 rows to packed codes spill 40 to 72 bytes at 80
+// registers.)
 template <int BITS, class T>
 __global__ void __launch_bounds__(256, 3) append_packed_kernel(const AppendParams p) {
     constexpr int kBatch = 2;

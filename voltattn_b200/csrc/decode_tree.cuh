@@ -37,12 +37,12 @@
 // are cleared. A drafted float row with inf or nan entries reaches only the rows
 // that see it (`special` below).
 //
-// Bound by instruction issue and the latency between dependent instructions: 23
-// warp-instructions a position and tile for q8+ (f16+ 17, q4+ 27, q3+ 31) with three CTAs
-// of 168 registers an SM, issue slots 51 % busy. 16 query rows because 32 spill at that count, and
-// two CTAs of more registers were slower; four CTAs of 128 registers took 183 us where this took 113.
-// Measured: 16 sequences of 1024 to 8192 rows, q8+, 16 nodes, 32 query / 8 KV heads, 102 us
-// (the cache at the copy rate would take 26); one sequence of 1024, q4+, 8 nodes, 10.3 us.
+// Bound by instruction issue and the latency between dependent instructions: 27 warp-instructions a
+// position and tile for q8+, start and merge included, with three CTAs of 168 registers an SM, issue
+// slots 50 % busy. 16 query rows because 32 spill far more at that count (these spill 4 to 52 bytes at D = 128),
+// and two CTAs of more registers were slower; four CTAs of 128 registers took 183 us where this took 113.
+// Measured: 16 sequences of 1024 to 8192 rows, q8+, 16 nodes, 32 query / 8 KV heads, 101 us
+// (the cache at the copy rate would take 26); one sequence of 1024, q4+, 8 nodes, 10.6 us.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -2,8 +2,9 @@
 // operator of decode_tree.cuh (its mathematics, masks, splits and slots) for many
 // query rows, with tcgen05.mma and accumulators in tensor memory.
 //
-// One CTA per (sequence, KV head, tile of query rows, range of positions), one
-// per SM, 23 warps:
+// One CTA per SM, each with an equal window of the call's blocks of positions (with S = 1 a CTA per
+// tile of query rows): the ranges in it, of one (sequence, KV head, tile) each, one after the other.
+// 23 warps:
 //   warps 0-15   softmax: thread (group w, half hf, row r) has 32 of the 64 positions of
 //                query row r (TMEM lane r) in the jobs of group w;
 //   warps 16, 17  producers of K tiles, 18, 19 of V tiles: codes -> exact fp16 codes in
@@ -37,13 +38,14 @@
 // 32-bit word ((0, 4), (1, 5), ...), which costs no byte permutes; Q's columns are
 // stored in the same order and the output's are put back.
 //
-// Bound by what the roles share: issue slots (58 % busy) and shared memory. A block of 64
-// positions against 128 rows takes 1.27 us and 5600 warp-instructions. In copies with parts
-// cut out (303 us then): no loads of scales 270, no stores of decoded tiles 261, a quarter of
-// the MMAs 293, no exponentials 295. Measured: 8 sequences of 16384 to 32768 rows, q4+,
-// 32 nodes, 32 query / 8 KV heads, 231 us, 470 TFLOP/s (598 us in tiles of 16); 16 of 2048
-// to 8192, f16+, 64 nodes, 32 / 4 heads, 120 us, 760 TFLOP/s (144 in a loop of seconds, at
-// the 1000 W power cap).
+// Bound by what the roles share: issue slots (60 % busy) and shared memory. A block of 64
+// positions against 128 rows takes 1.32 us and 5650 warp-instructions, start and merge included. In
+// copies with parts cut out (303 us before the windows): no loads of scales 270, no stores of decoded
+// tiles 261, a quarter of the MMAs 293, no exponentials 295. 736 threads leave 80 registers each: the
+// softmax spills 28 to 172 bytes at D = 128 (20 to 116 at 64), and where it does decides a few percent.
+// Measured: 8 sequences of 16384 to 32768 rows, q4+, 32 nodes, 32 query / 8 KV heads, 232 us, 470
+// TFLOP/s (598 us in tiles of 16); 16 of 2048 to 8192, f16+, 64 nodes, 32 / 4 heads, 146 us, 627
+// TFLOP/s, in a loop of seconds at the 1000 W power cap, 121 to 124 in a burst.
 #pragma once
 
 #include "decode_tree.cuh"

@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kAcceptThreads) accept_tree_kernel(const Accep
 // shared memory and a warp has the first 32 entries of kAhead sequences in flight. 96 new
 // sequences of 200 to 1500 rows: about 14 us.
 constexpr int kAhead = 2;
-constexpr int kFreeHere = 1024;  // pages of the free list kept in shared memory as well
+constexpr int kFreeHere = 1024;  // free pages kept in shared memory (further ones in free_list)
 __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const ForkParams p) {
     extern __shared__ int sm[];
     int* kids = sm;              // [Bin]
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const Compac
 }
 
 // The moved pages' bytes (chunks of kMoveChunk 16-byte words, over all CTAs) and
-// the tables' entries. Bound by HBM: 1400 pages of 64 rows, q4+, 8 heads, 4 layers move in 145 us with
+// the tables' entries. Bound by HBM: 1400 pages of 64 rows, q4+, 8 heads, 4 layers move in 143 us with
 // the plan, 5.4 TB/s.
 constexpr int kMoveThreads = 256, kMoveWords = 4 * kMoveThreads;
 __global__ void __launch_bounds__(kMoveThreads) compact_move_kernel(const CompactParams p) {

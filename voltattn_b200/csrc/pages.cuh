@@ -31,7 +31,7 @@ struct ForkParams {
     int* new_table;     // [Bout][max_pages]
     int* new_lens;
     int* shortage;
-    int* free_list;     // workspace [Bout * max_pages]
+    int* free_list;     // workspace [num_pages]: the free pages to give out, past the first kFreeHere
     int* copy;          // workspace [3][Bout]: from, to, rows
     int Bin, Bout, max_pages, reserve;
 };
